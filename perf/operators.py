@@ -108,8 +108,10 @@ def prepare(case, seed):
     if own:  # a program packs its weights once, when it loads them
         from kadan_amd import ops
         for name in ("w", "gate", "up"):
-            if name in state:
+            if name in state and c["path"] != "backward":
                 state[name + "_packed"] = ops.mxfp4_pack(*state[name])
+            if name in state and c["path"] in ("backward", "train"):
+                state[name + "_transposed"] = ops.mxfp4_pack(*state[name], transposed=True)
     return state
 
 
@@ -148,13 +150,15 @@ def own_pass(state):
     if c["path"] == "quantized":
         return ops.mxfp4_product_quantized(*state["x"], state["w_packed"], c["n"],
                                            dtype=TYPES[c["y"]])
-    gate, up = state["gate_packed"], state["up_packed"]
     if c["path"] == "gated":
-        return ops.mxfp4_gated(state["x"], gate, up, c["n"])
+        return ops.mxfp4_gated(state["x"], state["gate_packed"], state["up_packed"], c["n"])
     if c["path"] == "backward":
-        return ops.mxfp4_gated_backward(state["dh"], state["saved"], gate, up, c["k"])
-    h, saved = ops.mxfp4_gated(state["x"], gate, up, c["n"], save="q8")
-    dx, dgu = ops.mxfp4_gated_backward(state["dh"], saved, gate, up, c["k"])
+        return ops.mxfp4_gated_backward(state["dh"], state["saved"], state["gate_transposed"],
+                                        state["up_transposed"], c["k"])
+    h, saved = ops.mxfp4_gated(state["x"], state["gate_packed"], state["up_packed"], c["n"],
+                               save="q8")
+    dx, dgu = ops.mxfp4_gated_backward(state["dh"], saved, state["gate_transposed"],
+                                       state["up_transposed"], c["k"])
     return h, dx, dgu
 
 
