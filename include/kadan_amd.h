@@ -392,6 +392,80 @@ int kdq_moe_mxfp4_packed_noalloc(const uint16_t* x_bf16, const float* logits, si
                                  const uint8_t* down_packed, float* y, int32_t* idx,
                                  float* w, int32_t* offsets, int32_t* perm, void* stream);
 
+/* ---- MXFP4 dense layers (the reference multiplies MXFP4 rows on the host only:
+ * IW/src/weights/quantization.cpp:207-247).  A matrix of `rows` x `cols` values is
+ * blocks u8 [rows, cols/2] and scales u8 [rows, cols/32] as above, cols % 32 == 0, any
+ * number of rows.  Calls on different streams share nothing: what scratch a call needs is
+ * the caller's `workspace` (device memory, 16-byte aligned, at least what the _workspace
+ * function of the call says; null where that is 0), which two calls that may overlap must
+ * not share.  Nothing allocates, so every call may be captured in a graph.
+ * Sizes: m <= 2^20 rows of activations, k <= 2^20, n <= 2^24; strides count values, are
+ * multiples of 8 and at most 2^21 for inputs, and any for outputs (products: outputs 2- or
+ * 4-byte aligned); other pointers 16-byte aligned.  Scale bytes above 252 take the largest
+ * codes past fp32's range: such weights are infinite, or NaN (255). */
+
+/* x [rows x cols] (type KDQ_F32, KDQ_F16 or KDQ_BF16, rows x_stride values apart) as
+ * MXFP4: per 32 values the scale is 2^(floor(log2(largest magnitude)) - 2) (byte at least
+ * 0), codes value / scale rounded to the nearest E2M1 value, ties to the even code,
+ * magnitudes above 6 to 6.  A block with a value that is not finite gets scale byte 255
+ * and codes 0, and *status |= 1 (status may be null; the caller zeroes it).
+ * x 16-byte, blocks 4-byte aligned. */
+int kdq_mxfp4_quantize(int type, const void* x, size_t x_stride, size_t rows, size_t cols,
+                       uint8_t* blocks, uint8_t* scales, unsigned* status, void* stream);
+
+/* Packs a matrix for the products, once per weight: `packed` 16-byte aligned,
+ * kdq_mxfp4_packed_bytes long (0 for sizes that have no packed form).  The form is that of
+ * kdq_moe_mxfp4_pack with one expert, with rows rounded up to 32 and cols to 64. */
+size_t kdq_mxfp4_packed_bytes(size_t rows, size_t cols);
+int kdq_mxfp4_pack(const uint8_t* blocks, const uint8_t* scales, size_t rows, size_t cols,
+                   uint8_t* packed, void* stream);
+
+/* Packs a matrix for kdq_mxfp4_gated_backward, which sums over its rows (at most 2^19). */
+size_t kdq_mxfp4_packed_transposed_bytes(size_t rows, size_t cols);
+int kdq_mxfp4_pack_transposed(const uint8_t* blocks, const uint8_t* scales, size_t rows,
+                              size_t cols, uint8_t* packed, void* stream);
+
+/* y [m x n] = x [m x k] W^T: W packed (n rows of k), x bf16 rows x_stride apart, y of
+ * type KDQ_F32 or KDQ_BF16, rows y_stride apart.  Products of decoded weights and x are
+ * exact, sums are fp32. */
+size_t kdq_mxfp4_product_workspace(size_t m, size_t n, size_t k, int quantized);
+int kdq_mxfp4_product(const uint16_t* x_bf16, size_t x_stride, size_t m, const uint8_t* packed,
+                      size_t n, size_t k, int type, void* y, size_t y_stride, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
+/* The same over MXFP4 activations (kdq_mxfp4_quantize; workspace with quantized = 1). */
+int kdq_mxfp4_product_quantized(const uint8_t* x_blocks, const uint8_t* x_scales, size_t m,
+                                const uint8_t* packed, size_t n, size_t k, int type, void* y,
+                                size_t y_stride, void* workspace, size_t workspace_bytes,
+                                void* stream);
+
+/* The gated feed-forward projection in one pass over x: g = x Wg^T, u = x Wu^T (n rows of
+ * k each, n % 32 == 0), h [m x n] bf16 = g * sigmoid(g) * u.  For a backward pass the
+ * pre-activations may be kept (workspace with kept = 1): as bf16 [m x 2n], g then u
+ * (kept_bf16), or in 8 bits as kdq_quantize_q8 does, int8 [m x 2n] (kept_q8) and fp32
+ * [m x 2n/32] (kept_scales; blocks under 2^-120 are kept as zeros, blocks with a value
+ * that is not finite have a NaN scale); null pointers keep nothing. */
+size_t kdq_mxfp4_gated_workspace(size_t m, size_t n, size_t k, int kept);
+int kdq_mxfp4_gated(const uint16_t* x_bf16, size_t x_stride, size_t m,
+                    const uint8_t* gate_packed, const uint8_t* up_packed, size_t n, size_t k,
+                    uint16_t* h_bf16, size_t h_stride, uint16_t* kept_bf16, int8_t* kept_q8,
+                    float* kept_scales, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Its backward pass over frozen weights: from dh [m x n] bf16 and the kept pre-activations
+ * (one of kept_bf16 and kept_q8 with kept_scales), with s = sigmoid(g):
+ * dg = dh * u * s * (1 + g * (1 - s)) and du = dh * g * s, written as dgu [m x 2n] bf16
+ * (dg, then du: the gradients that adapters of the two projections need, or x^T products
+ * for a float copy of the weights), and dx [m x k] bf16 = dg Wg + du Wu, the products of
+ * the rounded dg and du exact and their sums fp32.  Weights from
+ * kdq_mxfp4_pack_transposed(n rows, k cols). */
+size_t kdq_mxfp4_gated_backward_workspace(size_t m, size_t n, size_t k);
+int kdq_mxfp4_gated_backward(const uint16_t* dh_bf16, size_t dh_stride, size_t m,
+                             const uint16_t* kept_bf16, const int8_t* kept_q8,
+                             const float* kept_scales, const uint8_t* gate_transposed,
+                             const uint8_t* up_transposed, size_t n, size_t k,
+                             uint16_t* dgu_bf16, uint16_t* dx_bf16, size_t dx_stride,
+                             void* workspace, size_t workspace_bytes, void* stream);
+
 /* Measurement aid, no counterpart in the reference: one streaming read of `bytes`
  * (a multiple of 16; `src` 16-byte aligned) over `workgroups` workgroups of `threads`
  * (256 or 1024) lanes.  Workgroup b folds (xor) the 32-bit words of its share, units of

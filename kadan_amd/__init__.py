@@ -87,6 +87,15 @@ _SIGNATURES = {
                              _VP, _VP, _VP],
     "kdq_moe_mxfp4_packed_noalloc": [_VP, _VP, _SZ, _SZ, _SZ, _SZ, _SZ, _VP, _VP, _VP, _VP,
                                      _VP, _VP, _VP, _VP, _VP],
+    "kdq_mxfp4_quantize": [_I, _VP, _SZ, _SZ, _SZ, _VP, _VP, _VP, _VP],
+    "kdq_mxfp4_pack": [_VP, _VP, _SZ, _SZ, _VP, _VP],
+    "kdq_mxfp4_pack_transposed": [_VP, _VP, _SZ, _SZ, _VP, _VP],
+    "kdq_mxfp4_product": [_VP, _SZ, _SZ, _VP, _SZ, _SZ, _I, _VP, _SZ, _VP, _SZ, _VP],
+    "kdq_mxfp4_product_quantized": [_VP, _VP, _SZ, _VP, _SZ, _SZ, _I, _VP, _SZ, _VP, _SZ, _VP],
+    "kdq_mxfp4_gated": [_VP, _SZ, _SZ, _VP, _VP, _SZ, _SZ, _VP, _SZ, _VP, _VP, _VP, _VP, _SZ,
+                        _VP],
+    "kdq_mxfp4_gated_backward": [_VP, _SZ, _SZ, _VP, _VP, _VP, _VP, _VP, _SZ, _SZ, _VP, _VP, _SZ,
+                                 _VP, _SZ, _VP],
     "kdq_hbm_read": [_VP, _SZ, _VP, _SZ, _I, _I, C.c_uint, _VP],
     "kdq_release_scratch": [],
 }
@@ -100,6 +109,11 @@ _OTHER = {
     "kdq_gemm_rows_values": (_SZ, [_I]),
     "kdq_gemv_packed_supported": (_I, [_I, _SZ]),
     "kdq_moe_mxfp4_packed_bytes": (_SZ, [_SZ, _SZ, _SZ]),
+    "kdq_mxfp4_packed_bytes": (_SZ, [_SZ, _SZ]),
+    "kdq_mxfp4_packed_transposed_bytes": (_SZ, [_SZ, _SZ]),
+    "kdq_mxfp4_product_workspace": (_SZ, [_SZ, _SZ, _SZ, _I]),
+    "kdq_mxfp4_gated_workspace": (_SZ, [_SZ, _SZ, _SZ, _I]),
+    "kdq_mxfp4_gated_backward_workspace": (_SZ, [_SZ, _SZ, _SZ]),
 }
 
 _lib = None

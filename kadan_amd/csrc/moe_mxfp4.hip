@@ -1670,32 +1670,34 @@ __global__ __launch_bounds__(kDecodeWaves * 64) void decode_down_kernel(
     }
 }
 
+// Eight codes of a row to a lane (four lanes a 32-value block): a wavefront's reads and
+// writes are whole lines.
 __global__ __launch_bounds__(256) void mxfp4_dequant_kernel(const uint8_t* __restrict__ blocks,
                                                             const uint8_t* __restrict__ scales,
-                                                            size_t rows, size_t cols,
+                                                            size_t eighths,
                                                             float* __restrict__ out,
                                                             unsigned* status) {
-    const size_t i = size_t(blockIdx.x) * blockDim.x + threadIdx.x;  // one byte = 2 values
+    const size_t i = size_t(blockIdx.x) * blockDim.x + threadIdx.x;  // 4 bytes = 8 values
     unsigned bad = 0;
-    if (i < rows * cols / 2) {
-        const size_t r = i / (cols / 2), c = (i % (cols / 2)) * 2;
-        const unsigned byte = blocks[i];
-        const unsigned s = scales[r * (cols / 32) + c / 32];
+    if (i < eighths) {
+        typedef unsigned any __attribute__((aligned(1)));  // (rows may lie anywhere)
+        const unsigned codes = *reinterpret_cast<const any*>(blocks + i * 4), s = scales[i / 4];
         if (s == 255)
             bad |= 1u;
+        float v[8];
+        auto pair = [&]<int SEL>() {  // codes 2 SEL, 2 SEL + 1 (at scale 1), times 2^(s - 127)
+            const auto p = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(codes, 1.0f, SEL);
+            v[2 * SEL] = __builtin_amdgcn_ldexpf(p[0], int(s) - 127);
+            v[2 * SEL + 1] = __builtin_amdgcn_ldexpf(p[1], int(s) - 127);
+        };
+        static_for<4>(pair);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const unsigned code = (byte >> (4 * h)) & 15u;
-            const float mag[8] = {0.f, 0.5f, 1.f, 1.5f, 2.f, 3.f, 4.f, 6.f};
-            float v = 0.f;
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-                v = (code & 7u) == unsigned(q) ? mag[q] : v;
-            v = ldexpf(v, int(s) - 127);
-            if (!isfinite(v))
+        for (int h = 0; h < 8; ++h)
+            if (!isfinite(v[h]))
                 bad |= 2u;
-            out[r * cols + c + h] = (code & 8u) ? -v : v;
-        }
+        typedef float quad __attribute__((ext_vector_type(4), aligned(4)));
+        *reinterpret_cast<quad*>(out + i * 8) = quad{v[0], v[1], v[2], v[3]};
+        *reinterpret_cast<quad*>(out + i * 8 + 4) = quad{v[4], v[5], v[6], v[7]};
     }
     if (status && bad)
         atomicOr(status, bad);
@@ -1963,10 +1965,9 @@ extern "C" int kdq_mxfp4_dequantize(const uint8_t* blocks, const uint8_t* scales
         return KDQ_ERR_ARGUMENT;
     if (cols % 32 || mul_overflows(rows, cols))
         return KDQ_ERR_SHAPE;
-    const size_t threads = rows * cols / 2;
-    hipLaunchKernelGGL(mxfp4_dequant_kernel, dim3(unsigned((threads + 255) / 256)), dim3(256), 0,
-                       static_cast<hipStream_t>(stream), blocks, scales, rows, cols, out,
-                       status);
+    const size_t eighths = rows * cols / 8;
+    hipLaunchKernelGGL(mxfp4_dequant_kernel, dim3(unsigned((eighths + 255) / 256)), dim3(256), 0,
+                       static_cast<hipStream_t>(stream), blocks, scales, eighths, out, status);
     KDQ_HIP(hipGetLastError());
     return KDQ_OK;
 }

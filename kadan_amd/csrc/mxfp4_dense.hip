@@ -1,0 +1,1366 @@
+// MXFP4 dense layers for gfx950: products with a packed matrix, the gated feed-forward
+// projection and its backward pass (include/kadan_amd.h).  The reference multiplies MXFP4
+// rows on the host only (IW/src/weights/quantization.cpp:207-247; IW =
+// services/hikari/inference_worker).
+//
+//   pack_kernel        rows -> the packed form every product reads
+//   pack_t_kernel      rows -> the form the backward pass reads (summed over the rows)
+//   decode_kernel      a few rows of x: one workgroup per 16 matrix rows, K over its
+//                      wavefronts, the weights read once as 256-byte runs
+//   gemm_kernel        more rows: 256 matrix rows x 32..256 rows of x a workgroup
+//   reduce_kernel      K slices of gemm_kernel summed in slice order, then its epilogue
+//   gate_grad_kernel   dg, du from dh and the kept pre-activations
+#include "kdq_common.hpp"
+
+#include <algorithm>
+#include <atomic>
+#include <utility>
+
+namespace kdq {
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
+
+// ------------------------------------------------------------------ packed forms
+//
+// Packed (kdq_mxfp4_pack): per group of 32 rows and step of 64 values one 1 KB block of
+// codes, lane i + 32h holding the 16 bytes of values 64q + 32h .. +31 of row 32g + i; then
+// per group and 4 steps one 256-byte block of scales, byte j of lane i + 32h's dword the
+// scale of step 4p + j.  Rows and values past the matrix are zero codes with scale 0.
+//
+// Transposed (kdq_mxfp4_pack_transposed), for sums over the rows: per group of 64 columns
+// and step of 64 rows one 2 KB block of codes in two 1 KB pieces, lane c + 32h of piece p
+// holding for rows 64q + 32h + 16p .. +15 the byte that holds columns 64g + 2c (low nibble)
+// and 64g + 2c + 1; then per group and step 128 bytes of scales, byte b of run 2h + e the
+// scale of row 64q + 32h + b for columns 64g + 32e .. +31.
+
+struct Form {
+    size_t groups, steps, code_bytes, scale_bytes;
+};
+
+__host__ __device__ inline size_t ceil_div(size_t a, size_t b) {
+    return (a + b - 1) / b;
+}
+
+__host__ __device__ inline Form packed_form(size_t rows, size_t cols) {
+    Form f;
+    f.groups = ceil_div(rows, 32);
+    f.steps = ceil_div(cols, 64);
+    f.code_bytes = f.groups * f.steps * 1024;
+    f.scale_bytes = f.groups * ceil_div(f.steps, 4) * 256;
+    return f;
+}
+
+__host__ __device__ inline Form transposed_form(size_t rows, size_t cols) {
+    Form f;
+    f.groups = ceil_div(cols, 64);
+    f.steps = ceil_div(rows, 64);
+    f.code_bytes = f.groups * f.steps * 2048;
+    f.scale_bytes = f.groups * f.steps * 128;
+    return f;
+}
+
+__global__ __launch_bounds__(256) void pack_kernel(const uint8_t* __restrict__ blocks,
+                                                   const uint8_t* __restrict__ scales,
+                                                   size_t rows, size_t cols, Form f,
+                                                   uint8_t* __restrict__ out) {
+    const size_t u = size_t(blockIdx.x) * 256 + threadIdx.x;
+    const size_t units = f.code_bytes / 16;
+    if (u < units) {  // 16 bytes of codes
+        const unsigned l = unsigned(u % 64);
+        const size_t q = u / 64 % f.steps, row = u / 64 / f.steps * 32 + l % 32;
+        const size_t at = q * 32 + 16 * (l / 32);
+        u32x4 v{0, 0, 0, 0};
+        if (row < rows && at < cols / 2)
+            v = load16(blocks + row * (cols / 2) + at);
+        *reinterpret_cast<u32x4*>(out + u * 16) = v;
+    } else if (u - units < f.scale_bytes / 4) {  // a dword of scales
+        const size_t w = u - units, sg = ceil_div(f.steps, 4);
+        const unsigned l = unsigned(w % 64);
+        const size_t p = w / 64 % sg, row = w / 64 / sg * 32 + l % 32;
+        unsigned word = 0;
+        for (unsigned j = 0; j < 4; ++j) {
+            const size_t b = 2 * (4 * p + j) + l / 32;  // the row's 32-value block
+            if (row < rows && b < cols / 32)
+                word |= unsigned(scales[row * (cols / 32) + b]) << (8 * j);
+        }
+        reinterpret_cast<unsigned*>(out + f.code_bytes)[w] = word;
+    }
+}
+
+__global__ __launch_bounds__(256) void pack_t_kernel(const uint8_t* __restrict__ blocks,
+                                                     const uint8_t* __restrict__ scales,
+                                                     size_t rows, size_t cols, Form f,
+                                                     uint8_t* __restrict__ out) {
+    const size_t u = size_t(blockIdx.x) * 256 + threadIdx.x;
+    const size_t units = f.code_bytes / 16, width = cols / 2;
+    if (u < units) {  // one column byte of 16 rows
+        const unsigned l = unsigned(u % 64), piece = unsigned(u / 64 % 2);
+        const size_t q = u / 128 % f.steps, g = u / 128 / f.steps;
+        const size_t byte = 32 * g + l % 32, row = 64 * q + 32 * (l / 32) + 16 * piece;
+        unsigned w[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (unsigned b = 0; b < 16; ++b)
+            if (row + b < rows && byte < width)
+                w[b / 4] |= unsigned(blocks[(row + b) * width + byte]) << (8 * (b % 4));
+        *reinterpret_cast<u32x4*>(out + u * 16) = u32x4{w[0], w[1], w[2], w[3]};
+    } else if (u - units < f.scale_bytes / 4) {
+        const size_t w = u - units, within = w % 32;  // 32 dwords per group and step
+        const size_t q = w / 32 % f.steps, g = w / 32 / f.steps;
+        const size_t run = within / 8, row = 64 * q + 32 * (run / 2) + 4 * (within % 8);
+        const size_t block = 2 * g + run % 2;
+        unsigned word = 0;
+        for (unsigned b = 0; b < 4; ++b)
+            if (row + b < rows && block < cols / 32)
+                word |= unsigned(scales[(row + b) * (cols / 32) + block]) << (8 * b);
+        reinterpret_cast<unsigned*>(out + f.code_bytes)[w] = word;
+    }
+}
+
+// ------------------------------------------------------------------ decoding
+
+// Byte j of a dword of E8M0 scales as the fp32 operand of the conversions, which take its
+// exponent field and nothing else (checked on the device for every scale byte, with other
+// bits set as well): a rotation puts the byte there.
+__device__ __forceinline__ float scale_of(unsigned word, unsigned j) {
+    return __uint_as_float(__builtin_amdgcn_alignbit(word, word, 9 + 8 * j));
+}
+
+__device__ __forceinline__ unsigned bits(bf16x2 v) {
+    return __builtin_bit_cast(unsigned, v);
+}
+
+// Eight E2M1 codes times their scale as bf16, which holds every such value (scale bytes up
+// to 252; past that the largest codes are infinite, as in fp32; 255 gives NaN).
+__device__ __forceinline__ bf16x8 decode8(unsigned codes, float scale) {
+    const u4 v{bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0)),
+               bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1)),
+               bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2)),
+               bits(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3))};
+    return __builtin_bit_cast(bf16x8, v);
+}
+
+// The transposed form: byte j of `codes` is row j's pair of columns, byte j of `scales` its
+// scale.  Eight rows as the operands of the even columns and of the odd ones.
+__device__ __forceinline__ void decode8_pair(const unsigned (&codes)[2],
+                                             const unsigned (&scales)[2], bf16x8& even,
+                                             bf16x8& odd) {
+    unsigned e[4], o[4];
+#pragma unroll
+    for (int d = 0; d < 2; ++d) {
+        const unsigned v0 = bits(
+            __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes[d], scale_of(scales[d], 0), 0));
+        const unsigned v1 = bits(
+            __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes[d], scale_of(scales[d], 1), 1));
+        const unsigned v2 = bits(
+            __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes[d], scale_of(scales[d], 2), 2));
+        const unsigned v3 = bits(
+            __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes[d], scale_of(scales[d], 3), 3));
+        e[2 * d] = __builtin_amdgcn_perm(v1, v0, 0x05040100);
+        o[2 * d] = __builtin_amdgcn_perm(v1, v0, 0x07060302);
+        e[2 * d + 1] = __builtin_amdgcn_perm(v3, v2, 0x05040100);
+        o[2 * d + 1] = __builtin_amdgcn_perm(v3, v2, 0x07060302);
+    }
+    even = __builtin_bit_cast(bf16x8, u4{e[0], e[1], e[2], e[3]});
+    odd = __builtin_bit_cast(bf16x8, u4{o[0], o[1], o[2], o[3]});
+}
+
+// ------------------------------------------------------------------ outputs
+
+enum Out { kOutF32, kOutBf16, kOutGated, kOutBackward };
+
+// Where results go.  Products: y [m][n].  Gated: y = h bf16 [m][n], and the kept
+// pre-activations if asked for: bf16 [m][2n] (gates, then ups), or int8 [m][2n] with an
+// fp32 scale per 32.  Backward: y = dx bf16 [m][n].
+struct Target {
+    void* y;
+    size_t stride;  // values per row of y
+    unsigned m, n;
+    uint16_t* kept;
+    int8_t* kept_q;
+    float* kept_d;
+};
+
+__device__ __forceinline__ unsigned bf16_pair(float a, float b) {
+    const bf16x2 v{__bf16(a), __bf16(b)};  // round to nearest even
+    return bits(v);
+}
+
+// silu(g) * u with the hardware exp2 and reciprocal (about 2^-22 relative; h leaves as bf16)
+__device__ __forceinline__ float gate_value(float g, float u) {
+    const float e = __builtin_amdgcn_exp2f(-1.44269504f * g);
+    return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
+}
+
+typedef unsigned pair_a2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef unsigned quad_a2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef float quadf_a4 __attribute__((ext_vector_type(4), aligned(4)));
+
+// Four values of consecutive columns c .. c+3 of row `row` as bf16 / fp32 (those below n).
+__device__ __forceinline__ void store4_bf16(uint16_t* y, size_t stride, unsigned n,
+                                            unsigned row, unsigned c, f32x4 v) {
+    uint16_t* at = y + size_t(row) * stride + c;
+    const unsigned lo = bf16_pair(v.x, v.y), hi = bf16_pair(v.z, v.w);
+    if (c + 3 < n) {
+        *reinterpret_cast<pair_a2*>(at) = pair_a2{lo, hi};
+    } else {
+        if (c < n)
+            at[0] = uint16_t(lo);
+        if (c + 1 < n)
+            at[1] = uint16_t(lo >> 16);
+        if (c + 2 < n)
+            at[2] = uint16_t(hi);
+    }
+}
+
+__device__ __forceinline__ void store4_f32(float* y, size_t stride, unsigned n, unsigned row,
+                                           unsigned c, f32x4 v) {
+    float* at = y + size_t(row) * stride + c;
+    if (c + 3 < n) {
+        *reinterpret_cast<quadf_a4*>(at) = quadf_a4{v.x, v.y, v.z, v.w};
+    } else {
+        if (c < n)
+            at[0] = v.x;
+        if (c + 1 < n)
+            at[1] = v.y;
+        if (c + 2 < n)
+            at[2] = v.z;
+    }
+}
+
+// Quad j of a wavefront's two 32 x 32 result tiles (group G, row `token` of x, lane half
+// h): values 8j + 4h .. +3 of the tiles' matrix rows.  Products: the tiles are rows 64G and
+// 64G + 32; gated: gate and up rows 32G; backward: columns 64G + 2i and 64G + 2i + 1.
+template <int OUT>
+__device__ __forceinline__ void store_quad(const Target& t, unsigned G, unsigned token,
+                                           unsigned h, unsigned j, f32x4 v0, f32x4 v1) {
+    if (token >= t.m)
+        return;
+    const unsigned r = 8 * j + 4 * h;
+    if constexpr (OUT == kOutF32) {
+        store4_f32(static_cast<float*>(t.y), t.stride, t.n, token, 64 * G + r, v0);
+        store4_f32(static_cast<float*>(t.y), t.stride, t.n, token, 64 * G + 32 + r, v1);
+    } else if constexpr (OUT == kOutBf16) {
+        store4_bf16(static_cast<uint16_t*>(t.y), t.stride, t.n, token, 64 * G + r, v0);
+        store4_bf16(static_cast<uint16_t*>(t.y), t.stride, t.n, token, 64 * G + 32 + r, v1);
+    } else if constexpr (OUT == kOutGated) {
+        const unsigned c = 32 * G + r;
+        const f32x4 hv{gate_value(v0.x, v1.x), gate_value(v0.y, v1.y), gate_value(v0.z, v1.z),
+                       gate_value(v0.w, v1.w)};
+        store4_bf16(static_cast<uint16_t*>(t.y), t.stride, t.n, token, c, hv);
+        if (t.kept && c < t.n) {  // (n % 32 == 0)
+            store4_bf16(t.kept, 2 * size_t(t.n), 2 * t.n, token, c, v0);
+            store4_bf16(t.kept, 2 * size_t(t.n), 2 * t.n, token, t.n + c, v1);
+        }
+    } else {
+        const unsigned c = 64 * G + 2 * r;  // (n % 32 == 0: all eight or none)
+        if (c < t.n)
+            *reinterpret_cast<quad_a2*>(static_cast<uint16_t*>(t.y) + size_t(token) * t.stride +
+                                        c) =
+                quad_a2{bf16_pair(v0.x, v1.x), bf16_pair(v0.y, v1.y), bf16_pair(v0.z, v1.z),
+                        bf16_pair(v0.w, v1.w)};
+    }
+}
+
+// One row's 32 pre-activations (a lane holds 16 of them, lane ^ 32 the others) as int8
+// codes with scale amax / 127, codes round-half-even(v * 127 / amax): kdq_quantize_q8's
+// format.  A block with a value that is not finite keeps a NaN scale; one whose largest
+// magnitude is below 2^-120 is kept as zeros (127 / amax would overflow).
+__device__ __forceinline__ void keep_q8(const Target& t, unsigned column, unsigned token,
+                                        unsigned h, const f32x4 (&v)[4]) {
+    float amax = 0.f;
+    unsigned top = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            top = max(top, __float_as_uint(v[j][i]) & 0x7fffffffu);
+    top = max(top, unsigned(__shfl_xor(int(top), 32, 64)));
+    const bool finite = top < 0x7f800000u;
+    amax = __uint_as_float(top);
+    const bool some = finite && amax >= 0x1p-120f;
+    const float inv = some ? 127.0f / amax : 0.f;
+    if (token >= t.m || column >= 2 * t.n)
+        return;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        unsigned word = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int q = some ? int(rintf(v[j][i] * inv)) : 0;
+            word |= (unsigned(q) & 255u) << (8 * i);
+        }
+        *reinterpret_cast<unsigned*>(t.kept_q + size_t(token) * 2 * t.n + column + 8 * j + 4 * h) =
+            word;
+    }
+    if (h == 0)
+        t.kept_d[size_t(token) * (2 * t.n / 32) + column / 32] =
+            !finite ? __uint_as_float(0x7fc00000u) : some ? amax / 127.0f : 0.f;
+}
+
+__device__ __forceinline__ f32x4 quad_of(const f32x16& a, int j) {
+    return f32x4{a[4 * j], a[4 * j + 1], a[4 * j + 2], a[4 * j + 3]};
+}
+
+template <int OUT>
+__device__ __forceinline__ void store_tiles(const Target& t, unsigned G, unsigned token,
+                                            unsigned h, const f32x16& a0, const f32x16& a1) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        store_quad<OUT>(t, G, token, h, j, quad_of(a0, j), quad_of(a1, j));
+    if constexpr (OUT == kOutGated) {
+        if (t.kept_q && 32 * G < t.n) {
+            const f32x4 g[4] = {quad_of(a0, 0), quad_of(a0, 1), quad_of(a0, 2), quad_of(a0, 3)};
+            const f32x4 u[4] = {quad_of(a1, 0), quad_of(a1, 1), quad_of(a1, 2), quad_of(a1, 3)};
+            keep_q8(t, 32 * G, token, h, g);
+            keep_q8(t, t.n + 32 * G, token, h, u);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ a few rows of x
+//
+// One workgroup takes 16 matrix rows (both matrices' for the gated projection) and all of
+// K, in units of 128 values that its wavefronts take in turn.  Per unit a lane holds 32
+// values of one matrix row (lane r + 16q: row r, values 128t + 32q ..) and of one row of x,
+// so four v_mfma_f32_16x16x32_bf16 multiply the unit without moving a value between lanes:
+// the sum over K may run in any order.  Weights are read once, as two 256-byte runs of a
+// block per unit.
+
+struct Decode {
+    const uint8_t *w0, *w1;
+    const uint8_t* x;         // bf16 rows, or MXFP4 blocks
+    const uint8_t* x_scales;  // MXFP4 scales
+    unsigned x_stride;        // bytes
+    unsigned k, steps, groups;
+    Target out;
+};
+
+constexpr int kOutside = 0x7ffffff0;  // past any buffer's range: such loads return zeros
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const uint8_t* p, unsigned bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, int(bytes), 0x00027000);
+}
+
+__device__ __forceinline__ u4 load_b128(const __amdgpu_buffer_rsrc_t& r, int at) {
+    const auto v = __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0);
+    return u4{unsigned(v[0]), unsigned(v[1]), unsigned(v[2]), unsigned(v[3])};
+}
+
+// The wavefronts' partial results of a workgroup: [wavefront][tile][lane].
+template <int TB, bool GATED, bool FP4, int OUT>
+__global__ __launch_bounds__(1024) void decode_kernel(Decode a) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    auto* red = reinterpret_cast<f32x4*>(lds);
+    const unsigned lane = threadIdx.x % 64, wave = threadIdx.x / 64, waves = blockDim.x / 64;
+    const unsigned r = lane % 16, q = lane / 16;
+    const unsigned group = blockIdx.x / 2, row = 16 * (blockIdx.x % 2) + r;
+    const unsigned share = GATED ? waves / 2 : waves;  // wavefronts on one matrix
+    const uint8_t* w = GATED && wave >= share ? a.w1 : a.w0;
+    const unsigned first = wave % share, units = (a.k + 127) / 128;
+    const unsigned scale_groups = (a.steps + 3) / 4;
+    const auto codes = buffer(w + size_t(group) * a.steps * 1024, a.steps * 1024);
+    const auto scales = buffer(w + size_t(a.groups) * a.steps * 1024 +
+                                   size_t(group) * scale_groups * 256,
+                               scale_groups * 256);
+    const unsigned lane_codes = (q / 2) * 1024 + (row + 32 * (q % 2)) * 16;
+    const unsigned lane_scales = (row + 32 * (q % 2)) * 4;
+    const unsigned row_bytes = FP4 ? a.k / 2 : a.k * 2;
+    const auto xs = buffer(a.x, (a.out.m - 1) * a.x_stride + row_bytes);
+    const auto xscales = buffer(a.x_scales, FP4 ? a.out.m * (a.k / 32) : 0);
+
+    f32x4 acc[TB] = {};
+    constexpr int kBatch = TB == 1 ? 4 : 2;
+    constexpr int kX = FP4 ? 1 : 4;
+    for (unsigned t0 = first; t0 < units; t0 += kBatch * share) {
+        u4 c[kBatch], x[kBatch][TB][kX];
+        unsigned s[kBatch], xb[kBatch][TB];
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            const unsigned t = t0 + b * share;  // past the last unit: zeros
+            c[b] = load_b128(codes, int(t * 2048 + lane_codes));
+            s[b] = __builtin_amdgcn_raw_buffer_load_b32(scales, int(t / 2 * 256 + lane_scales), 0,
+                                                        0);
+        }
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            const unsigned t = t0 + b * share;
+#pragma unroll
+            for (int i = 0; i < TB; ++i) {
+                const unsigned token = r + 16 * i;
+                const bool there = token < a.out.m && 128 * t + 32 * q < a.k;
+                if constexpr (FP4) {
+                    x[b][i][0] =
+                        load_b128(xs, there ? int(token * a.x_stride + (4 * t + q) * 16) : kOutside);
+                    xb[b][i] = __builtin_amdgcn_raw_buffer_load_b8(
+                        xscales, there ? int(token * (a.k / 32) + 4 * t + q) : kOutside, 0, 0);
+                } else {
+                    const int at = there ? int(token * a.x_stride + (128 * t + 32 * q) * 2)
+                                         : kOutside - 64;
+#pragma unroll
+                    for (int d = 0; d < 4; ++d)
+                        x[b][i][d] = load_b128(xs, at + 16 * d);
+                }
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            const unsigned t = t0 + b * share;
+            const float ws = scale_of(s[b], 2 * (t % 2) + q / 2);
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                const bf16x8 wv = decode8(c[b][d], ws);
+#pragma unroll
+                for (int i = 0; i < TB; ++i) {
+                    bf16x8 xv;
+                    if constexpr (FP4)
+                        xv = decode8(x[b][i][0][d], scale_of(xb[b][i], 0));
+                    else
+                        xv = __builtin_bit_cast(bf16x8, x[b][i][d]);
+                    acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, xv, acc[i], 0, 0, 0);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < TB; ++i)
+        red[(wave * TB + i) * 64 + lane] = acc[i];
+    __syncthreads();
+    if (wave >= TB)
+        return;
+    const unsigned token = 16 * wave + r, at = blockIdx.x * 16 + 4 * q;
+    if (token >= a.out.m)
+        return;
+    auto total = [&](unsigned from) {
+        f32x4 sum = red[(from * TB + wave) * 64 + lane];
+        for (unsigned i = 1; i < share; ++i)
+            sum += red[((from + i) * TB + wave) * 64 + lane];
+        return sum;
+    };
+    f32x4 v = total(0);
+    if constexpr (GATED) {
+        const f32x4 u = total(share);
+        v = f32x4{gate_value(v.x, u.x), gate_value(v.y, u.y), gate_value(v.z, u.z),
+                  gate_value(v.w, u.w)};
+    }
+    if constexpr (OUT == kOutF32)
+        store4_f32(static_cast<float*>(a.out.y), a.out.stride, a.out.n, token, at, v);
+    else
+        store4_bf16(static_cast<uint16_t*>(a.out.y), a.out.stride, a.out.n, token, at, v);
+}
+
+// ------------------------------------------------------------------ more rows of x
+//
+// A workgroup of eight wavefronts takes 256 matrix rows (four row groups of two 32-row
+// tiles) and, as two wavefront groups, either two parts of K of the same TT * 32 rows of x
+// (SPLIT; the groups' sums meet in LDS at the end) or two sets of TT * 32 rows.  x passes
+// through LDS in chunks of 128 bytes a row (64 bf16 values, or 256 MXFP4 values), copied
+// by DMA three chunks ahead into four buffers, eight rows to an instruction; a row's
+// 16-byte segments lie in it by (segment ^ row % 8), so the copies read whole lines and
+// the operands' reads are free of bank conflicts.  Weights go from memory to registers,
+// every one read and decoded by one wavefront (two where the groups share rows).
+//
+// Operands: bf16 x (v_mfma_f32_32x32x16_bf16, weights decoded to bf16, exact), MXFP4 x
+// (v_mfma_scale_f32_32x32x64_f8f6f4 over both codes as they lie), and the backward pass's
+// transposed weights under bf16 gradients.
+
+enum Operands { kBf16, kFp4, kTransposed };
+
+struct Gemm {
+    const uint8_t *w0, *w1;   // the matrices of the wavefront's two tiles; backward: of the groups
+    const uint8_t* x;
+    const uint8_t* x_scales;  // kFp4
+    unsigned x_stride;        // bytes
+    unsigned x_second;        // kTransposed: bytes to the second matrix's values in a row
+    unsigned segments;        // 16-byte segments of a row of x (of one matrix's part)
+    unsigned groups, steps;   // of the packed form
+    unsigned chunks, part;    // chunks of K, and how many a part has (a multiple of 4)
+    unsigned tiles_n, tiles_m;
+    Target out;
+    float* partial;           // K slices: results go here
+};
+
+constexpr int kStages = 4;
+constexpr unsigned kTileFloats = 2 * 16 * 64;  // a wavefront's two result tiles
+
+__device__ __forceinline__ void issue_order() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+template <int N, class F>
+__device__ __forceinline__ void static_for(F&& f) {
+    [&]<int... I>(std::integer_sequence<int, I...>) {
+        (f.template operator()<I>(), ...);
+    }(std::make_integer_sequence<int, N>{});
+}
+
+__device__ __forceinline__ i32x8 fp4_operand(const u4& c) {
+    const i32x4 v{int(c.x), int(c.y), int(c.z), int(c.w)};
+    return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1);
+}
+
+template <int TT, bool SPLIT, int OPS, int OUT>
+__global__ __launch_bounds__(512, 2) void gemm_kernel(Gemm a) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    constexpr int kStageBytes = TT * 8192;
+    const unsigned lane = threadIdx.x % 64, h = lane / 32;
+    const unsigned wave = unsigned(__builtin_amdgcn_readfirstlane(int(threadIdx.x / 64)));
+    const unsigned rg = wave % 4, kg = wave / 4;
+
+    // neighbouring tiles on one XCD (workgroups go round the eight of them), its matrix rows'
+    // tiles over all rows of x in turn
+    const unsigned tiles = a.tiles_n * a.tiles_m, xcd = blockIdx.x % 8;
+    const unsigned tile = xcd * (tiles / 8) + min(xcd, tiles % 8) + blockIdx.x / 8;
+    const unsigned tile_m = tile % a.tiles_m, tile_n = tile / a.tiles_m;
+    const unsigned G = tile_n * 4 + rg;  // the wavefront's pair of tiles
+
+    // this wavefront group's part of K, in chunks
+    constexpr bool kTwoParts = SPLIT && OPS != kTransposed;
+    const auto part_of = [&](unsigned set) {
+        return kTwoParts ? blockIdx.y * 2 + set : blockIdx.y;
+    };
+    const unsigned begin = min(a.chunks, part_of(kg) * a.part);
+    const unsigned end = min(a.chunks, begin + a.part);
+
+    // x: rows past the last are the last one again (such rows' results are not stored);
+    // segments past the part's end, or the row's, read as zeros
+    constexpr unsigned kRows = SPLIT ? TT * 32 : TT * 64;
+    const unsigned first_row = tile_m * kRows;
+    const unsigned rows = min(kRows, a.out.m - first_row);
+    const auto xs = buffer(a.x + size_t(first_row) * a.x_stride,
+                           (rows - 1) * a.x_stride + a.x_second * (OPS == kTransposed) +
+                               a.segments * 16);
+    int x_at[TT];            // this lane's offset in chunk 0 of its part
+    unsigned x_limit[TT];    // chunks * 8 it may read, counted from its segment
+#pragma unroll
+    for (int j = 0; j < TT; ++j) {
+        const unsigned u = j * 8 + wave;  // this instruction's eight rows
+        const unsigned set = SPLIT ? u / (4 * TT) : 0;
+        const unsigned row = min((SPLIT ? u % (4 * TT) : u) * 8 + lane / 8, rows - 1);
+        const unsigned seg = (lane % 8) ^ (lane / 8);
+        const unsigned b = min(a.chunks, part_of(set) * a.part);
+        const unsigned e = min(a.segments, min(a.chunks, b + a.part) * 8);
+        const unsigned from = b * 8 + seg;
+        x_at[j] = int(row * a.x_stride + from * 16 +
+                      (OPS == kTransposed && set ? a.x_second : 0));
+        x_limit[j] = e > from ? e - from : 0;
+    }
+    auto stage = [&](unsigned chunk, uint8_t* to) {  // chunk of the part
+#pragma unroll
+        for (int j = 0; j < TT; ++j) {
+            const int at = chunk * 8 < x_limit[j] ? x_at[j] + int(chunk * 128) : kOutside;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                xs, (__attribute__((address_space(3))) void*)(to + (j * 8 + wave) * 1024), 16, at,
+                0, 0, 0);
+        }
+        issue_order();
+    };
+
+    // weights: buffers that end with the part, so that steps past it are zero codes
+    constexpr unsigned kStepsPerChunk = OPS == kFp4 ? 4 : 1;
+    constexpr unsigned kStepBytes = OPS == kTransposed ? 2048 : 1024;
+    const unsigned end_step = min(a.steps, end * kStepsPerChunk);
+    const unsigned begin_step = begin * kStepsPerChunk;
+    const unsigned scale_groups = (a.steps + 3) / 4;
+    __amdgpu_buffer_rsrc_t codes_buf[2], scales_buf[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const bool second = OPS == kTransposed ? kg != 0 : t != 0;
+        const uint8_t* w = second ? a.w1 : a.w0;
+        const unsigned group = OPS == kTransposed || OUT == kOutGated ? G : 2 * G + t;
+        const bool there = group < a.groups;
+        const size_t g = there ? group : 0;
+        codes_buf[t] = buffer(w + g * a.steps * kStepBytes, there ? end_step * kStepBytes : 0);
+        const uint8_t* s = w + size_t(a.groups) * a.steps * kStepBytes;
+        if constexpr (OPS == kTransposed)
+            scales_buf[t] = buffer(s + g * a.steps * 128, there ? end_step * 128 : 0);
+        else
+            scales_buf[t] = buffer(s + g * scale_groups * 256, there ? scale_groups * 256 : 0);
+    }
+    constexpr int kAhead = 4;
+    struct Codes {
+        u4 w[2];
+        u4 s[OPS == kTransposed ? 2 : 1];
+    };
+    auto load_codes = [&](unsigned step, Codes& c) {
+        if constexpr (OPS == kTransposed) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+                c.w[t] = load_b128(codes_buf[0], int(step * 2048 + t * 1024 + lane * 16));
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+                c.s[t] = load_b128(scales_buf[0],
+                                   int(step * 128 + (2 * h + (lane % 32) / 16) * 32 + 16 * t));
+        } else {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+                c.w[t] = load_b128(codes_buf[t], int(step * 1024 + lane * 16));
+        }
+        issue_order();
+    };
+    struct Scales {
+        unsigned w[2], x[OPS == kFp4 ? TT : 1];
+    };
+    // kFp4: this lane's rows of x scales
+    const uint8_t* xscale_row[OPS == kFp4 ? TT : 1];
+    const unsigned x_blocks = a.segments;  // (a segment is 32 MXFP4 values)
+    if constexpr (OPS == kFp4) {
+#pragma unroll
+        for (int t = 0; t < TT; ++t) {
+            const unsigned row =
+                min((SPLIT ? 0 : kg * TT * 32) + t * 32 + lane % 32, rows - 1);
+            xscale_row[t] = a.x_scales + size_t(first_row + row) * x_blocks;
+        }
+    }
+    // Scales of the four steps from `step` (a multiple of 4).
+    auto load_scales = [&](unsigned step, Scales& s) {
+        if constexpr (OPS != kTransposed) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+                s.w[t] = __builtin_amdgcn_raw_buffer_load_b32(
+                    scales_buf[t], int(step * 64 + lane * 4), 0, 0);
+        }
+        if constexpr (OPS == kFp4) {
+            const unsigned block = step * 2;
+            if (block + 8 <= x_blocks) {
+#pragma unroll
+                for (int t = 0; t < TT; ++t) {
+                    typedef unsigned two __attribute__((ext_vector_type(2), aligned(1)));
+                    const two v = *reinterpret_cast<const two*>(xscale_row[t] + block);
+                    s.x[t] = __builtin_amdgcn_perm(v.y, v.x, h ? 0x07050301u : 0x06040200u);
+                }
+            } else {  // the last, short chunk of a row, or none: byte by byte
+#pragma unroll
+                for (int t = 0; t < TT; ++t) {
+                    unsigned word = 0;
+#pragma unroll
+                    for (unsigned j = 0; j < 4; ++j) {
+                        const unsigned b = block + 2 * j + h;
+                        const unsigned v = xscale_row[t][min(b, x_blocks - 1)];
+                        word |= (b < x_blocks ? v : 0u) << (8 * j);
+                    }
+                    s.x[t] = word;
+                }
+            }
+        }
+        issue_order();
+    };
+
+    f32x16 acc[2][TT];
+#pragma unroll
+    for (int t = 0; t < TT; ++t)
+        acc[0][t] = acc[1][t] = f32x16{};
+
+    // A wavefront's loads return in order.  Chunk c's copies were issued three chunks ago; at
+    // least the copies of the two chunks after it, the weights of three chunks and the
+    // scales of those were issued behind them, so a wait for all but that many is a wait for
+    // the chunk, and the barrier makes it everyone's.
+    constexpr int kCodeLoads = (OPS == kTransposed ? 4 : 2) * int(kStepsPerChunk);
+    auto arrive = [&]<int BEHIND>() {
+        static_assert(BEHIND < 64, "vmcnt holds six bits");
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(BEHIND) : "memory");
+        __builtin_amdgcn_s_barrier();
+        issue_order();
+    };
+    const uint8_t* x_lane = lds + kg * (TT * 4096) + (lane % 32) * 128;
+    auto x_operand = [&](const uint8_t* buf, int t, unsigned seg) {
+        return *reinterpret_cast<const u4*>(buf + t * 4096 + ((seg ^ (lane % 8)) * 16));
+    };
+
+    Codes codes[kAhead];
+    Scales scales, next;
+    issue_order();
+    stage(0, lds);
+    stage(1, lds + kStageBytes);
+    stage(2, lds + 2 * kStageBytes);
+    load_scales(begin_step, scales);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+        load_codes(begin_step + i, codes[i]);
+
+    if constexpr (OPS == kFp4) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // fewer loads than the loop counts on
+        unsigned slot = 0;
+        for (unsigned c = 0; c < a.part; ++c) {
+            // (the scales' loads: at least as many as on the whole-chunk path)
+            arrive.template operator()<2 * TT + 3 * kCodeLoads>();
+            const uint8_t* buf = x_lane + slot * kStageBytes;
+            stage(c + 3, lds + ((slot + 3) % kStages) * kStageBytes);
+            load_scales(begin_step + 4 * (c + 1), next);
+            static_for<4>([&]<int S>() {
+#pragma unroll
+                for (int t = 0; t < TT; ++t) {
+                    const i32x8 xv = fp4_operand(x_operand(buf, t, 2 * S + h));
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        acc[i][t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+                            fp4_operand(codes[S].w[i]), xv, acc[i][t], 4, 4, S,
+                            int(scales.w[i]), S, int(scales.x[t]));
+                }
+                issue_order();
+                load_codes(begin_step + 4 * (c + 1) + S, codes[S]);
+            });
+            scales = next;
+            slot = (slot + 1) % kStages;
+        }
+    } else {
+        for (unsigned c0 = 0; c0 < a.part; c0 += 4) {
+            static_for<4>([&]<int C>() {
+                constexpr int kScaleLoads = OPS == kTransposed || C == 0 ? 0 : 2;
+                arrive.template operator()<2 * TT + 3 * kCodeLoads + kScaleLoads>();
+                const uint8_t* buf = x_lane + C * kStageBytes;
+                stage(c0 + C + 3, lds + ((C + 3) % kStages) * kStageBytes);
+                if constexpr (C == 0)
+                    load_scales(begin_step + c0 + 4, next);
+                static_for<4>([&]<int S>() {
+                    bf16x8 wv[2];
+                    if constexpr (OPS == kTransposed) {
+                        const unsigned cw[2] = {codes[C].w[S / 2][2 * (S % 2)],
+                                                codes[C].w[S / 2][2 * (S % 2) + 1]};
+                        const unsigned sw[2] = {codes[C].s[S / 2][2 * (S % 2)],
+                                                codes[C].s[S / 2][2 * (S % 2) + 1]};
+                        decode8_pair(cw, sw, wv[0], wv[1]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            wv[i] = decode8(codes[C].w[i][S], scale_of(scales.w[i], C));
+                    }
+#pragma unroll
+                    for (int t = 0; t < TT; ++t) {
+                        const bf16x8 xv = __builtin_bit_cast(bf16x8, x_operand(buf, t, 4 * h + S));
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            acc[i][t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wv[i], xv,
+                                                                               acc[i][t], 0, 0, 0);
+                    }
+                });
+                issue_order();
+                load_codes(begin_step + c0 + C + kAhead, codes[C]);
+            });
+            scales = next;
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // no copy outlives the loop
+    __syncthreads();
+
+    // SPLIT: each group hands the other one half of its tiles and finishes the other half
+    // (TT == 1: the first group finishes both)
+    constexpr int kOwn = SPLIT ? (TT + 1) / 2 : TT;
+    const unsigned own = SPLIT ? (TT > 1 ? kg * kOwn : 0) : 0;
+    if constexpr (SPLIT) {
+        constexpr int kGiven = TT > 1 ? 2 : 1;  // groups that hand tiles over
+        auto* meet = reinterpret_cast<f32x4*>(lds) + rg * (kGiven * kOwn * 512) + lane;
+        if (TT > 1 || kg == 1) {
+#pragma unroll
+            for (int t = 0; t < kOwn; ++t)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        f32x4 v;
+                        if (TT > 1)
+                            v = kg ? quad_of(acc[i][t], j) : quad_of(acc[i][(t + kOwn) % TT], j);
+                        else
+                            v = quad_of(acc[i][0], j);
+                        meet[(TT > 1 ? kg : 0) * (kOwn * 512) + ((t * 2 + i) * 4 + j) * 64] = v;
+                    }
+        }
+        __syncthreads();
+        if (TT == 1 && kg == 1)
+            return;
+#pragma unroll
+        for (int t = 0; t < kOwn; ++t)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const f32x4 v =
+                        meet[(TT > 1 ? 1 - kg : 0) * (kOwn * 512) + ((t * 2 + i) * 4 + j) * 64];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if (TT > 1) {
+                            // (kept in place t: the group's own tiles move down)
+                            const float mine = kg ? acc[i][(t + kOwn) % TT][4 * j + e]
+                                                  : acc[i][t][4 * j + e];
+                            acc[i][t][4 * j + e] = kg ? v[e] + mine : mine + v[e];
+                        } else {
+                            acc[i][0][4 * j + e] += v[e];
+                        }
+                    }
+                }
+    }
+    const unsigned first_tile =
+        (first_row / 32) + (SPLIT ? own : kg * TT);  // of 32 rows of x, the wavefront's first
+#pragma unroll
+    for (int t = 0; t < kOwn; ++t) {
+        const unsigned T = first_tile + t;
+        if (a.partial) {
+            const unsigned row_tiles = (a.out.m + 31) / 32;
+            if (T < row_tiles) {
+                auto* to = reinterpret_cast<f32x4*>(
+                               a.partial + ((size_t(blockIdx.y) * (a.tiles_n * 4) + G) * row_tiles +
+                                            T) * kTileFloats) +
+                           lane;
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        to[(i * 4 + j) * 64] = quad_of(acc[i][t], j);
+            }
+        } else {
+            store_tiles<OUT>(a.out, G, T * 32 + lane % 32, h, acc[0][t], acc[1][t]);
+        }
+    }
+}
+
+// The K slices' partial results of one pair of tiles, summed in slice order: a wavefront
+// takes one quad of rows (four of them all of a pair's; kept pre-activations in 8 bits
+// need a row's 32 values together, so there one wavefront takes all).
+template <int OUT, bool WHOLE>
+__global__ __launch_bounds__(256) void reduce_kernel(const float* __restrict__ partial,
+                                                     unsigned slices, size_t pairs,
+                                                     unsigned row_tiles, Target out) {
+    const unsigned lane = threadIdx.x % 64;
+    const size_t w = size_t(blockIdx.x) * 4 + threadIdx.x / 64;
+    const size_t pair = WHOLE ? w : w / 4;
+    if (pair >= pairs)
+        return;
+    const unsigned G = unsigned(pair / row_tiles), T = unsigned(pair % row_tiles);
+    const auto* from = reinterpret_cast<const f32x4*>(partial + pair * kTileFloats) + lane;
+    const size_t step = pairs * (kTileFloats / 4);
+    constexpr int kQuads = WHOLE ? 4 : 1;
+    const unsigned j0 = WHOLE ? 0 : unsigned(w % 4);
+    f32x4 v[2][kQuads];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < kQuads; ++j)
+            v[i][j] = from[(i * 4 + j0 + j) * 64];
+    for (unsigned s = 1; s < slices; ++s)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < kQuads; ++j)
+                v[i][j] += from[s * step + (i * 4 + j0 + j) * 64];
+    const unsigned token = T * 32 + lane % 32, h = lane / 32;
+#pragma unroll
+    for (int j = 0; j < kQuads; ++j)
+        store_quad<OUT>(out, G, token, h, j0 + j, v[0][j], v[1][j]);
+    if constexpr (WHOLE) {
+        if (32 * G < out.n) {
+            keep_q8(out, 32 * G, token, h, v[0]);
+            keep_q8(out, out.n + 32 * G, token, h, v[1]);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ dg and du
+//
+// s = sigmoid(g): dg = dh * u * s * (1 + g * (1 - s)), du = dh * g * s.  One lane takes
+// eight columns; the traffic is dh, the kept g and u, and the two results, each once.
+// g and u come as bf16 [m][2n] or as 8-bit codes with a scale per 32.
+
+template <bool Q8>
+__global__ __launch_bounds__(256) void gate_grad_kernel(const uint16_t* __restrict__ dh,
+                                                        size_t dh_stride, unsigned m, unsigned n,
+                                                        const uint16_t* __restrict__ kept,
+                                                        const int8_t* __restrict__ kept_q,
+                                                        const float* __restrict__ kept_d,
+                                                        uint16_t* __restrict__ dgu) {
+    const unsigned eighths = n / 8;
+    const size_t u = size_t(blockIdx.x) * 256 + threadIdx.x;
+    if (u >= size_t(m) * eighths)
+        return;
+    const unsigned row = unsigned(u / eighths), c = unsigned(u % eighths) * 8;
+    const u32x4 dv = load16(reinterpret_cast<const uint8_t*>(dh + size_t(row) * dh_stride + c));
+    float g[8], up[8];
+    const size_t at = size_t(row) * 2 * n + c;
+    if constexpr (Q8) {
+        const float dg = kept_d[at / 32], du = kept_d[(at + n) / 32];
+        const uint2 gq = *reinterpret_cast<const uint2*>(kept_q + at);
+        const uint2 uq = *reinterpret_cast<const uint2*>(kept_q + at + n);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            g[i] = float(int8_t((i < 4 ? gq.x : gq.y) >> (8 * (i % 4)))) * dg;
+            up[i] = float(int8_t((i < 4 ? uq.x : uq.y) >> (8 * (i % 4)))) * du;
+        }
+    } else {
+        const u32x4 gv = load16(reinterpret_cast<const uint8_t*>(kept + at));
+        const u32x4 uv = load16(reinterpret_cast<const uint8_t*>(kept + at + n));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            g[2 * i] = __uint_as_float(gv[i] << 16);
+            g[2 * i + 1] = __uint_as_float(gv[i] & 0xffff0000u);
+            up[2 * i] = __uint_as_float(uv[i] << 16);
+            up[2 * i + 1] = __uint_as_float(uv[i] & 0xffff0000u);
+        }
+    }
+    float rg[8], ru[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float d = __uint_as_float(i % 2 ? dv[i / 2] & 0xffff0000u : dv[i / 2] << 16);
+        const float s =
+            __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * g[i]));
+        rg[i] = d * up[i] * (s * (1.0f + g[i] * (1.0f - s)));
+        ru[i] = d * (g[i] * s);
+    }
+    *reinterpret_cast<u32x4*>(dgu + at) = u32x4{bf16_pair(rg[0], rg[1]), bf16_pair(rg[2], rg[3]),
+                                                bf16_pair(rg[4], rg[5]), bf16_pair(rg[6], rg[7])};
+    *reinterpret_cast<u32x4*>(dgu + at + n) =
+        u32x4{bf16_pair(ru[0], ru[1]), bf16_pair(ru[2], ru[3]), bf16_pair(ru[4], ru[5]),
+              bf16_pair(ru[6], ru[7])};
+}
+
+// ------------------------------------------------------------------ launch plans
+
+constexpr size_t kMaxRows = size_t(1) << 20, kMaxK = size_t(1) << 20, kMaxN = size_t(1) << 24;
+
+// How a product runs: `decode` (decode_kernel), or gemm_kernel with TT tiles of 32 rows of
+// x, the groups splitting K or not, in `slices` of `part` chunks.
+struct Plan {
+    bool decode, split;
+    int tt;
+    unsigned tiles_n, tiles_m, slices, chunks, part;
+};
+
+constexpr size_t kDecodeRows = 32;
+
+Plan plan_gemm(size_t m, size_t wave_groups, size_t chunks, int ops) {
+    Plan p{};
+    p.tt = m <= 32 ? 1 : m <= 64 ? 2 : 4;
+    p.tiles_n = unsigned(ceil_div(wave_groups, 4));
+    p.split = true;
+    p.chunks = unsigned(chunks);
+    if (ops == kFp4 && m > 128) {
+        const size_t whole = size_t(p.tiles_n) * ceil_div(m, 256);
+        p.split = whole < compute_units();
+    }
+    p.tiles_m = unsigned(ceil_div(m, size_t(p.tt) * (p.split ? 32 : 64)));
+    const unsigned sets = p.split && ops != kTransposed ? 2 : 1;
+    const size_t tiles = size_t(p.tiles_n) * p.tiles_m;
+    // slices until the tiles fill the compute units, each group at least four chunks
+    const unsigned unit = ops == kFp4 ? 1 : 4;
+    const size_t most = std::max<size_t>(1, ceil_div(chunks, size_t(sets) * unit));
+    size_t slices = std::max<size_t>(1, std::min<size_t>(compute_units() / tiles, most));
+    p.part = unsigned(ceil_div(ceil_div(chunks, slices * sets), unit) * unit);
+    p.slices = unsigned(ceil_div(chunks, size_t(p.part) * sets));
+    return p;
+}
+
+size_t partial_bytes(const Plan& p, size_t m) {
+    return p.decode || p.slices == 1
+               ? 0
+               : size_t(p.slices) * p.tiles_n * 4 * ceil_div(m, 32) * kTileFloats * 4;
+}
+
+template <int TT, bool SPLIT, int OPS, int OUT>
+int launch_gemm(const Gemm& a, const Plan& p, hipStream_t st) {
+    const auto f = gemm_kernel<TT, SPLIT, OPS, OUT>;
+    constexpr int kLds = kStages * TT * 8192;
+    if constexpr (kLds > 64 * 1024) {
+        static std::atomic<uint64_t> configured{0};  // devices whose attribute is set
+        int device = 0;
+        KDQ_HIP(hipGetDevice(&device));
+        const uint64_t bit = uint64_t(1) << (device % 64);
+        if (device >= 64 || !(configured.load(std::memory_order_relaxed) & bit)) {
+            KDQ_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(f),
+                                        hipFuncAttributeMaxDynamicSharedMemorySize, kLds));
+            configured.fetch_or(bit, std::memory_order_relaxed);
+        }
+    }
+    hipLaunchKernelGGL(f, dim3(p.tiles_n * p.tiles_m, p.slices), dim3(512), kLds, st, a);
+    KDQ_HIP(hipGetLastError());
+    return KDQ_OK;
+}
+
+template <int OPS, int OUT> int run_gemm(Gemm a, const Plan& p, void* workspace, hipStream_t st) {
+    a.chunks = p.chunks;
+    a.part = p.part;
+    a.tiles_n = p.tiles_n;
+    a.tiles_m = p.tiles_m;
+    a.partial = p.slices > 1 ? static_cast<float*>(workspace) : nullptr;
+    int rc;
+    if (!p.split) {
+        if constexpr (OPS == kFp4)
+            rc = launch_gemm<4, false, OPS, OUT>(a, p, st);
+        else
+            return KDQ_ERR_UNSUPPORTED;
+    } else {
+        rc = p.tt == 1   ? launch_gemm<1, true, OPS, OUT>(a, p, st)
+             : p.tt == 2 ? launch_gemm<2, true, OPS, OUT>(a, p, st)
+                         : launch_gemm<4, true, OPS, OUT>(a, p, st);
+    }
+    if (rc || p.slices == 1)
+        return rc;
+    const unsigned row_tiles = unsigned(ceil_div(a.out.m, 32));
+    const size_t pairs = size_t(p.tiles_n) * 4 * row_tiles;
+    bool whole = false;
+    if constexpr (OUT == kOutGated)
+        whole = a.out.kept_q != nullptr;
+    if (whole) {
+        if constexpr (OUT == kOutGated)
+            hipLaunchKernelGGL((reduce_kernel<OUT, true>), dim3(unsigned(ceil_div(pairs, 4))),
+                               dim3(256), 0, st, a.partial, p.slices, pairs, row_tiles, a.out);
+    } else {
+        hipLaunchKernelGGL((reduce_kernel<OUT, false>), dim3(unsigned(pairs)), dim3(256), 0, st,
+                           a.partial, p.slices, pairs, row_tiles, a.out);
+    }
+    KDQ_HIP(hipGetLastError());
+    return KDQ_OK;
+}
+
+template <int TB, bool GATED, bool FP4, int OUT>
+int launch_decode(const Decode& a, hipStream_t st) {
+    const unsigned units = (a.k + 127) / 128;
+    const unsigned per = GATED ? 2 : 1;
+    const unsigned waves = per * (units <= 8 ? 2 : units <= 16 ? 4 : units <= 64 || GATED ? 8 : 16);
+    hipLaunchKernelGGL((decode_kernel<TB, GATED, FP4, OUT>), dim3(unsigned(ceil_div(a.out.n, 16))),
+                       dim3(waves * 64), waves * TB * 1024, st, a);
+    KDQ_HIP(hipGetLastError());
+    return KDQ_OK;
+}
+
+template <bool GATED, bool FP4, int OUT> int run_decode(const Decode& a, hipStream_t st) {
+    return a.out.m <= 16 ? launch_decode<1, GATED, FP4, OUT>(a, st)
+                         : launch_decode<2, GATED, FP4, OUT>(a, st);
+}
+
+Plan plan_product(size_t m, size_t n, size_t k, bool fp4) {
+    if (m <= kDecodeRows) {
+        Plan p{};
+        p.decode = true;
+        return p;
+    }
+    return plan_gemm(m, ceil_div(n, 64), ceil_div(k, fp4 ? 256 : 64), fp4 ? kFp4 : kBf16);
+}
+
+Plan plan_gated(size_t m, size_t n, size_t k, bool kept) {
+    if (m <= kDecodeRows && !kept) {
+        Plan p{};
+        p.decode = true;
+        return p;
+    }
+    return plan_gemm(m, ceil_div(n, 32), ceil_div(k, 64), kBf16);
+}
+
+Plan plan_backward(size_t m, size_t n, size_t k) {
+    return plan_gemm(m, ceil_div(k, 64), ceil_div(n, 64), kTransposed);
+}
+
+bool sizes_ok(size_t m, size_t n, size_t k) {
+    return m <= kMaxRows && n <= kMaxN && k <= kMaxK && k % 32 == 0;
+}
+
+// Bytes of `rows` rows `stride` values apart, `cols` values of `size` bytes each.
+size_t extent(size_t rows, size_t stride, size_t cols, size_t size) {
+    return ((rows - 1) * stride + cols) * size;
+}
+
+constexpr size_t kMaxStride = size_t(1) << 21;  // 256 rows stay within a buffer's range
+
+int check_workspace(size_t need, const void* workspace, size_t bytes) {
+    if (!need)
+        return KDQ_OK;
+    if (!workspace || bytes < need)
+        return KDQ_ERR_SCRATCH;
+    return misaligned(workspace, 16) ? KDQ_ERR_ALIGNMENT : KDQ_OK;
+}
+
+int check_form(const Form& f, const void* blocks, const void* scales, const void* packed,
+               size_t rows, size_t cols) {
+    if (misaligned(blocks, 16) || misaligned(packed, 16))
+        return KDQ_ERR_ALIGNMENT;
+    const size_t bytes = f.code_bytes + f.scale_bytes;
+    if (overlaps(packed, bytes, blocks, rows * (cols / 2)) ||
+        overlaps(packed, bytes, scales, rows * (cols / 32)))
+        return KDQ_ERR_ALIAS;
+    return KDQ_OK;
+}
+
+template <class K>
+int launch_pack(K kernel, const Form& f, const uint8_t* blocks, const uint8_t* scales,
+                size_t rows, size_t cols, uint8_t* packed, void* stream) {
+    const size_t units = f.code_bytes / 16 + f.scale_bytes / 4;
+    hipLaunchKernelGGL(kernel, dim3(unsigned(ceil_div(units, 256))), dim3(256), 0,
+                       static_cast<hipStream_t>(stream), blocks, scales, rows, cols, f, packed);
+    KDQ_HIP(hipGetLastError());
+    return KDQ_OK;
+}
+}  // namespace
+}  // namespace kdq
+
+using namespace kdq;
+
+extern "C" size_t kdq_mxfp4_packed_bytes(size_t rows, size_t cols) {
+    if (!rows || !cols || cols % 32 || rows > kMaxN || cols > kMaxK)
+        return 0;
+    const Form f = packed_form(rows, cols);
+    return f.code_bytes + f.scale_bytes;
+}
+
+extern "C" int kdq_mxfp4_pack(const uint8_t* blocks, const uint8_t* scales, size_t rows,
+                              size_t cols, uint8_t* packed, void* stream) {
+    if (!blocks || !scales || !packed || !rows || !cols)
+        return KDQ_ERR_ARGUMENT;
+    if (!kdq_mxfp4_packed_bytes(rows, cols))
+        return KDQ_ERR_SHAPE;
+    const Form f = packed_form(rows, cols);
+    if (const int rc = check_form(f, blocks, scales, packed, rows, cols))
+        return rc;
+    return launch_pack(pack_kernel, f, blocks, scales, rows, cols, packed, stream);
+}
+
+extern "C" size_t kdq_mxfp4_packed_transposed_bytes(size_t rows, size_t cols) {
+    if (!rows || !cols || cols % 32 || rows > kMaxK || cols > kMaxK)
+        return 0;
+    const Form f = transposed_form(rows, cols);
+    return f.code_bytes + f.scale_bytes;
+}
+
+extern "C" int kdq_mxfp4_pack_transposed(const uint8_t* blocks, const uint8_t* scales,
+                                         size_t rows, size_t cols, uint8_t* packed,
+                                         void* stream) {
+    if (!blocks || !scales || !packed || !rows || !cols)
+        return KDQ_ERR_ARGUMENT;
+    if (!kdq_mxfp4_packed_transposed_bytes(rows, cols))
+        return KDQ_ERR_SHAPE;
+    const Form f = transposed_form(rows, cols);
+    if (const int rc = check_form(f, blocks, scales, packed, rows, cols))
+        return rc;
+    return launch_pack(pack_t_kernel, f, blocks, scales, rows, cols, packed, stream);
+}
+
+extern "C" size_t kdq_mxfp4_product_workspace(size_t m, size_t n, size_t k, int quantized) {
+    if (!m || !n || !k || !sizes_ok(m, n, k))
+        return 0;
+    return partial_bytes(plan_product(m, n, k, quantized != 0), m);
+}
+
+extern "C" size_t kdq_mxfp4_gated_workspace(size_t m, size_t n, size_t k, int kept) {
+    if (!m || !n || !k || !sizes_ok(m, n, k) || n % 32)
+        return 0;
+    return partial_bytes(plan_gated(m, n, k, kept != 0), m);
+}
+
+extern "C" size_t kdq_mxfp4_gated_backward_workspace(size_t m, size_t n, size_t k) {
+    if (!m || !n || !k || !sizes_ok(m, n, k) || n % 32 || n > kMaxK / 2)
+        return 0;
+    return partial_bytes(plan_backward(m, n, k), m);
+}
+
+namespace kdq {
+namespace {
+int check_output(int type, const void* y, size_t y_stride, size_t m, size_t n) {
+    if (type != KDQ_F32 && type != KDQ_BF16)
+        return KDQ_ERR_UNSUPPORTED;
+    if (y_stride < n || y_stride > (SIZE_MAX >> 4) / m)
+        return KDQ_ERR_SHAPE;
+    return misaligned(y, type == KDQ_F32 ? 4 : 2) ? KDQ_ERR_ALIGNMENT : KDQ_OK;
+}
+
+template <int OPS> int product(Gemm g, const Plan& p, int type, void* workspace, hipStream_t st) {
+    if (p.decode) {
+        Decode d{g.w0, nullptr, g.x, g.x_scales, g.x_stride,
+                 unsigned(OPS == kFp4 ? g.segments * 32 : g.segments * 8), g.steps, g.groups,
+                 g.out};
+        constexpr bool kQ = OPS == kFp4;
+        return type == KDQ_F32 ? run_decode<false, kQ, kOutF32>(d, st)
+                               : run_decode<false, kQ, kOutBf16>(d, st);
+    }
+    return type == KDQ_F32 ? run_gemm<OPS, kOutF32>(g, p, workspace, st)
+                           : run_gemm<OPS, kOutBf16>(g, p, workspace, st);
+}
+}  // namespace
+}  // namespace kdq
+
+extern "C" int kdq_mxfp4_product(const uint16_t* x_bf16, size_t x_stride, size_t m,
+                                 const uint8_t* packed, size_t n, size_t k, int type, void* y,
+                                 size_t y_stride, void* workspace, size_t workspace_bytes,
+                                 void* stream) {
+    if (!x_bf16 || !packed || !y || !m || !n || !k)
+        return KDQ_ERR_ARGUMENT;
+    if (!sizes_ok(m, n, k) || x_stride < k || x_stride % 8 || x_stride > kMaxStride)
+        return KDQ_ERR_SHAPE;
+    if (const int rc = check_output(type, y, y_stride, m, n))
+        return rc;
+    if (misaligned(x_bf16, 16) || misaligned(packed, 16))
+        return KDQ_ERR_ALIGNMENT;
+    const size_t y_bytes = extent(m, y_stride, n, type == KDQ_F32 ? 4 : 2);
+    if (overlaps(y, y_bytes, x_bf16, extent(m, x_stride, k, 2)) ||
+        overlaps(y, y_bytes, packed, kdq_mxfp4_packed_bytes(n, k)) ||
+        overlaps(y, y_bytes, workspace, workspace_bytes))
+        return KDQ_ERR_ALIAS;
+    const Plan p = plan_product(m, n, k, false);
+    if (const int rc = check_workspace(partial_bytes(p, m), workspace, workspace_bytes))
+        return rc;
+    const Form f = packed_form(n, k);
+    Gemm g{};
+    g.w0 = g.w1 = packed;
+    g.x = reinterpret_cast<const uint8_t*>(x_bf16);
+    g.x_stride = unsigned(x_stride * 2);
+    g.segments = unsigned(k / 8);
+    g.groups = unsigned(f.groups);
+    g.steps = unsigned(f.steps);
+    g.out = {y, y_stride, unsigned(m), unsigned(n), nullptr, nullptr, nullptr};
+    return product<kBf16>(g, p, type, workspace, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int kdq_mxfp4_product_quantized(const uint8_t* x_blocks, const uint8_t* x_scales,
+                                           size_t m, const uint8_t* packed, size_t n, size_t k,
+                                           int type, void* y, size_t y_stride, void* workspace,
+                                           size_t workspace_bytes, void* stream) {
+    if (!x_blocks || !x_scales || !packed || !y || !m || !n || !k)
+        return KDQ_ERR_ARGUMENT;
+    if (!sizes_ok(m, n, k))
+        return KDQ_ERR_SHAPE;
+    if (const int rc = check_output(type, y, y_stride, m, n))
+        return rc;
+    if (misaligned(x_blocks, 16) || misaligned(packed, 16))
+        return KDQ_ERR_ALIGNMENT;
+    const size_t y_bytes = extent(m, y_stride, n, type == KDQ_F32 ? 4 : 2);
+    if (overlaps(y, y_bytes, x_blocks, m * (k / 2)) ||
+        overlaps(y, y_bytes, x_scales, m * (k / 32)) ||
+        overlaps(y, y_bytes, packed, kdq_mxfp4_packed_bytes(n, k)) ||
+        overlaps(y, y_bytes, workspace, workspace_bytes))
+        return KDQ_ERR_ALIAS;
+    const Plan p = plan_product(m, n, k, true);
+    if (const int rc = check_workspace(partial_bytes(p, m), workspace, workspace_bytes))
+        return rc;
+    const Form f = packed_form(n, k);
+    Gemm g{};
+    g.w0 = g.w1 = packed;
+    g.x = x_blocks;
+    g.x_scales = x_scales;
+    g.x_stride = unsigned(k / 2);
+    g.segments = unsigned(k / 32);
+    g.groups = unsigned(f.groups);
+    g.steps = unsigned(f.steps);
+    g.out = {y, y_stride, unsigned(m), unsigned(n), nullptr, nullptr, nullptr};
+    return product<kFp4>(g, p, type, workspace, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int kdq_mxfp4_gated(const uint16_t* x_bf16, size_t x_stride, size_t m,
+                               const uint8_t* gate_packed, const uint8_t* up_packed, size_t n,
+                               size_t k, uint16_t* h_bf16, size_t h_stride,
+                               uint16_t* kept_bf16, int8_t* kept_q8, float* kept_scales,
+                               void* workspace, size_t workspace_bytes, void* stream) {
+    if (!x_bf16 || !gate_packed || !up_packed || !h_bf16 || !m || !n || !k ||
+        (kept_bf16 && kept_q8) || !kept_q8 != !kept_scales)
+        return KDQ_ERR_ARGUMENT;
+    if (!sizes_ok(m, n, k) || n % 32 || x_stride < k || x_stride % 8 || x_stride > kMaxStride)
+        return KDQ_ERR_SHAPE;
+    if (const int rc = check_output(KDQ_BF16, h_bf16, h_stride, m, n))
+        return rc;
+    if (misaligned(x_bf16, 16) || misaligned(gate_packed, 16) || misaligned(up_packed, 16) ||
+        misaligned(kept_bf16, 16) || misaligned(kept_q8, 16) || misaligned(kept_scales, 4))
+        return KDQ_ERR_ALIGNMENT;
+    const struct {
+        const void* p;
+        size_t bytes;
+    } out[] = {{h_bf16, extent(m, h_stride, n, 2)},
+               {kept_bf16, 4 * m * n},
+               {kept_q8, 2 * m * n},
+               {kept_scales, m * n / 4},
+               {workspace, workspace_bytes}},
+      in[] = {{x_bf16, extent(m, x_stride, k, 2)},
+              {gate_packed, kdq_mxfp4_packed_bytes(n, k)},
+              {up_packed, kdq_mxfp4_packed_bytes(n, k)}};
+    for (size_t i = 0; i < 5; ++i) {
+        for (const auto& b : in)
+            if (overlaps(out[i].p, out[i].bytes, b.p, b.bytes))
+                return KDQ_ERR_ALIAS;
+        for (size_t j = 0; j < i; ++j)
+            if (overlaps(out[i].p, out[i].bytes, out[j].p, out[j].bytes))
+                return KDQ_ERR_ALIAS;
+    }
+    const Plan p = plan_gated(m, n, k, kept_bf16 || kept_q8);
+    if (const int rc = check_workspace(partial_bytes(p, m), workspace, workspace_bytes))
+        return rc;
+    const Form f = packed_form(n, k);
+    const auto st = static_cast<hipStream_t>(stream);
+    const Target t{h_bf16, h_stride, unsigned(m), unsigned(n), kept_bf16, kept_q8, kept_scales};
+    if (p.decode)
+        return run_decode<true, false, kOutBf16>(
+            {gate_packed, up_packed, reinterpret_cast<const uint8_t*>(x_bf16), nullptr,
+             unsigned(x_stride * 2), unsigned(k), unsigned(f.steps), unsigned(f.groups), t},
+            st);
+    Gemm g{};
+    g.w0 = gate_packed;
+    g.w1 = up_packed;
+    g.x = reinterpret_cast<const uint8_t*>(x_bf16);
+    g.x_stride = unsigned(x_stride * 2);
+    g.segments = unsigned(k / 8);
+    g.groups = unsigned(f.groups);
+    g.steps = unsigned(f.steps);
+    g.out = t;
+    return run_gemm<kBf16, kOutGated>(g, p, workspace, st);
+}
+
+extern "C" int kdq_mxfp4_gated_backward(const uint16_t* dh_bf16, size_t dh_stride, size_t m,
+                                        const uint16_t* kept_bf16, const int8_t* kept_q8,
+                                        const float* kept_scales, const uint8_t* gate_transposed,
+                                        const uint8_t* up_transposed, size_t n, size_t k,
+                                        uint16_t* dgu_bf16, uint16_t* dx_bf16, size_t dx_stride,
+                                        void* workspace, size_t workspace_bytes, void* stream) {
+    if (!dh_bf16 || !gate_transposed || !up_transposed || !dgu_bf16 || !dx_bf16 || !m || !n ||
+        !k || !kept_bf16 == !kept_q8 || !kept_q8 != !kept_scales)
+        return KDQ_ERR_ARGUMENT;
+    if (!sizes_ok(m, n, k) || n % 32 || n > kMaxK / 2 || dh_stride < n || dh_stride % 8 ||
+        dh_stride > kMaxStride)
+        return KDQ_ERR_SHAPE;
+    if (const int rc = check_output(KDQ_BF16, dx_bf16, dx_stride, m, k))
+        return rc;
+    if (misaligned(dh_bf16, 16) || misaligned(gate_transposed, 16) ||
+        misaligned(up_transposed, 16) || misaligned(kept_bf16, 16) || misaligned(kept_q8, 16) ||
+        misaligned(kept_scales, 4) || misaligned(dgu_bf16, 16))
+        return KDQ_ERR_ALIGNMENT;
+    const size_t w_bytes = kdq_mxfp4_packed_transposed_bytes(n, k);
+    const struct {
+        const void* p;
+        size_t bytes;
+    } out[] = {{dgu_bf16, 4 * m * n},
+               {dx_bf16, extent(m, dx_stride, k, 2)},
+               {workspace, workspace_bytes}},
+      in[] = {{dh_bf16, extent(m, dh_stride, n, 2)}, {kept_bf16, 4 * m * n},
+              {kept_q8, 2 * m * n},                  {kept_scales, m * n / 4},
+              {gate_transposed, w_bytes},            {up_transposed, w_bytes}};
+    for (size_t i = 0; i < 3; ++i) {
+        for (const auto& b : in)
+            if (overlaps(out[i].p, out[i].bytes, b.p, b.bytes))
+                return KDQ_ERR_ALIAS;
+        for (size_t j = 0; j < i; ++j)
+            if (overlaps(out[i].p, out[i].bytes, out[j].p, out[j].bytes))
+                return KDQ_ERR_ALIAS;
+    }
+    const Plan p = plan_backward(m, n, k);
+    if (const int rc = check_workspace(partial_bytes(p, m), workspace, workspace_bytes))
+        return rc;
+    const auto st = static_cast<hipStream_t>(stream);
+    const dim3 grid(unsigned(ceil_div(m * (n / 8), 256)));
+    if (kept_q8)
+        hipLaunchKernelGGL(gate_grad_kernel<true>, grid, dim3(256), 0, st, dh_bf16, dh_stride,
+                           unsigned(m), unsigned(n), kept_bf16, kept_q8, kept_scales, dgu_bf16);
+    else
+        hipLaunchKernelGGL(gate_grad_kernel<false>, grid, dim3(256), 0, st, dh_bf16, dh_stride,
+                           unsigned(m), unsigned(n), kept_bf16, kept_q8, kept_scales, dgu_bf16);
+    KDQ_HIP(hipGetLastError());
+    const Form f = transposed_form(n, k);
+    Gemm g{};
+    g.w0 = gate_transposed;
+    g.w1 = up_transposed;
+    g.x = reinterpret_cast<const uint8_t*>(dgu_bf16);
+    g.x_stride = unsigned(n * 4);
+    g.x_second = unsigned(n * 2);
+    g.segments = unsigned(n / 8);
+    g.groups = unsigned(f.groups);
+    g.steps = unsigned(f.steps);
+    g.out = {dx_bf16, dx_stride, unsigned(m), unsigned(k), nullptr, nullptr, nullptr};
+    return run_gemm<kTransposed, kOutBackward>(g, p, workspace, st);
+}

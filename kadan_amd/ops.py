@@ -377,6 +377,216 @@ def moe_mxfp4_packed(x_bf16: torch.Tensor, logits: torch.Tensor, top_k: int, int
     return (out, *extra) if routing else out
 
 
+def _here(*tensors: torch.Tensor) -> None:
+    """Kernels run on the current device's current stream: its tensors only."""
+    device = torch.cuda.current_device()
+    for t in tensors:
+        if t.get_device() != device:
+            raise ValueError("every tensor must be on the current device")
+
+
+def _row_stride(t: torch.Tensor, dtype, name: str, multiple: int = 8) -> int:
+    """Values from row to row of a 2-d device tensor whose rows are contiguous."""
+    if t.dtype != dtype or t.dim() != 2 or not t.is_cuda:
+        raise ValueError(f"{name}: expected a 2-d {dtype} device tensor")
+    rows, cols = t.shape
+    row, col = t.stride()
+    if cols > 1 and col != 1:
+        raise ValueError(f"{name}: values of a row must lie side by side")
+    if rows == 1:
+        return cols
+    if row < cols or row % multiple:
+        raise ValueError(f"{name}: rows must not overlap and lie a multiple of {multiple} "
+                         "values apart")
+    return row
+
+
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}  # KDQ_F32, _F16, _BF16
+
+
+def _type(dtype) -> int:
+    try:
+        return _TYPES[dtype]
+    except KeyError:
+        raise ValueError(f"no MXFP4 operator takes {dtype}") from None
+
+
+def _blocks(blocks: torch.Tensor, scales: torch.Tensor) -> tuple[int, int]:
+    """Rows and values of a row of an MXFP4 matrix."""
+    _need(blocks, torch.uint8, "blocks")
+    _need(scales, torch.uint8, "scales")
+    if (blocks.dim() != 2 or scales.dim() != 2 or blocks.shape[0] != scales.shape[0]
+            or blocks.shape[1] != 16 * scales.shape[1]):
+        raise ValueError("expected blocks [rows, cols/2] and scales [rows, cols/32]")
+    return blocks.shape[0], 2 * blocks.shape[1]
+
+
+@functools.lru_cache(maxsize=4096, typed=True)
+def _mxfp4_size(function: str, *sizes: int) -> int:
+    return int(getattr(lib(), function)(*sizes))
+
+
+def _scratch(size: int, device) -> tuple[torch.Tensor | None, int | None]:
+    """A call's workspace: torch's allocator keeps it to the current stream (and to a
+    graph's own pool under capture), so calls share none.  Keep the tensor until the call
+    is enqueued."""
+    if not size:
+        return None, None
+    t = torch.empty(size, dtype=torch.uint8, device=device)
+    return t, t.data_ptr()
+
+
+def _matrix(packed: torch.Tensor, function: str, rows: int, cols: int, name: str) -> int:
+    if packed.dtype != torch.uint8 or not packed.is_cuda or not packed.is_contiguous():
+        raise ValueError(f"{name}: expected a packed uint8 device tensor")
+    if not rows or packed.numel() != _mxfp4_size(function, rows, cols):
+        raise ValueError(f"{name}: packed size does not match {rows} x {cols}")
+    return packed.data_ptr()
+
+
+def _output(out: torch.Tensor | None, rows: int, cols: int, dtype, device,
+            name: str) -> tuple[torch.Tensor, int]:
+    if out is None:
+        return torch.empty(rows, cols, dtype=dtype, device=device), cols
+    if out.dim() != 2 or out.shape[0] != rows or out.shape[1] != cols:
+        raise ValueError(f"{name}: expected [{rows}, {cols}]")
+    _here(out)
+    return out, _row_stride(out, dtype, name, 1)
+
+
+def mxfp4_quantize(x: torch.Tensor, status: torch.Tensor | None = None):
+    """fp32, fp16 or bf16 [rows, cols] (cols % 32 == 0) as MXFP4: blocks uint8
+    [rows, cols/2] and scales uint8 [rows, cols/32] (kdq_mxfp4_quantize)."""
+    kind = _type(x.dtype)
+    stride = _row_stride(x, x.dtype, "x")
+    _here(x)
+    rows, cols = x.shape
+    if cols % 32:
+        raise ValueError("x: a row must be whole blocks of 32 values")
+    blocks = torch.empty(rows, cols // 2, dtype=torch.uint8, device=x.device)
+    scales = torch.empty(rows, cols // 32, dtype=torch.uint8, device=x.device)
+    call("kdq_mxfp4_quantize", kind, x.data_ptr(), stride, rows, cols, blocks.data_ptr(),
+         scales.data_ptr(), _ptr(status), _stream())
+    return blocks, scales
+
+
+def mxfp4_pack(blocks: torch.Tensor, scales: torch.Tensor,
+               transposed: bool = False) -> torch.Tensor:
+    """An MXFP4 matrix in the form the products read (kdq_mxfp4_pack), or, ``transposed``,
+    in the one that mxfp4_gated_backward reads (kdq_mxfp4_pack_transposed)."""
+    rows, cols = _blocks(blocks, scales)
+    _here(blocks, scales)
+    name = "kdq_mxfp4_pack_transposed" if transposed else "kdq_mxfp4_pack"
+    size = _mxfp4_size("kdq_mxfp4_packed_transposed_bytes" if transposed
+                       else "kdq_mxfp4_packed_bytes", rows, cols)
+    if not size:
+        raise ValueError(f"a matrix of {rows} x {cols} has no packed form")
+    packed = torch.empty(size, dtype=torch.uint8, device=blocks.device)
+    call(name, blocks.data_ptr(), scales.data_ptr(), rows, cols, packed.data_ptr(), _stream())
+    return packed
+
+
+def mxfp4_product(x: torch.Tensor, packed: torch.Tensor, n_out: int,
+                  dtype: torch.dtype = torch.float32,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """bf16 [m, k] times a packed MXFP4 matrix (mxfp4_pack) of n_out rows of k values ->
+    fp32 or bf16 [m, n_out] (kdq_mxfp4_product)."""
+    stride = _row_stride(x, torch.bfloat16, "x")
+    _here(x, packed)
+    m, k = x.shape
+    w = _matrix(packed, "kdq_mxfp4_packed_bytes", n_out, k, "packed")
+    y, y_stride = _output(out, m, n_out, dtype, x.device, "out")
+    size = _mxfp4_size("kdq_mxfp4_product_workspace", m, n_out, k, 0)
+    scratch, at = _scratch(size, x.device)
+    call("kdq_mxfp4_product", x.data_ptr(), stride, m, w, n_out, k, _type(dtype), y.data_ptr(),
+         y_stride, at, size, _stream())
+    return y
+
+
+def mxfp4_product_quantized(blocks: torch.Tensor, scales: torch.Tensor, packed: torch.Tensor,
+                            n_out: int, dtype: torch.dtype = torch.float32,
+                            out: torch.Tensor | None = None) -> torch.Tensor:
+    """MXFP4 activations (mxfp4_quantize) times a packed MXFP4 matrix of n_out rows -> fp32
+    or bf16 [m, n_out] (kdq_mxfp4_product_quantized)."""
+    m, k = _blocks(blocks, scales)
+    _here(blocks, scales, packed)
+    w = _matrix(packed, "kdq_mxfp4_packed_bytes", n_out, k, "packed")
+    y, y_stride = _output(out, m, n_out, dtype, blocks.device, "out")
+    size = _mxfp4_size("kdq_mxfp4_product_workspace", m, n_out, k, 1)
+    scratch, at = _scratch(size, blocks.device)
+    call("kdq_mxfp4_product_quantized", blocks.data_ptr(), scales.data_ptr(), m, w, n_out, k,
+         _type(dtype), y.data_ptr(), y_stride, at, size, _stream())
+    return y
+
+
+def mxfp4_gated(x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, n_out: int,
+                save: str | None = None, out: torch.Tensor | None = None):
+    """h = silu(x Wg^T) * (x Wu^T): bf16 [m, k] and two packed MXFP4 matrices (mxfp4_pack) of
+    n_out rows (n_out % 32 == 0) -> bf16 [m, n_out] (kdq_mxfp4_gated).  With ``save`` the
+    pre-activations are kept for mxfp4_gated_backward, and (h, saved) returned: "bf16" as one
+    tensor [m, 2 n_out], "q8" as int8 [m, 2 n_out] and fp32 scales [m, 2 n_out / 32]."""
+    stride = _row_stride(x, torch.bfloat16, "x")
+    _here(x, gate, up)
+    if save not in (None, "bf16", "q8"):
+        raise ValueError('save: None, "bf16" or "q8"')
+    m, k = x.shape
+    if n_out % 32:
+        raise ValueError("n_out must be a multiple of 32")
+    wg = _matrix(gate, "kdq_mxfp4_packed_bytes", n_out, k, "gate")
+    wu = _matrix(up, "kdq_mxfp4_packed_bytes", n_out, k, "up")
+    h, h_stride = _output(out, m, n_out, torch.bfloat16, x.device, "out")
+    saved = kept = codes = scales = None
+    if save == "bf16":
+        saved = torch.empty(m, 2 * n_out, dtype=torch.bfloat16, device=x.device)
+        kept = saved.data_ptr()
+    elif save == "q8":
+        saved = (torch.empty(m, 2 * n_out, dtype=torch.int8, device=x.device),
+                 torch.empty(m, n_out // 16, dtype=torch.float32, device=x.device))
+        codes, scales = saved[0].data_ptr(), saved[1].data_ptr()
+    size = _mxfp4_size("kdq_mxfp4_gated_workspace", m, n_out, k, int(save is not None))
+    scratch, at = _scratch(size, x.device)
+    call("kdq_mxfp4_gated", x.data_ptr(), stride, m, wg, wu, n_out, k, h.data_ptr(), h_stride,
+         kept, codes, scales, at, size, _stream())
+    return h if save is None else (h, saved)
+
+
+def mxfp4_gated_backward(dh: torch.Tensor, saved, gate: torch.Tensor, up: torch.Tensor,
+                         n_in: int, out: torch.Tensor | None = None):
+    """The backward pass of mxfp4_gated over frozen weights: dh bf16 [m, n_out], ``saved``
+    from its forward pass, the matrices from mxfp4_pack(..., transposed=True) -> dx bf16
+    [m, n_in] and the pre-activations' gradients bf16 [m, 2 n_out], gates then ups
+    (kdq_mxfp4_gated_backward)."""
+    stride = _row_stride(dh, torch.bfloat16, "dh")
+    _here(dh, gate, up)
+    m, n = dh.shape
+    if n % 32 or n_in % 32 or not n_in:
+        raise ValueError("n_out and n_in must be multiples of 32")
+    wg = _matrix(gate, "kdq_mxfp4_packed_transposed_bytes", n, n_in, "gate")
+    wu = _matrix(up, "kdq_mxfp4_packed_transposed_bytes", n, n_in, "up")
+    kept = codes = scales = None
+    if isinstance(saved, torch.Tensor):
+        _need(saved, torch.bfloat16, "saved")
+        parts = (saved,)
+        kept = saved.data_ptr()
+    else:
+        parts = q, d = saved
+        _need(q, torch.int8, "saved codes")
+        _need(d, torch.float32, "saved scales")
+        if d.shape != (m, n // 16):
+            raise ValueError("saved: scales of another shape")
+        codes, scales = q.data_ptr(), d.data_ptr()
+    if parts[0].shape != (m, 2 * n):
+        raise ValueError("saved: of another shape than dh")
+    _here(*parts)
+    dgu = torch.empty(m, 2 * n, dtype=torch.bfloat16, device=dh.device)
+    dx, dx_stride = _output(out, m, n_in, torch.bfloat16, dh.device, "out")
+    size = _mxfp4_size("kdq_mxfp4_gated_backward_workspace", m, n, n_in)
+    scratch, at = _scratch(size, dh.device)
+    call("kdq_mxfp4_gated_backward", dh.data_ptr(), stride, m, kept, codes, scales, wg, wu, n,
+         n_in, dgu.data_ptr(), dx.data_ptr(), dx_stride, at, size, _stream())
+    return dx, dgu
+
+
 def hbm_read(buffer: torch.Tensor, sink: torch.Tensor, workgroups: int,
              threads: int = 256, store_all: bool = True, match: int = 0) -> None:
     """kdq_hbm_read: one streaming read of `buffer` (the HBM read ceiling's probe) over
@@ -392,5 +602,7 @@ def hbm_read(buffer: torch.Tensor, sink: torch.Tensor, workgroups: int,
 __all__ = ["dequantize", "gemv", "gemv_batch", "quantize_q8", "gemm_q4_0", "gemm_q4_0_packed",
            "gemm_packed", "hbm_read",
            "moe_gguf", "moe_route",
+           "mxfp4_quantize", "mxfp4_pack", "mxfp4_product", "mxfp4_product_quantized",
+           "mxfp4_gated", "mxfp4_gated_backward",
            "mxfp4_dequantize", "moe_mxfp4", "moe_mxfp4_pack", "moe_mxfp4_packed", "lib",
            "BLOCK_BYTES", "BLOCK_VALUES"]

@@ -1,0 +1,194 @@
+"""CPU checks of the MXFP4 dense operators: sizes, workspaces and refusals of the C ABI
+before any launch, and the reference that the GPU tests compare with."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import kadan_amd
+from kadan_amd import ops
+
+import mxfp4_reference as ref
+
+W, X, Y, Z, V = (0x10000000 * i for i in range(1, 6))  # never dereferenced
+K256 = dict(argument=1, shape=2, unsupported=3, alias=4, scratch=6, alignment=7)
+
+
+def test_packed_sizes():
+    lib = kadan_amd.lib()
+    size, transposed = lib.kdq_mxfp4_packed_bytes, lib.kdq_mxfp4_packed_transposed_bytes
+    assert size(32, 64) == 1024 + 256 == lib.kdq_moe_mxfp4_packed_bytes(1, 32, 64)
+    assert size(2880, 2880) == lib.kdq_moe_mxfp4_packed_bytes(1, 2880, 2880)
+    assert size(1, 32) == 1024 + 256
+    assert size(33, 288) == 2 * 5 * 1024 + 2 * 2 * 256
+    assert transposed(64, 64) == 2048 + 128
+    assert transposed(65, 96) == 2 * 2 * (2048 + 128)
+    for f in (size, transposed):
+        assert f(0, 64) == f(64, 0) == f(64, 48) == f(64, (1 << 20) + 32) == 0
+
+
+def test_pack_refusals():
+    lib = kadan_amd.lib()
+    for f in (lib.kdq_mxfp4_pack, lib.kdq_mxfp4_pack_transposed):
+        assert f(None, X, 32, 64, Y, None) == 1
+        assert f(W, X, 0, 64, Y, None) == 1
+        assert f(W, X, 32, 48, Y, None) == 2
+        assert f(W + 8, X, 32, 64, Y, None) == 7
+        assert f(W, X, 32, 64, Y + 8, None) == 7
+        assert f(W, X, 32, 64, W + 512, None) == 4
+        assert f(W, Y + 512, 32, 64, Y, None) == 4
+
+
+def test_quantize_refusals():
+    f = kadan_amd.lib().kdq_mxfp4_quantize
+    assert f(0, None, 64, 2, 64, Y, Z, None, None) == 1
+    assert f(0, X, 64, 0, 64, Y, Z, None, None) == 1
+    assert f(8, X, 64, 2, 64, Y, Z, None, None) == 3
+    assert f(0, X, 64, 2, 48, Y, Z, None, None) == 2
+    assert f(0, X, 63, 2, 64, Y, Z, None, None) == 2
+    assert f(0, X, 68, 2, 64, Y, Z, None, None) == 2
+    assert f(0, X, 1 << 62, 1 << 10, 64, Y, Z, None, None) == 2
+    assert f(0, X + 8, 64, 2, 64, Y, Z, None, None) == 7
+    assert f(0, X, 64, 2, 64, Y + 2, Z, None, None) == 7
+    assert f(0, X, 64, 2, 64, X + 256, Z, None, None) == 4
+    assert f(0, X, 64, 2, 64, Y, X + 64, None, None) == 4
+    assert f(0, X, 64, 2, 64, Y, Y + 16, None, None) == 4
+
+
+def test_product_refusals():
+    lib = kadan_amd.lib()
+    f = lib.kdq_mxfp4_product
+    good = dict(x=X, xs=64, m=2, w=W, n=40, k=64, t=0, y=Y, ys=40, ws=None, wb=0)
+
+    def call(**change):
+        a = {**good, **change}
+        return f(a["x"], a["xs"], a["m"], a["w"], a["n"], a["k"], a["t"], a["y"], a["ys"],
+                 a["ws"], a["wb"], None)
+
+    for name in ("x", "w", "y"):
+        assert call(**{name: None}) == 1
+    for name in ("m", "n", "k"):
+        assert call(**{name: 0}) == 1
+    assert call(k=48, xs=48) == 2 and call(xs=63) == 2 and call(xs=68) == 2
+    assert call(xs=(1 << 21) + 8) == 2 and call(m=(1 << 20) + 1) == 2
+    assert call(n=(1 << 24) + 1, ys=1 << 25) == 2 and call(ys=39) == 2
+    assert call(t=1) == 3 and call(t=8) == 3
+    assert call(x=X + 8) == 7 and call(w=W + 8) == 7 and call(y=Y + 2) == 7
+    assert call(t=30, y=Y + 1) == 7
+    assert call(y=X + 128) == 4 and call(y=W + 64) == 4
+    # K slices need their workspace, aligned and apart from the output
+    need = lib.kdq_mxfp4_product_workspace(77, 4096, 14336, 0)
+    assert need > 0
+    big = dict(m=77, n=4096, k=14336, xs=14336, ys=4096, y=Y * 4, x=X * 4, w=W * 8)
+    assert call(**big) == 6 and call(**big, ws=Z * 8, wb=need - 1) == 6
+    assert call(**big, ws=Z * 8 + 8, wb=need) == 7
+    assert call(**big, ws=Y * 4 + 256, wb=need) == 4
+
+
+def test_product_quantized_refusals():
+    f = kadan_amd.lib().kdq_mxfp4_product_quantized
+    ok = [X, Z, 2, W, 40, 64, 0, Y, 40, None, 0, None]
+
+    def call(at, value):
+        return f(*[value if i == at else v for i, v in enumerate(ok)])
+
+    for at in (0, 1, 3, 7):
+        assert call(at, None) == 1
+    for at in (2, 4, 5):
+        assert call(at, 0) == 1
+    assert call(5, 48) == 2 and call(8, 39) == 2 and call(6, 1) == 3
+    assert call(0, X + 4) == 7 and call(3, W + 4) == 7 and call(7, Y + 2) == 7
+    assert call(7, X) == 4 and call(7, Z) == 4 and call(7, W) == 4
+
+
+def test_gated_refusals():
+    f = kadan_amd.lib().kdq_mxfp4_gated
+    ok = [X, 64, 2, W, W + 65536, 32, 64, Y, 32, None, None, None, None, 0, None]
+
+    def call(**change):
+        return f(*[change.get(f"a{i}", v) for i, v in enumerate(ok)])
+
+    for at in (0, 3, 4, 7):
+        assert call(**{f"a{at}": None}) == 1
+    for at in (2, 5, 6):
+        assert call(**{f"a{at}": 0}) == 1
+    assert call(a10=Z) == 1 and call(a11=Z) == 1 and call(a9=Z, a10=V, a11=V + 4096) == 1
+    assert call(a5=40, a8=40) == 2 and call(a6=48) == 2 and call(a1=60) == 2 and call(a8=31) == 2
+    assert call(a0=X + 8) == 7 and call(a4=W + 65544) == 7 and call(a9=Z + 8) == 7
+    assert call(a10=Z + 4, a11=V) == 7
+    assert call(a7=X + 32) == 4 and call(a7=W + 64) == 4 and call(a9=Y + 16) == 4
+    assert call(a10=Z, a11=Z + 64) == 4 and call(a10=W, a11=V) == 4
+
+
+def test_gated_backward_refusals():
+    f = kadan_amd.lib().kdq_mxfp4_gated_backward
+    ok = [X, 32, 2, Z, None, None, W, W + 65536, 32, 64, Y, Y + 65536, 64, None, 0, None]
+
+    def call(**change):
+        return f(*[change.get(f"a{i}", v) for i, v in enumerate(ok)])
+
+    for at in (0, 3, 6, 7, 10, 11):
+        assert call(**{f"a{at}": None}) == 1
+    for at in (2, 8, 9):
+        assert call(**{f"a{at}": 0}) == 1
+    assert call(a4=V) == 1 and call(a3=None, a4=V) == 1 and call(a5=V) == 1
+    assert call(a8=40, a1=40) == 2 and call(a9=48) == 2 and call(a1=36) == 2 and call(a12=63) == 2
+    assert call(a0=X + 2) == 7 and call(a3=Z + 8) == 7 and call(a10=Y + 8) == 7
+    assert call(a11=Y + 65537) == 7
+    assert call(a10=X) == 4 and call(a10=Z) == 4 and call(a11=Y) == 4 and call(a11=W) == 4
+
+
+def test_sizes_without_a_workspace_and_with_one():
+    lib = kadan_amd.lib()
+    assert lib.kdq_mxfp4_product_workspace(1, 14336, 4096, 0) == 0
+    assert lib.kdq_mxfp4_product_workspace(0, 14336, 4096, 0) == 0
+    assert lib.kdq_mxfp4_product_workspace(8, 64, 48, 0) == 0
+    assert lib.kdq_mxfp4_gated_workspace(1, 14336, 4096, 0) == 0
+    # a slice's results are 8 KB per pair of 32 x 32 tiles
+    for got in (lib.kdq_mxfp4_product_workspace(77, 4096, 14336, 0),
+                lib.kdq_mxfp4_gated_workspace(1, 64, 4096, 1),
+                lib.kdq_mxfp4_gated_backward_workspace(40, 4096, 64)):
+        assert got % 8192 == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_wrappers_refuse_host_tensors(dtype):
+    x = torch.zeros(2, 64, dtype=dtype)
+    u8 = torch.zeros(1280, dtype=torch.uint8)
+    with pytest.raises(ValueError):
+        ops.mxfp4_quantize(x)
+    with pytest.raises(ValueError):
+        ops.mxfp4_product(x, u8, 32)
+    with pytest.raises(ValueError):
+        ops.mxfp4_gated(x, u8, u8, 32)
+    with pytest.raises(ValueError):
+        ops.mxfp4_gated_backward(x, x, u8, u8, 64)
+    with pytest.raises(ValueError):
+        ops.mxfp4_pack(u8.view(1, -1), u8[:80].view(1, -1))
+
+
+def test_reference_quantiser_is_nearest_and_ties_to_even():
+    """The oracle of the GPU tests, by hand: the format's own values, ties, and saturation."""
+    row = np.zeros((1, 32))
+    row[0, :12] = [6.0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, -0.5, -6.9, 0.26, 7.0]
+    blocks, scales = ref.quantize(row)
+    assert scales.tolist() == [[127]]
+    codes = [int(b) >> s & 15 for b in blocks[0] for s in (0, 4)]
+    assert codes[:12] == [7, 0, 2, 2, 4, 4, 6, 6, 9, 15, 1, 7]
+    for e in (-127, -3, 90):
+        got = ref.quantize(row * 2.0 ** e)
+        assert got[1].tolist() == [[127 + e]] and np.array_equal(got[0], blocks)
+    values = ref.decode(torch.from_numpy(blocks), torch.from_numpy(scales))[0, :12].tolist()
+    assert values == [6, 0, 1, 1, 2, 2, 4, 4, -0.5, -6, 0.5, 6]
+
+
+def test_gradient_formula_against_differences():
+    g, u, dh = (torch.randn(3, 32, dtype=torch.float64) * 3 for _ in range(3))
+    want, _ = ref.gate_gradients(dh, g, u)
+    f = lambda a, b: dh * a * torch.sigmoid(a) * b
+    e = 1e-6
+    numeric = torch.cat([(f(g + e, u) - f(g - e, u)) / (2 * e),
+                         (f(g, u + e) - f(g, u - e)) / (2 * e)], 1)
+    # central differences: e^2 / 6 times the third derivative, and cancellation of 2^-53 / e
+    assert float((want - numeric).abs().max()) < 1e-12 * 50 + 1e-7
