@@ -433,7 +433,8 @@ int kdq_mxfp4_product(const uint16_t* x_bf16, size_t x_stride, size_t m, const u
                       size_t n, size_t k, int type, void* y, size_t y_stride, void* workspace,
                       size_t workspace_bytes, void* stream);
 
-/* The same over MXFP4 activations (kdq_mxfp4_quantize; workspace with quantized = 1). */
+/* The same over MXFP4 activations (kdq_mxfp4_quantize; workspace with quantized = 1);
+ * x_blocks 16-byte, x_scales 4-byte aligned. */
 int kdq_mxfp4_product_quantized(const uint8_t* x_blocks, const uint8_t* x_scales, size_t m,
                                 const uint8_t* packed, size_t n, size_t k, int type, void* y,
                                 size_t y_stride, void* workspace, size_t workspace_bytes,

@@ -360,6 +360,7 @@ __global__ __launch_bounds__(1024) void decode_kernel(Decode a) {
     auto* red = reinterpret_cast<f32x4*>(lds);
     const unsigned lane = threadIdx.x % 64, wave = threadIdx.x / 64, waves = blockDim.x / 64;
     const unsigned r = lane % 16, q = lane / 16;
+    const unsigned first_row = blockIdx.y * (16 * TB), rows = min(a.out.m - first_row, 16u * TB);
     const unsigned group = blockIdx.x / 2, row = 16 * (blockIdx.x % 2) + r;
     const unsigned share = GATED ? waves / 2 : waves;  // wavefronts on one matrix
     const uint8_t* w = GATED && wave >= share ? a.w1 : a.w0;
@@ -372,8 +373,10 @@ __global__ __launch_bounds__(1024) void decode_kernel(Decode a) {
     const unsigned lane_codes = (q / 2) * 1024 + (row + 32 * (q % 2)) * 16;
     const unsigned lane_scales = (row + 32 * (q % 2)) * 4;
     const unsigned row_bytes = FP4 ? a.k / 2 : a.k * 2;
-    const auto xs = buffer(a.x, (a.out.m - 1) * a.x_stride + row_bytes);
-    const auto xscales = buffer(a.x_scales, FP4 ? a.out.m * (a.k / 32) : 0);
+    const auto xs = buffer(a.x + size_t(first_row) * a.x_stride,
+                           (rows - 1) * a.x_stride + row_bytes);
+    const auto xscales = buffer(a.x_scales + size_t(first_row) * (a.k / 32),
+                                FP4 ? rows * (a.k / 32) : 0);
 
     f32x4 acc[TB] = {};
     constexpr int kBatch = TB == 1 ? 4 : 2;
@@ -394,7 +397,7 @@ __global__ __launch_bounds__(1024) void decode_kernel(Decode a) {
 #pragma unroll
             for (int i = 0; i < TB; ++i) {
                 const unsigned token = r + 16 * i;
-                const bool there = token < a.out.m && 128 * t + 32 * q < a.k;
+                const bool there = token < rows && 128 * t + 32 * q < a.k;
                 if constexpr (FP4) {
                     x[b][i][0] =
                         load_b128(xs, there ? int(token * a.x_stride + (4 * t + q) * 16) : kOutside);
@@ -434,7 +437,7 @@ __global__ __launch_bounds__(1024) void decode_kernel(Decode a) {
     __syncthreads();
     if (wave >= TB)
         return;
-    const unsigned token = 16 * wave + r, at = blockIdx.x * 16 + 4 * q;
+    const unsigned token = first_row + 16 * wave + r, at = blockIdx.x * 16 + 4 * q;
     if (token >= a.out.m)
         return;
     auto total = [&](unsigned from) {
@@ -462,8 +465,9 @@ __global__ __launch_bounds__(1024) void decode_kernel(Decode a) {
 // (SPLIT; the groups' sums meet in LDS at the end) or two sets of TT * 32 rows.  x passes
 // through LDS in chunks of 128 bytes a row (64 bf16 values, or 256 MXFP4 values), copied
 // by DMA three chunks ahead into four buffers, eight rows to an instruction; a row's
-// 16-byte segments lie in it by (segment ^ row % 8), so the copies read whole lines and
-// the operands' reads are free of bank conflicts.  Weights go from memory to registers,
+// 16-byte segments lie in it by (segment ^ row / 2 % 8), so the copies read whole lines and
+// any 16 neighbouring rows' operands lie in all 64 banks (by row % 8, which two rows of 16
+// share: a conflict in one cycle of eight).  Weights go from memory to registers,
 // every one read and decoded by one wavefront (two where the groups share rows).
 //
 // Operands: bf16 x (v_mfma_f32_32x32x16_bf16, weights decoded to bf16, exact), MXFP4 x
@@ -494,6 +498,10 @@ __device__ __forceinline__ void issue_order() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
+__device__ __forceinline__ unsigned uniform(unsigned v) {
+    return unsigned(__builtin_amdgcn_readfirstlane(int(v)));
+}
+
 template <int N, class F>
 __device__ __forceinline__ void static_for(F&& f) {
     [&]<int... I>(std::integer_sequence<int, I...>) {
@@ -511,7 +519,7 @@ __global__ __launch_bounds__(512, 2) void gemm_kernel(Gemm a) {
     extern __shared__ __align__(16) uint8_t lds[];
     constexpr int kStageBytes = TT * 8192;
     const unsigned lane = threadIdx.x % 64, h = lane / 32;
-    const unsigned wave = unsigned(__builtin_amdgcn_readfirstlane(int(threadIdx.x / 64)));
+    const unsigned wave = uniform(threadIdx.x / 64);
     const unsigned rg = wave % 4, kg = wave / 4;
 
     // neighbouring tiles on one XCD (workgroups go round the eight of them), its matrix rows'
@@ -543,8 +551,9 @@ __global__ __launch_bounds__(512, 2) void gemm_kernel(Gemm a) {
     for (int j = 0; j < TT; ++j) {
         const unsigned u = j * 8 + wave;  // this instruction's eight rows
         const unsigned set = SPLIT ? u / (4 * TT) : 0;
-        const unsigned row = min((SPLIT ? u % (4 * TT) : u) * 8 + lane / 8, rows - 1);
-        const unsigned seg = (lane % 8) ^ (lane / 8);
+        const unsigned place = (SPLIT ? u % (4 * TT) : u) * 8 + lane / 8;
+        const unsigned row = min(place, rows - 1);
+        const unsigned seg = (lane % 8) ^ (place / 2 % 8);
         const unsigned b = min(a.chunks, part_of(set) * a.part);
         const unsigned e = min(a.segments, min(a.chunks, b + a.part) * 8);
         const unsigned from = b * 8 + seg;
@@ -552,7 +561,28 @@ __global__ __launch_bounds__(512, 2) void gemm_kernel(Gemm a) {
                       (OPS == kTransposed && set ? a.x_second : 0));
         x_limit[j] = e > from ? e - from : 0;
     }
-    auto stage = [&](unsigned chunk, uint8_t* to) {  // chunk of the part
+    // kFp4: a chunk is eight scale bytes of a row, copied as the three dwords that hold them
+    // (a row's bytes start anywhere; the buffer ends with the dword of the last one) into 16
+    // bytes of LDS, sixteen rows to an instruction
+    constexpr int kScaleCopies = OPS != kFp4 ? 0 : TT > 2 ? TT / 2 : 1;
+    const unsigned x_blocks = a.segments;  // scale bytes of a row: a segment is 32 values
+    const size_t scales_from = size_t(first_row) * x_blocks;
+    const unsigned odd = unsigned(scales_from % 4);
+    const auto xscales = buffer(a.x_scales + (scales_from - odd),
+                                OPS == kFp4 ? (odd + rows * x_blocks + 3) / 4 * 4 : 0);
+    int scale_at[TT];
+    if constexpr (OPS == kFp4) {
+#pragma unroll
+        for (int j = 0; j < kScaleCopies; ++j) {
+            const unsigned place = (j * 8 + wave) % (4 * TT) * 16 + lane / 4;
+            const unsigned set = SPLIT ? place / (TT * 32) : 0;
+            const unsigned row = min(SPLIT ? place % (TT * 32) : place, rows - 1);
+            const unsigned from = odd + row * x_blocks + min(a.chunks, part_of(set) * a.part) * 8;
+            scale_at[j] = lane % 4 < 3 ? int(from / 4 * 4 + lane % 4 * 4) : kOutside / 2;
+        }
+    }
+    auto stage = [&](unsigned chunk, unsigned slot) {  // chunk of the part
+        uint8_t* to = lds + slot * kStageBytes;
 #pragma unroll
         for (int j = 0; j < TT; ++j) {
             const int at = chunk * 8 < x_limit[j] ? x_at[j] + int(chunk * 128) : kOutside;
@@ -560,14 +590,23 @@ __global__ __launch_bounds__(512, 2) void gemm_kernel(Gemm a) {
                 xs, (__attribute__((address_space(3))) void*)(to + (j * 8 + wave) * 1024), 16, at,
                 0, 0, 0);
         }
+#pragma unroll
+        for (int j = 0; j < kScaleCopies; ++j)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                xscales,
+                (__attribute__((address_space(3))) void*)(lds + kStages * kStageBytes +
+                                                          slot * (TT * 1024) +
+                                                          (j * 8 + wave) % (4 * TT) * 256),
+                4, scale_at[j] + int(chunk * 8), 0, 0, 0);
         issue_order();
     };
 
     // weights: buffers that end with the part, so that steps past it are zero codes
     constexpr unsigned kStepsPerChunk = OPS == kFp4 ? 4 : 1;
     constexpr unsigned kStepBytes = OPS == kTransposed ? 2048 : 1024;
-    const unsigned end_step = min(a.steps, end * kStepsPerChunk);
-    const unsigned begin_step = begin * kStepsPerChunk;
+    // (in scalar registers, or every load would loop over its buffer's possible values)
+    const unsigned end_step = uniform(min(a.steps, end * kStepsPerChunk));
+    const unsigned begin_step = uniform(begin * kStepsPerChunk);
     const unsigned scale_groups = (a.steps + 3) / 4;
     __amdgpu_buffer_rsrc_t codes_buf[2], scales_buf[2];
 #pragma unroll
@@ -606,19 +645,8 @@ __global__ __launch_bounds__(512, 2) void gemm_kernel(Gemm a) {
         issue_order();
     };
     struct Scales {
-        unsigned w[2], x[OPS == kFp4 ? TT : 1];
+        unsigned w[2];
     };
-    // kFp4: this lane's rows of x scales
-    const uint8_t* xscale_row[OPS == kFp4 ? TT : 1];
-    const unsigned x_blocks = a.segments;  // (a segment is 32 MXFP4 values)
-    if constexpr (OPS == kFp4) {
-#pragma unroll
-        for (int t = 0; t < TT; ++t) {
-            const unsigned row =
-                min((SPLIT ? 0 : kg * TT * 32) + t * 32 + lane % 32, rows - 1);
-            xscale_row[t] = a.x_scales + size_t(first_row + row) * x_blocks;
-        }
-    }
     // Scales of the four steps from `step` (a multiple of 4).
     auto load_scales = [&](unsigned step, Scales& s) {
         if constexpr (OPS != kTransposed) {
@@ -626,29 +654,6 @@ __global__ __launch_bounds__(512, 2) void gemm_kernel(Gemm a) {
             for (int t = 0; t < 2; ++t)
                 s.w[t] = __builtin_amdgcn_raw_buffer_load_b32(
                     scales_buf[t], int(step * 64 + lane * 4), 0, 0);
-        }
-        if constexpr (OPS == kFp4) {
-            const unsigned block = step * 2;
-            if (block + 8 <= x_blocks) {
-#pragma unroll
-                for (int t = 0; t < TT; ++t) {
-                    typedef unsigned two __attribute__((ext_vector_type(2), aligned(1)));
-                    const two v = *reinterpret_cast<const two*>(xscale_row[t] + block);
-                    s.x[t] = __builtin_amdgcn_perm(v.y, v.x, h ? 0x07050301u : 0x06040200u);
-                }
-            } else {  // the last, short chunk of a row, or none: byte by byte
-#pragma unroll
-                for (int t = 0; t < TT; ++t) {
-                    unsigned word = 0;
-#pragma unroll
-                    for (unsigned j = 0; j < 4; ++j) {
-                        const unsigned b = block + 2 * j + h;
-                        const unsigned v = xscale_row[t][min(b, x_blocks - 1)];
-                        word |= (b < x_blocks ? v : 0u) << (8 * j);
-                    }
-                    s.x[t] = word;
-                }
-            }
         }
         issue_order();
     };
@@ -671,15 +676,15 @@ __global__ __launch_bounds__(512, 2) void gemm_kernel(Gemm a) {
     };
     const uint8_t* x_lane = lds + kg * (TT * 4096) + (lane % 32) * 128;
     auto x_operand = [&](const uint8_t* buf, int t, unsigned seg) {
-        return *reinterpret_cast<const u4*>(buf + t * 4096 + ((seg ^ (lane % 8)) * 16));
+        return *reinterpret_cast<const u4*>(buf + t * 4096 + ((seg ^ (lane / 2 % 8)) * 16));
     };
 
     Codes codes[kAhead];
     Scales scales, next;
     issue_order();
-    stage(0, lds);
-    stage(1, lds + kStageBytes);
-    stage(2, lds + 2 * kStageBytes);
+    stage(0, 0);
+    stage(1, 1);
+    stage(2, 2);
     load_scales(begin_step, scales);
 #pragma unroll
     for (int i = 0; i < kAhead; ++i)
@@ -687,28 +692,50 @@ __global__ __launch_bounds__(512, 2) void gemm_kernel(Gemm a) {
 
     if constexpr (OPS == kFp4) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // fewer loads than the loop counts on
-        unsigned slot = 0;
-        for (unsigned c = 0; c < a.part; ++c) {
-            // (the scales' loads: at least as many as on the whole-chunk path)
-            arrive.template operator()<2 * TT + 3 * kCodeLoads>();
-            const uint8_t* buf = x_lane + slot * kStageBytes;
-            stage(c + 3, lds + ((slot + 3) % kStages) * kStageBytes);
-            load_scales(begin_step + 4 * (c + 1), next);
-            static_for<4>([&]<int S>() {
+        // (32 rows on, a row's bytes start the same)
+        const unsigned scale_shift = (odd + lane % 32 * x_blocks) % 4;
+        // (two chunks a turn: their scales stay in registers of their own, and are put in
+        // order only where they are used, so that no load is waited for where it is issued)
+        for (unsigned c0 = 0; c0 < a.part; c0 += 2) {
+            static_for<2>([&]<int C>() {
+                arrive.template operator()<2 * (TT + kScaleCopies) + 3 * kCodeLoads + 4>();
+                const unsigned slot = c0 % kStages + C;
+                const uint8_t* buf = x_lane + slot * kStageBytes;
+                Scales& now = C ? next : scales;
+                load_scales(begin_step + 4 * (c0 + C + 1), C ? scales : next);
+                stage(c0 + C + 3, (slot + 3) % kStages);
+                // a row's eight scales, those past its end (the next row's, or none) as zero;
+                // the lane's half has every other one
+                const unsigned block = (begin + c0 + C) * 8;
+                const unsigned there = x_blocks - min(x_blocks, block);
+                unsigned xs_now[TT];
 #pragma unroll
                 for (int t = 0; t < TT; ++t) {
-                    const i32x8 xv = fp4_operand(x_operand(buf, t, 2 * S + h));
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-                        acc[i][t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-                            fp4_operand(codes[S].w[i]), xv, acc[i][t], 4, 4, S,
-                            int(scales.w[i]), S, int(scales.x[t]));
+                    const u4 v = *reinterpret_cast<const u4*>(
+                        lds + kStages * kStageBytes + slot * (TT * 1024) +
+                        (kg * (TT * 32) + t * 32 + lane % 32) * 16);
+                    uint64_t bytes = uint64_t(__builtin_amdgcn_alignbyte(v.z, v.y, scale_shift))
+                                         << 32 |
+                                     __builtin_amdgcn_alignbyte(v.y, v.x, scale_shift);
+                    if (there < 8)
+                        bytes &= (uint64_t(1) << (8 * there)) - 1;
+                    xs_now[t] = __builtin_amdgcn_perm(unsigned(bytes >> 32), unsigned(bytes),
+                                                      h ? 0x07050301u : 0x06040200u);
                 }
-                issue_order();
-                load_codes(begin_step + 4 * (c + 1) + S, codes[S]);
+                static_for<4>([&]<int S>() {
+#pragma unroll
+                    for (int t = 0; t < TT; ++t) {
+                        const i32x8 xv = fp4_operand(x_operand(buf, t, 2 * S + h));
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            acc[i][t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+                                fp4_operand(codes[S].w[i]), xv, acc[i][t], 4, 4, S,
+                                int(now.w[i]), S, int(xs_now[t]));
+                    }
+                    issue_order();
+                    load_codes(begin_step + 4 * (c0 + C + 1) + S, codes[S]);
+                });
             });
-            scales = next;
-            slot = (slot + 1) % kStages;
         }
     } else {
         for (unsigned c0 = 0; c0 < a.part; c0 += 4) {
@@ -716,7 +743,7 @@ __global__ __launch_bounds__(512, 2) void gemm_kernel(Gemm a) {
                 constexpr int kScaleLoads = OPS == kTransposed || C == 0 ? 0 : 2;
                 arrive.template operator()<2 * TT + 3 * kCodeLoads + kScaleLoads>();
                 const uint8_t* buf = x_lane + C * kStageBytes;
-                stage(c0 + C + 3, lds + ((C + 3) % kStages) * kStageBytes);
+                stage(c0 + C + 3, (C + 3) % kStages);
                 if constexpr (C == 0)
                     load_scales(begin_step + c0 + 4, next);
                 static_for<4>([&]<int S>() {
@@ -963,7 +990,7 @@ size_t partial_bytes(const Plan& p, size_t m) {
 template <int TT, bool SPLIT, int OPS, int OUT>
 int launch_gemm(const Gemm& a, const Plan& p, hipStream_t st) {
     const auto f = gemm_kernel<TT, SPLIT, OPS, OUT>;
-    constexpr int kLds = kStages * TT * 8192;
+    constexpr int kLds = kStages * TT * (OPS == kFp4 ? 9216 : 8192);
     if constexpr (kLds > 64 * 1024) {
         static std::atomic<uint64_t> configured{0};  // devices whose attribute is set
         int device = 0;
@@ -1021,7 +1048,9 @@ int launch_decode(const Decode& a, hipStream_t st) {
     const unsigned units = (a.k + 127) / 128;
     const unsigned per = GATED ? 2 : 1;
     const unsigned waves = per * (units <= 8 ? 2 : units <= 16 ? 4 : units <= 64 || GATED ? 8 : 16);
-    hipLaunchKernelGGL((decode_kernel<TB, GATED, FP4, OUT>), dim3(unsigned(ceil_div(a.out.n, 16))),
+    hipLaunchKernelGGL((decode_kernel<TB, GATED, FP4, OUT>),
+                       dim3(unsigned(ceil_div(a.out.n, 16)),
+                            unsigned(ceil_div(a.out.m, 16 * TB))),
                        dim3(waves * 64), waves * TB * 1024, st, a);
     KDQ_HIP(hipGetLastError());
     return KDQ_OK;
@@ -1222,7 +1251,7 @@ extern "C" int kdq_mxfp4_product_quantized(const uint8_t* x_blocks, const uint8_
         return KDQ_ERR_SHAPE;
     if (const int rc = check_output(type, y, y_stride, m, n))
         return rc;
-    if (misaligned(x_blocks, 16) || misaligned(packed, 16))
+    if (misaligned(x_blocks, 16) || misaligned(x_scales, 4) || misaligned(packed, 16))
         return KDQ_ERR_ALIGNMENT;
     const size_t y_bytes = extent(m, y_stride, n, type == KDQ_F32 ? 4 : 2);
     if (overlaps(y, y_bytes, x_blocks, m * (k / 2)) ||
