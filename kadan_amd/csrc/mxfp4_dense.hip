@@ -308,12 +308,94 @@ __device__ __forceinline__ f32x4 quad_of(const f32x16& a, int j) {
     return f32x4{a[4 * j], a[4 * j + 1], a[4 * j + 2], a[4 * j + 3]};
 }
 
-template <int OUT>
-__device__ __forceinline__ void store_tiles(const Target& t, unsigned G, unsigned token,
-                                            unsigned h, const f32x16& a0, const f32x16& a1) {
+// 32 rows of 128 bytes, a wavefront's own in LDS, to rows `first` .. of y (their bytes from
+// byte column `c` on, those below `bytes`): whole lines in 16-byte pieces, where a lane's own
+// values would be 8- or 16-byte pieces of 32 rows (each a request of its own to the L2: 3.7
+// million of 10 million for 2048 x 14336 bf16 results).
+constexpr unsigned kPatchBytes = 4096;
+
+__device__ __forceinline__ unsigned patch_at(unsigned row, unsigned piece) {
+    return row * 128 + (piece ^ (row / 2 % 8)) * 16;
+}
+
+__device__ __forceinline__ void store_patch(const uint8_t* patch, uint8_t* y, size_t row_bytes,
+                                            unsigned first, unsigned m, size_t c, size_t bytes) {
+    const unsigned lane = threadIdx.x % 64, piece = lane % 8;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    u4 v[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-        store_quad<OUT>(t, G, token, h, j, quad_of(a0, j), quad_of(a1, j));
+    for (int i = 0; i < 4; ++i)
+        v[i] = *reinterpret_cast<const u4*>(patch + patch_at(8 * i + lane / 8, piece));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const unsigned row = first + 8 * i + lane / 8;
+        const size_t at = c + 16 * piece;
+        if (row >= m || at >= bytes)
+            continue;
+        uint8_t* to = y + size_t(row) * row_bytes + at;
+        if (at + 16 <= bytes) {
+            *reinterpret_cast<quad_a2*>(to) = quad_a2{v[i].x, v[i].y, v[i].z, v[i].w};
+        } else {
+#pragma unroll
+            for (unsigned e = 0; e < 7; ++e)  // (values are 2 or 4 bytes)
+                if (at + 2 * e < bytes)
+                    *reinterpret_cast<uint16_t*>(to + 2 * e) =
+                        uint16_t(v[i][e / 2] >> (16 * (e % 2)));
+        }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// Two tiles of 32 columns as bf16, side by side in the patch.
+__device__ __forceinline__ void patch_pair(uint8_t* patch, unsigned token, unsigned h,
+                                           const f32x16& a0, const f32x16& a1) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const f32x4 v0 = quad_of(a0, j), v1 = quad_of(a1, j);
+        *reinterpret_cast<uint2*>(patch + patch_at(token, j) + 8 * h) =
+            make_uint2(bf16_pair(v0.x, v0.y), bf16_pair(v0.z, v0.w));
+        *reinterpret_cast<uint2*>(patch + patch_at(token, 4 + j) + 8 * h) =
+            make_uint2(bf16_pair(v1.x, v1.y), bf16_pair(v1.z, v1.w));
+    }
+}
+
+// A wavefront's two 32 x 32 result tiles (group G, rows 32T .. of x): as store_quad, through
+// `patch`, kPatchBytes of LDS that are the wavefront's own.
+template <int OUT>
+__device__ __forceinline__ void store_tiles(const Target& t, unsigned G, unsigned T,
+                                            uint8_t* patch, const f32x16& a0, const f32x16& a1) {
+    const unsigned lane = threadIdx.x % 64, row = lane % 32, h = lane / 32;
+    const unsigned token = T * 32 + row;
+    auto* y = static_cast<uint8_t*>(t.y);
+    if constexpr (OUT == kOutF32) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                *reinterpret_cast<f32x4*>(patch + patch_at(row, 2 * j + h)) =
+                    quad_of(i ? a1 : a0, j);
+            store_patch(patch, y, t.stride * 4, T * 32, t.m, (size_t(64) * G + 32 * i) * 4,
+                        size_t(t.n) * 4);
+        }
+    } else if constexpr (OUT == kOutBf16) {
+        patch_pair(patch, row, h, a0, a1);
+        store_patch(patch, y, t.stride * 2, T * 32, t.m, size_t(64) * G * 2, size_t(t.n) * 2);
+    } else if constexpr (OUT == kOutBackward) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const f32x4 v0 = quad_of(a0, j), v1 = quad_of(a1, j);
+            *reinterpret_cast<u4*>(patch + patch_at(row, 2 * j + h)) =
+                u4{bf16_pair(v0.x, v1.x), bf16_pair(v0.y, v1.y), bf16_pair(v0.z, v1.z),
+                   bf16_pair(v0.w, v1.w)};
+        }
+        store_patch(patch, y, t.stride * 2, T * 32, t.m, size_t(64) * G * 2, size_t(t.n) * 2);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            store_quad<OUT>(t, G, token, h, j, quad_of(a0, j), quad_of(a1, j));
+    }
     if constexpr (OUT == kOutGated) {
         if (t.kept_q && 32 * G < t.n) {
             const f32x4 g[4] = {quad_of(a0, 0), quad_of(a0, 1), quad_of(a0, 2), quad_of(a0, 3)};
@@ -517,7 +599,7 @@ __device__ __forceinline__ i32x8 fp4_operand(const u4& c) {
 template <int TT, bool SPLIT, int OPS, int OUT>
 __global__ __launch_bounds__(512, 2) void gemm_kernel(Gemm a) {
     extern __shared__ __align__(16) uint8_t lds[];
-    constexpr int kStageBytes = TT * 8192;
+    constexpr int GROUPS = 2, kWaves = 4 * GROUPS, kStageBytes = TT * 8192;
     const unsigned lane = threadIdx.x % 64, h = lane / 32;
     const unsigned wave = uniform(threadIdx.x / 64);
     const unsigned rg = wave % 4, kg = wave / 4;
@@ -549,7 +631,7 @@ __global__ __launch_bounds__(512, 2) void gemm_kernel(Gemm a) {
     unsigned x_limit[TT];    // chunks * 8 it may read, counted from its segment
 #pragma unroll
     for (int j = 0; j < TT; ++j) {
-        const unsigned u = j * 8 + wave;  // this instruction's eight rows
+        const unsigned u = j * kWaves + wave;  // this instruction's eight rows
         const unsigned set = SPLIT ? u / (4 * TT) : 0;
         const unsigned place = (SPLIT ? u % (4 * TT) : u) * 8 + lane / 8;
         const unsigned row = min(place, rows - 1);
@@ -561,43 +643,48 @@ __global__ __launch_bounds__(512, 2) void gemm_kernel(Gemm a) {
                       (OPS == kTransposed && set ? a.x_second : 0));
         x_limit[j] = e > from ? e - from : 0;
     }
-    // kFp4: a chunk is eight scale bytes of a row, copied as the three dwords that hold them
-    // (a row's bytes start anywhere; the buffer ends with the dword of the last one) into 16
-    // bytes of LDS, sixteen rows to an instruction
-    constexpr int kScaleCopies = OPS != kFp4 ? 0 : TT > 2 ? TT / 2 : 1;
+    // kFp4: the scales of four chunks are 32 bytes of a row, copied as the nine dwords that
+    // hold them (a row's bytes start anywhere; the buffer ends with the dword of the last one)
+    // into 40 bytes of LDS: read by single chunks, each row's line would come four times
+    constexpr int kScaleRows = GROUPS * TT * 32;
+    constexpr int kScaleBytes = OPS == kFp4 ? kScaleRows * 40 : 0;
+    constexpr int kScaleCopies = (kScaleBytes / 256 + kWaves - 1) / kWaves;
     const unsigned x_blocks = a.segments;  // scale bytes of a row: a segment is 32 values
     const size_t scales_from = size_t(first_row) * x_blocks;
     const unsigned odd = unsigned(scales_from % 4);
     const auto xscales = buffer(a.x_scales + (scales_from - odd),
                                 OPS == kFp4 ? (odd + rows * x_blocks + 3) / 4 * 4 : 0);
-    int scale_at[TT];
-    if constexpr (OPS == kFp4) {
+    int scale_at[kScaleCopies + 1];
+    unsigned scale_to[kScaleCopies + 1];
 #pragma unroll
-        for (int j = 0; j < kScaleCopies; ++j) {
-            const unsigned place = (j * 8 + wave) % (4 * TT) * 16 + lane / 4;
-            const unsigned set = SPLIT ? place / (TT * 32) : 0;
-            const unsigned row = min(SPLIT ? place % (TT * 32) : place, rows - 1);
-            const unsigned from = odd + row * x_blocks + min(a.chunks, part_of(set) * a.part) * 8;
-            scale_at[j] = lane % 4 < 3 ? int(from / 4 * 4 + lane % 4 * 4) : kOutside / 2;
-        }
+    for (int j = 0; j < kScaleCopies; ++j) {
+        // (the last round's spare wavefronts repeat its last copy)
+        const unsigned copy = min(j * kWaves + wave, unsigned(kScaleBytes / 256 - 1));
+        const unsigned place = (copy * 64 + lane) / 10, dword = (copy * 64 + lane) % 10;
+        const unsigned set = SPLIT ? place / (TT * 32) : 0;
+        const unsigned row = min(SPLIT ? place % (TT * 32) : place, rows - 1);
+        const unsigned from = odd + row * x_blocks + min(a.chunks, part_of(set) * a.part) * 8;
+        scale_at[j] = int(from / 4 * 4 + dword * 4);
+        scale_to[j] = uniform(kStages * kStageBytes + copy * 256);
     }
+    auto stage_scales = [&](unsigned chunk, unsigned slot) {  // of the four chunks from `chunk`
+#pragma unroll
+        for (int j = 0; j < kScaleCopies; ++j)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                xscales,
+                (__attribute__((address_space(3))) void*)(lds + scale_to[j] + slot * kScaleBytes),
+                4, scale_at[j] + int(chunk * 8), 0, 0, 0);
+        issue_order();
+    };
     auto stage = [&](unsigned chunk, unsigned slot) {  // chunk of the part
         uint8_t* to = lds + slot * kStageBytes;
 #pragma unroll
         for (int j = 0; j < TT; ++j) {
             const int at = chunk * 8 < x_limit[j] ? x_at[j] + int(chunk * 128) : kOutside;
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                xs, (__attribute__((address_space(3))) void*)(to + (j * 8 + wave) * 1024), 16, at,
-                0, 0, 0);
+                xs, (__attribute__((address_space(3))) void*)(to + (j * kWaves + wave) * 1024),
+                16, at, 0, 0, 0);
         }
-#pragma unroll
-        for (int j = 0; j < kScaleCopies; ++j)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                xscales,
-                (__attribute__((address_space(3))) void*)(lds + kStages * kStageBytes +
-                                                          slot * (TT * 1024) +
-                                                          (j * 8 + wave) % (4 * TT) * 256),
-                4, scale_at[j] + int(chunk * 8), 0, 0, 0);
         issue_order();
     };
 
@@ -623,7 +710,7 @@ __global__ __launch_bounds__(512, 2) void gemm_kernel(Gemm a) {
         else
             scales_buf[t] = buffer(s + g * scale_groups * 256, there ? scale_groups * 256 : 0);
     }
-    constexpr int kAhead = 4;
+    constexpr int kAhead = OPS == kTransposed ? 2 : 4;  // steps (registers for two are left)
     struct Codes {
         u4 w[2];
         u4 s[OPS == kTransposed ? 2 : 1];
@@ -681,7 +768,28 @@ __global__ __launch_bounds__(512, 2) void gemm_kernel(Gemm a) {
 
     Codes codes[kAhead];
     Scales scales, next;
+    // the x operands of a chunk's step S, and (bf16) the chunk's weights of it
+    auto read_x = [&]<int S>(const uint8_t* buf, u4 (&v)[TT]) {
+#pragma unroll
+        for (int t = 0; t < TT; ++t)
+            v[t] = x_operand(buf, t, OPS == kFp4 ? 2 * S + h : 4 * h + S);
+    };
+    auto decode_w = [&]<int C, int S>(bf16x8 (&v)[2]) {
+        if constexpr (OPS == kTransposed) {
+            const unsigned cw[2] = {codes[C % kAhead].w[S / 2][2 * (S % 2)],
+                                    codes[C % kAhead].w[S / 2][2 * (S % 2) + 1]};
+            const unsigned sw[2] = {codes[C % kAhead].s[S / 2][2 * (S % 2)],
+                                    codes[C % kAhead].s[S / 2][2 * (S % 2) + 1]};
+            decode8_pair(cw, sw, v[0], v[1]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                v[i] = decode8(codes[C % kAhead].w[i][S], scale_of(scales.w[i], C));
+        }
+    };
     issue_order();
+    if constexpr (OPS == kFp4)
+        stage_scales(0, 0);
     stage(0, 0);
     stage(1, 1);
     stage(2, 2);
@@ -694,16 +802,20 @@ __global__ __launch_bounds__(512, 2) void gemm_kernel(Gemm a) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // fewer loads than the loop counts on
         // (32 rows on, a row's bytes start the same)
         const unsigned scale_shift = (odd + lane % 32 * x_blocks) % 4;
-        // (two chunks a turn: their scales stay in registers of their own, and are put in
-        // order only where they are used, so that no load is waited for where it is issued)
-        for (unsigned c0 = 0; c0 < a.part; c0 += 2) {
-            static_for<2>([&]<int C>() {
-                arrive.template operator()<2 * (TT + kScaleCopies) + 3 * kCodeLoads + 4>();
-                const unsigned slot = c0 % kStages + C;
-                const uint8_t* buf = x_lane + slot * kStageBytes;
-                Scales& now = C ? next : scales;
-                load_scales(begin_step + 4 * (c0 + C + 1), C ? scales : next);
-                stage(c0 + C + 3, (slot + 3) % kStages);
+        for (unsigned c0 = 0; c0 < a.part; c0 += 4) {
+            static_for<4>([&]<int C>() {
+                // (the next four chunks' scales go out ahead of chunk 0 of them)
+                constexpr int kScalesBehind = C == 2 || C == 3 ? kScaleCopies : 0;
+                arrive.template operator()<2 * TT + kScalesBehind + 3 * kCodeLoads + 4>();
+                const uint8_t* buf = x_lane + C * kStageBytes;
+                Scales& now = C % 2 ? next : scales;
+                load_scales(begin_step + 4 * (c0 + C + 1), C % 2 ? scales : next);
+                const unsigned group = c0 / 4 % 2;
+                if constexpr (C == 1)
+                    stage_scales(c0 + 4, 1 - group);
+                stage(c0 + C + 3, (C + 3) % kStages);
+                // (chunks past the part's end multiply nothing, but every load is issued)
+                const bool active = c0 + C < a.part;
                 // a row's eight scales, those past its end (the next row's, or none) as zero;
                 // the lane's half has every other one
                 const unsigned block = (begin + c0 + C) * 8;
@@ -711,26 +823,32 @@ __global__ __launch_bounds__(512, 2) void gemm_kernel(Gemm a) {
                 unsigned xs_now[TT];
 #pragma unroll
                 for (int t = 0; t < TT; ++t) {
-                    const u4 v = *reinterpret_cast<const u4*>(
-                        lds + kStages * kStageBytes + slot * (TT * 1024) +
-                        (kg * (TT * 32) + t * 32 + lane % 32) * 16);
-                    uint64_t bytes = uint64_t(__builtin_amdgcn_alignbyte(v.z, v.y, scale_shift))
-                                         << 32 |
-                                     __builtin_amdgcn_alignbyte(v.y, v.x, scale_shift);
+                    const auto* at = reinterpret_cast<const unsigned*>(
+                        lds + kStages * kStageBytes + group * kScaleBytes +
+                        (kg * (TT * 32) + t * 32 + lane % 32) * 40 + C * 8);
+                    const uint2 v = *reinterpret_cast<const uint2*>(at);
+                    uint64_t bytes =
+                        uint64_t(__builtin_amdgcn_alignbyte(at[2], v.y, scale_shift)) << 32 |
+                        __builtin_amdgcn_alignbyte(v.y, v.x, scale_shift);
                     if (there < 8)
                         bytes &= (uint64_t(1) << (8 * there)) - 1;
                     xs_now[t] = __builtin_amdgcn_perm(unsigned(bytes >> 32), unsigned(bytes),
                                                       h ? 0x07050301u : 0x06040200u);
                 }
+                u4 xv[2][TT];  // a step's operands are read while the one before multiplies
+                read_x.template operator()<0>(buf, xv[0]);
                 static_for<4>([&]<int S>() {
+                    if (active) {
+                        if constexpr (S < 3)
+                            read_x.template operator()<S + 1>(buf, xv[(S + 1) % 2]);
+                        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int t = 0; t < TT; ++t) {
-                        const i32x8 xv = fp4_operand(x_operand(buf, t, 2 * S + h));
+                        for (int t = 0; t < TT; ++t)
 #pragma unroll
-                        for (int i = 0; i < 2; ++i)
-                            acc[i][t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-                                fp4_operand(codes[S].w[i]), xv, acc[i][t], 4, 4, S,
-                                int(now.w[i]), S, int(xs_now[t]));
+                            for (int i = 0; i < 2; ++i)
+                                acc[i][t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+                                    fp4_operand(codes[S].w[i]), fp4_operand(xv[S % 2][t]),
+                                    acc[i][t], 4, 4, S, int(now.w[i]), S, int(xs_now[t]));
                     }
                     issue_order();
                     load_codes(begin_step + 4 * (c0 + C + 1) + S, codes[S]);
@@ -746,30 +864,26 @@ __global__ __launch_bounds__(512, 2) void gemm_kernel(Gemm a) {
                 stage(c0 + C + 3, (C + 3) % kStages);
                 if constexpr (C == 0)
                     load_scales(begin_step + c0 + 4, next);
+                u4 xv[2][TT];  // operands are read, and weights decoded, a step ahead
+                bf16x8 wv[2][2];
+                read_x.template operator()<0>(buf, xv[0]);
+                decode_w.template operator()<C, 0>(wv[0]);
                 static_for<4>([&]<int S>() {
-                    bf16x8 wv[2];
-                    if constexpr (OPS == kTransposed) {
-                        const unsigned cw[2] = {codes[C].w[S / 2][2 * (S % 2)],
-                                                codes[C].w[S / 2][2 * (S % 2) + 1]};
-                        const unsigned sw[2] = {codes[C].s[S / 2][2 * (S % 2)],
-                                                codes[C].s[S / 2][2 * (S % 2) + 1]};
-                        decode8_pair(cw, sw, wv[0], wv[1]);
-                    } else {
+                    if constexpr (S < 3)
+                        read_x.template operator()<S + 1>(buf, xv[(S + 1) % 2]);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if constexpr (S < 3)
+                        decode_w.template operator()<C, S + 1>(wv[(S + 1) % 2]);
+#pragma unroll
+                    for (int t = 0; t < TT; ++t)
 #pragma unroll
                         for (int i = 0; i < 2; ++i)
-                            wv[i] = decode8(codes[C].w[i][S], scale_of(scales.w[i], C));
-                    }
-#pragma unroll
-                    for (int t = 0; t < TT; ++t) {
-                        const bf16x8 xv = __builtin_bit_cast(bf16x8, x_operand(buf, t, 4 * h + S));
-#pragma unroll
-                        for (int i = 0; i < 2; ++i)
-                            acc[i][t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wv[i], xv,
-                                                                               acc[i][t], 0, 0, 0);
-                    }
+                            acc[i][t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                                wv[S % 2][i], __builtin_bit_cast(bf16x8, xv[S % 2][t]),
+                                acc[i][t], 0, 0, 0);
                 });
                 issue_order();
-                load_codes(begin_step + c0 + C + kAhead, codes[C]);
+                load_codes(begin_step + c0 + C + kAhead, codes[C % kAhead]);
             });
             scales = next;
         }
@@ -823,6 +937,10 @@ __global__ __launch_bounds__(512, 2) void gemm_kernel(Gemm a) {
                     }
                 }
     }
+    // (SPLIT: of the tiles handed to this wavefront, which it alone read)
+    uint8_t* patch =
+        SPLIT ? lds + (rg * (TT > 1 ? 2 : 1) + (TT > 1 ? 1 - kg : 0)) * (kOwn * 8192)
+              : lds + wave * kPatchBytes;
     const unsigned first_tile =
         (first_row / 32) + (SPLIT ? own : kg * TT);  // of 32 rows of x, the wavefront's first
 #pragma unroll
@@ -842,7 +960,7 @@ __global__ __launch_bounds__(512, 2) void gemm_kernel(Gemm a) {
                         to[(i * 4 + j) * 64] = quad_of(acc[i][t], j);
             }
         } else {
-            store_tiles<OUT>(a.out, G, T * 32 + lane % 32, h, acc[0][t], acc[1][t]);
+            store_tiles<OUT>(a.out, G, T, patch, acc[0][t], acc[1][t]);
         }
     }
 }
@@ -990,7 +1108,7 @@ size_t partial_bytes(const Plan& p, size_t m) {
 template <int TT, bool SPLIT, int OPS, int OUT>
 int launch_gemm(const Gemm& a, const Plan& p, hipStream_t st) {
     const auto f = gemm_kernel<TT, SPLIT, OPS, OUT>;
-    constexpr int kLds = kStages * TT * (OPS == kFp4 ? 9216 : 8192);
+    constexpr int kLds = kStages * TT * 8192 + (OPS == kFp4 ? 2 * TT * 64 * 40 : 0);
     if constexpr (kLds > 64 * 1024) {
         static std::atomic<uint64_t> configured{0};  // devices whose attribute is set
         int device = 0;
