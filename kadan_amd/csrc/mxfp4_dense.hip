@@ -408,83 +408,154 @@ __device__ __forceinline__ void store_tiles(const Target& t, unsigned G, unsigne
 
 // ------------------------------------------------------------------ a few rows of x
 //
-// One workgroup takes 16 matrix rows (both matrices' for the gated projection) and all of
-// K, in units of 128 values that its wavefronts take in turn.  Per unit a lane holds 32
-// values of one matrix row (lane r + 16q: row r, values 128t + 32q ..) and of one row of x,
-// so four v_mfma_f32_16x16x32_bf16 multiply the unit without moving a value between lanes:
-// the sum over K may run in any order.  Weights are read once, as two 256-byte runs of a
-// block per unit.
+// One workgroup takes R tiles of 16 matrix rows (of both matrices for the gated projection)
+// and all of K, a run of 128-value units to each wavefront.  Per unit a lane holds 32 values
+// of one matrix row (lane r + 16q: row r, values 128t + 32q ..) and of one row of x, so four
+// v_mfma_f32_16x16x32_bf16 multiply the unit without moving a value between lanes: the sum
+// over K may run in any order.  Weights are read once, whole lines (R == 2: whole 1 KB
+// blocks), and not kept in the caches.
+//
+// STAGED: x, up to kStagedBytes, passes through LDS, requested before the weights (a compute
+// unit's loads return in order); otherwise every wavefront reads its operands of x itself.
 
 struct Decode {
     const uint8_t *w0, *w1;
     const uint8_t* x;         // bf16 rows, or MXFP4 blocks
     const uint8_t* x_scales;  // MXFP4 scales
     unsigned x_stride;        // bytes
-    unsigned k, steps, groups;
+    unsigned k, steps, groups, units;  // units of a wavefront
     Target out;
 };
 
 constexpr int kOutside = 0x7ffffff0;  // past any buffer's range: such loads return zeros
+constexpr unsigned kStagedBytes = 32 * 1024;
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const uint8_t* p, unsigned bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, int(bytes), 0x00027000);
 }
 
+template <int POLICY = 0>
 __device__ __forceinline__ u4 load_b128(const __amdgpu_buffer_rsrc_t& r, int at) {
-    const auto v = __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0);
+    const auto v = __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, POLICY);
     return u4{unsigned(v[0]), unsigned(v[1]), unsigned(v[2]), unsigned(v[3])};
 }
 
-// The wavefronts' partial results of a workgroup: [wavefront][tile][lane].
-template <int TB, bool GATED, bool FP4, int OUT>
+// Bytes between the rows of a staged x: 16 more than a row has, so that rows start in
+// different banks.
+__host__ __device__ inline unsigned staged_pitch(unsigned row_bytes) {
+    return row_bytes + 16;
+}
+
+template <int R, int TB, bool GATED, bool FP4, bool STAGED, int OUT>
 __global__ __launch_bounds__(1024) void decode_kernel(Decode a) {
     extern __shared__ __align__(16) uint8_t lds[];
-    auto* red = reinterpret_cast<f32x4*>(lds);
-    const unsigned lane = threadIdx.x % 64, wave = threadIdx.x / 64, waves = blockDim.x / 64;
+    constexpr int kNt = 2;  // cache policy of loads that nothing reads again
+    constexpr int TILES = GATED ? 2 * R : R;
+    constexpr int kBatch = TB == 1 ? 4 : 2;
+    constexpr int kX = FP4 ? 1 : 4;
+    const unsigned lane = threadIdx.x % 64, waves = blockDim.x / 64;
+    const unsigned wave = unsigned(__builtin_amdgcn_readfirstlane(int(threadIdx.x / 64)));
     const unsigned r = lane % 16, q = lane / 16;
     const unsigned first_row = blockIdx.y * (16 * TB), rows = min(a.out.m - first_row, 16u * TB);
-    const unsigned group = blockIdx.x / 2, row = 16 * (blockIdx.x % 2) + r;
-    const unsigned share = GATED ? waves / 2 : waves;  // wavefronts on one matrix
-    const uint8_t* w = GATED && wave >= share ? a.w1 : a.w0;
-    const unsigned first = wave % share, units = (a.k + 127) / 128;
-    const unsigned scale_groups = (a.steps + 3) / 4;
-    const auto codes = buffer(w + size_t(group) * a.steps * 1024, a.steps * 1024);
-    const auto scales = buffer(w + size_t(a.groups) * a.steps * 1024 +
-                                   size_t(group) * scale_groups * 256,
-                               scale_groups * 256);
-    const unsigned lane_codes = (q / 2) * 1024 + (row + 32 * (q % 2)) * 16;
-    const unsigned lane_scales = (row + 32 * (q % 2)) * 4;
     const unsigned row_bytes = FP4 ? a.k / 2 : a.k * 2;
     const auto xs = buffer(a.x + size_t(first_row) * a.x_stride,
                            (rows - 1) * a.x_stride + row_bytes);
     const auto xscales = buffer(a.x_scales + size_t(first_row) * (a.k / 32),
                                 FP4 ? rows * (a.k / 32) : 0);
 
-    f32x4 acc[TB] = {};
-    constexpr int kBatch = TB == 1 ? 4 : 2;
-    constexpr int kX = FP4 ? 1 : 4;
-    for (unsigned t0 = first; t0 < units; t0 += kBatch * share) {
-        u4 c[kBatch], x[kBatch][TB][kX];
-        unsigned s[kBatch], xb[kBatch][TB];
+    constexpr unsigned kPieces = kStagedBytes / 16 / 256;  // of a thread, at 256 threads
+    u4 piece[STAGED ? kPieces : 1];
+    const unsigned row_pieces = row_bytes / 16, pieces = rows * row_pieces;
+    if constexpr (STAGED) {
 #pragma unroll
-        for (int b = 0; b < kBatch; ++b) {
-            const unsigned t = t0 + b * share;  // past the last unit: zeros
-            c[b] = load_b128(codes, int(t * 2048 + lane_codes));
-            s[b] = __builtin_amdgcn_raw_buffer_load_b32(scales, int(t / 2 * 256 + lane_scales), 0,
-                                                        0);
+        for (unsigned j = 0; j < kPieces; ++j) {
+            const unsigned i = j * blockDim.x + threadIdx.x;
+            if (j * blockDim.x < pieces)
+                piece[j] = load_b128(
+                    xs, i < pieces ? int(i / row_pieces * a.x_stride + i % row_pieces * 16)
+                                   : kOutside);
         }
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    }
+
+    // tile i: rows 16 (R * blockIdx.x + i % R) .. of matrix i / R
+    const unsigned scale_groups = (a.steps + 3) / 4;
+    __amdgpu_buffer_rsrc_t codes[GATED ? 2 : 1], scales[GATED ? 2 : 1];
+    const unsigned group = R == 2 ? blockIdx.x : blockIdx.x / 2;
+#pragma unroll
+    for (int i = 0; i < (GATED ? 2 : 1); ++i) {
+        const uint8_t* w = i ? a.w1 : a.w0;
+        codes[i] = buffer(w + size_t(group) * a.steps * 1024, a.steps * 1024);
+        scales[i] = buffer(w + size_t(a.groups) * a.steps * 1024 +
+                               size_t(group) * scale_groups * 256,
+                           scale_groups * 256);
+    }
+    const unsigned block_row = 16 * (R == 2 ? 0 : blockIdx.x % 2) + r + 32 * (q % 2);
+    const unsigned lane_codes = (q / 2) * 1024 + block_row * 16, lane_scales = block_row * 4;
+    // (an even number of units: a dword of scales is two)
+    const unsigned begin = wave * a.units, end = begin + a.units;
+    u4 c[kBatch][TILES];
+    unsigned s[kBatch / 2][TILES];
+    auto load = [&](unsigned t0) {  // units past K, or past the wavefront's run, are zeros
+#pragma unroll
+        for (int i = 0; i < TILES; ++i) {
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b)
+                c[b][i] = load_b128<kNt>(
+                    codes[i / R],
+                    t0 + b < end ? int((t0 + b) * 2048 + lane_codes + i % R * 256) : kOutside);
+#pragma unroll
+            for (int b = 0; b < kBatch; b += 2)
+                s[b / 2][i] = __builtin_amdgcn_raw_buffer_load_b32(
+                    scales[i / R], int((t0 + b) / 2 * 256 + lane_scales + i % R * 64), 0, kNt);
+        }
+    };
+    load(begin);
+    const unsigned pitch = staged_pitch(row_bytes);
+    if constexpr (STAGED) {
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (unsigned j = 0; j < kPieces; ++j) {
+            const unsigned i = j * blockDim.x + threadIdx.x;
+            if (i < pieces)
+                *reinterpret_cast<u4*>(lds + i / row_pieces * pitch + i % row_pieces * 16) =
+                    piece[j];
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the weights stay in flight)
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    }
+
+    f32x4 acc[TILES][TB] = {};
+    const unsigned staged_row = min(r, rows - 1) * pitch;  // (others' results are not stored)
+    for (unsigned t0 = begin; t0 < end; t0 += kBatch) {
+        if (t0 != begin)
+            load(t0);
+        u4 x[kBatch][TB][kX];
+        unsigned xb[kBatch][TB];
 #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
-            const unsigned t = t0 + b * share;
+            const unsigned t = t0 + b;
+            const bool inside = 128 * t + 32 * q < a.k;
 #pragma unroll
             for (int i = 0; i < TB; ++i) {
                 const unsigned token = r + 16 * i;
-                const bool there = token < rows && 128 * t + 32 * q < a.k;
-                if constexpr (FP4) {
-                    x[b][i][0] =
-                        load_b128(xs, there ? int(token * a.x_stride + (4 * t + q) * 16) : kOutside);
+                const bool there = token < rows && inside;
+                if constexpr (FP4)
                     xb[b][i] = __builtin_amdgcn_raw_buffer_load_b8(
                         xscales, there ? int(token * (a.k / 32) + 4 * t + q) : kOutside, 0, 0);
+                if constexpr (STAGED) {
+#pragma unroll
+                    for (int d = 0; d < kX; ++d) {
+                        const unsigned at = FP4 ? (4 * t + q) * 16 : (128 * t + 32 * q + 8 * d) * 2;
+                        const u4 v = *reinterpret_cast<const u4*>(
+                            lds + staged_row + (inside ? at : 0));
+                        x[b][i][d] = inside ? v : u4{0, 0, 0, 0};
+                    }
+                } else if constexpr (FP4) {
+                    x[b][i][0] =
+                        load_b128(xs, there ? int(token * a.x_stride + (4 * t + q) * 16) : kOutside);
                 } else {
                     const int at = there ? int(token * a.x_stride + (128 * t + 32 * q) * 2)
                                          : kOutside - 64;
@@ -496,41 +567,56 @@ __global__ __launch_bounds__(1024) void decode_kernel(Decode a) {
         }
 #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
-            const unsigned t = t0 + b * share;
-            const float ws = scale_of(s[b], 2 * (t % 2) + q / 2);
+            float ws[TILES];
+#pragma unroll
+            for (int i = 0; i < TILES; ++i)  // (t0 is even)
+                ws[i] = scale_of(s[b / 2][i], 2 * (b % 2) + q / 2);
 #pragma unroll
             for (int d = 0; d < 4; ++d) {
-                const bf16x8 wv = decode8(c[b][d], ws);
+                bf16x8 xv[TB];
 #pragma unroll
                 for (int i = 0; i < TB; ++i) {
-                    bf16x8 xv;
                     if constexpr (FP4)
-                        xv = decode8(x[b][i][0][d], scale_of(xb[b][i], 0));
+                        xv[i] = decode8(x[b][i][0][d], scale_of(xb[b][i], 0));
                     else
-                        xv = __builtin_bit_cast(bf16x8, x[b][i][d]);
-                    acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, xv, acc[i], 0, 0, 0);
+                        xv[i] = __builtin_bit_cast(bf16x8, x[b][i][d]);
+                }
+#pragma unroll
+                for (int j = 0; j < TILES; ++j) {
+                    const bf16x8 wv = decode8(c[b][j][d], ws[j]);
+#pragma unroll
+                    for (int i = 0; i < TB; ++i)
+                        acc[j][i] =
+                            __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, xv[i], acc[j][i], 0, 0, 0);
                 }
             }
         }
     }
+    // the wavefronts' sums meet in wavefront order
+    if constexpr (STAGED)
+        __syncthreads();
+    auto* red = reinterpret_cast<f32x4*>(lds);
 #pragma unroll
-    for (int i = 0; i < TB; ++i)
-        red[(wave * TB + i) * 64 + lane] = acc[i];
+    for (int j = 0; j < TILES; ++j)
+#pragma unroll
+        for (int i = 0; i < TB; ++i)
+            red[((wave * TILES + j) * TB + i) * 64 + lane] = acc[j][i];
     __syncthreads();
-    if (wave >= TB)
+    if (wave >= R * TB)
         return;
-    const unsigned token = first_row + 16 * wave + r, at = blockIdx.x * 16 + 4 * q;
+    const unsigned tile = wave / TB, tb = wave % TB;
+    const unsigned token = first_row + 16 * tb + r, at = (blockIdx.x * R + tile) * 16 + 4 * q;
     if (token >= a.out.m)
         return;
-    auto total = [&](unsigned from) {
-        f32x4 sum = red[(from * TB + wave) * 64 + lane];
-        for (unsigned i = 1; i < share; ++i)
-            sum += red[((from + i) * TB + wave) * 64 + lane];
+    auto total = [&](unsigned j) {
+        f32x4 sum = red[(j * TB + tb) * 64 + lane];
+        for (unsigned i = 1; i < waves; ++i)
+            sum += red[((i * TILES + j) * TB + tb) * 64 + lane];
         return sum;
     };
-    f32x4 v = total(0);
+    f32x4 v = total(tile);
     if constexpr (GATED) {
-        const f32x4 u = total(share);
+        const f32x4 u = total(R + tile);
         v = f32x4{gate_value(v.x, u.x), gate_value(v.y, u.y), gate_value(v.z, u.z),
                   gate_value(v.w, u.w)};
     }
@@ -1161,22 +1247,37 @@ template <int OPS, int OUT> int run_gemm(Gemm a, const Plan& p, void* workspace,
     return KDQ_OK;
 }
 
-template <int TB, bool GATED, bool FP4, int OUT>
-int launch_decode(const Decode& a, hipStream_t st) {
-    const unsigned units = (a.k + 127) / 128;
-    const unsigned per = GATED ? 2 : 1;
-    const unsigned waves = per * (units <= 8 ? 2 : units <= 16 ? 4 : units <= 64 || GATED ? 8 : 16);
-    hipLaunchKernelGGL((decode_kernel<TB, GATED, FP4, OUT>),
-                       dim3(unsigned(ceil_div(a.out.n, 16)),
+template <int R, int TB, bool GATED, bool FP4, bool STAGED, int OUT>
+int launch_decode(Decode a, unsigned waves, hipStream_t st) {
+    const unsigned tiles = GATED ? 2 * R : R;
+    const unsigned row_bytes = FP4 ? a.k / 2 : a.k * 2;
+    unsigned bytes = waves * tiles * TB * 1024;
+    if (STAGED)
+        bytes = std::max(bytes, std::min(a.out.m, 16u * TB) * staged_pitch(row_bytes));
+    hipLaunchKernelGGL((decode_kernel<R, TB, GATED, FP4, STAGED, OUT>),
+                       dim3(unsigned(ceil_div(a.out.n, 16 * R)),
                             unsigned(ceil_div(a.out.m, 16 * TB))),
-                       dim3(waves * 64), waves * TB * 1024, st, a);
+                       dim3(waves * 64), bytes, st, a);
     KDQ_HIP(hipGetLastError());
     return KDQ_OK;
 }
 
-template <bool GATED, bool FP4, int OUT> int run_decode(const Decode& a, hipStream_t st) {
-    return a.out.m <= 16 ? launch_decode<1, GATED, FP4, OUT>(a, st)
-                         : launch_decode<2, GATED, FP4, OUT>(a, st);
+template <bool GATED, bool FP4, int OUT> int run_decode(Decode a, hipStream_t st) {
+    const unsigned units = (a.k + 127) / 128;
+    // whole blocks of 32 rows a workgroup where those fill the compute units
+    const bool wide = a.groups >= compute_units();
+    unsigned waves = units <= 8 ? 2 : units <= 16 ? 4 : units <= 64 || wide ? 8 : 16;
+    a.units = (unsigned(ceil_div(units, waves)) + 1) / 2 * 2;
+    if (a.out.m > 16)
+        return wide ? launch_decode<2, 2, GATED, FP4, false, OUT>(a, waves, st)
+                    : launch_decode<1, 2, GATED, FP4, false, OUT>(a, waves, st);
+    const bool staged = a.out.m * staged_pitch(FP4 ? a.k / 2 : a.k * 2) <= kStagedBytes &&
+                        a.out.m * (FP4 ? a.k / 2 : a.k * 2) <= waves * 64 * 16 * 8;
+    if (staged)
+        return wide ? launch_decode<2, 1, GATED, FP4, true, OUT>(a, waves, st)
+                    : launch_decode<1, 1, GATED, FP4, true, OUT>(a, waves, st);
+    return wide ? launch_decode<2, 1, GATED, FP4, false, OUT>(a, waves, st)
+                : launch_decode<1, 1, GATED, FP4, false, OUT>(a, waves, st);
 }
 
 Plan plan_product(size_t m, size_t n, size_t k, bool fp4) {
@@ -1316,7 +1417,7 @@ template <int OPS> int product(Gemm g, const Plan& p, int type, void* workspace,
     if (p.decode) {
         Decode d{g.w0, nullptr, g.x, g.x_scales, g.x_stride,
                  unsigned(OPS == kFp4 ? g.segments * 32 : g.segments * 8), g.steps, g.groups,
-                 g.out};
+                 0, g.out};
         constexpr bool kQ = OPS == kFp4;
         return type == KDQ_F32 ? run_decode<false, kQ, kOutF32>(d, st)
                                : run_decode<false, kQ, kOutBf16>(d, st);
@@ -1436,7 +1537,7 @@ extern "C" int kdq_mxfp4_gated(const uint16_t* x_bf16, size_t x_stride, size_t m
     if (p.decode)
         return run_decode<true, false, kOutBf16>(
             {gate_packed, up_packed, reinterpret_cast<const uint8_t*>(x_bf16), nullptr,
-             unsigned(x_stride * 2), unsigned(k), unsigned(f.steps), unsigned(f.groups), t},
+             unsigned(x_stride * 2), unsigned(k), unsigned(f.steps), unsigned(f.groups), 0, t},
             st);
     Gemm g{};
     g.w0 = gate_packed;

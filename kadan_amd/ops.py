@@ -377,12 +377,14 @@ def moe_mxfp4_packed(x_bf16: torch.Tensor, logits: torch.Tensor, top_k: int, int
     return (out, *extra) if routing else out
 
 
-def _here(*tensors: torch.Tensor) -> None:
-    """Kernels run on the current device's current stream: its tensors only."""
+def _stream_for(*tensors: torch.Tensor) -> int:
+    """The current device's current stream, where every tensor is on that device."""
     device = torch.cuda.current_device()
     for t in tensors:
         if t.get_device() != device:
             raise ValueError("every tensor must be on the current device")
+    return (torch.cuda.current_stream().cuda_stream if _raw_stream is None
+            else _raw_stream(device))
 
 
 def _row_stride(t: torch.Tensor, dtype, name: str, multiple: int = 8) -> int:
@@ -401,72 +403,80 @@ def _row_stride(t: torch.Tensor, dtype, name: str, multiple: int = 8) -> int:
     return row
 
 
-_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}  # KDQ_F32, _F16, _BF16
+_BF16 = torch.bfloat16
+_TYPES = {torch.float32: 0, torch.float16: 1, _BF16: 30}  # KDQ_F32, KDQ_F16, KDQ_BF16
 
 
 def _type(dtype) -> int:
-    try:
-        return _TYPES[dtype]
-    except KeyError:
-        raise ValueError(f"no MXFP4 operator takes {dtype}") from None
+    kind = _TYPES.get(dtype)
+    if kind is None:
+        raise ValueError(f"no MXFP4 operator takes {dtype}")
+    return kind
 
 
 def _blocks(blocks: torch.Tensor, scales: torch.Tensor) -> tuple[int, int]:
     """Rows and values of a row of an MXFP4 matrix."""
     _need(blocks, torch.uint8, "blocks")
     _need(scales, torch.uint8, "scales")
-    if (blocks.dim() != 2 or scales.dim() != 2 or blocks.shape[0] != scales.shape[0]
-            or blocks.shape[1] != 16 * scales.shape[1]):
-        raise ValueError("expected blocks [rows, cols/2] and scales [rows, cols/32]")
-    return blocks.shape[0], 2 * blocks.shape[1]
+    if blocks.dim() == 2 and scales.dim() == 2:
+        rows, width = blocks.shape
+        if scales.shape == (rows, width // 16) and width % 16 == 0:
+            return rows, 2 * width
+    raise ValueError("expected blocks [rows, cols/2] and scales [rows, cols/32]")
 
 
+# Device bytes that a call's matrices and workspace take.  (A decode product takes 6-8 us on
+# the device and its wrapper must not take longer, so they are asked for once.)
 @functools.lru_cache(maxsize=4096, typed=True)
 def _mxfp4_size(function: str, *sizes: int) -> int:
     return int(getattr(lib(), function)(*sizes))
 
 
-def _scratch(size: int, device) -> tuple[torch.Tensor | None, int | None]:
-    """A call's workspace: torch's allocator keeps it to the current stream (and to a
-    graph's own pool under capture), so calls share none.  Keep the tensor until the call
-    is enqueued."""
-    if not size:
-        return None, None
-    t = torch.empty(size, dtype=torch.uint8, device=device)
-    return t, t.data_ptr()
+@functools.lru_cache(maxsize=4096, typed=True)
+def _mxfp4_sizes(matrix: str, rows: int, cols: int, workspace: str, *sizes: int):
+    return _mxfp4_size(matrix, rows, cols), _mxfp4_size(workspace, *sizes)
 
 
-def _matrix(packed: torch.Tensor, function: str, rows: int, cols: int, name: str) -> int:
+_PACKED, _TRANSPOSED = "kdq_mxfp4_packed_bytes", "kdq_mxfp4_packed_transposed_bytes"
+
+
+def _matrix(packed: torch.Tensor, size: int, name: str) -> int:
     if packed.dtype != torch.uint8 or not packed.is_cuda or not packed.is_contiguous():
         raise ValueError(f"{name}: expected a packed uint8 device tensor")
-    if not rows or packed.numel() != _mxfp4_size(function, rows, cols):
-        raise ValueError(f"{name}: packed size does not match {rows} x {cols}")
+    if not size or packed.numel() != size:
+        raise ValueError(f"{name}: not the packed size of this call's matrix")
     return packed.data_ptr()
 
 
-def _output(out: torch.Tensor | None, rows: int, cols: int, dtype, device,
-            name: str) -> tuple[torch.Tensor, int]:
-    if out is None:
-        return torch.empty(rows, cols, dtype=dtype, device=device), cols
+def _output(out: torch.Tensor, rows: int, cols: int, dtype, name: str) -> int:
+    """Values from row to row of a given output."""
     if out.dim() != 2 or out.shape[0] != rows or out.shape[1] != cols:
         raise ValueError(f"{name}: expected [{rows}, {cols}]")
-    _here(out)
-    return out, _row_stride(out, dtype, name, 1)
+    return _row_stride(out, dtype, name, 1)
+
+
+def _scratch(size: int, device) -> torch.Tensor | None:
+    """A call's workspace: torch's allocator keeps it to the current stream (and to a
+    graph's own pool under capture), so calls share none.  Keep it until the call is
+    enqueued."""
+    return torch.empty(size, dtype=torch.uint8, device=device) if size else None
 
 
 def mxfp4_quantize(x: torch.Tensor, status: torch.Tensor | None = None):
     """fp32, fp16 or bf16 [rows, cols] (cols % 32 == 0) as MXFP4: blocks uint8
     [rows, cols/2] and scales uint8 [rows, cols/32] (kdq_mxfp4_quantize)."""
-    kind = _type(x.dtype)
-    stride = _row_stride(x, x.dtype, "x")
-    _here(x)
+    dtype = x.dtype
+    kind = _type(dtype)
+    stride = _row_stride(x, dtype, "x")
+    stream = _stream_for(x)
     rows, cols = x.shape
     if cols % 32:
         raise ValueError("x: a row must be whole blocks of 32 values")
-    blocks = torch.empty(rows, cols // 2, dtype=torch.uint8, device=x.device)
-    scales = torch.empty(rows, cols // 32, dtype=torch.uint8, device=x.device)
+    device = x.device
+    blocks = torch.empty(rows, cols // 2, dtype=torch.uint8, device=device)
+    scales = torch.empty(rows, cols // 32, dtype=torch.uint8, device=device)
     call("kdq_mxfp4_quantize", kind, x.data_ptr(), stride, rows, cols, blocks.data_ptr(),
-         scales.data_ptr(), _ptr(status), _stream())
+         scales.data_ptr(), _ptr(status), stream)
     return blocks, scales
 
 
@@ -475,14 +485,13 @@ def mxfp4_pack(blocks: torch.Tensor, scales: torch.Tensor,
     """An MXFP4 matrix in the form the products read (kdq_mxfp4_pack), or, ``transposed``,
     in the one that mxfp4_gated_backward reads (kdq_mxfp4_pack_transposed)."""
     rows, cols = _blocks(blocks, scales)
-    _here(blocks, scales)
-    name = "kdq_mxfp4_pack_transposed" if transposed else "kdq_mxfp4_pack"
-    size = _mxfp4_size("kdq_mxfp4_packed_transposed_bytes" if transposed
-                       else "kdq_mxfp4_packed_bytes", rows, cols)
+    stream = _stream_for(blocks, scales)
+    size = _mxfp4_size(_TRANSPOSED if transposed else _PACKED, rows, cols)
     if not size:
         raise ValueError(f"a matrix of {rows} x {cols} has no packed form")
     packed = torch.empty(size, dtype=torch.uint8, device=blocks.device)
-    call(name, blocks.data_ptr(), scales.data_ptr(), rows, cols, packed.data_ptr(), _stream())
+    call("kdq_mxfp4_pack_transposed" if transposed else "kdq_mxfp4_pack", blocks.data_ptr(),
+         scales.data_ptr(), rows, cols, packed.data_ptr(), stream)
     return packed
 
 
@@ -491,16 +500,21 @@ def mxfp4_product(x: torch.Tensor, packed: torch.Tensor, n_out: int,
                   out: torch.Tensor | None = None) -> torch.Tensor:
     """bf16 [m, k] times a packed MXFP4 matrix (mxfp4_pack) of n_out rows of k values ->
     fp32 or bf16 [m, n_out] (kdq_mxfp4_product)."""
-    stride = _row_stride(x, torch.bfloat16, "x")
-    _here(x, packed)
+    stride = _row_stride(x, _BF16, "x")
     m, k = x.shape
-    w = _matrix(packed, "kdq_mxfp4_packed_bytes", n_out, k, "packed")
-    y, y_stride = _output(out, m, n_out, dtype, x.device, "out")
-    size = _mxfp4_size("kdq_mxfp4_product_workspace", m, n_out, k, 0)
-    scratch, at = _scratch(size, x.device)
-    call("kdq_mxfp4_product", x.data_ptr(), stride, m, w, n_out, k, _type(dtype), y.data_ptr(),
-         y_stride, at, size, _stream())
-    return y
+    kind = _type(dtype)
+    weights, size = _mxfp4_sizes(_PACKED, n_out, k, "kdq_mxfp4_product_workspace", m, n_out, k, 0)
+    w = _matrix(packed, weights, "packed")
+    if out is None:
+        stream, y_stride = _stream_for(x, packed), n_out
+        out = torch.empty(m, n_out, dtype=dtype, device=x.device)
+    else:
+        y_stride = _output(out, m, n_out, dtype, "out")
+        stream = _stream_for(x, packed, out)
+    scratch = _scratch(size, x.device)
+    call("kdq_mxfp4_product", x.data_ptr(), stride, m, w, n_out, k, kind, out.data_ptr(),
+         y_stride, _ptr(scratch), size, stream)
+    return out
 
 
 def mxfp4_product_quantized(blocks: torch.Tensor, scales: torch.Tensor, packed: torch.Tensor,
@@ -509,14 +523,19 @@ def mxfp4_product_quantized(blocks: torch.Tensor, scales: torch.Tensor, packed: 
     """MXFP4 activations (mxfp4_quantize) times a packed MXFP4 matrix of n_out rows -> fp32
     or bf16 [m, n_out] (kdq_mxfp4_product_quantized)."""
     m, k = _blocks(blocks, scales)
-    _here(blocks, scales, packed)
-    w = _matrix(packed, "kdq_mxfp4_packed_bytes", n_out, k, "packed")
-    y, y_stride = _output(out, m, n_out, dtype, blocks.device, "out")
-    size = _mxfp4_size("kdq_mxfp4_product_workspace", m, n_out, k, 1)
-    scratch, at = _scratch(size, blocks.device)
+    kind = _type(dtype)
+    weights, size = _mxfp4_sizes(_PACKED, n_out, k, "kdq_mxfp4_product_workspace", m, n_out, k, 1)
+    w = _matrix(packed, weights, "packed")
+    if out is None:
+        stream, y_stride = _stream_for(blocks, scales, packed), n_out
+        out = torch.empty(m, n_out, dtype=dtype, device=blocks.device)
+    else:
+        y_stride = _output(out, m, n_out, dtype, "out")
+        stream = _stream_for(blocks, scales, packed, out)
+    scratch = _scratch(size, blocks.device)
     call("kdq_mxfp4_product_quantized", blocks.data_ptr(), scales.data_ptr(), m, w, n_out, k,
-         _type(dtype), y.data_ptr(), y_stride, at, size, _stream())
-    return y
+         kind, out.data_ptr(), y_stride, _ptr(scratch), size, stream)
+    return out
 
 
 def mxfp4_gated(x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, n_out: int,
@@ -525,29 +544,34 @@ def mxfp4_gated(x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, n_out: in
     n_out rows (n_out % 32 == 0) -> bf16 [m, n_out] (kdq_mxfp4_gated).  With ``save`` the
     pre-activations are kept for mxfp4_gated_backward, and (h, saved) returned: "bf16" as one
     tensor [m, 2 n_out], "q8" as int8 [m, 2 n_out] and fp32 scales [m, 2 n_out / 32]."""
-    stride = _row_stride(x, torch.bfloat16, "x")
-    _here(x, gate, up)
+    stride = _row_stride(x, _BF16, "x")
     if save not in (None, "bf16", "q8"):
         raise ValueError('save: None, "bf16" or "q8"')
     m, k = x.shape
     if n_out % 32:
         raise ValueError("n_out must be a multiple of 32")
-    wg = _matrix(gate, "kdq_mxfp4_packed_bytes", n_out, k, "gate")
-    wu = _matrix(up, "kdq_mxfp4_packed_bytes", n_out, k, "up")
-    h, h_stride = _output(out, m, n_out, torch.bfloat16, x.device, "out")
+    weights, size = _mxfp4_sizes(_PACKED, n_out, k, "kdq_mxfp4_gated_workspace", m, n_out, k,
+                                 0 if save is None else 1)
+    wg, wu = _matrix(gate, weights, "gate"), _matrix(up, weights, "up")
+    device = x.device
+    if out is None:
+        stream, h_stride = _stream_for(x, gate, up), n_out
+        out = torch.empty(m, n_out, dtype=_BF16, device=device)
+    else:
+        h_stride = _output(out, m, n_out, _BF16, "out")
+        stream = _stream_for(x, gate, up, out)
     saved = kept = codes = scales = None
     if save == "bf16":
-        saved = torch.empty(m, 2 * n_out, dtype=torch.bfloat16, device=x.device)
+        saved = torch.empty(m, 2 * n_out, dtype=_BF16, device=device)
         kept = saved.data_ptr()
     elif save == "q8":
-        saved = (torch.empty(m, 2 * n_out, dtype=torch.int8, device=x.device),
-                 torch.empty(m, n_out // 16, dtype=torch.float32, device=x.device))
+        saved = (torch.empty(m, 2 * n_out, dtype=torch.int8, device=device),
+                 torch.empty(m, n_out // 16, dtype=torch.float32, device=device))
         codes, scales = saved[0].data_ptr(), saved[1].data_ptr()
-    size = _mxfp4_size("kdq_mxfp4_gated_workspace", m, n_out, k, int(save is not None))
-    scratch, at = _scratch(size, x.device)
-    call("kdq_mxfp4_gated", x.data_ptr(), stride, m, wg, wu, n_out, k, h.data_ptr(), h_stride,
-         kept, codes, scales, at, size, _stream())
-    return h if save is None else (h, saved)
+    scratch = _scratch(size, device)
+    call("kdq_mxfp4_gated", x.data_ptr(), stride, m, wg, wu, n_out, k, out.data_ptr(), h_stride,
+         kept, codes, scales, _ptr(scratch), size, stream)
+    return out if save is None else (out, saved)
 
 
 def mxfp4_gated_backward(dh: torch.Tensor, saved, gate: torch.Tensor, up: torch.Tensor,
@@ -556,16 +580,16 @@ def mxfp4_gated_backward(dh: torch.Tensor, saved, gate: torch.Tensor, up: torch.
     from its forward pass, the matrices from mxfp4_pack(..., transposed=True) -> dx bf16
     [m, n_in] and the pre-activations' gradients bf16 [m, 2 n_out], gates then ups
     (kdq_mxfp4_gated_backward)."""
-    stride = _row_stride(dh, torch.bfloat16, "dh")
-    _here(dh, gate, up)
+    stride = _row_stride(dh, _BF16, "dh")
     m, n = dh.shape
     if n % 32 or n_in % 32 or not n_in:
         raise ValueError("n_out and n_in must be multiples of 32")
-    wg = _matrix(gate, "kdq_mxfp4_packed_transposed_bytes", n, n_in, "gate")
-    wu = _matrix(up, "kdq_mxfp4_packed_transposed_bytes", n, n_in, "up")
+    weights, size = _mxfp4_sizes(_TRANSPOSED, n, n_in, "kdq_mxfp4_gated_backward_workspace", m,
+                                 n, n_in)
+    wg, wu = _matrix(gate, weights, "gate"), _matrix(up, weights, "up")
     kept = codes = scales = None
     if isinstance(saved, torch.Tensor):
-        _need(saved, torch.bfloat16, "saved")
+        _need(saved, _BF16, "saved")
         parts = (saved,)
         kept = saved.data_ptr()
     else:
@@ -577,14 +601,18 @@ def mxfp4_gated_backward(dh: torch.Tensor, saved, gate: torch.Tensor, up: torch.
         codes, scales = q.data_ptr(), d.data_ptr()
     if parts[0].shape != (m, 2 * n):
         raise ValueError("saved: of another shape than dh")
-    _here(*parts)
-    dgu = torch.empty(m, 2 * n, dtype=torch.bfloat16, device=dh.device)
-    dx, dx_stride = _output(out, m, n_in, torch.bfloat16, dh.device, "out")
-    size = _mxfp4_size("kdq_mxfp4_gated_backward_workspace", m, n, n_in)
-    scratch, at = _scratch(size, dh.device)
+    device = dh.device
+    if out is None:
+        stream, dx_stride = _stream_for(dh, gate, up, *parts), n_in
+        out = torch.empty(m, n_in, dtype=_BF16, device=device)
+    else:
+        dx_stride = _output(out, m, n_in, _BF16, "out")
+        stream = _stream_for(dh, gate, up, out, *parts)
+    dgu = torch.empty(m, 2 * n, dtype=_BF16, device=device)
+    scratch = _scratch(size, device)
     call("kdq_mxfp4_gated_backward", dh.data_ptr(), stride, m, kept, codes, scales, wg, wu, n,
-         n_in, dgu.data_ptr(), dx.data_ptr(), dx_stride, at, size, _stream())
-    return dx, dgu
+         n_in, dgu.data_ptr(), out.data_ptr(), dx_stride, _ptr(scratch), size, stream)
+    return out, dgu
 
 
 def hbm_read(buffer: torch.Tensor, sink: torch.Tensor, workgroups: int,
