@@ -451,7 +451,8 @@ __global__ __launch_bounds__(1024) void decode_kernel(Decode a) {
     extern __shared__ __align__(16) uint8_t lds[];
     constexpr int kNt = 2;  // cache policy of loads that nothing reads again
     constexpr int TILES = GATED ? 2 * R : R;
-    constexpr int kBatch = TB == 1 ? 4 : 2;
+    constexpr int kBatch = TB == 1 ? 4 : TB == 2 ? 2 : 1;
+    constexpr int kScales = (kBatch + 1) / 2;  // dwords of scales
     constexpr int kX = FP4 ? 1 : 4;
     const unsigned lane = threadIdx.x % 64, waves = blockDim.x / 64;
     const unsigned wave = unsigned(__builtin_amdgcn_readfirstlane(int(threadIdx.x / 64)));
@@ -496,7 +497,7 @@ __global__ __launch_bounds__(1024) void decode_kernel(Decode a) {
     // (an even number of units: a dword of scales is two)
     const unsigned begin = wave * a.units, end = begin + a.units;
     u4 c[kBatch][TILES];
-    unsigned s[kBatch / 2][TILES];
+    unsigned s[kScales][TILES];
     auto load = [&](unsigned t0) {  // units past K, or past the wavefront's run, are zeros
 #pragma unroll
         for (int i = 0; i < TILES; ++i) {
@@ -506,9 +507,9 @@ __global__ __launch_bounds__(1024) void decode_kernel(Decode a) {
                     codes[i / R],
                     t0 + b < end ? int((t0 + b) * 2048 + lane_codes + i % R * 256) : kOutside);
 #pragma unroll
-            for (int b = 0; b < kBatch; b += 2)
-                s[b / 2][i] = __builtin_amdgcn_raw_buffer_load_b32(
-                    scales[i / R], int((t0 + b) / 2 * 256 + lane_scales + i % R * 64), 0, kNt);
+            for (int b = 0; b < kScales; ++b)
+                s[b][i] = __builtin_amdgcn_raw_buffer_load_b32(
+                    scales[i / R], int((t0 / 2 + b) * 256 + lane_scales + i % R * 64), 0, kNt);
         }
     };
     load(begin);
@@ -569,8 +570,8 @@ __global__ __launch_bounds__(1024) void decode_kernel(Decode a) {
         for (int b = 0; b < kBatch; ++b) {
             float ws[TILES];
 #pragma unroll
-            for (int i = 0; i < TILES; ++i)  // (t0 is even)
-                ws[i] = scale_of(s[b / 2][i], 2 * (b % 2) + q / 2);
+            for (int i = 0; i < TILES; ++i)  // (t0 is even, but for batches of one)
+                ws[i] = scale_of(s[b / 2][i], 2 * (kBatch == 1 ? t0 % 2 : b % 2) + q / 2);
 #pragma unroll
             for (int d = 0; d < 4; ++d) {
                 bf16x8 xv[TB];
@@ -602,28 +603,122 @@ __global__ __launch_bounds__(1024) void decode_kernel(Decode a) {
         for (int i = 0; i < TB; ++i)
             red[((wave * TILES + j) * TB + i) * 64 + lane] = acc[j][i];
     __syncthreads();
-    if (wave >= R * TB)
-        return;
-    const unsigned tile = wave / TB, tb = wave % TB;
-    const unsigned token = first_row + 16 * tb + r, at = (blockIdx.x * R + tile) * 16 + 4 * q;
-    if (token >= a.out.m)
-        return;
-    auto total = [&](unsigned j) {
+    auto total = [&](unsigned j, unsigned tb) {
         f32x4 sum = red[(j * TB + tb) * 64 + lane];
         for (unsigned i = 1; i < waves; ++i)
             sum += red[((i * TILES + j) * TB + tb) * 64 + lane];
         return sum;
     };
-    f32x4 v = total(tile);
-    if constexpr (GATED) {
-        const f32x4 u = total(R + tile);
-        v = f32x4{gate_value(v.x, u.x), gate_value(v.y, u.y), gate_value(v.z, u.z),
-                  gate_value(v.w, u.w)};
+    for (unsigned i = wave; i < R * TB; i += waves) {
+        const unsigned tile = i / TB, tb = i % TB;
+        const unsigned token = first_row + 16 * tb + r, at = (blockIdx.x * R + tile) * 16 + 4 * q;
+        if (token >= a.out.m)
+            continue;
+        f32x4 v = total(tile, tb);
+        if constexpr (GATED) {
+            const f32x4 u = total(R + tile, tb);
+            v = f32x4{gate_value(v.x, u.x), gate_value(v.y, u.y), gate_value(v.z, u.z),
+                      gate_value(v.w, u.w)};
+        }
+        if constexpr (OUT == kOutF32)
+            store4_f32(static_cast<float*>(a.out.y), a.out.stride, a.out.n, token, at, v);
+        else
+            store4_bf16(static_cast<uint16_t*>(a.out.y), a.out.stride, a.out.n, token, at, v);
     }
-    if constexpr (OUT == kOutF32)
-        store4_f32(static_cast<float*>(a.out.y), a.out.stride, a.out.n, token, at, v);
-    else
-        store4_bf16(static_cast<uint16_t*>(a.out.y), a.out.stride, a.out.n, token, at, v);
+}
+
+// The backward pass's product for a few rows: x = [dg | du], the matrices in the transposed
+// form.  A workgroup takes 32 columns (16 byte lanes e = blockIdx.x % 2 of a group, as a tile
+// of even and a tile of odd columns), half its wavefronts the gate's rows and half the up's,
+// in units of 128 rows: lane r + 16q holds byte lane r's rows 128t + 32q .. +31.
+template <int TB>
+__global__ __launch_bounds__(1024) void decode_t_kernel(Decode a) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    constexpr int kNt = 2;
+    constexpr int kBatch = TB == 1 ? 2 : 1;
+    const unsigned lane = threadIdx.x % 64, waves = blockDim.x / 64, share = waves / 2;
+    const unsigned wave = unsigned(__builtin_amdgcn_readfirstlane(int(threadIdx.x / 64)));
+    const unsigned r = lane % 16, q = lane / 16;
+    const unsigned group = blockIdx.x / 2, e = blockIdx.x % 2, matrix = wave / share;
+    const uint8_t* w = matrix ? a.w1 : a.w0;
+    const auto codes = buffer(w + size_t(group) * a.steps * 2048, a.steps * 2048);
+    const auto scales = buffer(w + size_t(a.groups) * a.steps * 2048 +
+                                   size_t(group) * a.steps * 128,
+                               a.steps * 128);
+    const unsigned first_row = blockIdx.y * (16 * TB), rows = min(a.out.m - first_row, 16u * TB);
+    const auto xs = buffer(a.x + size_t(first_row) * a.x_stride + matrix * (a.k * 2),
+                           (rows - 1) * a.x_stride + a.k * 2);
+    const unsigned lane_codes = (q / 2) * 2048 + (16 * e + r + 32 * (q % 2)) * 16;
+    const unsigned lane_scales = (q / 2) * 128 + (2 * (q % 2) + e) * 32;
+    const unsigned begin = wave % share * a.units, end = begin + a.units;
+    f32x4 acc[2][TB] = {};
+    for (unsigned t0 = begin; t0 < end; t0 += kBatch) {
+        u4 c[kBatch][2], s[kBatch][2], x[kBatch][TB][4];
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            const unsigned t = t0 + b;
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+                c[b][p] = load_b128<kNt>(
+                    codes, t < end ? int(t * 4096 + p * 1024 + lane_codes) : kOutside);
+                s[b][p] = load_b128(scales, int(t * 256 + lane_scales + 16 * p));
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            const unsigned from = 128 * (t0 + b) + 32 * q;
+#pragma unroll
+            for (int i = 0; i < TB; ++i) {
+                const unsigned token = r + 16 * i;
+                const int at = token < rows && from < a.k ? int(token * a.x_stride + from * 2)
+                                                          : kOutside - 64;
+#pragma unroll
+                for (int d = 0; d < 4; ++d)
+                    x[b][i][d] = load_b128(xs, at + 16 * d);
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b)
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                const unsigned cw[2] = {c[b][d / 2][2 * (d % 2)], c[b][d / 2][2 * (d % 2) + 1]};
+                const unsigned sw[2] = {s[b][d / 2][2 * (d % 2)], s[b][d / 2][2 * (d % 2) + 1]};
+                bf16x8 even, odd;
+                decode8_pair(cw, sw, even, odd);
+#pragma unroll
+                for (int i = 0; i < TB; ++i) {
+                    const bf16x8 xv = __builtin_bit_cast(bf16x8, x[b][i][d]);
+                    acc[0][i] =
+                        __builtin_amdgcn_mfma_f32_16x16x32_bf16(even, xv, acc[0][i], 0, 0, 0);
+                    acc[1][i] =
+                        __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd, xv, acc[1][i], 0, 0, 0);
+                }
+            }
+    }
+    auto* red = reinterpret_cast<f32x4*>(lds);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < TB; ++i)
+            red[((wave * 2 + j) * TB + i) * 64 + lane] = acc[j][i];
+    __syncthreads();
+    const unsigned col = blockIdx.x * 32 + 8 * q;  // (n % 32 == 0)
+    for (unsigned tb = wave; tb < TB; tb += waves) {
+        const unsigned token = first_row + 16 * tb + r;
+        if (token >= a.out.m)
+            continue;
+        f32x4 v[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            v[j] = red[(j * TB + tb) * 64 + lane];
+            for (unsigned i = 1; i < waves; ++i)
+                v[j] += red[((i * 2 + j) * TB + tb) * 64 + lane];
+        }
+        *reinterpret_cast<quad_a2*>(static_cast<uint16_t*>(a.out.y) +
+                                    size_t(token) * a.out.stride + col) =
+            quad_a2{bf16_pair(v[0].x, v[1].x), bf16_pair(v[0].y, v[1].y),
+                    bf16_pair(v[0].z, v[1].z), bf16_pair(v[0].w, v[1].w)};
+    }
 }
 
 // ------------------------------------------------------------------ more rows of x
@@ -1161,7 +1256,7 @@ struct Plan {
     unsigned tiles_n, tiles_m, slices, chunks, part;
 };
 
-constexpr size_t kDecodeRows = 32;
+constexpr size_t kDecodeTraffic = size_t(32) << 20;
 
 Plan plan_gemm(size_t m, size_t wave_groups, size_t chunks, int ops) {
     Plan p{};
@@ -1265,9 +1360,13 @@ int launch_decode(Decode a, unsigned waves, hipStream_t st) {
 template <bool GATED, bool FP4, int OUT> int run_decode(Decode a, hipStream_t st) {
     const unsigned units = (a.k + 127) / 128;
     // whole blocks of 32 rows a workgroup where those fill the compute units
-    const bool wide = a.groups >= compute_units();
-    unsigned waves = units <= 8 ? 2 : units <= 16 ? 4 : units <= 64 || wide ? 8 : 16;
+    const bool wide = a.groups >= compute_units() && a.out.m <= 32;
+    unsigned waves = units <= 8 ? 2 : units <= 16 ? 4
+                     : units <= 64 || wide || a.out.m > 32 ? 8
+                                                           : 16;
     a.units = (unsigned(ceil_div(units, waves)) + 1) / 2 * 2;
+    if (a.out.m > 32)
+        return launch_decode<1, 4, GATED, FP4, false, OUT>(a, waves, st);
     if (a.out.m > 16)
         return wide ? launch_decode<2, 2, GATED, FP4, false, OUT>(a, waves, st)
                     : launch_decode<1, 2, GATED, FP4, false, OUT>(a, waves, st);
@@ -1280,8 +1379,32 @@ template <bool GATED, bool FP4, int OUT> int run_decode(Decode a, hipStream_t st
                 : launch_decode<1, 1, GATED, FP4, false, OUT>(a, waves, st);
 }
 
+template <int TB> int launch_decode_t(const Decode& a, unsigned waves, hipStream_t st) {
+    hipLaunchKernelGGL((decode_t_kernel<TB>),
+                       dim3(a.out.n / 32, unsigned(ceil_div(a.out.m, 16 * TB))),
+                       dim3(waves * 64), waves * 2 * TB * 1024, st, a);
+    KDQ_HIP(hipGetLastError());
+    return KDQ_OK;
+}
+
+int run_decode_t(Decode a, hipStream_t st) {
+    const unsigned units = (a.k + 127) / 128;  // of each matrix
+    const unsigned waves =
+        2 * (units <= 4 ? 1 : units <= 8 ? 2 : units <= 16 || a.out.m > 32 ? 4 : 8);
+    a.units = unsigned(ceil_div(units, waves / 2));
+    return a.out.m <= 16   ? launch_decode_t<1>(a, waves, st)
+           : a.out.m <= 32 ? launch_decode_t<2>(a, waves, st)
+                           : launch_decode_t<4>(a, waves, st);
+}
+
+// Whether decode_kernel takes a product of m rows of k values whose workgroups are `blocks`:
+// each reads all of x.
+bool decode_takes(size_t m, size_t k_bytes, size_t blocks) {
+    return m <= 32 || (m <= 64 && m * k_bytes * blocks <= kDecodeTraffic);
+}
+
 Plan plan_product(size_t m, size_t n, size_t k, bool fp4) {
-    if (m <= kDecodeRows) {
+    if (decode_takes(m, fp4 ? k / 2 : k * 2, ceil_div(n, 16))) {
         Plan p{};
         p.decode = true;
         return p;
@@ -1290,7 +1413,7 @@ Plan plan_product(size_t m, size_t n, size_t k, bool fp4) {
 }
 
 Plan plan_gated(size_t m, size_t n, size_t k, bool kept) {
-    if (m <= kDecodeRows && !kept) {
+    if (!kept && decode_takes(m, k * 2, ceil_div(n, 16))) {
         Plan p{};
         p.decode = true;
         return p;
@@ -1299,6 +1422,11 @@ Plan plan_gated(size_t m, size_t n, size_t k, bool kept) {
 }
 
 Plan plan_backward(size_t m, size_t n, size_t k) {
+    if (decode_takes(m, n * 4, k / 32)) {
+        Plan p{};
+        p.decode = true;
+        return p;
+    }
     return plan_gemm(m, ceil_div(k, 64), ceil_div(n, 64), kTransposed);
 }
 
@@ -1600,6 +1728,13 @@ extern "C" int kdq_mxfp4_gated_backward(const uint16_t* dh_bf16, size_t dh_strid
                            unsigned(m), unsigned(n), kept_bf16, kept_q8, kept_scales, dgu_bf16);
     KDQ_HIP(hipGetLastError());
     const Form f = transposed_form(n, k);
+    const Target t{dx_bf16, dx_stride, unsigned(m), unsigned(k), nullptr, nullptr, nullptr};
+    if (p.decode)
+        return run_decode_t({gate_transposed, up_transposed,
+                             reinterpret_cast<const uint8_t*>(dgu_bf16), nullptr,
+                             unsigned(n * 4), unsigned(n), unsigned(f.steps), unsigned(f.groups),
+                             0, t},
+                            st);
     Gemm g{};
     g.w0 = gate_transposed;
     g.w1 = up_transposed;
@@ -1609,6 +1744,6 @@ extern "C" int kdq_mxfp4_gated_backward(const uint16_t* dh_bf16, size_t dh_strid
     g.segments = unsigned(n / 8);
     g.groups = unsigned(f.groups);
     g.steps = unsigned(f.steps);
-    g.out = {dx_bf16, dx_stride, unsigned(m), unsigned(k), nullptr, nullptr, nullptr};
+    g.out = t;
     return run_gemm<kTransposed, kOutBackward>(g, p, workspace, st);
 }
