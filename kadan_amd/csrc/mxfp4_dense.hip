@@ -1072,60 +1072,52 @@ __global__ __launch_bounds__(512, 2) void gemm_kernel(Gemm a) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // no copy outlives the loop
     __syncthreads();
 
-    // SPLIT: each group hands the other one half of its tiles and finishes the other half
-    // (TT == 1: the first group finishes both)
-    constexpr int kOwn = SPLIT ? (TT + 1) / 2 : TT;
-    const unsigned own = SPLIT ? (TT > 1 ? kg * kOwn : 0) : 0;
+    // SPLIT: the first group finishes the first kOwn tiles and is handed the second one's sums
+    // of them, and the other way round
+    constexpr int kOwn = SPLIT ? (TT + 1) / 2 : TT, kOther = TT - kOwn;
     if constexpr (SPLIT) {
-        constexpr int kGiven = TT > 1 ? 2 : 1;  // groups that hand tiles over
-        auto* meet = reinterpret_cast<f32x4*>(lds) + rg * (kGiven * kOwn * 512) + lane;
-        if (TT > 1 || kg == 1) {
+        auto* meet = reinterpret_cast<f32x4*>(lds) + rg * (TT * 512) + lane;
+        auto hand = [&]<int FROM, int COUNT>() {
 #pragma unroll
-            for (int t = 0; t < kOwn; ++t)
+            for (int t = FROM; t < FROM + COUNT; ++t)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        meet[((t * 2 + i) * 4 + j) * 64] = quad_of(acc[i][t], j);
+        };
+        auto add = [&]<int FROM, int COUNT>() {  // (kept from place 0 on)
+#pragma unroll
+            for (int t = 0; t < COUNT; ++t)
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        f32x4 v;
-                        if (TT > 1)
-                            v = kg ? quad_of(acc[i][t], j) : quad_of(acc[i][(t + kOwn) % TT], j);
-                        else
-                            v = quad_of(acc[i][0], j);
-                        meet[(TT > 1 ? kg : 0) * (kOwn * 512) + ((t * 2 + i) * 4 + j) * 64] = v;
+                        const f32x4 v = meet[(((FROM + t) * 2 + i) * 4 + j) * 64];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            acc[i][t][4 * j + e] = acc[i][FROM + t][4 * j + e] + v[e];
                     }
-        }
+        };
+        if (kg)
+            hand.template operator()<0, kOwn>();
+        else
+            hand.template operator()<kOwn, kOther>();
         __syncthreads();
-        if (TT == 1 && kg == 1)
-            return;
-#pragma unroll
-        for (int t = 0; t < kOwn; ++t)
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const f32x4 v =
-                        meet[(TT > 1 ? 1 - kg : 0) * (kOwn * 512) + ((t * 2 + i) * 4 + j) * 64];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        if (TT > 1) {
-                            // (kept in place t: the group's own tiles move down)
-                            const float mine = kg ? acc[i][(t + kOwn) % TT][4 * j + e]
-                                                  : acc[i][t][4 * j + e];
-                            acc[i][t][4 * j + e] = kg ? v[e] + mine : mine + v[e];
-                        } else {
-                            acc[i][0][4 * j + e] += v[e];
-                        }
-                    }
-                }
+        if (kg)
+            add.template operator()<kOwn, kOther>();
+        else
+            add.template operator()<0, kOwn>();
     }
-    // (SPLIT: of the tiles handed to this wavefront, which it alone read)
-    uint8_t* patch =
-        SPLIT ? lds + (rg * (TT > 1 ? 2 : 1) + (TT > 1 ? 1 - kg : 0)) * (kOwn * 8192)
-              : lds + wave * kPatchBytes;
+    // (SPLIT: LDS that only this wavefront read from)
+    uint8_t* patch = lds + (SPLIT ? (rg * TT + (kg ? kOwn : 0)) * 8192 : wave * kPatchBytes);
+    const unsigned own = SPLIT && kg ? kOther : kOwn;
     const unsigned first_tile =
-        (first_row / 32) + (SPLIT ? own : kg * TT);  // of 32 rows of x, the wavefront's first
+        (first_row / 32) + kg * (SPLIT ? kOwn : TT);  // of 32 rows of x, the wavefront's first
 #pragma unroll
     for (int t = 0; t < kOwn; ++t) {
+        if (t >= int(own))
+            break;
         const unsigned T = first_tile + t;
         if (a.partial) {
             const unsigned row_tiles = (a.out.m + 31) / 32;
@@ -1169,7 +1161,8 @@ __global__ __launch_bounds__(256) void reduce_kernel(const float* __restrict__ p
 #pragma unroll
         for (int j = 0; j < kQuads; ++j)
             v[i][j] = from[(i * 4 + j0 + j) * 64];
-    for (unsigned s = 1; s < slices; ++s)
+#pragma unroll 4
+    for (unsigned s = 1; s < slices; ++s)  // (loads of four slices in flight)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -1260,13 +1253,14 @@ constexpr size_t kDecodeTraffic = size_t(32) << 20;
 
 Plan plan_gemm(size_t m, size_t wave_groups, size_t chunks, int ops) {
     Plan p{};
-    p.tt = m <= 32 ? 1 : m <= 64 ? 2 : 4;
+    p.tt = m <= 32 ? 1 : m <= 64 ? 2 : ceil_div(m, 96) * 3 < ceil_div(m, 128) * 4 ? 3 : 4;
     p.tiles_n = unsigned(ceil_div(wave_groups, 4));
     p.split = true;
     p.chunks = unsigned(chunks);
     if (ops == kFp4 && m > 128) {
         const size_t whole = size_t(p.tiles_n) * ceil_div(m, 256);
         p.split = whole < compute_units();
+        p.tt = 4;
     }
     p.tiles_m = unsigned(ceil_div(m, size_t(p.tt) * (p.split ? 32 : 64)));
     const unsigned sets = p.split && ops != kTransposed ? 2 : 1;
@@ -1321,6 +1315,7 @@ template <int OPS, int OUT> int run_gemm(Gemm a, const Plan& p, void* workspace,
     } else {
         rc = p.tt == 1   ? launch_gemm<1, true, OPS, OUT>(a, p, st)
              : p.tt == 2 ? launch_gemm<2, true, OPS, OUT>(a, p, st)
+             : p.tt == 3 ? launch_gemm<3, true, OPS, OUT>(a, p, st)
                          : launch_gemm<4, true, OPS, OUT>(a, p, st);
     }
     if (rc || p.slices == 1)
