@@ -777,8 +777,11 @@ __device__ __forceinline__ i32x8 fp4_operand(const u4& c) {
     return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1);
 }
 
+// Tiles small enough for two workgroups to a compute unit (128 registers).
+template <int TT, int OPS> constexpr bool shares_unit = TT == 1 || (TT == 2 && OPS != kFp4);
+
 template <int TT, bool SPLIT, int OPS, int OUT>
-__global__ __launch_bounds__(512, 2) void gemm_kernel(Gemm a) {
+__global__ __launch_bounds__(512, (shares_unit<TT, OPS> ? 4 : 2)) void gemm_kernel(Gemm a) {
     extern __shared__ __align__(16) uint8_t lds[];
     constexpr int GROUPS = 2, kWaves = 4 * GROUPS, kStageBytes = TT * 8192;
     const unsigned lane = threadIdx.x % 64, h = lane / 32;
@@ -891,7 +894,9 @@ __global__ __launch_bounds__(512, 2) void gemm_kernel(Gemm a) {
         else
             scales_buf[t] = buffer(s + g * scale_groups * 256, there ? scale_groups * 256 : 0);
     }
-    constexpr int kAhead = OPS == kTransposed ? 2 : 4;  // steps (registers for two are left)
+    // steps (registers for two are left, or several workgroups share a compute unit)
+    constexpr int kAhead =
+        OPS == kFp4 ? 4 : OPS == kTransposed || shares_unit<TT, OPS> ? 2 : 4;
     struct Codes {
         u4 w[2];
         u4 s[OPS == kTransposed ? 2 : 1];
@@ -947,6 +952,9 @@ __global__ __launch_bounds__(512, 2) void gemm_kernel(Gemm a) {
         return *reinterpret_cast<const u4*>(buf + t * 4096 + ((seg ^ (lane / 2 % 8)) * 16));
     };
 
+    // operands are read (and weights decoded) a step ahead of their products where one
+    // workgroup has the compute unit, at their step where two share it
+    constexpr int kBuffers = shares_unit<TT, OPS> ? 1 : 2;
     Codes codes[kAhead];
     Scales scales, next;
     // the x operands of a chunk's step S, and (bf16) the chunk's weights of it
@@ -1016,19 +1024,22 @@ __global__ __launch_bounds__(512, 2) void gemm_kernel(Gemm a) {
                     xs_now[t] = __builtin_amdgcn_perm(unsigned(bytes >> 32), unsigned(bytes),
                                                       h ? 0x07050301u : 0x06040200u);
                 }
-                u4 xv[2][TT];  // a step's operands are read while the one before multiplies
-                read_x.template operator()<0>(buf, xv[0]);
+                u4 xv[kBuffers][TT];
+                if constexpr (kBuffers == 2)
+                    read_x.template operator()<0>(buf, xv[0]);
                 static_for<4>([&]<int S>() {
                     if (active) {
-                        if constexpr (S < 3)
-                            read_x.template operator()<S + 1>(buf, xv[(S + 1) % 2]);
-                        __builtin_amdgcn_sched_barrier(0);
+                        if constexpr (S + kBuffers < 5)
+                            read_x.template operator()<S + kBuffers - 1>(
+                                buf, xv[(S + kBuffers - 1) % kBuffers]);
+                        if constexpr (kBuffers == 2)
+                            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                         for (int t = 0; t < TT; ++t)
 #pragma unroll
                             for (int i = 0; i < 2; ++i)
                                 acc[i][t] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-                                    fp4_operand(codes[S].w[i]), fp4_operand(xv[S % 2][t]),
+                                    fp4_operand(codes[S].w[i]), fp4_operand(xv[S % kBuffers][t]),
                                     acc[i][t], 4, 4, S, int(now.w[i]), S, int(xs_now[t]));
                     }
                     issue_order();
@@ -1045,22 +1056,28 @@ __global__ __launch_bounds__(512, 2) void gemm_kernel(Gemm a) {
                 stage(c0 + C + 3, (C + 3) % kStages);
                 if constexpr (C == 0)
                     load_scales(begin_step + c0 + 4, next);
-                u4 xv[2][TT];  // operands are read, and weights decoded, a step ahead
-                bf16x8 wv[2][2];
-                read_x.template operator()<0>(buf, xv[0]);
-                decode_w.template operator()<C, 0>(wv[0]);
+                u4 xv[kBuffers][TT];
+                bf16x8 wv[kBuffers][2];
+                if constexpr (kBuffers == 2) {
+                    read_x.template operator()<0>(buf, xv[0]);
+                    decode_w.template operator()<C, 0>(wv[0]);
+                }
                 static_for<4>([&]<int S>() {
-                    if constexpr (S < 3)
-                        read_x.template operator()<S + 1>(buf, xv[(S + 1) % 2]);
-                    __builtin_amdgcn_sched_barrier(0);
-                    if constexpr (S < 3)
-                        decode_w.template operator()<C, S + 1>(wv[(S + 1) % 2]);
+                    if constexpr (S + kBuffers < 5)
+                        read_x.template operator()<S + kBuffers - 1>(
+                            buf, xv[(S + kBuffers - 1) % kBuffers]);
+                    if constexpr (kBuffers == 2)
+                        __builtin_amdgcn_sched_barrier(0);
+                    if constexpr (S + kBuffers < 5)
+                        decode_w.template operator()<C, S + kBuffers - 1>(
+                            wv[(S + kBuffers - 1) % kBuffers]);
 #pragma unroll
                     for (int t = 0; t < TT; ++t)
 #pragma unroll
                         for (int i = 0; i < 2; ++i)
                             acc[i][t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                                wv[S % 2][i], __builtin_bit_cast(bf16x8, xv[S % 2][t]),
+                                wv[S % kBuffers][i],
+                                __builtin_bit_cast(bf16x8, xv[S % kBuffers][t]),
                                 acc[i][t], 0, 0, 0);
                 });
                 issue_order();
@@ -1251,27 +1268,58 @@ struct Plan {
 
 constexpr size_t kDecodeTraffic = size_t(32) << 20;
 
+// What a product in tiles of tt * 32 rows and `slices` K slices takes, in microseconds, up to
+// what every choice shares: a workgroup's fixed part and its turns, alone on a compute unit or
+// beside another, and the slices' sum.  Fitted to sweeps over tt and slices at 18 sizes per
+// kind: 64 x 14336 -> 4096 16 us in 6 slices of 32 rows, 18 in 14 of 64, 23 in 14 of 128;
+// 333 x 2880 -> 2880 gated 14 us in tiles of 32, 20 of 64, 25 of 128; 512 x 4096 -> 14336 51 us
+// in tiles of 128, 53 of 64, 60 of 32; 512 x 4096 -> 4096 18 of 32, 26 of 64, 30 of 128.
+struct Cost {
+    double fixed, turn, turn_of_two;
+};
+
+Cost cost_of(int ops, int tt) {
+    if (ops == kFp4)
+        return {2.0 + 0.75 * tt, 0.05 + 0.55 * tt, 0.1 + 1.35 * tt};
+    const double fixed = 2.5 + 0.9 * tt;
+    return ops == kTransposed ? Cost{fixed, 0.4 + 0.3 * tt, 0.7 + 0.6 * tt}
+                              : Cost{fixed, 0.03 + 0.33 * tt, 0.05 + 0.68 * tt};
+}
+
 Plan plan_gemm(size_t m, size_t wave_groups, size_t chunks, int ops) {
-    Plan p{};
-    p.tt = m <= 32 ? 1 : m <= 64 ? 2 : ceil_div(m, 96) * 3 < ceil_div(m, 128) * 4 ? 3 : 4;
-    p.tiles_n = unsigned(ceil_div(wave_groups, 4));
-    p.split = true;
-    p.chunks = unsigned(chunks);
-    if (ops == kFp4 && m > 128) {
-        const size_t whole = size_t(p.tiles_n) * ceil_div(m, 256);
-        p.split = whole < compute_units();
-        p.tt = 4;
-    }
-    p.tiles_m = unsigned(ceil_div(m, size_t(p.tt) * (p.split ? 32 : 64)));
-    const unsigned sets = p.split && ops != kTransposed ? 2 : 1;
-    const size_t tiles = size_t(p.tiles_n) * p.tiles_m;
-    // slices until the tiles fill the compute units, each group at least four chunks
-    const unsigned unit = ops == kFp4 ? 1 : 4;
-    const size_t most = std::max<size_t>(1, ceil_div(chunks, size_t(sets) * unit));
-    size_t slices = std::max<size_t>(1, std::min<size_t>(compute_units() / tiles, most));
-    p.part = unsigned(ceil_div(ceil_div(chunks, slices * sets), unit) * unit);
-    p.slices = unsigned(ceil_div(chunks, size_t(p.part) * sets));
-    return p;
+    const size_t cus = compute_units();
+    Plan best{};
+    double least = 0;
+    const auto consider = [&](int tt, bool split, size_t slices) {
+        Plan p{};
+        p.tt = tt;
+        p.split = split;
+        p.tiles_n = unsigned(ceil_div(wave_groups, 4));
+        p.tiles_m = unsigned(ceil_div(m, size_t(tt) * (split ? 32 : 64)));
+        p.chunks = unsigned(chunks);
+        const unsigned sets = split && ops != kTransposed ? 2 : 1, unit = ops == kFp4 ? 1 : 4;
+        p.part = unsigned(ceil_div(ceil_div(chunks, slices * sets), unit) * unit);
+        p.slices = unsigned(ceil_div(chunks, size_t(p.part) * sets));
+        const Cost c = cost_of(ops, tt);
+        const bool shared = tt == 1 || (tt == 2 && ops != kFp4);
+        const size_t tiles = size_t(p.tiles_n) * p.tiles_m;
+        const size_t each = ceil_div(tiles * p.slices, cus);  // workgroups of a compute unit
+        const double alone = c.fixed + p.part * c.turn, both = c.fixed + p.part * c.turn_of_two;
+        double t = shared ? double(each / 2) * both + double(each % 2) * alone
+                          : double(each) * (split ? alone : 0.93 * alone);
+        if (p.slices > 1)
+            t += 3.5 + double(p.slices) * p.tiles_n * 4 * ceil_div(m, 32) * kTileFloats * 4 / 2.5e6;
+        if (!best.slices || t < least) {
+            least = t;
+            best = p;
+        }
+    };
+    for (int tt = 1; tt <= 4; ++tt)
+        for (size_t slices = 1; slices <= 16; ++slices)
+            consider(tt, true, slices);
+    if (ops == kFp4)
+        consider(4, false, 1);
+    return best;
 }
 
 size_t partial_bytes(const Plan& p, size_t m) {
