@@ -652,18 +652,26 @@ __global__ __launch_bounds__(1024) void decode_t_kernel(Decode a) {
     const unsigned lane_scales = (q / 2) * 128 + (2 * (q % 2) + e) * 32;
     const unsigned begin = wave % share * a.units, end = begin + a.units;
     f32x4 acc[2][TB] = {};
-    for (unsigned t0 = begin; t0 < end; t0 += kBatch) {
-        u4 c[kBatch][2], s[kBatch][2], x[kBatch][TB][4];
+    struct Batch {
+        u4 c[kBatch][2], s[kBatch][2];
+    };
+    auto load = [&](unsigned t0, Batch& v) {  // units past the wavefront's run are zeros
 #pragma unroll
-        for (int b = 0; b < kBatch; ++b) {
-            const unsigned t = t0 + b;
+        for (int b = 0; b < kBatch; ++b)
 #pragma unroll
             for (int p = 0; p < 2; ++p) {
-                c[b][p] = load_b128<kNt>(
+                const unsigned t = t0 + b;
+                v.c[b][p] = load_b128<kNt>(
                     codes, t < end ? int(t * 4096 + p * 1024 + lane_codes) : kOutside);
-                s[b][p] = load_b128(scales, int(t * 256 + lane_scales + 16 * p));
+                v.s[b][p] = load_b128(scales, int(t * 256 + lane_scales + 16 * p));
             }
-        }
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // a batch's x is requested before the next batch's weights, which then stream while it is
+    // multiplied (loads return in order)
+    auto multiply = [&](unsigned t0, const Batch& now, Batch& next) {
+        u4 x[kBatch][TB][4];
 #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
             const unsigned from = 128 * (t0 + b) + 32 * q;
@@ -677,12 +685,17 @@ __global__ __launch_bounds__(1024) void decode_t_kernel(Decode a) {
                     x[b][i][d] = load_b128(xs, at + 16 * d);
             }
         }
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        load(t0 + kBatch, next);
 #pragma unroll
         for (int b = 0; b < kBatch; ++b)
 #pragma unroll
             for (int d = 0; d < 4; ++d) {
-                const unsigned cw[2] = {c[b][d / 2][2 * (d % 2)], c[b][d / 2][2 * (d % 2) + 1]};
-                const unsigned sw[2] = {s[b][d / 2][2 * (d % 2)], s[b][d / 2][2 * (d % 2) + 1]};
+                const unsigned cw[2] = {now.c[b][d / 2][2 * (d % 2)],
+                                        now.c[b][d / 2][2 * (d % 2) + 1]};
+                const unsigned sw[2] = {now.s[b][d / 2][2 * (d % 2)],
+                                        now.s[b][d / 2][2 * (d % 2) + 1]};
                 bf16x8 even, odd;
                 decode8_pair(cw, sw, even, odd);
 #pragma unroll
@@ -694,6 +707,12 @@ __global__ __launch_bounds__(1024) void decode_t_kernel(Decode a) {
                         __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd, xv, acc[1][i], 0, 0, 0);
                 }
             }
+    };
+    Batch first, second;
+    load(begin, first);
+    for (unsigned t0 = begin; t0 < end; t0 += 2 * kBatch) {
+        multiply(t0, first, second);
+        multiply(t0 + kBatch, second, first);
     }
     auto* red = reinterpret_cast<f32x4*>(lds);
 #pragma unroll
@@ -1264,9 +1283,9 @@ struct Plan {
     bool decode, split;
     int tt;
     unsigned tiles_n, tiles_m, slices, chunks, part;
+    double cost;
 };
 
-constexpr size_t kDecodeTraffic = size_t(32) << 20;
 
 // What a product in tiles of tt * 32 rows and `slices` K slices takes, in microseconds, up to
 // what every choice shares: a workgroup's fixed part and its turns, alone on a compute unit or
@@ -1289,7 +1308,6 @@ Cost cost_of(int ops, int tt) {
 Plan plan_gemm(size_t m, size_t wave_groups, size_t chunks, int ops) {
     const size_t cus = compute_units();
     Plan best{};
-    double least = 0;
     const auto consider = [&](int tt, bool split, size_t slices) {
         Plan p{};
         p.tt = tt;
@@ -1309,9 +1327,9 @@ Plan plan_gemm(size_t m, size_t wave_groups, size_t chunks, int ops) {
                           : double(each) * (split ? alone : 0.93 * alone);
         if (p.slices > 1)
             t += 3.5 + double(p.slices) * p.tiles_n * 4 * ceil_div(m, 32) * kTileFloats * 4 / 2.5e6;
-        if (!best.slices || t < least) {
-            least = t;
+        if (!best.slices || t < best.cost) {
             best = p;
+            best.cost = t;
         }
     };
     for (int tt = 1; tt <= 4; ++tt)
@@ -1408,8 +1426,9 @@ template <bool GATED, bool FP4, int OUT> int run_decode(Decode a, hipStream_t st
                      : units <= 64 || wide || a.out.m > 32 ? 8
                                                            : 16;
     a.units = (unsigned(ceil_div(units, waves)) + 1) / 2 * 2;
-    if (a.out.m > 32)
-        return launch_decode<1, 4, GATED, FP4, false, OUT>(a, waves, st);
+    if constexpr (FP4)
+        if (a.out.m > 32)
+            return launch_decode<1, 4, GATED, FP4, false, OUT>(a, waves, st);
     if (a.out.m > 16)
         return wide ? launch_decode<2, 2, GATED, FP4, false, OUT>(a, waves, st)
                     : launch_decode<1, 2, GATED, FP4, false, OUT>(a, waves, st);
@@ -1433,44 +1452,55 @@ template <int TB> int launch_decode_t(const Decode& a, unsigned waves, hipStream
 int run_decode_t(Decode a, hipStream_t st) {
     const unsigned units = (a.k + 127) / 128;  // of each matrix
     const unsigned waves =
-        2 * (units <= 4 ? 1 : units <= 8 ? 2 : units <= 16 || a.out.m > 32 ? 4 : 8);
+        2 * (units <= 4 ? 1 : units <= 8 ? 2 : units <= 16 ? 4 : 8);
     a.units = unsigned(ceil_div(units, waves / 2));
-    return a.out.m <= 16   ? launch_decode_t<1>(a, waves, st)
-           : a.out.m <= 32 ? launch_decode_t<2>(a, waves, st)
-                           : launch_decode_t<4>(a, waves, st);
+    return a.out.m <= 16 ? launch_decode_t<1>(a, waves, st) : launch_decode_t<2>(a, waves, st);
 }
 
-// Whether decode_kernel takes a product of m rows of k values whose workgroups are `blocks`:
-// each reads all of x.
-bool decode_takes(size_t m, size_t k_bytes, size_t blocks) {
-    return m <= 32 || (m <= 64 && m * k_bytes * blocks <= kDecodeTraffic);
+// What decode_kernel takes, in microseconds: its weights at 6 GB/ms, and each workgroup's own
+// reading of x (m rows of row_bytes; none to speak of where x is staged) at what a compute
+// unit takes of strided rows, 33 KB/us.  Swept against gemm_kernel over 11 sizes per kind and
+// 1 to 64 rows: 4096 -> 14336 8 rows 10.7 us against 12.1, 16 rows 13.5 against 12.3; 14336
+// -> 4096 4 rows 11.2 against 12.6, 8 rows 14.0 against 12.7; 8192 -> 1024 12 rows 9.1
+// against 9.3, 20 rows 14.6 against 9.4; 2880 -> 2880 20 rows 7.5 against 8.2, 32 rows 9.4
+// against 8.3.
+bool decode_is_quicker(size_t m, size_t row_bytes, size_t row_tiles, size_t weight_bytes,
+                       bool fp4, const Plan& gemm) {
+    const double weights = double(weight_bytes) / 6.0e6;
+    const double rounds = std::max(1.0, double(row_tiles) / compute_units());
+    const double x = m * staged_pitch(unsigned(row_bytes)) <= kStagedBytes
+                         ? 0.0
+                         : double(m * row_bytes) * rounds / 33.0e3;
+    return weights + x < std::max(gemm.cost - (fp4 ? 1.0 : 3.0), weights + 2.5);
 }
 
 Plan plan_product(size_t m, size_t n, size_t k, bool fp4) {
-    if (decode_takes(m, fp4 ? k / 2 : k * 2, ceil_div(n, 16))) {
-        Plan p{};
-        p.decode = true;
-        return p;
-    }
-    return plan_gemm(m, ceil_div(n, 64), ceil_div(k, fp4 ? 256 : 64), fp4 ? kFp4 : kBf16);
+    Plan p = plan_gemm(m, ceil_div(n, 64), ceil_div(k, fp4 ? 256 : 64), fp4 ? kFp4 : kBf16);
+    const size_t groups = ceil_div(n, 32);
+    p.decode = m <= (fp4 ? 64 : 32) &&
+               decode_is_quicker(m, fp4 ? k / 2 : k * 2,
+                                 groups >= compute_units() ? groups : ceil_div(n, 16),
+                                 n * k * 17 / 32, fp4, p);
+    return p;
 }
 
 Plan plan_gated(size_t m, size_t n, size_t k, bool kept) {
-    if (!kept && decode_takes(m, k * 2, ceil_div(n, 16))) {
-        Plan p{};
-        p.decode = true;
-        return p;
-    }
-    return plan_gemm(m, ceil_div(n, 32), ceil_div(k, 64), kBf16);
+    Plan p = plan_gemm(m, ceil_div(n, 32), ceil_div(k, 64), kBf16);
+    const size_t groups = ceil_div(n, 32);
+    p.decode = !kept && m <= 32 &&
+               decode_is_quicker(m, k * 2, groups >= compute_units() ? groups : ceil_div(n, 16),
+                                 n * k * 17 / 16, false, p);
+    return p;
 }
 
+// (decode_t_kernel is bound by decoding the weights, which half the compute units do where
+// there are 4096 columns: 1 row of 14336 -> 4096 26 us against 21, of 2880 -> 2880 10.3
+// against 13.0, 16 rows of that 15.0 against 13.2, 1 row of 1024 -> 8192 6.6 against 11.6)
 Plan plan_backward(size_t m, size_t n, size_t k) {
-    if (decode_takes(m, n * 4, k / 32)) {
-        Plan p{};
-        p.decode = true;
-        return p;
-    }
-    return plan_gemm(m, ceil_div(k, 64), ceil_div(n, 64), kTransposed);
+    Plan p = plan_gemm(m, ceil_div(k, 64), ceil_div(n, 64), kTransposed);
+    const double units = double(ceil_div(n, 128)) * double(ceil_div(k / 32, compute_units()));
+    p.decode = m <= 32 && 2.5 + 0.2 * units * (1.0 + double(m) / 14) < p.cost;
+    return p;
 }
 
 bool sizes_ok(size_t m, size_t n, size_t k) {
