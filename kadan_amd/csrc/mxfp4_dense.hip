@@ -1301,7 +1301,7 @@ Cost cost_of(int ops, int tt) {
     if (ops == kFp4)
         return {2.0 + 0.75 * tt, 0.05 + 0.55 * tt, 0.1 + 1.35 * tt};
     const double fixed = 2.5 + 0.9 * tt;
-    return ops == kTransposed ? Cost{fixed, 0.4 + 0.3 * tt, 0.7 + 0.6 * tt}
+    return ops == kTransposed ? Cost{fixed, tt == 1 ? 0.5 : 0.4 + 0.3 * tt, 0.7 + 0.6 * tt}
                               : Cost{fixed, 0.03 + 0.33 * tt, 0.05 + 0.68 * tt};
 }
 
@@ -1325,8 +1325,8 @@ Plan plan_gemm(size_t m, size_t wave_groups, size_t chunks, int ops) {
         const double alone = c.fixed + p.part * c.turn, both = c.fixed + p.part * c.turn_of_two;
         double t = shared ? double(each / 2) * both + double(each % 2) * alone
                           : double(each) * (split ? alone : 0.93 * alone);
-        if (p.slices > 1)
-            t += 3.5 + double(p.slices) * p.tiles_n * 4 * ceil_div(m, 32) * kTileFloats * 4 / 2.5e6;
+        if (p.slices > 1)  // (the backward pass's third launch, which is its caller's time too)
+            t += (ops == kTransposed ? 4.5 : 3.5) + double(p.slices) * p.tiles_n * 4 * ceil_div(m, 32) * kTileFloats * 4 / 2.5e6;
         if (!best.slices || t < best.cost) {
             best = p;
             best.cost = t;
