@@ -272,9 +272,12 @@ __device__ __forceinline__ void store_quad(const Target& t, unsigned G, unsigned
 // codes with scale amax / 127, codes round-half-even(v * 127 / amax): kdq_quantize_q8's
 // format.  A block with a value that is not finite keeps a NaN scale; one whose largest
 // magnitude is below 2^-120 is kept as zeros (127 / amax would overflow).
-__device__ __forceinline__ void keep_q8(const Target& t, unsigned column, unsigned token,
-                                        unsigned h, const f32x4 (&v)[4]) {
-    float amax = 0.f;
+struct Q8 {
+    unsigned codes[4];
+    float scale;
+};
+
+__device__ __forceinline__ Q8 q8_of(const f32x4 (&v)[4]) {
     unsigned top = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -283,25 +286,34 @@ __device__ __forceinline__ void keep_q8(const Target& t, unsigned column, unsign
             top = max(top, __float_as_uint(v[j][i]) & 0x7fffffffu);
     top = max(top, unsigned(__shfl_xor(int(top), 32, 64)));
     const bool finite = top < 0x7f800000u;
-    amax = __uint_as_float(top);
+    const float amax = __uint_as_float(top);
     const bool some = finite && amax >= 0x1p-120f;
     const float inv = some ? 127.0f / amax : 0.f;
+    Q8 q;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        q.codes[j] = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int code = some ? int(rintf(v[j][i] * inv)) : 0;
+            q.codes[j] |= (unsigned(code) & 255u) << (8 * i);
+        }
+    }
+    q.scale = !finite ? __uint_as_float(0x7fc00000u) : some ? amax / 127.0f : 0.f;
+    return q;
+}
+
+__device__ __forceinline__ void keep_q8(const Target& t, unsigned column, unsigned token,
+                                        unsigned h, const f32x4 (&v)[4]) {
+    const Q8 q = q8_of(v);
     if (token >= t.m || column >= 2 * t.n)
         return;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        unsigned word = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int q = some ? int(rintf(v[j][i] * inv)) : 0;
-            word |= (unsigned(q) & 255u) << (8 * i);
-        }
+    for (int j = 0; j < 4; ++j)
         *reinterpret_cast<unsigned*>(t.kept_q + size_t(token) * 2 * t.n + column + 8 * j + 4 * h) =
-            word;
-    }
+            q.codes[j];
     if (h == 0)
-        t.kept_d[size_t(token) * (2 * t.n / 32) + column / 32] =
-            !finite ? __uint_as_float(0x7fc00000u) : some ? amax / 127.0f : 0.f;
+        t.kept_d[size_t(token) * (2 * t.n / 32) + column / 32] = q.scale;
 }
 
 __device__ __forceinline__ f32x4 quad_of(const f32x16& a, int j) {
@@ -361,13 +373,12 @@ __device__ __forceinline__ void patch_pair(uint8_t* patch, unsigned token, unsig
     }
 }
 
-// A wavefront's two 32 x 32 result tiles (group G, rows 32T .. of x): as store_quad, through
-// `patch`, kPatchBytes of LDS that are the wavefront's own.
+// A wavefront's two 32 x 32 result tiles (group G, rows 32T .. of x), but for the gated
+// projection's: as store_quad, through `patch`, kPatchBytes of LDS that are the wavefront's own.
 template <int OUT>
 __device__ __forceinline__ void store_tiles(const Target& t, unsigned G, unsigned T,
                                             uint8_t* patch, const f32x16& a0, const f32x16& a1) {
     const unsigned lane = threadIdx.x % 64, row = lane % 32, h = lane / 32;
-    const unsigned token = T * 32 + row;
     auto* y = static_cast<uint8_t*>(t.y);
     if constexpr (OUT == kOutF32) {
 #pragma unroll
@@ -382,7 +393,8 @@ __device__ __forceinline__ void store_tiles(const Target& t, unsigned G, unsigne
     } else if constexpr (OUT == kOutBf16) {
         patch_pair(patch, row, h, a0, a1);
         store_patch(patch, y, t.stride * 2, T * 32, t.m, size_t(64) * G * 2, size_t(t.n) * 2);
-    } else if constexpr (OUT == kOutBackward) {
+    } else {
+        static_assert(OUT == kOutBackward);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const f32x4 v0 = quad_of(a0, j), v1 = quad_of(a1, j);
@@ -391,18 +403,83 @@ __device__ __forceinline__ void store_tiles(const Target& t, unsigned G, unsigne
                    bf16_pair(v0.w, v1.w)};
         }
         store_patch(patch, y, t.stride * 2, T * 32, t.m, size_t(64) * G * 2, size_t(t.n) * 2);
-    } else {
+    }
+}
+
+// The gated projection's results of four wavefronts (32 features each, side by side) and 32
+// rows meet in LDS, so that they leave in whole lines: h and kept bf16 values 256 bytes a
+// row, kept codes 128.  (Each wavefront by itself: pieces of 8 bytes for h, of 4 for codes;
+// 2048 x 4096 -> 14336 with kept codes 445 us against 387 with nothing kept.)
+constexpr unsigned kWidePitch = 272, kCodePitch = 144;
+constexpr unsigned kGatedPatch = 32 * 3 * kWidePitch;  // h, g, u; or h, codes and scales
+
+__device__ __forceinline__ void gather_gated(const Target& t, uint8_t* patch, unsigned rg,
+                                             unsigned row, unsigned h, const f32x16& a0,
+                                             const f32x16& a1) {
+    uint8_t* kept = patch + 32 * kWidePitch;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const f32x4 g = quad_of(a0, j), u = quad_of(a1, j);
+        const unsigned at = row * kWidePitch + (32 * rg + 8 * j + 4 * h) * 2;
+        *reinterpret_cast<uint2*>(patch + at) =
+            make_uint2(bf16_pair(gate_value(g.x, u.x), gate_value(g.y, u.y)),
+                       bf16_pair(gate_value(g.z, u.z), gate_value(g.w, u.w)));
+        if (t.kept) {
+            *reinterpret_cast<uint2*>(kept + at) =
+                make_uint2(bf16_pair(g.x, g.y), bf16_pair(g.z, g.w));
+            *reinterpret_cast<uint2*>(kept + 32 * kWidePitch + at) =
+                make_uint2(bf16_pair(u.x, u.y), bf16_pair(u.z, u.w));
+        }
+    }
+    if (!t.kept_q)
+        return;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const f32x16& a = i ? a1 : a0;
+        const f32x4 v[4] = {quad_of(a, 0), quad_of(a, 1), quad_of(a, 2), quad_of(a, 3)};
+        const Q8 q = q8_of(v);
+        uint8_t* codes = kept + i * 32 * kCodePitch + row * kCodePitch;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            store_quad<OUT>(t, G, token, h, j, quad_of(a0, j), quad_of(a1, j));
+            *reinterpret_cast<unsigned*>(codes + 32 * rg + 8 * j + 4 * h) = q.codes[j];
+        if (h == 0)  // (the pitch's last 16 bytes: the four wavefronts' scales)
+            *reinterpret_cast<float*>(codes + 128 + 4 * rg) = q.scale;
     }
-    if constexpr (OUT == kOutGated) {
-        if (t.kept_q && 32 * G < t.n) {
-            const f32x4 g[4] = {quad_of(a0, 0), quad_of(a0, 1), quad_of(a0, 2), quad_of(a0, 3)};
-            const f32x4 u[4] = {quad_of(a1, 0), quad_of(a1, 1), quad_of(a1, 2), quad_of(a1, 3)};
-            keep_q8(t, 32 * G, token, h, g);
-            keep_q8(t, t.n + 32 * G, token, h, u);
+}
+
+// Thread `i` of 256; features first .. first + 127, rows of x from 32T on.
+__device__ __forceinline__ void store_gated(const Target& t, const uint8_t* patch, unsigned i,
+                                            unsigned first, unsigned T) {
+    const uint8_t* kept = patch + 32 * kWidePitch;
+    auto wide = [&](const uint8_t* from, uint16_t* to, size_t stride) {  // 512 pieces
+#pragma unroll
+        for (unsigned e = 0; e < 2; ++e) {
+            const unsigned row = 16 * e + i / 16, c = i % 16 * 8;
+            const u4 v = *reinterpret_cast<const u4*>(from + row * kWidePitch + c * 2);
+            if (32 * T + row < t.m && first + c < t.n)  // (n % 32 == 0)
+                *reinterpret_cast<quad_a2*>(to + size_t(32 * T + row) * stride + first + c) =
+                    quad_a2{v.x, v.y, v.z, v.w};
         }
+    };
+    wide(patch, static_cast<uint16_t*>(t.y), t.stride);
+    if (t.kept) {
+        wide(kept, t.kept, 2 * size_t(t.n));
+        wide(kept + 32 * kWidePitch, t.kept + t.n, 2 * size_t(t.n));
+    }
+    if (!t.kept_q)
+        return;
+    const unsigned row = i / 8, c = i % 8 * 16, token = 32 * T + row;
+#pragma unroll
+    for (unsigned e = 0; e < 2; ++e) {
+        const uint8_t* codes = kept + (e * 32 + row) * kCodePitch;
+        const u4 v = *reinterpret_cast<const u4*>(codes + c);
+        if (token < t.m && first + c < t.n)
+            *reinterpret_cast<quad_a2*>(t.kept_q + size_t(token) * 2 * t.n + e * t.n + first + c) =
+                quad_a2{v.x, v.y, v.z, v.w};
+        // four of the eight threads of a row: a scale each
+        if (token < t.m && i % 8 < 4 && first + 32 * (i % 8) < t.n)
+            t.kept_d[size_t(token) * (t.n / 16) + e * (t.n / 32) + first / 32 + i % 8] =
+                *reinterpret_cast<const float*>(codes + 128 + 4 * (i % 8));
     }
 }
 
@@ -1148,6 +1225,24 @@ __global__ __launch_bounds__(512, (shares_unit<TT, OPS> ? 4 : 2)) void gemm_kern
     // (SPLIT: LDS that only this wavefront read from)
     uint8_t* patch = lds + (SPLIT ? (rg * TT + (kg ? kOwn : 0)) * 8192 : wave * kPatchBytes);
     const unsigned own = SPLIT && kg ? kOther : kOwn;
+    if constexpr (OUT == kOutGated) {
+        if (!a.partial) {
+            uint8_t* shared = lds + kg * kGatedPatch;
+            const unsigned from = first_row / 32 + kg * (SPLIT ? kOwn : TT);
+            __syncthreads();
+#pragma unroll
+            for (int t = 0; t < kOwn; ++t) {
+                const bool mine = t < int(own) && (from + t) * 32 < a.out.m;
+                if (mine)
+                    gather_gated(a.out, shared, rg, lane % 32, h, acc[0][t], acc[1][t]);
+                __syncthreads();
+                if (mine)
+                    store_gated(a.out, shared, rg * 64 + lane, tile_n * 128, from + t);
+                __syncthreads();
+            }
+            return;
+        }
+    }
     const unsigned first_tile =
         (first_row / 32) + kg * (SPLIT ? kOwn : TT);  // of 32 rows of x, the wavefront's first
 #pragma unroll
@@ -1168,7 +1263,7 @@ __global__ __launch_bounds__(512, (shares_unit<TT, OPS> ? 4 : 2)) void gemm_kern
                     for (int j = 0; j < 4; ++j)
                         to[(i * 4 + j) * 64] = quad_of(acc[i][t], j);
             }
-        } else {
+        } else if constexpr (OUT != kOutGated) {
             store_tiles<OUT>(a.out, G, T, patch, acc[0][t], acc[1][t]);
         }
     }
@@ -1302,7 +1397,7 @@ Cost cost_of(int ops, int tt) {
         return {2.0 + 0.75 * tt, 0.05 + 0.55 * tt, 0.1 + 1.35 * tt};
     const double fixed = 2.5 + 0.9 * tt;
     return ops == kTransposed ? Cost{fixed, tt == 1 ? 0.5 : 0.4 + 0.3 * tt, 0.7 + 0.6 * tt}
-                              : Cost{fixed, 0.03 + 0.33 * tt, 0.05 + 0.68 * tt};
+                              : Cost{fixed, 0.03 + 0.33 * tt, 0.05 + 0.66 * tt};
 }
 
 Plan plan_gemm(size_t m, size_t wave_groups, size_t chunks, int ops) {
@@ -1323,7 +1418,8 @@ Plan plan_gemm(size_t m, size_t wave_groups, size_t chunks, int ops) {
         const size_t tiles = size_t(p.tiles_n) * p.tiles_m;
         const size_t each = ceil_div(tiles * p.slices, cus);  // workgroups of a compute unit
         const double alone = c.fixed + p.part * c.turn, both = c.fixed + p.part * c.turn_of_two;
-        double t = shared ? double(each / 2) * both + double(each % 2) * alone
+        // (two to a unit begin and end together: what their turns hide is paid once)
+        double t = shared ? double(each / 2) * both + double(each % 2) * alone + (each > 1 ? 1.5 : 0.0)
                           : double(each) * (split ? alone : 0.93 * alone);
         if (p.slices > 1)  // (the backward pass's third launch, which is its caller's time too)
             t += (ops == kTransposed ? 4.5 : 3.5) + double(p.slices) * p.tiles_n * 4 * ceil_div(m, 32) * kTileFloats * 4 / 2.5e6;
