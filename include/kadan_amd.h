@@ -401,7 +401,8 @@ int kdq_moe_mxfp4_packed_noalloc(const uint16_t* x_bf16, const float* logits, si
  * not share.  Nothing allocates, so every call may be captured in a graph.
  * Sizes: m <= 2^20 rows of activations, k <= 2^20, n <= 2^24; strides count values, are
  * multiples of 8 and at most 2^21 for inputs, and any for outputs (products: outputs 2- or
- * 4-byte aligned); other pointers 16-byte aligned.  Scale bytes above 252 take the largest
+ * 4-byte aligned); other pointers 16-byte aligned.  No output may lie between the first
+ * and the last byte of an input or of another output.  Scale bytes above 252 take the largest
  * codes past fp32's range: such weights are infinite, or NaN (255). */
 
 /* x [rows x cols] (type KDQ_F32, KDQ_F16 or KDQ_BF16, rows x_stride values apart) as
@@ -409,7 +410,7 @@ int kdq_moe_mxfp4_packed_noalloc(const uint16_t* x_bf16, const float* logits, si
  * 0), codes value / scale rounded to the nearest E2M1 value, ties to the even code,
  * magnitudes above 6 to 6.  A block with a value that is not finite gets scale byte 255
  * and codes 0, and *status |= 1 (status may be null; the caller zeroes it).
- * x 16-byte, blocks 4-byte aligned. */
+ * x 16-byte, blocks 4-byte aligned; x_stride a multiple of 8; up to 2^35 values. */
 int kdq_mxfp4_quantize(int type, const void* x, size_t x_stride, size_t rows, size_t cols,
                        uint8_t* blocks, uint8_t* scales, unsigned* status, void* stream);
 
@@ -434,7 +435,8 @@ int kdq_mxfp4_product(const uint16_t* x_bf16, size_t x_stride, size_t m, const u
                       size_t workspace_bytes, void* stream);
 
 /* The same over MXFP4 activations (kdq_mxfp4_quantize; workspace with quantized = 1);
- * x_blocks 16-byte, x_scales 4-byte aligned. */
+ * x_blocks 16-byte, x_scales 4-byte aligned
+ * (its last bytes are read with the rest of their dword). */
 int kdq_mxfp4_product_quantized(const uint8_t* x_blocks, const uint8_t* x_scales, size_t m,
                                 const uint8_t* packed, size_t n, size_t k, int type, void* y,
                                 size_t y_stride, void* workspace, size_t workspace_bytes,
@@ -458,7 +460,7 @@ int kdq_mxfp4_gated(const uint16_t* x_bf16, size_t x_stride, size_t m,
  * (dg, then du: the gradients that adapters of the two projections need, or x^T products
  * for a float copy of the weights), and dx [m x k] bf16 = dg Wg + du Wu, the products of
  * the rounded dg and du exact and their sums fp32.  Weights from
- * kdq_mxfp4_pack_transposed(n rows, k cols). */
+ * kdq_mxfp4_pack_transposed(n rows, k cols).  m * n up to 2^35. */
 size_t kdq_mxfp4_gated_backward_workspace(size_t m, size_t n, size_t k);
 int kdq_mxfp4_gated_backward(const uint16_t* dh_bf16, size_t dh_stride, size_t m,
                              const uint16_t* kept_bf16, const int8_t* kept_q8,

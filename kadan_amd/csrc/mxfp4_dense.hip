@@ -1416,6 +1416,8 @@ Plan plan_gemm(size_t m, size_t wave_groups, size_t chunks, int ops) {
         const Cost c = cost_of(ops, tt);
         const bool shared = tt == 1 || (tt == 2 && ops != kFp4);
         const size_t tiles = size_t(p.tiles_n) * p.tiles_m;
+        if (best.slices && tiles * 512 > UINT32_MAX)
+            return;  // (a launch's threads are counted in 32 bits)
         const size_t each = ceil_div(tiles * p.slices, cus);  // workgroups of a compute unit
         const double alone = c.fixed + p.part * c.turn, both = c.fixed + p.part * c.turn_of_two;
         // (two to a unit begin and end together: what their turns hide is paid once)
@@ -1428,7 +1430,7 @@ Plan plan_gemm(size_t m, size_t wave_groups, size_t chunks, int ops) {
             best.cost = t;
         }
     };
-    for (int tt = 1; tt <= 4; ++tt)
+    for (int tt = 4; tt >= 1; --tt)
         for (size_t slices = 1; slices <= 16; ++slices)
             consider(tt, true, slices);
     if (ops == kFp4)
@@ -1858,7 +1860,7 @@ extern "C" int kdq_mxfp4_gated_backward(const uint16_t* dh_bf16, size_t dh_strid
         !k || !kept_bf16 == !kept_q8 || !kept_q8 != !kept_scales)
         return KDQ_ERR_ARGUMENT;
     if (!sizes_ok(m, n, k) || n % 32 || n > kMaxK / 2 || dh_stride < n || dh_stride % 8 ||
-        dh_stride > kMaxStride)
+        dh_stride > kMaxStride || m * (n / 8) > UINT32_MAX - 255)
         return KDQ_ERR_SHAPE;
     if (const int rc = check_output(KDQ_BF16, dx_bf16, dx_stride, m, k))
         return rc;

@@ -99,7 +99,7 @@ extern "C" int kdq_mxfp4_quantize(int type, const void* x, size_t x_stride, size
     if (type != KDQ_F32 && type != KDQ_F16 && type != KDQ_BF16)
         return KDQ_ERR_UNSUPPORTED;
     if (cols % 32 || cols > (size_t(1) << 31) || x_stride < cols || x_stride % 8 ||
-        x_stride > (SIZE_MAX >> 4) / rows || rows * (cols / 8) > (size_t(1) << 39))
+        x_stride > (SIZE_MAX >> 4) / rows || rows * (cols / 8) > UINT32_MAX - 255)
         return KDQ_ERR_SHAPE;
     if (misaligned(x, 16) || misaligned(blocks, 4))
         return KDQ_ERR_ALIGNMENT;

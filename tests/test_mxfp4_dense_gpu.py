@@ -105,10 +105,16 @@ SIZES = [  # m, n, k: each side of every tile, block, part and slice
     (129, 63, 4128), (200, 600, 2880), (255, 31, 64), (257, 1030, 288), (300, 14336, 96),
     (77, 4096, 1440), (520, 5000, 608), (1025, 2100, 320),
 ]
+# and sizes that reach every tile of the larger kernel (64, 96 and 128 rows; MXFP4 x: 256),
+# with and without K slices, ragged in each direction
+TILES = [(2933, 525, 544), (833, 4756, 544), (2083, 2856, 1632), (3219, 17, 12704),
+         (65, 11414, 12448), (2167, 770, 10272)]
+TILES_MXFP4 = [(2821, 531, 1312), (2049, 1867, 1312), (843, 9332, 1248), (2401, 2423, 1248),
+               (399, 13133, 32), (75, 30, 3872)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("m,n,k", SIZES)
+@pytest.mark.parametrize("m,n,k", SIZES + TILES)
 def test_product(device, gen, m, n, k, dtype):
     w = ref.matrix(gen, n, k)
     x = normal(gen, m, k).bfloat16()
@@ -118,7 +124,7 @@ def test_product(device, gen, m, n, k, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("m,n,k", SIZES)
+@pytest.mark.parametrize("m,n,k", SIZES + TILES_MXFP4)
 def test_product_quantized(device, gen, m, n, k, dtype):
     w, x = ref.matrix(gen, n, k), ref.matrix(gen, m, k)
     y = ops.mxfp4_product_quantized(*x, ops.mxfp4_pack(*w), n, dtype)
@@ -201,6 +207,73 @@ def test_strided_rows_and_untouched_neighbours(device, gen, m, n, k):
         assert bool((frame == 3.5).all())
 
 
+@pytest.mark.parametrize("m,k", [(5, 96), (50, 288), (300, 1056), (2100, 288)])
+def test_a_block_that_is_not_finite_stays_in_its_row_of_x(device, gen, m, k):
+    n = 1100
+    packed = ops.mxfp4_pack(*ref.matrix(gen, n, k))
+    x = normal(gen, m, k)
+    clean = ops.mxfp4_product_quantized(*ops.mxfp4_quantize(x), packed, n)
+    x[m - 2, k - 1] = float("inf")
+    blocks, scales = ops.mxfp4_quantize(x)
+    assert int(scales[m - 2, -1]) == 255
+    y = ops.mxfp4_product_quantized(blocks, scales, packed, n)
+    assert bool(torch.isnan(y[m - 2]).all())
+    rest = torch.arange(m, device=device) != m - 2
+    assert torch.equal(y[rest], clean[rest])
+
+
+@pytest.mark.parametrize("k", [32, 96, 288, 2080])
+@pytest.mark.parametrize("m", [3, 70, 260])
+def test_scales_of_x_that_start_anywhere_in_a_dword(device, gen, m, k):
+    """Rows of 1, 3, 9 and 65 scale bytes; the tensor's end followed by other data."""
+    n = 96
+    w, (blocks, scales) = ref.matrix(gen, n, k), ref.matrix(gen, m, k)
+    held = torch.full((scales.numel() + 64,), 255, dtype=torch.uint8, device=device)
+    held[:scales.numel()] = scales.reshape(-1)
+    view = held[:scales.numel()].view(m, k // 32)
+    y = ops.mxfp4_product_quantized(blocks, view, ops.mxfp4_pack(*w), n)
+    want, bound = ref.sum_bound(ref.decode(blocks, scales), ref.decode(*w))
+    ref.within(y, want, bound)
+
+
+@pytest.mark.parametrize("m", [2, 40, 300])
+def test_gated_strided_rows_and_untouched_neighbours(device, gen, m):
+    n, k = 96, 160
+    wg, wu = ref.matrix(gen, n, k), ref.matrix(gen, n, k)
+    packed = [ops.mxfp4_pack(*w) for w in (wg, wu)]
+    x = normal(gen, m, k + 8).bfloat16()[:, 8:]
+    plain = ops.mxfp4_gated(x.contiguous(), *packed, n)
+    frame = torch.full((m + 2, n + 3), 3.5, dtype=BF16, device=device)
+    assert torch.equal(ops.mxfp4_gated(x, *packed, n, out=frame[1:m + 1, 1:n + 1]), plain)
+    tg, tu = (ops.mxfp4_pack(*w, transposed=True) for w in (wg, wu))
+    dh = normal(gen, m, n + 16).bfloat16()[:, 8:8 + n]
+    kept = normal(gen, m, 2 * n).bfloat16()
+    dx, dgu = ops.mxfp4_gated_backward(dh.contiguous(), kept, tg, tu, k)
+    wide = torch.full((m + 2, k + 5), 3.5, dtype=BF16, device=device)
+    got, again = ops.mxfp4_gated_backward(dh, kept, tg, tu, k, out=wide[1:m + 1, 2:k + 2])
+    assert torch.equal(got, dx) and torch.equal(again, dgu)
+    for f, inner in ((frame, (slice(1, m + 1), slice(1, n + 1))),
+                     (wide, (slice(1, m + 1), slice(2, k + 2)))):
+        f[inner] = 3.5
+        assert bool((f == 3.5).all())
+
+
+def test_the_same_matrix_twice_and_the_same_rows_twice(device, gen):
+    """Gate and up of one tensor; rows that are each other's copies."""
+    n, k = 64, 96
+    w = ref.matrix(gen, n, k)
+    p, t = ops.mxfp4_pack(*w), ops.mxfp4_pack(*w, transposed=True)
+    for m in (4, 70):
+        row = (normal(gen, 1, k) * 0.5).bfloat16()
+        x = row.repeat(m, 1)
+        h, saved = ops.mxfp4_gated(x, p, p, n, save="bf16")
+        assert torch.equal(h, h[:1].expand_as(h)) and torch.equal(saved[:, :n], saved[:, n:])
+        *_, (want, bound) = ref.gated(x.double(), ref.decode(*w), ref.decode(*w))
+        ref.within(h, want, bound)
+        dx, dgu = ops.mxfp4_gated_backward(h, saved, t, t, k)
+        assert torch.equal(dx, dx[:1].expand_as(dx))
+
+
 def test_rows_do_not_depend_on_their_number_within_a_kernel(device, gen):
     """The same rows in calls of the same kernel give the same bits, whatever lies behind."""
     n, k = 96, 512
@@ -238,6 +311,15 @@ GATED = [(1, 32, 32), (3, 64, 96), (16, 96, 2048), (17, 2880, 320), (32, 32, 409
          (64, 160, 1056), (100, 96, 2880), (129, 2048, 96), (260, 1056, 512), (600, 288, 160)]
 
 
+# sizes that reach every tile, with and without K slices: with nothing kept, and kept
+GATED_TILES = [(67, 11456, 608), (133, 13344, 544), (2211, 1312, 1632), (3005, 32, 12512),
+               (65, 11072, 7968), (397, 2496, 9120)]
+GATED_TILES_KEPT = [(77, 10976, 544), (3291, 544, 544), (325, 9024, 1632), (2735, 32, 12448),
+                    (73, 5440, 12640), (101, 9344, 8864)]
+BACKWARD_TILES = [(129, 32, 13152), (289, 32, 13408), (385, 32, 13152), (35, 6208, 11744),
+                  (65, 4864, 11360), (109, 4896, 8288)]
+
+
 def check_q8(saved, exact, error):
     """Codes and scales against the pre-activations they stand for: a value is off by half a
     code of its block's scale, which is off by the largest error of the block."""
@@ -252,8 +334,9 @@ def check_q8(saved, exact, error):
     assert int(q.to(torch.int32).abs().max()) <= 127
 
 
-@pytest.mark.parametrize("save", [None, "bf16", "q8"])
-@pytest.mark.parametrize("m,n,k", GATED)
+@pytest.mark.parametrize("m,n,k,save", [
+    (*size, save) for save in (None, "bf16", "q8")
+    for size in GATED + (GATED_TILES_KEPT if save else GATED_TILES)])
 def test_gated(device, gen, m, n, k, save):
     wg, wu = ref.matrix(gen, n, k), ref.matrix(gen, n, k)
     x = (normal(gen, m, k) * (8 / k ** 0.5)).bfloat16()
@@ -319,7 +402,8 @@ def test_gated_q8_blocks_that_cannot_be_kept(device, gen):
 # ---------------------------------------------------------------- its backward pass
 
 @pytest.mark.parametrize("save", ["bf16", "q8"])
-@pytest.mark.parametrize("m,n,k", GATED + [(40, 2048, 2080), (7, 4128, 96), (200, 320, 5000 // 32 * 32)])
+@pytest.mark.parametrize("m,n,k", GATED + BACKWARD_TILES + [(40, 2048, 2080), (7, 4128, 96),
+                                                          (200, 320, 4992)])
 def test_gated_backward(device, gen, m, n, k, save):
     wg, wu = ref.matrix(gen, n, k), ref.matrix(gen, n, k)
     tg, tu = (ops.mxfp4_pack(*w, transposed=True) for w in (wg, wu))
@@ -430,7 +514,7 @@ def passes(gen, m, n, k):
                lambda: ops.mxfp4_gated_backward(dh, kept, t, t2, k)]
 
 
-@pytest.mark.parametrize("m,n,k", [(2, 64, 256), (70, 64, 2048)])
+@pytest.mark.parametrize("m,n,k", [(2, 64, 256), (70, 64, 2048), (300, 2880, 288)])
 def test_captured_and_replayed(device, gen, m, n, k):
     """Each operator captured once and replayed with new inputs, eager calls (one of a larger
     size, so of a larger workspace) between the replays; two graphs alive together."""
@@ -438,8 +522,7 @@ def test_captured_and_replayed(device, gen, m, n, k):
     _, larger = passes(gen, 300, 96, 2112)
     torch.cuda.synchronize()
     graphs = []
-    for f in fs:
-        f()
+    for f in fs:  # (captured before any eager call)
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             out = f()
