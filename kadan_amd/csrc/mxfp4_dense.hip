@@ -1430,9 +1430,13 @@ Plan plan_gemm(size_t m, size_t wave_groups, size_t chunks, int ops) {
             best.cost = t;
         }
     };
-    for (int tt = 4; tt >= 1; --tt)
-        for (size_t slices = 1; slices <= 16; ++slices)
+    for (int tt = 4; tt >= 1; --tt) {  // (slices up to two workgroups a compute unit)
+        const size_t tiles = ceil_div(wave_groups, 4) * ceil_div(m, size_t(tt) * 32);
+        const size_t most = std::min<size_t>({16, std::max<size_t>(1, 2 * cus / tiles),
+                                              ceil_div(chunks, ops == kFp4 ? 2 : 4)});
+        for (size_t slices = 1; slices <= most; ++slices)
             consider(tt, true, slices);
+    }
     if (ops == kFp4)
         consider(4, false, 1);
     return best;
@@ -1520,9 +1524,11 @@ template <bool GATED, bool FP4, int OUT> int run_decode(Decode a, hipStream_t st
     const unsigned units = (a.k + 127) / 128;
     // whole blocks of 32 rows a workgroup where those fill the compute units
     const bool wide = a.groups >= compute_units() && a.out.m <= 32;
-    unsigned waves = units <= 8 ? 2 : units <= 16 ? 4
-                     : units <= 64 || wide || a.out.m > 32 ? 8
-                                                           : 16;
+    // (1 row, 14336 -> 4096: 8.7 us over 16 wavefronts, 9.9 over 8; the gated projection's
+    // two matrices 14.9 and 14.1; 4096 -> 4096 5.5 and 4.9; 4096 -> 14336 13.1 and 8.1)
+    const unsigned waves = units <= 8 ? 2 : units <= 16 ? 4
+                           : units <= 48 || wide || GATED || a.out.m > 32 ? 8
+                                                                          : 16;
     a.units = (unsigned(ceil_div(units, waves)) + 1) / 2 * 2;
     if constexpr (FP4)
         if (a.out.m > 32)
@@ -1562,33 +1568,48 @@ int run_decode_t(Decode a, hipStream_t st) {
 // -> 4096 4 rows 11.2 against 12.6, 8 rows 14.0 against 12.7; 8192 -> 1024 12 rows 9.1
 // against 9.3, 20 rows 14.6 against 9.4; 2880 -> 2880 20 rows 7.5 against 8.2, 32 rows 9.4
 // against 8.3.
-bool decode_is_quicker(size_t m, size_t row_bytes, size_t row_tiles, size_t weight_bytes,
-                       bool fp4, const Plan& gemm) {
-    const double weights = double(weight_bytes) / 6.0e6;
-    const double rounds = std::max(1.0, double(row_tiles) / compute_units());
-    const double x = m * staged_pitch(unsigned(row_bytes)) <= kStagedBytes
-                         ? 0.0
-                         : double(m * row_bytes) * rounds / 33.0e3;
-    return weights + x < std::max(gemm.cost - (fp4 ? 1.0 : 3.0), weights + 2.5);
+// Where x takes less than 2.5 us no plan of gemm_kernel is the quicker, and none is made: it
+// would cost the caller about a microsecond.
+struct DecodeCost {
+    double weights, x;
+    bool certain() const {
+        return x < 2.5;
+    }
+    bool quicker_than(const Plan& gemm, bool fp4) const {
+        return certain() || x + weights < gemm.cost - (fp4 ? 1.0 : 3.0);
+    }
+};
+
+DecodeCost decode_cost(size_t m, size_t row_bytes, size_t n, size_t weight_bytes) {
+    const size_t groups = ceil_div(n, 32), cus = compute_units();
+    const size_t row_tiles = groups >= cus ? groups : ceil_div(n, 16);
+    const double rounds = std::max(1.0, double(row_tiles) / double(cus));
+    const bool staged = m * staged_pitch(unsigned(row_bytes)) <= kStagedBytes;
+    return {double(weight_bytes) / 6.0e6, staged ? 0.0 : double(m * row_bytes) * rounds / 33.0e3};
+}
+
+Plan decode_plan() {
+    Plan p{};
+    p.decode = true;
+    return p;
 }
 
 Plan plan_product(size_t m, size_t n, size_t k, bool fp4) {
-    Plan p = plan_gemm(m, ceil_div(n, 64), ceil_div(k, fp4 ? 256 : 64), fp4 ? kFp4 : kBf16);
-    const size_t groups = ceil_div(n, 32);
-    p.decode = m <= (fp4 ? 64 : 32) &&
-               decode_is_quicker(m, fp4 ? k / 2 : k * 2,
-                                 groups >= compute_units() ? groups : ceil_div(n, 16),
-                                 n * k * 17 / 32, fp4, p);
-    return p;
+    const bool few = m <= (fp4 ? 64 : 32);
+    const DecodeCost d = decode_cost(few ? m : 0, fp4 ? k / 2 : k * 2, n, n * k * 17 / 32);
+    if (few && d.certain())
+        return decode_plan();
+    const Plan p = plan_gemm(m, ceil_div(n, 64), ceil_div(k, fp4 ? 256 : 64), fp4 ? kFp4 : kBf16);
+    return few && d.quicker_than(p, fp4) ? decode_plan() : p;
 }
 
 Plan plan_gated(size_t m, size_t n, size_t k, bool kept) {
-    Plan p = plan_gemm(m, ceil_div(n, 32), ceil_div(k, 64), kBf16);
-    const size_t groups = ceil_div(n, 32);
-    p.decode = !kept && m <= 32 &&
-               decode_is_quicker(m, k * 2, groups >= compute_units() ? groups : ceil_div(n, 16),
-                                 n * k * 17 / 16, false, p);
-    return p;
+    const bool few = !kept && m <= 32;
+    const DecodeCost d = decode_cost(few ? m : 0, k * 2, n, n * k * 17 / 16);
+    if (few && d.certain())
+        return decode_plan();
+    const Plan p = plan_gemm(m, ceil_div(n, 32), ceil_div(k, 64), kBf16);
+    return few && d.quicker_than(p, false) ? decode_plan() : p;
 }
 
 // (decode_t_kernel is bound by decoding the weights, which half the compute units do where
