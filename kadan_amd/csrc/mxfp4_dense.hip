@@ -573,6 +573,9 @@ __global__ __launch_bounds__(1024) void decode_kernel(Decode a) {
     const unsigned lane_codes = (q / 2) * 1024 + block_row * 16, lane_scales = block_row * 4;
     // (an even number of units: a dword of scales is two)
     const unsigned begin = wave * a.units, end = begin + a.units;
+    // x ends with the run as well: a batch past it would multiply the zeros that stand for its
+    // weights by the next wavefront's x, which may be infinite
+    const unsigned limit = min(a.k, end * 128);
     u4 c[kBatch][TILES];
     unsigned s[kScales][TILES];
     auto load = [&](unsigned t0) {  // units past K, or past the wavefront's run, are zeros
@@ -615,7 +618,7 @@ __global__ __launch_bounds__(1024) void decode_kernel(Decode a) {
 #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
             const unsigned t = t0 + b;
-            const bool inside = 128 * t + 32 * q < a.k;
+            const bool inside = 128 * t + 32 * q < limit;
 #pragma unroll
             for (int i = 0; i < TB; ++i) {
                 const unsigned token = r + 16 * i;
@@ -728,6 +731,7 @@ __global__ __launch_bounds__(1024) void decode_t_kernel(Decode a) {
     const unsigned lane_codes = (q / 2) * 2048 + (16 * e + r + 32 * (q % 2)) * 16;
     const unsigned lane_scales = (q / 2) * 128 + (2 * (q % 2) + e) * 32;
     const unsigned begin = wave % share * a.units, end = begin + a.units;
+    const unsigned limit = min(a.k, end * 128);  // x ends with the run, as decode_kernel's
     f32x4 acc[2][TB] = {};
     struct Batch {
         u4 c[kBatch][2], s[kBatch][2];
@@ -755,7 +759,7 @@ __global__ __launch_bounds__(1024) void decode_t_kernel(Decode a) {
 #pragma unroll
             for (int i = 0; i < TB; ++i) {
                 const unsigned token = r + 16 * i;
-                const int at = token < rows && from < a.k ? int(token * a.x_stride + from * 2)
+                const int at = token < rows && from < limit ? int(token * a.x_stride + from * 2)
                                                           : kOutside - 64;
 #pragma unroll
                 for (int d = 0; d < 4; ++d)

@@ -191,6 +191,44 @@ def test_values_that_are_not_finite_stay_in_their_row(device, gen, m, k):
     assert torch.equal(torch.nan_to_num(y[1].double(), nan=7.0), torch.nan_to_num(want, nan=7.0))
 
 
+def without_zeros(blocks):
+    """The codes with 0 made 0.5, so that an infinity's products are infinite."""
+    return blocks | ((blocks & 0x07) == 0).to(torch.uint8) | \
+        (((blocks & 0x70) == 0).to(torch.uint8) << 4)
+
+
+@pytest.mark.parametrize("k", [512, 640, 1440, 4352, 9600])
+@pytest.mark.parametrize("m", [4, 12, 20, 32, 70])
+def test_an_infinity_anywhere_in_a_row_is_the_rows_result(device, gen, m, k):
+    """Wherever the wavefronts' shares of a row end, and a batch past such an end."""
+    n = 48
+    blocks, scales = ref.matrix(gen, n, k)
+    blocks = without_zeros(blocks)
+    packed, w = ops.mxfp4_pack(blocks, scales), ref.decode(blocks, scales)
+    for first in range(0, k, 32 * m):
+        at = (torch.arange(m, device=device) * 32 + first) % k
+        x = normal(gen, m, k).bfloat16()
+        x[torch.arange(m, device=device), at] = float("inf")
+        want = w[:, at].t().sign() * float("inf")
+        assert torch.equal(ops.mxfp4_product(x, packed, n).double(), want)
+
+
+@pytest.mark.parametrize("n", [512, 640, 1440, 4352])
+@pytest.mark.parametrize("m", [4, 12, 20, 32, 70])
+def test_an_infinite_gradient_anywhere_in_a_row_is_the_rows_result(device, gen, m, n):
+    k = 96
+    blocks, scales = ref.matrix(gen, n, k)
+    blocks = without_zeros(blocks)
+    packed, w = ops.mxfp4_pack(blocks, scales, transposed=True), ref.decode(blocks, scales)
+    kept = torch.ones(m, 2 * n, dtype=BF16, device=device)
+    for first in range(0, n, 32 * m):
+        at = (torch.arange(m, device=device) * 32 + first) % n
+        dh = normal(gen, m, n).bfloat16()
+        dh[torch.arange(m, device=device), at] = float("inf")
+        dx, _ = ops.mxfp4_gated_backward(dh, kept, packed, packed, k)
+        assert torch.equal(dx.double(), w[at].sign() * float("inf"))
+
+
 @pytest.mark.parametrize("m,n,k", [(1, 40, 96), (20, 70, 64), (50, 100, 160), (140, 300, 96)])
 def test_strided_rows_and_untouched_neighbours(device, gen, m, n, k):
     w = ref.matrix(gen, n, k)
