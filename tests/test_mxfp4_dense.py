@@ -190,5 +190,19 @@ def test_gradient_formula_against_differences():
     e = 1e-6
     numeric = torch.cat([(f(g + e, u) - f(g - e, u)) / (2 * e),
                          (f(g, u + e) - f(g, u - e)) / (2 * e)], 1)
-    # central differences: e^2 / 6 times the third derivative, and cancellation of 2^-53 / e
-    assert float((want - numeric).abs().max()) < 1e-12 * 50 + 1e-7
+    # Central differences of f in x are off by e^2 / 6 times the third derivative, which is below
+    # |dh u| in g (silu's is below 1) and 0 in u; by the rounding of f's two values, 8 * 2^-53 of
+    # them (three products and a sigmoid of at most five roundings), over e; and by that of
+    # x + e and x - e, 2^-53 of them each, times the slope, over e.  Slopes are at most
+    # 1.1 |dh u| in g and |dh g| in u.  The formula itself is off by a few of its terms' roundings.
+    half = 2.0 ** -53
+
+    def bound(x, slope, third):
+        value = f(g, u).abs() + slope * e
+        return third * e * e / 6 + (8 * half * value + half * (x.abs() + e) * slope) / e
+
+    terms = (dh * u).abs() * (2 + 2 * g.abs()) + (dh * g).abs()
+    limit = torch.cat([bound(g, 1.1 * (dh * u).abs(), (dh * u).abs()),
+                       bound(u, (dh * g).abs(), torch.zeros_like(g))], 1)
+    limit = limit + 16 * half * torch.cat([terms, terms], 1)
+    assert bool(((want - numeric).abs() <= limit).all())
