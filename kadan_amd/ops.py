@@ -464,11 +464,19 @@ def _scratch(size: int, device) -> torch.Tensor | None:
 
 def mxfp4_quantize(x: torch.Tensor, status: torch.Tensor | None = None):
     """fp32, fp16 or bf16 [rows, cols] (cols % 32 == 0) as MXFP4: blocks uint8
-    [rows, cols/2] and scales uint8 [rows, cols/32] (kdq_mxfp4_quantize)."""
+    [rows, cols/2] and scales uint8 [rows, cols/32]; ``status``, an int32, is set to 1 where
+    a value is not finite (kdq_mxfp4_quantize)."""
+    if status is None:
+        flag, parts = None, (x,)
+    else:
+        _need(status, torch.int32, "status")
+        if not status.numel():
+            raise ValueError("status: expected one value")
+        flag, parts = status.data_ptr(), (x, status)
     dtype = x.dtype
     kind = _type(dtype)
     stride = _row_stride(x, dtype, "x")
-    stream = _stream_for(x)
+    stream = _stream_for(*parts)
     rows, cols = x.shape
     if cols % 32:
         raise ValueError("x: a row must be whole blocks of 32 values")
@@ -476,7 +484,7 @@ def mxfp4_quantize(x: torch.Tensor, status: torch.Tensor | None = None):
     blocks = torch.empty(rows, cols // 2, dtype=torch.uint8, device=device)
     scales = torch.empty(rows, cols // 32, dtype=torch.uint8, device=device)
     call("kdq_mxfp4_quantize", kind, x.data_ptr(), stride, rows, cols, blocks.data_ptr(),
-         scales.data_ptr(), _ptr(status), stream)
+         scales.data_ptr(), flag, stream)
     return blocks, scales
 
 

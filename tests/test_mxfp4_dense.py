@@ -168,6 +168,13 @@ def test_wrappers_refuse_host_tensors(dtype):
         ops.mxfp4_pack(u8.view(1, -1), u8[:80].view(1, -1))
 
 
+@pytest.mark.parametrize("status", [torch.zeros(1, dtype=torch.int32), torch.zeros(1),
+                                    torch.zeros(0, dtype=torch.int32)])
+def test_quantize_refuses_a_status_that_the_device_cannot_write(status):
+    with pytest.raises(ValueError, match="status"):
+        ops.mxfp4_quantize(torch.zeros(2, 64), status)
+
+
 def test_reference_quantiser_is_nearest_and_ties_to_even():
     """The oracle of the GPU tests, by hand: the format's own values, ties, and saturation."""
     row = np.zeros((1, 32))
