@@ -1421,7 +1421,7 @@ Plan plan_gemm(size_t m, size_t wave_groups, size_t chunks, int ops) {
         const bool shared = tt == 1 || (tt == 2 && ops != kFp4);
         const size_t tiles = size_t(p.tiles_n) * p.tiles_m;
         if (best.slices && tiles * 512 > UINT32_MAX)
-            return;  // (a launch's threads are counted in 32 bits)
+            return;  // (a launch's threads are counted in 32 bits; the largest tiles come first)
         const size_t each = ceil_div(tiles * p.slices, cus);  // workgroups of a compute unit
         const double alone = c.fixed + p.part * c.turn, both = c.fixed + p.part * c.turn_of_two;
         // (two to a unit begin and end together: what their turns hide is paid once)
@@ -1626,8 +1626,25 @@ Plan plan_backward(size_t m, size_t n, size_t k) {
     return p;
 }
 
+// (a packing launch counts its threads, one per 16 bytes of codes or 4 of scales, in 32 bits)
+constexpr size_t kMaxCodes = size_t(1) << 35;
+
+bool packs(size_t rows, size_t cols) {
+    return rows && cols && cols % 32 == 0 && rows <= kMaxN && cols <= kMaxK &&
+           packed_form(rows, cols).code_bytes <= kMaxCodes;
+}
+
+bool packs_transposed(size_t rows, size_t cols) {
+    return rows && cols && cols % 32 == 0 && rows <= kMaxK && cols <= kMaxK &&
+           transposed_form(rows, cols).code_bytes <= kMaxCodes;
+}
+
 bool sizes_ok(size_t m, size_t n, size_t k) {
-    return m <= kMaxRows && n <= kMaxN && k <= kMaxK && k % 32 == 0;
+    return m <= kMaxRows && packs(n, k);
+}
+
+bool backward_sizes_ok(size_t m, size_t n, size_t k) {
+    return m <= kMaxRows && n % 32 == 0 && n <= kMaxK / 2 && packs_transposed(n, k);
 }
 
 // Bytes of `rows` rows `stride` values apart, `cols` values of `size` bytes each.
@@ -1671,7 +1688,7 @@ int launch_pack(K kernel, const Form& f, const uint8_t* blocks, const uint8_t* s
 using namespace kdq;
 
 extern "C" size_t kdq_mxfp4_packed_bytes(size_t rows, size_t cols) {
-    if (!rows || !cols || cols % 32 || rows > kMaxN || cols > kMaxK)
+    if (!packs(rows, cols))
         return 0;
     const Form f = packed_form(rows, cols);
     return f.code_bytes + f.scale_bytes;
@@ -1690,7 +1707,7 @@ extern "C" int kdq_mxfp4_pack(const uint8_t* blocks, const uint8_t* scales, size
 }
 
 extern "C" size_t kdq_mxfp4_packed_transposed_bytes(size_t rows, size_t cols) {
-    if (!rows || !cols || cols % 32 || rows > kMaxK || cols > kMaxK)
+    if (!packs_transposed(rows, cols))
         return 0;
     const Form f = transposed_form(rows, cols);
     return f.code_bytes + f.scale_bytes;
@@ -1722,7 +1739,7 @@ extern "C" size_t kdq_mxfp4_gated_workspace(size_t m, size_t n, size_t k, int ke
 }
 
 extern "C" size_t kdq_mxfp4_gated_backward_workspace(size_t m, size_t n, size_t k) {
-    if (!m || !n || !k || !sizes_ok(m, n, k) || n % 32 || n > kMaxK / 2)
+    if (!m || !n || !k || !backward_sizes_ok(m, n, k))
         return 0;
     return partial_bytes(plan_backward(m, n, k), m);
 }
@@ -1884,7 +1901,7 @@ extern "C" int kdq_mxfp4_gated_backward(const uint16_t* dh_bf16, size_t dh_strid
     if (!dh_bf16 || !gate_transposed || !up_transposed || !dgu_bf16 || !dx_bf16 || !m || !n ||
         !k || !kept_bf16 == !kept_q8 || !kept_q8 != !kept_scales)
         return KDQ_ERR_ARGUMENT;
-    if (!sizes_ok(m, n, k) || n % 32 || n > kMaxK / 2 || dh_stride < n || dh_stride % 8 ||
+    if (!backward_sizes_ok(m, n, k) || dh_stride < n || dh_stride % 8 ||
         dh_stride > kMaxStride || m * (n / 8) > UINT32_MAX - 255)
         return KDQ_ERR_SHAPE;
     if (const int rc = check_output(KDQ_BF16, dx_bf16, dx_stride, m, k))

@@ -175,6 +175,27 @@ def test_quantize_refuses_a_status_that_the_device_cannot_write(status):
         ops.mxfp4_quantize(torch.zeros(2, 64), status)
 
 
+def test_matrices_past_a_launch_of_32_bits_are_refused():
+    """A packing launch counts its threads in 32 bits: up to 2^36 values, 32 GB of codes."""
+    lib = kadan_amd.lib()
+    far = 1 << 45
+    assert lib.kdq_mxfp4_packed_bytes(1 << 23, 1 << 13) == (1 << 35) + (1 << 31)
+    assert lib.kdq_mxfp4_packed_bytes((1 << 23) + 1, 1 << 13) == 0
+    assert lib.kdq_mxfp4_pack(W, far, 1 << 24, 1 << 13, 2 * far, None) == 2
+    assert lib.kdq_mxfp4_packed_transposed_bytes(1 << 18, 1 << 18) == (1 << 35) + (1 << 31)
+    assert lib.kdq_mxfp4_packed_transposed_bytes(1 << 18, (1 << 18) + 32) == 0
+    assert lib.kdq_mxfp4_pack_transposed(W, far, 1 << 20, 1 << 18, 2 * far, None) == 2
+    n, k = 1 << 24, 1 << 13
+    assert lib.kdq_mxfp4_product_workspace(1, n, k, 0) == 0
+    assert lib.kdq_mxfp4_product(X, k, 1, far, n, k, 0, 2 * far, n, None, 0, None) == 2
+    assert lib.kdq_mxfp4_product_quantized(X, Z, 1, far, n, k, 0, 2 * far, n, None, 0, None) == 2
+    assert lib.kdq_mxfp4_gated(X, k, 1, far, 2 * far, n, k, 4 * far, n, None, None, None, None, 0,
+                               None) == 2
+    n = k = 1 << 19
+    assert lib.kdq_mxfp4_gated_backward(X, n, 1, Y, None, None, far, 2 * far, n, k, Z, W, k, None,
+                                        0, None) == 2
+
+
 def test_reference_quantiser_is_nearest_and_ties_to_even():
     """The oracle of the GPU tests, by hand: the format's own values, ties, and saturation."""
     row = np.zeros((1, 32))
