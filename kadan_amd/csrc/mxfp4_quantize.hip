@@ -33,7 +33,8 @@ __device__ __forceinline__ unsigned quad_max(unsigned v) {
 // block's largest magnitude less 2 (E2M1's largest exponent), at least 0; the conversion
 // rounds value / 2^(byte - 127) to the nearest code, ties to the even one, past 6 to 6
 // (checked on the device around every tie, for the smallest and largest scales too).
-// Bound by memory: 2048 x 4096 bf16 read and 4.25 bits a value written.
+// Bound by memory: 14336 x 4096 fp32 58 us (235 MB read, 31 written, 4.6 TB/s); a few rows by
+// the launch (4 x 2880 2 us).
 template <int TYPE, bool DENSE>
 __global__ __launch_bounds__(256) void quantize_kernel(const void* __restrict__ x, size_t stride,
                                                        size_t eighths, unsigned per_row,
