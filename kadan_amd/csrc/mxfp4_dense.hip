@@ -1071,11 +1071,15 @@ __global__ __launch_bounds__(512, (shares_unit<TT, OPS> ? 4 : 2)) void gemm_kern
     for (int t = 0; t < TT; ++t)
         acc[0][t] = acc[1][t] = f32x16{};
 
-    // A wavefront's loads return in order.  Chunk c's copies were issued three chunks ago; at
-    // least the copies of the two chunks after it, the weights of three chunks and the
-    // scales of those were issued behind them, so a wait for all but that many is a wait for
-    // the chunk, and the barrier makes it everyone's.
-    constexpr int kCodeLoads = (OPS == kTransposed ? 4 : 2) * int(kStepsPerChunk);
+    // A wavefront's loads return in order.  Chunk c's copies were issued three chunks ago; the
+    // copies of the two chunks after it, the weights of three chunks and their scales were
+    // issued behind them, so a wait for all but that many is a wait for the chunk, and the
+    // barrier makes it everyone's.  The first three chunks' copies are issued before the loop,
+    // and only kAhead steps of weights behind them: kBehindFirst loads lie behind chunk 0's.
+    constexpr int kStepLoads = OPS == kTransposed ? 4 : 2;
+    constexpr int kCodeLoads = kStepLoads * int(kStepsPerChunk);
+    constexpr int kScaleLoads = OPS == kTransposed ? 0 : 2;  // of four steps
+    constexpr int kBehindFirst = 2 * TT + kScaleLoads + kAhead * kStepLoads;
     auto arrive = [&]<int BEHIND>() {
         static_assert(BEHIND < 64, "vmcnt holds six bits");
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(BEHIND) : "memory");
@@ -1123,7 +1127,7 @@ __global__ __launch_bounds__(512, (shares_unit<TT, OPS> ? 4 : 2)) void gemm_kern
         load_codes(begin_step + i, codes[i]);
 
     if constexpr (OPS == kFp4) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // fewer loads than the loop counts on
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (the first turn's loads are fewer)
         // (32 rows on, a row's bytes start the same)
         const unsigned scale_shift = (odd + lane % 32 * x_blocks) % 4;
         for (unsigned c0 = 0; c0 < a.part; c0 += 4) {
@@ -1183,10 +1187,17 @@ __global__ __launch_bounds__(512, (shares_unit<TT, OPS> ? 4 : 2)) void gemm_kern
             });
         }
     } else {
+        // scales are loaded in chunk 0 of four, which is one of the three behind the others
+        constexpr int kBehind = 2 * TT + 3 * kCodeLoads;
+        // (the first turn's chunks 1 and 2: what the loop issued for the chunks before them too)
+        static_assert(kBehindFirst + kCodeLoads + kScaleLoads >= kBehind + kScaleLoads &&
+                          kBehindFirst + 2 * kCodeLoads + kScaleLoads >= kBehind + kScaleLoads,
+                      "a wait of the first turn counts loads that were not issued");
+        if constexpr (kBehindFirst < kBehind)  // (kTransposed: 8 loads of weights, not 12)
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kBehindFirst) : "memory");
         for (unsigned c0 = 0; c0 < a.part; c0 += 4) {
             static_for<4>([&]<int C>() {
-                constexpr int kScaleLoads = OPS == kTransposed || C == 0 ? 0 : 2;
-                arrive.template operator()<2 * TT + 3 * kCodeLoads + kScaleLoads>();
+                arrive.template operator()<kBehind + (C == 0 ? 0 : kScaleLoads)>();
                 const uint8_t* buf = x_lane + C * kStageBytes;
                 stage(c0 + C + 3, (C + 3) % kStages);
                 if constexpr (C == 0)

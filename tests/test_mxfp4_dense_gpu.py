@@ -465,6 +465,25 @@ def test_gated_backward(device, gen, m, n, k, save):
     ref.within(dx, full, bound @ both.abs().T + rounded(y, e, BF16) + 1e-30, "dx")
 
 
+@pytest.mark.parametrize("m,n,k", BACKWARD_TILES + [(64, 768, 2048)])
+def test_gated_backward_reads_nothing_of_the_kernel_before(device, gen, m, n, k):
+    """Calls right behind a product whose rows are NaN, which leaves NaN in every compute unit's
+    LDS, and behind nothing, with dgu out of the caches: the same bits."""
+    t, t2 = (ops.mxfp4_pack(*ref.matrix(gen, n, k), transposed=True) for _ in range(2))
+    dh, kept = normal(gen, m, n).bfloat16(), normal(gen, m, 2 * n).bfloat16()
+    want = ops.mxfp4_gated_backward(dh, kept, t, t2, k)
+    packed = ops.mxfp4_pack(*ref.matrix(gen, 8192, 1024))
+    bad = torch.full((1024, 1024), float("nan"), dtype=BF16, device=device)
+    other = torch.empty(1 << 29, dtype=torch.uint8, device=device)
+    for i in range(12):
+        if i % 2:
+            other.fill_(i)
+        ops.mxfp4_product(bad, packed, 8192, BF16)
+        got = ops.mxfp4_gated_backward(dh, kept, t, t2, k)
+        assert bool(torch.isfinite(got[0]).all())
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_gated_backward_against_differences(device, gen):
     """The loss sum(dh * h(x)) in 64 bits along random directions, by central differences."""
     m, n, k = 12, 64, 96
