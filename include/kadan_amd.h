@@ -422,7 +422,9 @@ size_t kdq_mxfp4_packed_bytes(size_t rows, size_t cols);
 int kdq_mxfp4_pack(const uint8_t* blocks, const uint8_t* scales, size_t rows, size_t cols,
                    uint8_t* packed, void* stream);
 
-/* Packs a matrix for kdq_mxfp4_gated_backward, which sums over its rows (at most 2^19). */
+/* Packs a matrix for kdq_mxfp4_gated_backward, which sums over its rows (at most 2^19).  The
+ * two forms of a matrix may take the same number of bytes and carry no mark: the caller keeps
+ * them apart. */
 size_t kdq_mxfp4_packed_transposed_bytes(size_t rows, size_t cols);
 int kdq_mxfp4_pack_transposed(const uint8_t* blocks, const uint8_t* scales, size_t rows,
                               size_t cols, uint8_t* packed, void* stream);

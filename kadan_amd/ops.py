@@ -440,11 +440,33 @@ def _mxfp4_sizes(matrix: str, rows: int, cols: int, workspace: str, *sizes: int)
 _PACKED, _TRANSPOSED = "kdq_mxfp4_packed_bytes", "kdq_mxfp4_packed_transposed_bytes"
 
 
-def _matrix(packed: torch.Tensor, size: int, name: str) -> int:
+def _packed(packed: torch.Tensor, size: int, name: str) -> None:
     if packed.dtype != torch.uint8 or not packed.is_cuda or not packed.is_contiguous():
         raise ValueError(f"{name}: expected a packed uint8 device tensor")
     if not size or packed.numel() != size:
         raise ValueError(f"{name}: not the packed size of this call's matrix")
+
+
+# The two packed forms of a matrix may take the same number of bytes (14336 x 4096 does), so
+# they are told apart by their shape: flat for the products, a row per 64 columns transposed.
+def _matrix(packed: torch.Tensor, size: int, name: str) -> int:
+    _packed(packed, size, name)
+    if packed.dim() != 1:
+        raise ValueError(f"{name}: expected mxfp4_pack's flat tensor (not the transposed form)")
+    return packed.data_ptr()
+
+
+def _transposed_shape(size: int, cols: int) -> tuple[int, int]:
+    groups = (cols + 63) // 64
+    return groups, size // groups
+
+
+def _transposed_matrix(packed: torch.Tensor, size: int, cols: int, name: str) -> int:
+    _packed(packed, size, name)
+    groups, width = _transposed_shape(size, cols)
+    if packed.dim() != 2 or packed.shape[0] != groups:
+        raise ValueError(f"{name}: expected mxfp4_pack(..., transposed=True)'s "
+                         f"[{groups}, {width}]")
     return packed.data_ptr()
 
 
@@ -490,14 +512,17 @@ def mxfp4_quantize(x: torch.Tensor, status: torch.Tensor | None = None):
 
 def mxfp4_pack(blocks: torch.Tensor, scales: torch.Tensor,
                transposed: bool = False) -> torch.Tensor:
-    """An MXFP4 matrix in the form the products read (kdq_mxfp4_pack), or, ``transposed``,
-    in the one that mxfp4_gated_backward reads (kdq_mxfp4_pack_transposed)."""
+    """An MXFP4 matrix in the form the products read, uint8 [bytes] (kdq_mxfp4_pack), or,
+    ``transposed``, in the one that mxfp4_gated_backward reads, uint8 [ceil(cols / 64), bytes of
+    64 columns] (kdq_mxfp4_pack_transposed).  The shape is what tells the two forms apart; of
+    matrices of other sizes the calls see the number of bytes alone."""
     rows, cols = _blocks(blocks, scales)
     stream = _stream_for(blocks, scales)
     size = _mxfp4_size(_TRANSPOSED if transposed else _PACKED, rows, cols)
     if not size:
         raise ValueError(f"a matrix of {rows} x {cols} has no packed form")
-    packed = torch.empty(size, dtype=torch.uint8, device=blocks.device)
+    packed = torch.empty(_transposed_shape(size, cols) if transposed else size,
+                         dtype=torch.uint8, device=blocks.device)
     call("kdq_mxfp4_pack_transposed" if transposed else "kdq_mxfp4_pack", blocks.data_ptr(),
          scales.data_ptr(), rows, cols, packed.data_ptr(), stream)
     return packed
@@ -594,7 +619,8 @@ def mxfp4_gated_backward(dh: torch.Tensor, saved, gate: torch.Tensor, up: torch.
         raise ValueError("n_out and n_in must be multiples of 32")
     weights, size = _mxfp4_sizes(_TRANSPOSED, n, n_in, "kdq_mxfp4_gated_backward_workspace", m,
                                  n, n_in)
-    wg, wu = _matrix(gate, weights, "gate"), _matrix(up, weights, "up")
+    wg = _transposed_matrix(gate, weights, n_in, "gate")
+    wu = _transposed_matrix(up, weights, n_in, "up")
     kept = codes = scales = None
     if isinstance(saved, torch.Tensor):
         _need(saved, _BF16, "saved")

@@ -175,6 +175,37 @@ def test_quantize_refuses_a_status_that_the_device_cannot_write(status):
         ops.mxfp4_quantize(torch.zeros(2, 64), status)
 
 
+class Packed:
+    """What the wrappers look at of a packed device tensor."""
+    dtype, is_cuda = torch.uint8, True
+
+    def __init__(self, *shape):
+        self.shape = torch.Size(shape)
+        self.dim, self.numel = lambda: len(shape), self.shape.numel
+        self.is_contiguous, self.data_ptr = lambda: True, lambda: W
+
+
+@pytest.mark.parametrize("rows,cols", [(64, 256), (14336, 4096), (4096, 8192), (64, 64)])
+def test_the_two_packed_forms_are_told_apart(rows, cols):
+    """Also where they take the same number of bytes, or the same but for a few."""
+    lib = kadan_amd.lib()
+    size = lib.kdq_mxfp4_packed_bytes(rows, cols)
+    transposed = lib.kdq_mxfp4_packed_transposed_bytes(rows, cols)
+    assert (size == transposed) == (cols != 64)
+    groups = cols // 64
+    t = Packed(groups, transposed // groups)
+    assert ops._matrix(Packed(size), size, "packed") == W
+    assert ops._transposed_matrix(t, transposed, cols, "gate") == W
+    with pytest.raises(ValueError, match="gate"):
+        ops._transposed_matrix(Packed(size), transposed, cols, "gate")
+    with pytest.raises(ValueError, match="packed"):
+        ops._matrix(t, size, "packed")
+    if groups > 1:  # another matrix of as many bytes
+        with pytest.raises(ValueError, match="gate"):
+            ops._transposed_matrix(Packed(groups // 2, 2 * transposed // groups), transposed, cols,
+                                   "gate")
+
+
 def test_matrices_past_a_launch_of_32_bits_are_refused():
     """A packing launch counts its threads in 32 bits: up to 2^36 values, 32 GB of codes."""
     lib = kadan_amd.lib()

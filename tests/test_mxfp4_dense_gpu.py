@@ -660,3 +660,21 @@ def test_refusals_on_the_device(device, gen):
     with pytest.raises(ValueError):
         ops.mxfp4_product_quantized(w[0], w[1][:, :3].contiguous(), p, 64)
     torch.cuda.synchronize()
+
+
+def test_the_other_packed_form_is_refused(device, gen):
+    n, k = 64, 256  # 8704 bytes in both
+    w = ref.matrix(gen, n, k)
+    p, t = ops.mxfp4_pack(*w), ops.mxfp4_pack(*w, transposed=True)
+    assert p.numel() == t.numel() and t.shape == (4, 2176)
+    x, dh = normal(gen, 3, k).bfloat16(), normal(gen, 3, n).bfloat16()
+    kept = normal(gen, 3, 2 * n).bfloat16()
+    for call in (lambda: ops.mxfp4_product(x, t, n),
+                 lambda: ops.mxfp4_product_quantized(*ops.mxfp4_quantize(x), t, n),
+                 lambda: ops.mxfp4_gated(x, t, p, n), lambda: ops.mxfp4_gated(x, p, t, n),
+                 lambda: ops.mxfp4_gated_backward(dh, kept, p, t, k),
+                 lambda: ops.mxfp4_gated_backward(dh, kept, t, p, k),
+                 lambda: ops.mxfp4_gated_backward(dh, kept, t, t.view(-1), k)):
+        with pytest.raises(ValueError):
+            call()
+    torch.cuda.synchronize()
