@@ -402,9 +402,10 @@ int kdq_moe_mxfp4_packed_noalloc(const uint16_t* x_bf16, const float* logits, si
  * Sizes: m <= 2^20 rows of activations, k <= 2^20, n <= 2^24, and a matrix of at most 2^36
  * values (its rows rounded up to 32, or 64 transposed, its columns to 64); strides count
  * values, are multiples of 8 and at most 2^21 for inputs, and any for outputs (products:
- * outputs 2- or 4-byte aligned); other pointers 16-byte aligned.  No output may lie between
- * the first and the last byte of an input or of another output.  Scale bytes above 252 take
- * the largest codes past fp32's range: such weights are infinite, or NaN (255). */
+ * outputs 2- or 4-byte aligned); other pointers 16-byte aligned.  No output, and no byte of
+ * the workspace, may lie between the first and the last byte of an input or of another output.
+ * Scale bytes above 252 take the largest codes past fp32's range: such weights are infinite,
+ * or NaN (255). */
 
 /* x [rows x cols] (type KDQ_F32, KDQ_F16 or KDQ_BF16, rows x_stride values apart) as
  * MXFP4: per 32 values the scale is 2^(floor(log2(largest magnitude)) - 2) (byte at least

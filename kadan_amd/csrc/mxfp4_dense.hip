@@ -1704,6 +1704,25 @@ size_t extent(size_t rows, size_t stride, size_t cols, size_t size) {
     return ((rows - 1) * stride + cols) * size;
 }
 
+struct Range {
+    const void* p;
+    size_t bytes;
+};
+
+// Whether one of the ranges that a call writes (its workspace among them, as far as the caller
+// says it may) overlaps one that it reads, or another that it writes.
+template <size_t N, size_t M> bool any_overlap(const Range (&out)[N], const Range (&in)[M]) {
+    for (size_t i = 0; i < N; ++i) {
+        for (const Range& b : in)
+            if (overlaps(out[i].p, out[i].bytes, b.p, b.bytes))
+                return true;
+        for (size_t j = 0; j < i; ++j)
+            if (overlaps(out[i].p, out[i].bytes, out[j].p, out[j].bytes))
+                return true;
+    }
+    return false;
+}
+
 constexpr size_t kMaxStride = size_t(1) << 21;  // 256 rows stay within a buffer's range
 
 int check_workspace(size_t need, const void* workspace, size_t bytes) {
@@ -1833,10 +1852,11 @@ extern "C" int kdq_mxfp4_product(const uint16_t* x_bf16, size_t x_stride, size_t
         return rc;
     if (misaligned(x_bf16, 16) || misaligned(packed, 16))
         return KDQ_ERR_ALIGNMENT;
-    const size_t y_bytes = extent(m, y_stride, n, type == KDQ_F32 ? 4 : 2);
-    if (overlaps(y, y_bytes, x_bf16, extent(m, x_stride, k, 2)) ||
-        overlaps(y, y_bytes, packed, kdq_mxfp4_packed_bytes(n, k)) ||
-        overlaps(y, y_bytes, workspace, workspace_bytes))
+    const Range out[] = {{y, extent(m, y_stride, n, type == KDQ_F32 ? 4 : 2)},
+                         {workspace, workspace_bytes}},
+                in[] = {{x_bf16, extent(m, x_stride, k, 2)},
+                        {packed, kdq_mxfp4_packed_bytes(n, k)}};
+    if (any_overlap(out, in))
         return KDQ_ERR_ALIAS;
     const Plan p = plan_product(m, n, k, false);
     if (const int rc = check_workspace(partial_bytes(p, m), workspace, workspace_bytes))
@@ -1865,11 +1885,12 @@ extern "C" int kdq_mxfp4_product_quantized(const uint8_t* x_blocks, const uint8_
         return rc;
     if (misaligned(x_blocks, 16) || misaligned(x_scales, 4) || misaligned(packed, 16))
         return KDQ_ERR_ALIGNMENT;
-    const size_t y_bytes = extent(m, y_stride, n, type == KDQ_F32 ? 4 : 2);
-    if (overlaps(y, y_bytes, x_blocks, m * (k / 2)) ||
-        overlaps(y, y_bytes, x_scales, m * (k / 32)) ||
-        overlaps(y, y_bytes, packed, kdq_mxfp4_packed_bytes(n, k)) ||
-        overlaps(y, y_bytes, workspace, workspace_bytes))
+    const Range out[] = {{y, extent(m, y_stride, n, type == KDQ_F32 ? 4 : 2)},
+                         {workspace, workspace_bytes}},
+                in[] = {{x_blocks, m * (k / 2)},
+                        {x_scales, m * (k / 32)},
+                        {packed, kdq_mxfp4_packed_bytes(n, k)}};
+    if (any_overlap(out, in))
         return KDQ_ERR_ALIAS;
     const Plan p = plan_product(m, n, k, true);
     if (const int rc = check_workspace(partial_bytes(p, m), workspace, workspace_bytes))
@@ -1902,25 +1923,16 @@ extern "C" int kdq_mxfp4_gated(const uint16_t* x_bf16, size_t x_stride, size_t m
     if (misaligned(x_bf16, 16) || misaligned(gate_packed, 16) || misaligned(up_packed, 16) ||
         misaligned(kept_bf16, 16) || misaligned(kept_q8, 16) || misaligned(kept_scales, 4))
         return KDQ_ERR_ALIGNMENT;
-    const struct {
-        const void* p;
-        size_t bytes;
-    } out[] = {{h_bf16, extent(m, h_stride, n, 2)},
-               {kept_bf16, 4 * m * n},
-               {kept_q8, 2 * m * n},
-               {kept_scales, m * n / 4},
-               {workspace, workspace_bytes}},
-      in[] = {{x_bf16, extent(m, x_stride, k, 2)},
-              {gate_packed, kdq_mxfp4_packed_bytes(n, k)},
-              {up_packed, kdq_mxfp4_packed_bytes(n, k)}};
-    for (size_t i = 0; i < 5; ++i) {
-        for (const auto& b : in)
-            if (overlaps(out[i].p, out[i].bytes, b.p, b.bytes))
-                return KDQ_ERR_ALIAS;
-        for (size_t j = 0; j < i; ++j)
-            if (overlaps(out[i].p, out[i].bytes, out[j].p, out[j].bytes))
-                return KDQ_ERR_ALIAS;
-    }
+    const Range out[] = {{h_bf16, extent(m, h_stride, n, 2)},
+                         {kept_bf16, 4 * m * n},
+                         {kept_q8, 2 * m * n},
+                         {kept_scales, m * n / 4},
+                         {workspace, workspace_bytes}},
+                in[] = {{x_bf16, extent(m, x_stride, k, 2)},
+                        {gate_packed, kdq_mxfp4_packed_bytes(n, k)},
+                        {up_packed, kdq_mxfp4_packed_bytes(n, k)}};
+    if (any_overlap(out, in))
+        return KDQ_ERR_ALIAS;
     const Plan p = plan_gated(m, n, k, kept_bf16 || kept_q8);
     if (const int rc = check_workspace(partial_bytes(p, m), workspace, workspace_bytes))
         return rc;
@@ -1963,23 +1975,14 @@ extern "C" int kdq_mxfp4_gated_backward(const uint16_t* dh_bf16, size_t dh_strid
         misaligned(kept_scales, 4) || misaligned(dgu_bf16, 16))
         return KDQ_ERR_ALIGNMENT;
     const size_t w_bytes = kdq_mxfp4_packed_transposed_bytes(n, k);
-    const struct {
-        const void* p;
-        size_t bytes;
-    } out[] = {{dgu_bf16, 4 * m * n},
-               {dx_bf16, extent(m, dx_stride, k, 2)},
-               {workspace, workspace_bytes}},
-      in[] = {{dh_bf16, extent(m, dh_stride, n, 2)}, {kept_bf16, 4 * m * n},
-              {kept_q8, 2 * m * n},                  {kept_scales, m * n / 4},
-              {gate_transposed, w_bytes},            {up_transposed, w_bytes}};
-    for (size_t i = 0; i < 3; ++i) {
-        for (const auto& b : in)
-            if (overlaps(out[i].p, out[i].bytes, b.p, b.bytes))
-                return KDQ_ERR_ALIAS;
-        for (size_t j = 0; j < i; ++j)
-            if (overlaps(out[i].p, out[i].bytes, out[j].p, out[j].bytes))
-                return KDQ_ERR_ALIAS;
-    }
+    const Range out[] = {{dgu_bf16, 4 * m * n},
+                         {dx_bf16, extent(m, dx_stride, k, 2)},
+                         {workspace, workspace_bytes}},
+                in[] = {{dh_bf16, extent(m, dh_stride, n, 2)}, {kept_bf16, 4 * m * n},
+                        {kept_q8, 2 * m * n},                  {kept_scales, m * n / 4},
+                        {gate_transposed, w_bytes},            {up_transposed, w_bytes}};
+    if (any_overlap(out, in))
+        return KDQ_ERR_ALIAS;
     const Plan p = plan_backward(m, n, k);
     if (const int rc = check_workspace(partial_bytes(p, m), workspace, workspace_bytes))
         return rc;

@@ -175,6 +175,34 @@ def test_quantize_refuses_a_status_that_the_device_cannot_write(status):
         ops.mxfp4_quantize(torch.zeros(2, 64), status)
 
 
+@pytest.mark.parametrize("quantized", [0, 1])
+def test_a_workspace_over_an_input_is_refused(quantized):
+    """K slices' partial results would replace x or the matrix while others still read them."""
+    lib = kadan_amd.lib()
+    m, n, k = (77, 4096, 14336) if not quantized else (200, 4096, 14336)
+    need = lib.kdq_mxfp4_product_workspace(m, n, k, quantized)
+    assert need > 0
+    x, scales, w, y, ws = (i << 40 for i in range(1, 6))
+    x_bytes, w_bytes = m * k * 2 // (1 if not quantized else 4), lib.kdq_mxfp4_packed_bytes(n, k)
+
+    def call(workspace, size=need):
+        if quantized:
+            return lib.kdq_mxfp4_product_quantized(x, scales, m, w, n, k, 0, y, n, workspace, size,
+                                                   None)
+        return lib.kdq_mxfp4_product(x, k, m, w, n, k, 0, y, n, workspace, size, None)
+
+    for base, size in ((x, x_bytes), (w, w_bytes), (y, m * n * 4)) + (
+            ((scales, m * k // 32),) if quantized else ()):
+        assert call(base) == 4 and call(base + size - 16) == 4 and call(base - need + 16) == 4
+    assert call(ws, need - 1) == 6  # (apart from all of them: the next check)
+    # a workspace that the call does not need is the caller's word for what it may write, too
+    assert lib.kdq_mxfp4_product_workspace(1, 64, 64, quantized) == 0
+    if quantized:
+        assert lib.kdq_mxfp4_product_quantized(x, scales, 1, w, 64, 64, 0, y, 64, x, 16, None) == 4
+    else:
+        assert lib.kdq_mxfp4_product(x, 64, 1, w, 64, 64, 0, y, 64, w, 16, None) == 4
+
+
 class Packed:
     """What the wrappers look at of a packed device tensor."""
     dtype, is_cuda = torch.uint8, True
