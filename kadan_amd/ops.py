@@ -15,6 +15,8 @@ from . import BLOCK_BYTES, BLOCK_VALUES, MatvecJob, call, lib
 
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # (not a public name)
+# (the same, without a check that the device runtime is up, which a device tensor stands for)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
 def _stream() -> int:
@@ -379,7 +381,7 @@ def moe_mxfp4_packed(x_bf16: torch.Tensor, logits: torch.Tensor, top_k: int, int
 
 def _stream_for(*tensors: torch.Tensor) -> int:
     """The current device's current stream, where every tensor is on that device."""
-    device = torch.cuda.current_device()
+    device = _current_device()
     for t in tensors:
         if t.get_device() != device:
             raise ValueError("every tensor must be on the current device")
@@ -433,41 +435,37 @@ def _mxfp4_size(function: str, *sizes: int) -> int:
 
 
 @functools.lru_cache(maxsize=4096, typed=True)
-def _mxfp4_sizes(matrix: str, rows: int, cols: int, workspace: str, *sizes: int):
-    return _mxfp4_size(matrix, rows, cols), _mxfp4_size(workspace, *sizes)
+def _mxfp4_sizes_on(device: int, matrix: str, rows: int, cols: int, workspace: str, *sizes: int):
+    return _mxfp4_size(matrix, rows, cols), int(getattr(lib(), workspace)(*sizes))
+
+
+def _mxfp4_sizes(*sizes):
+    """The matrix's bytes and the workspace's, which depend on the current device's compute
+    units."""
+    return _mxfp4_sizes_on(_current_device(), *sizes)
 
 
 _PACKED, _TRANSPOSED = "kdq_mxfp4_packed_bytes", "kdq_mxfp4_packed_transposed_bytes"
 
 
-def _packed(packed: torch.Tensor, size: int, name: str) -> None:
+# The two packed forms of a matrix may take the same number of bytes (14336 x 4096 does), so
+# they are told apart by their shape: flat for the products, a row per 64 columns transposed.
+def _matrix(packed: torch.Tensor, size: int, name: str, dims: int = 1) -> int:
     if packed.dtype != torch.uint8 or not packed.is_cuda or not packed.is_contiguous():
         raise ValueError(f"{name}: expected a packed uint8 device tensor")
     if not size or packed.numel() != size:
         raise ValueError(f"{name}: not the packed size of this call's matrix")
-
-
-# The two packed forms of a matrix may take the same number of bytes (14336 x 4096 does), so
-# they are told apart by their shape: flat for the products, a row per 64 columns transposed.
-def _matrix(packed: torch.Tensor, size: int, name: str) -> int:
-    _packed(packed, size, name)
-    if packed.dim() != 1:
-        raise ValueError(f"{name}: expected mxfp4_pack's flat tensor (not the transposed form)")
+    if packed.dim() != dims:
+        raise ValueError(f"{name}: expected mxfp4_pack's flat form" if dims == 1 else
+                         f"{name}: expected the form of mxfp4_pack(..., transposed=True)")
     return packed.data_ptr()
-
-
-def _transposed_shape(size: int, cols: int) -> tuple[int, int]:
-    groups = (cols + 63) // 64
-    return groups, size // groups
 
 
 def _transposed_matrix(packed: torch.Tensor, size: int, cols: int, name: str) -> int:
-    _packed(packed, size, name)
-    groups, width = _transposed_shape(size, cols)
-    if packed.dim() != 2 or packed.shape[0] != groups:
-        raise ValueError(f"{name}: expected mxfp4_pack(..., transposed=True)'s "
-                         f"[{groups}, {width}]")
-    return packed.data_ptr()
+    at = _matrix(packed, size, name, 2)
+    if packed.shape[0] != (cols + 63) // 64:
+        raise ValueError(f"{name}: another matrix's packed form")
+    return at
 
 
 def _output(out: torch.Tensor, rows: int, cols: int, dtype, name: str) -> int:
@@ -521,8 +519,9 @@ def mxfp4_pack(blocks: torch.Tensor, scales: torch.Tensor,
     size = _mxfp4_size(_TRANSPOSED if transposed else _PACKED, rows, cols)
     if not size:
         raise ValueError(f"a matrix of {rows} x {cols} has no packed form")
-    packed = torch.empty(_transposed_shape(size, cols) if transposed else size,
-                         dtype=torch.uint8, device=blocks.device)
+    groups = (cols + 63) // 64
+    packed = torch.empty((groups, size // groups) if transposed else size, dtype=torch.uint8,
+                         device=blocks.device)
     call("kdq_mxfp4_pack_transposed" if transposed else "kdq_mxfp4_pack", blocks.data_ptr(),
          scales.data_ptr(), rows, cols, packed.data_ptr(), stream)
     return packed

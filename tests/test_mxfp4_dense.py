@@ -175,6 +175,25 @@ def test_quantize_refuses_a_status_that_the_device_cannot_write(status):
         ops.mxfp4_quantize(torch.zeros(2, 64), status)
 
 
+def test_workspaces_are_asked_for_on_each_device(monkeypatch):
+    """Their sizes follow from the current device's compute units."""
+    current = 0
+
+    class Library:
+        kdq_mxfp4_packed_bytes = staticmethod(lambda rows, cols: rows * cols)
+        kdq_mxfp4_product_workspace = staticmethod(lambda *sizes: 8192 * (1 + current))
+
+    monkeypatch.setattr(ops, "lib", lambda: Library)
+    monkeypatch.setattr(ops, "_current_device", lambda: current, raising=False)
+    sizes = ("kdq_mxfp4_packed_bytes", 7, 32, "kdq_mxfp4_product_workspace", 5, 7, 32, 0)
+    try:
+        for current in (0, 1, 0):
+            assert ops._mxfp4_sizes(*sizes) == (7 * 32, 8192 * (1 + current))
+    finally:  # (sizes of the stand-in stay in no cache)
+        for name in ("_mxfp4_size", "_mxfp4_sizes", "_mxfp4_sizes_on"):
+            getattr(getattr(ops, name, None), "cache_clear", lambda: None)()
+
+
 @pytest.mark.parametrize("quantized", [0, 1])
 def test_a_workspace_over_an_input_is_refused(quantized):
     """K slices' partial results would replace x or the matrix while others still read them."""
