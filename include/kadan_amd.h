@@ -404,8 +404,9 @@ int kdq_moe_mxfp4_packed_noalloc(const uint16_t* x_bf16, const float* logits, si
  * values, are multiples of 8 and at most 2^21 for inputs, and any for outputs (products:
  * outputs 2- or 4-byte aligned); other pointers 16-byte aligned.  No output, and no byte of
  * the workspace, may lie between the first and the last byte of an input or of another output.
- * Scale bytes above 252 take the largest codes past fp32's range: such weights are infinite,
- * or NaN (255). */
+ * Scale bytes 253 and 254, which kdq_mxfp4_quantize does not write, take the largest codes
+ * past fp32's range: with bf16 rows such weights are infinite; kdq_mxfp4_product_quantized may
+ * take them, in the matrix or in x, as infinite or at their value (by m).  255 is NaN. */
 
 /* x [rows x cols] (type KDQ_F32, KDQ_F16 or KDQ_BF16, rows x_stride values apart) as
  * MXFP4: per 32 values the scale is 2^(floor(log2(largest magnitude)) - 2) (byte at least

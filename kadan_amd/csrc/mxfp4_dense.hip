@@ -853,7 +853,8 @@ __global__ __launch_bounds__(1024) void decode_t_kernel(Decode a) {
 // decoded by one wavefront (two where the groups share rows).
 //
 // Operands: bf16 x (v_mfma_f32_32x32x16_bf16, weights decoded to bf16, exact), MXFP4 x
-// (v_mfma_scale_f32_32x32x64_f8f6f4 over both codes as they lie), and the backward pass's
+// (v_mfma_scale_f32_32x32x64_f8f6f4 over both codes as they lie, so that 6 at scale byte 254 is
+// its value, where decode_kernel's bf16 weight is infinite), and the backward pass's
 // transposed weights under bf16 gradients (their scales lie along the columns, which are not
 // summed over, so the scaled MFMA cannot take them).
 //

@@ -152,6 +152,52 @@ def test_product_scales_over_the_whole_range(device, gen, m):
                torch.where(inside, want, torch.zeros_like(want)), bound)
 
 
+@pytest.mark.parametrize("k", [32, 96, 288])
+@pytest.mark.parametrize("m", [4, 20, 60, 70, 300])
+def test_product_quantized_scales_over_the_whole_range(device, gen, m, k):
+    """Every scale byte of the matrix against bytes of x from 0 to 254, in both kernels."""
+    n = 255
+    (blocks, _), (x_blocks, _) = ref.matrix(gen, n, k), ref.matrix(gen, m, k)
+    byte = torch.arange(n, device=device).to(torch.uint8)[:, None].repeat(1, k // 32)
+    x_byte = torch.randint(0, 253, (m, 1), generator=gen, device=device).to(torch.uint8)
+    x_byte[:4, 0] = torch.tensor([0, 252, 253, 254]).to(torch.uint8)
+    x_byte = x_byte.repeat(1, k // 32)
+    packed = ops.mxfp4_pack(blocks, byte)
+    y = ops.mxfp4_product_quantized(x_blocks, x_byte, packed, n)
+    x, w = ref.decode(x_blocks, x_byte), ref.decode(blocks, byte)
+    want, bound = ref.sum_bound(x, w)
+    # (as for bf16 x: terms below fp32's normal numbers are off by at most 2^-126 each, and sums
+    # may overflow on the way where the terms' magnitudes add up to 2^128)
+    bound = bound + k * ref.TINY
+    inside = x.abs() @ w.abs().T < 2.0 ** 127
+    zero = torch.zeros_like(want)
+    # bytes 253 and 254 take 4 and 6 past fp32: at their value, or infinite (NaN beside zeros)
+    fits = (byte[:, 0] <= 252)[None] & (x_byte[:, 0] <= 252)[:, None]
+    assert int((inside & fits).sum()) > m * n // 4 and bool((inside & ~fits).any())
+    held = inside & (fits | torch.isfinite(y))
+    ref.within(torch.where(held, y.double(), zero), torch.where(held, want, zero), bound)
+    # 255 is NaN in its row of x
+    x_byte[1] = 255
+    y = ops.mxfp4_product_quantized(x_blocks, x_byte, packed, n)
+    assert bool(torch.isnan(y[1]).all())
+
+
+@pytest.mark.parametrize("m", [3, 40, 200])
+def test_scales_past_252_are_infinite_weights_of_bf16_rows(device, gen, m):
+    """4 and 6 are infinite from the byte on that takes them past fp32, the others their value."""
+    n, k = 64, 32
+    code = torch.arange(n, device=device) % 8  # a row's first code; the others are zero
+    blocks = torch.zeros(n, k // 2, dtype=torch.uint8, device=device)
+    blocks[:, 0] = code.to(torch.uint8)
+    byte = (253 + torch.arange(n, device=device) // 32).to(torch.uint8)[:, None].contiguous()
+    x = torch.zeros(m, k, dtype=BF16, device=device)
+    x[:, 0] = 2.0 ** -126
+    y = ops.mxfp4_product(x, ops.mxfp4_pack(blocks, byte), n).double()
+    value = ref.decode(blocks, byte)[:, 0]  # past fp32 from 2^128 on
+    want = torch.where(value >= 2.0 ** 128, float("inf"), value * 2.0 ** -126)
+    assert torch.equal(y, want.expand(m, n))
+
+
 @pytest.mark.parametrize("m", [4, 40, 200])
 @pytest.mark.parametrize("quantized", [False, True])
 def test_scale_255_is_nan_in_its_rows_only(device, gen, m, quantized):
