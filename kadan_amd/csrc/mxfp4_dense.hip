@@ -15,6 +15,7 @@
 // Times below are of one MI355X (others: up to 6 % apart where the matrix cores are the bound),
 // whose 1 GB copy runs at 5.2 TB/s and whose library 8192^3 bf16 product at 1.25 PFLOP/s.
 #include "kdq_common.hpp"
+#include "mxfp4_plan.hpp"
 
 #include <algorithm>
 #include <atomic>
@@ -22,6 +23,8 @@
 
 namespace kdq {
 namespace {
+
+using namespace mxfp4;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -47,10 +50,6 @@ typedef unsigned u4 __attribute__((ext_vector_type(4)));
 struct Form {
     size_t groups, steps, code_bytes, scale_bytes;
 };
-
-__host__ __device__ inline size_t ceil_div(size_t a, size_t b) {
-    return (a + b - 1) / b;
-}
 
 __host__ __device__ inline Form packed_form(size_t rows, size_t cols) {
     Form f;
@@ -520,7 +519,6 @@ struct Decode {
 };
 
 constexpr int kOutside = 0x7ffffff0;  // past any buffer's range: such loads return zeros
-constexpr unsigned kStagedBytes = 32 * 1024;
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const uint8_t* p, unsigned bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p), 0, int(bytes), 0x00027000);
@@ -530,12 +528,6 @@ template <int POLICY = 0>
 __device__ __forceinline__ u4 load_b128(const __amdgpu_buffer_rsrc_t& r, int at) {
     const auto v = __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, POLICY);
     return u4{unsigned(v[0]), unsigned(v[1]), unsigned(v[2]), unsigned(v[3])};
-}
-
-// Bytes between the rows of a staged x: 16 more than a row has, so that rows start in
-// different banks.
-__host__ __device__ inline unsigned staged_pitch(unsigned row_bytes) {
-    return row_bytes + 16;
 }
 
 template <int R, int TB, bool GATED, bool FP4, bool STAGED, int OUT>
@@ -873,8 +865,6 @@ __global__ __launch_bounds__(1024) void decode_t_kernel(Decode a) {
 // 13.6 us, 77 x 14336 -> 4096 22.1 -> 17.5.  There the launch, the first loads and the slices'
 // sum are the larger part.
 
-enum Operands { kBf16, kFp4, kTransposed };
-
 struct Gemm {
     const uint8_t *w0, *w1;   // the matrices of the wavefront's two tiles; backward: of the groups
     const uint8_t* x;
@@ -890,7 +880,6 @@ struct Gemm {
 };
 
 constexpr int kStages = 4;
-constexpr unsigned kTileFloats = 2 * 16 * 64;  // a wavefront's two result tiles
 
 __device__ __forceinline__ void issue_order() {
     asm volatile("" ::: "memory");
@@ -1426,85 +1415,9 @@ __global__ __launch_bounds__(256) void gate_grad_kernel(const uint16_t* __restri
               bf16_pair(ru[6], ru[7])};
 }
 
-// ------------------------------------------------------------------ launch plans
+// ------------------------------------------------------------------ launches
 
 constexpr size_t kMaxRows = size_t(1) << 20, kMaxK = size_t(1) << 20, kMaxN = size_t(1) << 24;
-
-// How a product runs: `decode` (decode_kernel), or gemm_kernel with TT tiles of 32 rows of
-// x, the groups splitting K or not, in `slices` of `part` chunks.
-struct Plan {
-    bool decode, split;
-    int tt;
-    unsigned tiles_n, tiles_m, slices, chunks, part;
-    double cost;
-};
-
-// What a product in tiles of tt * 32 rows and `slices` K slices takes, in microseconds, up to
-// what every choice shares: a workgroup's fixed part and its turns, alone on a compute unit or
-// beside another, and the slices' sum.  Fitted to sweeps over tt and slices at 18 sizes per
-// kind: 64 x 14336 -> 4096 16 us in 6 slices of 32 rows, 18 in 14 of 64, 23 in 14 of 128;
-// 333 x 2880 -> 2880 gated 14 us in tiles of 32, 20 of 64, 25 of 128; 512 x 4096 -> 14336 51 us
-// in tiles of 128, 53 of 64, 60 of 32; 512 x 4096 -> 4096 18 of 32, 26 of 64, 30 of 128.
-struct Cost {
-    double fixed, turn, turn_of_two;
-};
-
-Cost cost_of(int ops, int tt) {
-    if (ops == kFp4)
-        return {2.0 + 0.75 * tt, 0.05 + 0.55 * tt, 0.1 + 1.35 * tt};
-    const double fixed = 2.5 + 0.9 * tt;
-    return ops == kTransposed ? Cost{fixed, tt == 1 ? 0.5 : 0.4 + 0.3 * tt, 0.7 + 0.6 * tt}
-                              : Cost{fixed, 0.03 + 0.33 * tt, 0.05 + 0.66 * tt};
-}
-
-size_t partial_bytes(const Plan& p, size_t m) {
-    return p.decode || p.slices == 1
-               ? 0
-               : size_t(p.slices) * p.tiles_n * 4 * ceil_div(m, 32) * kTileFloats * 4;
-}
-
-Plan plan_gemm(size_t m, size_t wave_groups, size_t chunks, int ops) {
-    const size_t cus = compute_units();
-    Plan best{};
-    const auto consider = [&](int tt, bool split, size_t slices) {
-        Plan p{};
-        p.tt = tt;
-        p.split = split;
-        p.tiles_n = unsigned(ceil_div(wave_groups, 4));
-        p.tiles_m = unsigned(ceil_div(m, size_t(tt) * (split ? 32 : 64)));
-        p.chunks = unsigned(chunks);
-        const unsigned sets = split && ops != kTransposed ? 2 : 1, unit = ops == kFp4 ? 1 : 4;
-        p.part = unsigned(ceil_div(ceil_div(chunks, slices * sets), unit) * unit);
-        p.slices = unsigned(ceil_div(chunks, size_t(p.part) * sets));
-        const Cost c = cost_of(ops, tt);
-        const bool shared = tt == 1 || (tt == 2 && ops != kFp4);
-        const size_t tiles = size_t(p.tiles_n) * p.tiles_m;
-        if (best.slices && tiles * 512 > UINT32_MAX)
-            return;  // (a launch's threads are counted in 32 bits; the largest tiles come first)
-        const size_t each = ceil_div(tiles * p.slices, cus);  // workgroups of a compute unit
-        const double alone = c.fixed + p.part * c.turn, both = c.fixed + p.part * c.turn_of_two;
-        // (two to a unit begin and end together: what their turns hide is paid once)
-        double t = shared ? double(each / 2) * both + double(each % 2) * alone +
-                                (each > 1 ? 1.5 : 0.0)
-                          : double(each) * (split ? alone : 0.93 * alone);
-        if (p.slices > 1)  // (the backward pass's third launch, which is its caller's time too)
-            t += (ops == kTransposed ? 4.5 : 3.5) + double(partial_bytes(p, m)) / 2.5e6;
-        if (!best.slices || t < best.cost) {
-            best = p;
-            best.cost = t;
-        }
-    };
-    for (int tt = 4; tt >= 1; --tt) {  // (slices up to two workgroups a compute unit)
-        const size_t tiles = ceil_div(wave_groups, 4) * ceil_div(m, size_t(tt) * 32);
-        const size_t most = std::min<size_t>({16, std::max<size_t>(1, 2 * cus / tiles),
-                                              ceil_div(chunks, ops == kFp4 ? 2 : 4)});
-        for (size_t slices = 1; slices <= most; ++slices)
-            consider(tt, true, slices);
-    }
-    if (ops == kFp4)
-        consider(4, false, 1);
-    return best;
-}
 
 template <int TT, bool SPLIT, int OPS, int OUT>
 int launch_gemm(const Gemm& a, const Plan& p, hipStream_t st) {
@@ -1579,28 +1492,19 @@ int launch_decode(Decode a, unsigned waves, hipStream_t st) {
 }
 
 template <bool GATED, bool FP4, int OUT> int run_decode(Decode a, hipStream_t st) {
-    const unsigned units = (a.k + 127) / 128;
-    // whole blocks of 32 rows a workgroup where those fill the compute units
-    const bool wide = a.groups >= compute_units() && a.out.m <= 32;
-    // (1 row, 14336 -> 4096: 8.7 us over 16 wavefronts, 9.9 over 8; the gated projection's
-    // two matrices 14.9 and 14.1; 4096 -> 4096 5.5 and 4.9; 4096 -> 14336 13.1 and 8.1)
-    const unsigned waves = units <= 8 ? 2 : units <= 16 ? 4
-                           : units <= 48 || wide || GATED || a.out.m > 32 ? 8
-                                                                          : 16;
-    a.units = (unsigned(ceil_div(units, waves)) + 1) / 2 * 2;
+    const DecodeShape s = decode_shape(a.out.m, a.out.n, a.k, GATED, FP4, compute_units());
+    a.units = s.units;
     if constexpr (FP4)
-        if (a.out.m > 32)
-            return launch_decode<1, 4, GATED, FP4, false, OUT>(a, waves, st);
-    if (a.out.m > 16)
-        return wide ? launch_decode<2, 2, GATED, FP4, false, OUT>(a, waves, st)
-                    : launch_decode<1, 2, GATED, FP4, false, OUT>(a, waves, st);
-    const bool staged = a.out.m * staged_pitch(FP4 ? a.k / 2 : a.k * 2) <= kStagedBytes &&
-                        a.out.m * (FP4 ? a.k / 2 : a.k * 2) <= waves * 64 * 16 * 8;
-    if (staged)
-        return wide ? launch_decode<2, 1, GATED, FP4, true, OUT>(a, waves, st)
-                    : launch_decode<1, 1, GATED, FP4, true, OUT>(a, waves, st);
-    return wide ? launch_decode<2, 1, GATED, FP4, false, OUT>(a, waves, st)
-                : launch_decode<1, 1, GATED, FP4, false, OUT>(a, waves, st);
+        if (s.tb == 4)
+            return launch_decode<1, 4, GATED, FP4, false, OUT>(a, s.waves, st);
+    if (s.tb == 2)
+        return s.wide ? launch_decode<2, 2, GATED, FP4, false, OUT>(a, s.waves, st)
+                      : launch_decode<1, 2, GATED, FP4, false, OUT>(a, s.waves, st);
+    if (s.staged)
+        return s.wide ? launch_decode<2, 1, GATED, FP4, true, OUT>(a, s.waves, st)
+                      : launch_decode<1, 1, GATED, FP4, true, OUT>(a, s.waves, st);
+    return s.wide ? launch_decode<2, 1, GATED, FP4, false, OUT>(a, s.waves, st)
+                  : launch_decode<1, 1, GATED, FP4, false, OUT>(a, s.waves, st);
 }
 
 template <int TB> int launch_decode_t(const Decode& a, unsigned waves, hipStream_t st) {
@@ -1616,67 +1520,6 @@ int run_decode_t(Decode a, hipStream_t st) {
     const unsigned waves = 2 * (units <= 4 ? 1 : units <= 8 ? 2 : units <= 16 ? 4 : 8);
     a.units = unsigned(ceil_div(units, waves / 2));
     return a.out.m <= 16 ? launch_decode_t<1>(a, waves, st) : launch_decode_t<2>(a, waves, st);
-}
-
-// What decode_kernel takes, in microseconds: its weights at 6 GB/ms, and each workgroup's own
-// reading of x (m rows of row_bytes; none to speak of where x is staged) at what a compute
-// unit takes of strided rows, 33 KB/us.  Swept against gemm_kernel over 11 sizes per kind and
-// 1 to 64 rows: 4096 -> 14336 8 rows 10.7 us against 12.1, 16 rows 13.5 against 12.3; 14336
-// -> 4096 4 rows 11.2 against 12.6, 8 rows 14.0 against 12.7; 8192 -> 1024 12 rows 9.1
-// against 9.3, 20 rows 14.6 against 9.4; 2880 -> 2880 20 rows 7.5 against 8.2, 32 rows 9.4
-// against 8.3.
-// Where x takes less than 2.5 us no plan of gemm_kernel is the quicker, and none is made: it
-// would cost the caller about a microsecond.
-struct DecodeCost {
-    double weights, x;
-    bool certain() const {
-        return x < 2.5;
-    }
-    bool quicker_than(const Plan& gemm, bool fp4) const {
-        return certain() || x + weights < gemm.cost - (fp4 ? 1.0 : 3.0);
-    }
-};
-
-DecodeCost decode_cost(size_t m, size_t row_bytes, size_t n, size_t weight_bytes) {
-    const size_t groups = ceil_div(n, 32), cus = compute_units();
-    const size_t row_tiles = groups >= cus ? groups : ceil_div(n, 16);
-    const double rounds = std::max(1.0, double(row_tiles) / double(cus));
-    const bool staged = m * staged_pitch(unsigned(row_bytes)) <= kStagedBytes;
-    return {double(weight_bytes) / 6.0e6, staged ? 0.0 : double(m * row_bytes) * rounds / 33.0e3};
-}
-
-Plan decode_plan() {
-    Plan p{};
-    p.decode = true;
-    return p;
-}
-
-Plan plan_product(size_t m, size_t n, size_t k, bool fp4) {
-    const bool few = m <= (fp4 ? 64 : 32);
-    const DecodeCost d = decode_cost(few ? m : 0, fp4 ? k / 2 : k * 2, n, n * k * 17 / 32);
-    if (few && d.certain())
-        return decode_plan();
-    const Plan p = plan_gemm(m, ceil_div(n, 64), ceil_div(k, fp4 ? 256 : 64), fp4 ? kFp4 : kBf16);
-    return few && d.quicker_than(p, fp4) ? decode_plan() : p;
-}
-
-Plan plan_gated(size_t m, size_t n, size_t k, bool kept) {
-    const bool few = !kept && m <= 32;
-    const DecodeCost d = decode_cost(few ? m : 0, k * 2, n, n * k * 17 / 16);
-    if (few && d.certain())
-        return decode_plan();
-    const Plan p = plan_gemm(m, ceil_div(n, 32), ceil_div(k, 64), kBf16);
-    return few && d.quicker_than(p, false) ? decode_plan() : p;
-}
-
-// (decode_t_kernel is bound by decoding the weights, which half the compute units do where
-// there are 4096 columns: 1 row of 14336 -> 4096 26 us against 21, of 2880 -> 2880 10.3
-// against 13.0, 16 rows of that 15.0 against 13.2, 1 row of 1024 -> 8192 6.6 against 11.6)
-Plan plan_backward(size_t m, size_t n, size_t k) {
-    Plan p = plan_gemm(m, ceil_div(k, 64), ceil_div(n, 64), kTransposed);
-    const double units = double(ceil_div(n, 128)) * double(ceil_div(k / 32, compute_units()));
-    p.decode = m <= 32 && 2.5 + 0.2 * units * (1.0 + double(m) / 14) < p.cost;
-    return p;
 }
 
 // (a packing launch counts its threads, one per 16 bytes of codes or 4 of scales, in 32 bits)
@@ -1801,19 +1644,19 @@ extern "C" int kdq_mxfp4_pack_transposed(const uint8_t* blocks, const uint8_t* s
 extern "C" size_t kdq_mxfp4_product_workspace(size_t m, size_t n, size_t k, int quantized) {
     if (!m || !n || !k || !sizes_ok(m, n, k))
         return 0;
-    return partial_bytes(plan_product(m, n, k, quantized != 0), m);
+    return partial_bytes(plan_product(m, n, k, quantized != 0, compute_units()), m);
 }
 
 extern "C" size_t kdq_mxfp4_gated_workspace(size_t m, size_t n, size_t k, int kept) {
     if (!m || !n || !k || !sizes_ok(m, n, k) || n % 32)
         return 0;
-    return partial_bytes(plan_gated(m, n, k, kept != 0), m);
+    return partial_bytes(plan_gated(m, n, k, kept != 0, compute_units()), m);
 }
 
 extern "C" size_t kdq_mxfp4_gated_backward_workspace(size_t m, size_t n, size_t k) {
     if (!m || !n || !k || !backward_sizes_ok(m, n, k))
         return 0;
-    return partial_bytes(plan_backward(m, n, k), m);
+    return partial_bytes(plan_backward(m, n, k, compute_units()), m);
 }
 
 namespace kdq {
@@ -1859,7 +1702,7 @@ extern "C" int kdq_mxfp4_product(const uint16_t* x_bf16, size_t x_stride, size_t
                         {packed, kdq_mxfp4_packed_bytes(n, k)}};
     if (any_overlap(out, in))
         return KDQ_ERR_ALIAS;
-    const Plan p = plan_product(m, n, k, false);
+    const Plan p = plan_product(m, n, k, false, compute_units());
     if (const int rc = check_workspace(partial_bytes(p, m), workspace, workspace_bytes))
         return rc;
     const Form f = packed_form(n, k);
@@ -1893,7 +1736,7 @@ extern "C" int kdq_mxfp4_product_quantized(const uint8_t* x_blocks, const uint8_
                         {packed, kdq_mxfp4_packed_bytes(n, k)}};
     if (any_overlap(out, in))
         return KDQ_ERR_ALIAS;
-    const Plan p = plan_product(m, n, k, true);
+    const Plan p = plan_product(m, n, k, true, compute_units());
     if (const int rc = check_workspace(partial_bytes(p, m), workspace, workspace_bytes))
         return rc;
     const Form f = packed_form(n, k);
@@ -1934,7 +1777,7 @@ extern "C" int kdq_mxfp4_gated(const uint16_t* x_bf16, size_t x_stride, size_t m
                         {up_packed, kdq_mxfp4_packed_bytes(n, k)}};
     if (any_overlap(out, in))
         return KDQ_ERR_ALIAS;
-    const Plan p = plan_gated(m, n, k, kept_bf16 || kept_q8);
+    const Plan p = plan_gated(m, n, k, kept_bf16 || kept_q8, compute_units());
     if (const int rc = check_workspace(partial_bytes(p, m), workspace, workspace_bytes))
         return rc;
     const Form f = packed_form(n, k);
@@ -1984,7 +1827,7 @@ extern "C" int kdq_mxfp4_gated_backward(const uint16_t* dh_bf16, size_t dh_strid
                         {gate_transposed, w_bytes},            {up_transposed, w_bytes}};
     if (any_overlap(out, in))
         return KDQ_ERR_ALIAS;
-    const Plan p = plan_backward(m, n, k);
+    const Plan p = plan_backward(m, n, k, compute_units());
     if (const int rc = check_workspace(partial_bytes(p, m), workspace, workspace_bytes))
         return rc;
     const auto st = static_cast<hipStream_t>(stream);

@@ -132,6 +132,30 @@ def test_product_quantized(device, gen, m, n, k, dtype):
     ref.within(y, want, rounded(want, bound, dtype), f"{m}x{n}x{k}")
 
 
+# a few rows of matrices whose 32-row blocks fill the compute units, and MXFP4 rows too long for
+# LDS: n on both sides of whole blocks, K on both sides of whole units
+WIDE = [(1, 8161, 32), (7, 8224, 1056), (11, 8163, 768), (16, 9001, 4128), (17, 8335, 32),
+        (32, 8192, 672)]
+WIDE_MXFP4 = [(14, 1, 4672), (16, 130, 5408), (1, 8360, 32), (8, 8192, 4128), (9, 8531, 7264),
+              (17, 8839, 32), (32, 8200, 672)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("quantized,m,n,k", [(False, *size) for size in WIDE] +
+                         [(True, *size) for size in WIDE_MXFP4])
+def test_few_rows_of_a_wide_matrix(device, gen, quantized, m, n, k, dtype):
+    w = ref.matrix(gen, n, k)
+    packed = ops.mxfp4_pack(*w)
+    if quantized:
+        x = ref.matrix(gen, m, k)
+        y, x = ops.mxfp4_product_quantized(*x, packed, n, dtype), ref.decode(*x)
+    else:
+        x = normal(gen, m, k).bfloat16()
+        y, x = ops.mxfp4_product(x, packed, n, dtype), x.double()
+    want, bound = ref.sum_bound(x, ref.decode(*w))
+    ref.within(y, want, rounded(want, bound, dtype), f"{m}x{n}x{k}")
+
+
 @pytest.mark.parametrize("m", [1, 20, 70, 300])
 def test_product_scales_over_the_whole_range(device, gen, m):
     """Scale bytes from 0 to 252 in one matrix, against x whose size makes up for them."""
@@ -402,6 +426,19 @@ GATED_TILES_KEPT = [(77, 10976, 544), (3291, 544, 544), (325, 9024, 1632), (2735
                     (73, 5440, 12640), (101, 9344, 8864)]
 BACKWARD_TILES = [(129, 32, 13152), (289, 32, 13408), (385, 32, 13152), (35, 6208, 11744),
                   (65, 4864, 11360), (109, 4896, 8288)]
+
+
+GATED_WIDE = [(1, 8224, 32), (7, 8192, 1056), (11, 8672, 768), (16, 8224, 4128), (17, 8256, 32),
+              (32, 8192, 672)]
+
+
+@pytest.mark.parametrize("m,n,k", GATED_WIDE)
+def test_gated_few_rows_of_wide_matrices(device, gen, m, n, k):
+    wg, wu = ref.matrix(gen, n, k), ref.matrix(gen, n, k)
+    x = (normal(gen, m, k) * (8 / k ** 0.5)).bfloat16()
+    h = ops.mxfp4_gated(x, ops.mxfp4_pack(*wg), ops.mxfp4_pack(*wu), n)
+    *_, (want, bound) = ref.gated(x.double(), ref.decode(*wg), ref.decode(*wu))
+    ref.within(h, want, bound, "h")
 
 
 def check_q8(saved, exact, error):
