@@ -123,12 +123,16 @@ inline DecodeShape decode_shape(size_t m, size_t n, size_t k, bool gated, bool f
 }
 
 // What decode_kernel takes, in microseconds: its weights at 6 GB/ms, and each workgroup's own
-// reading of x (m rows of row_bytes; none to speak of where x is staged) at what a compute
-// unit takes of strided rows, 33 KB/us.  Swept against gemm_kernel over 11 sizes per kind and
-// 1 to 64 rows: 4096 -> 14336 8 rows 10.7 us against 12.1, 16 rows 13.5 against 12.3; 14336
-// -> 4096 4 rows 11.2 against 12.6, 8 rows 14.0 against 12.7; 8192 -> 1024 12 rows 9.1
+// reading of x (m rows of row_bytes; none to speak of where x is staged, up to 16 rows) at what
+// a compute unit takes of strided rows, 33 KB/us.  Swept against gemm_kernel over 11 sizes per
+// kind and 1 to 64 rows: 4096 -> 14336 8 rows 10.7 us against 12.1, 16 rows 13.5 against 12.3;
+// 14336 -> 4096 4 rows 11.2 against 12.6, 8 rows 14.0 against 12.7; 8192 -> 1024 12 rows 9.1
 // against 9.3, 20 rows 14.6 against 9.4; 2880 -> 2880 20 rows 7.5 against 8.2, 32 rows 9.4
-// against 8.3.
+// against 8.3.  Rows of short K and wide outputs: 512 -> 131072 17 rows 17.4 against 10.1, 512 ->
+// 4096 32 rows 3.6 against 4.5; MXFP4 896 -> 65536 64 rows 25.5 against 11.9, 17 rows 10.6
+// against 10.3, 512 -> 262144 17 rows 20.6 against 25.7 (which the estimate misses: the GEMM's
+// many rounds of short tiles are dearer than it counts).  What a workgroup costs by itself is in
+// neither side: 128 -> 131072 1 row 10.5 against 7.1.
 // Where x takes less than 2.5 us no plan of gemm_kernel is the quicker, and none is made: it
 // would cost the caller about a microsecond.
 struct DecodeCost {
@@ -141,13 +145,12 @@ struct DecodeCost {
     }
 };
 
-inline DecodeCost decode_cost(size_t m, size_t row_bytes, size_t n, size_t weight_bytes,
-                              size_t cus) {
-    const size_t groups = ceil_div(n, 32);
-    const size_t row_tiles = groups >= cus ? groups : ceil_div(n, 16);
-    const double rounds = std::max(1.0, double(row_tiles) / double(cus));
-    const bool staged = m * staged_pitch(unsigned(row_bytes)) <= kStagedBytes;
-    return {double(weight_bytes) / 6.0e6, staged ? 0.0 : double(m * row_bytes) * rounds / 33.0e3};
+inline DecodeCost decode_cost(size_t m, size_t n, size_t k, bool gated, bool fp4, size_t cus) {
+    const DecodeShape s = decode_shape(m, n, k, gated, fp4, cus);
+    const double rounds = std::max(1.0, double(ceil_div(n, s.wide ? 32 : 16)) / double(cus));
+    const size_t row_bytes = fp4 ? k / 2 : k * 2, weight_bytes = n * k * 17 / 32 * (gated ? 2 : 1);
+    return {double(weight_bytes) / 6.0e6,
+            s.staged ? 0.0 : double(m * row_bytes) * rounds / 33.0e3};
 }
 
 inline Plan decode_plan() {
@@ -158,7 +161,7 @@ inline Plan decode_plan() {
 
 inline Plan plan_product(size_t m, size_t n, size_t k, bool fp4, size_t cus) {
     const bool few = m <= (fp4 ? 64 : 32);
-    const DecodeCost d = decode_cost(few ? m : 0, fp4 ? k / 2 : k * 2, n, n * k * 17 / 32, cus);
+    const DecodeCost d = few ? decode_cost(m, n, k, false, fp4, cus) : DecodeCost{};
     if (few && d.certain())
         return decode_plan();
     const Plan p = plan_gemm(m, ceil_div(n, 64), ceil_div(k, fp4 ? 256 : 64), fp4 ? kFp4 : kBf16,
@@ -168,7 +171,7 @@ inline Plan plan_product(size_t m, size_t n, size_t k, bool fp4, size_t cus) {
 
 inline Plan plan_gated(size_t m, size_t n, size_t k, bool kept, size_t cus) {
     const bool few = !kept && m <= 32;
-    const DecodeCost d = decode_cost(few ? m : 0, k * 2, n, n * k * 17 / 16, cus);
+    const DecodeCost d = few ? decode_cost(m, n, k, true, false, cus) : DecodeCost{};
     if (few && d.certain())
         return decode_plan();
     const Plan p = plan_gemm(m, ceil_div(n, 32), ceil_div(k, 64), kBf16, cus);

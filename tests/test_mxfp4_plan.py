@@ -70,3 +70,18 @@ def test_every_variant_is_reached_by_a_tested_size(plan, path):
         found.setdefault(variant, call)
     assert {v[1] for v in found if v[0] == "gemm"} == {1, 2, 3, 4}
     assert not {v: call for v, call in found.items() if v not in tested}
+
+
+@pytest.mark.parametrize("call,kernel", [
+    (("product", 31, 131072, 512, 0), "gemm"), (("product", 17, 65536, 896, 0), "gemm"),
+    (("product", 64, 65536, 896, 1), "gemm"), (("product", 31, 131072, 1984, 1), "gemm"),
+    (("gated", 17, 65536, 512, 0), "gemm"), (("product", 32, 4096, 512, 0), "decode"),
+    (("product", 64, 4096, 896, 1), "decode"), (("gated", 32, 4096, 512, 0), "decode"),
+    (("product", 16, 14336, 512, 0), "decode")])
+def test_rows_that_every_workgroup_reads_again_are_counted(plan, call, kernel):
+    """More than 16 rows never pass through LDS, however short they are: over many workgroups
+    their reading outweighs the weights'."""
+    variant, = plan([call])
+    assert variant[0] == kernel
+    if call[1] > 16 and kernel == "decode":
+        assert not variant[2]  # (not staged)
