@@ -405,6 +405,13 @@ def _row_stride(t: torch.Tensor, dtype, name: str, multiple: int = 8) -> int:
     return row
 
 
+def _no_graph(t: torch.Tensor, name: str) -> None:
+    """Refuses a tensor whose gradient would be lost: the calls record none."""
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient, which this call does not record: make it "
+                         "under torch.no_grad(), or within a torch.autograd.Function")
+
+
 _BF16 = torch.bfloat16
 _TYPES = {torch.float32: 0, torch.float16: 1, _BF16: 30}  # KDQ_F32, KDQ_F16, KDQ_BF16
 
@@ -532,6 +539,7 @@ def mxfp4_product(x: torch.Tensor, packed: torch.Tensor, n_out: int,
                   out: torch.Tensor | None = None) -> torch.Tensor:
     """bf16 [m, k] times a packed MXFP4 matrix (mxfp4_pack) of n_out rows of k values ->
     fp32 or bf16 [m, n_out] (kdq_mxfp4_product)."""
+    _no_graph(x, "x")
     stride = _row_stride(x, _BF16, "x")
     m, k = x.shape
     kind = _type(dtype)
@@ -575,7 +583,9 @@ def mxfp4_gated(x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, n_out: in
     """h = silu(x Wg^T) * (x Wu^T): bf16 [m, k] and two packed MXFP4 matrices (mxfp4_pack) of
     n_out rows (n_out % 32 == 0) -> bf16 [m, n_out] (kdq_mxfp4_gated).  With ``save`` the
     pre-activations are kept for mxfp4_gated_backward, and (h, saved) returned: "bf16" as one
-    tensor [m, 2 n_out], "q8" as int8 [m, 2 n_out] and fp32 scales [m, 2 n_out / 32]."""
+    tensor [m, 2 n_out], "q8" as int8 [m, 2 n_out] and fp32 scales [m, 2 n_out / 32].  Nothing
+    is recorded for autograd: the two calls are the halves of a torch.autograd.Function."""
+    _no_graph(x, "x")
     stride = _row_stride(x, _BF16, "x")
     if save not in (None, "bf16", "q8"):
         raise ValueError('save: None, "bf16" or "q8"')
@@ -612,6 +622,7 @@ def mxfp4_gated_backward(dh: torch.Tensor, saved, gate: torch.Tensor, up: torch.
     from its forward pass, the matrices from mxfp4_pack(..., transposed=True) -> dx bf16
     [m, n_in] and the pre-activations' gradients bf16 [m, 2 n_out], gates then ups
     (kdq_mxfp4_gated_backward)."""
+    _no_graph(dh, "dh")
     stride = _row_stride(dh, _BF16, "dh")
     m, n = dh.shape
     if n % 32 or n_in % 32 or not n_in:

@@ -222,6 +222,19 @@ def test_a_workspace_over_an_input_is_refused(quantized):
         assert lib.kdq_mxfp4_product(x, 64, 1, w, 64, 64, 0, y, 64, w, 16, None) == 4
 
 
+def test_a_gradient_that_would_be_lost_is_refused():
+    """Before anything else about the call; not where no graph is recorded."""
+    x, u8 = torch.zeros(2, 64, dtype=torch.bfloat16, requires_grad=True), torch.zeros(
+        1280, dtype=torch.uint8)
+    calls = (lambda: ops.mxfp4_product(x, u8, 32), lambda: ops.mxfp4_gated(x, u8, u8, 32),
+             lambda: ops.mxfp4_gated_backward(x, x, u8, u8, 64))
+    for call in calls:
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+        with torch.no_grad(), pytest.raises(ValueError, match="device tensor"):
+            call()
+
+
 class Packed:
     """What the wrappers look at of a packed device tensor."""
     dtype, is_cuda = torch.uint8, True

@@ -761,3 +761,37 @@ def test_the_other_packed_form_is_refused(device, gen):
         with pytest.raises(ValueError):
             call()
     torch.cuda.synchronize()
+
+
+class Gated(torch.autograd.Function):
+    """The gated projection over frozen weights as a user's program records it."""
+
+    @staticmethod
+    def forward(ctx, x, gate, up, gate_t, up_t, n):
+        h, saved = ops.mxfp4_gated(x, gate, up, n, save="bf16")
+        ctx.save_for_backward(saved, gate_t, up_t)
+        return h
+
+    @staticmethod
+    def backward(ctx, dh):
+        saved, gate_t, up_t = ctx.saved_tensors
+        k = 2 * gate_t.shape[0] * 32
+        dx, _ = ops.mxfp4_gated_backward(dh, saved, gate_t, up_t, k)
+        return dx, None, None, None, None, None
+
+
+def test_recorded_by_a_function_and_refused_without_one(device, gen):
+    m, n, k = 40, 96, 128
+    wg, wu = ref.matrix(gen, n, k), ref.matrix(gen, n, k)
+    packed = [ops.mxfp4_pack(*w) for w in (wg, wu)]
+    transposed = [ops.mxfp4_pack(*w, transposed=True) for w in (wg, wu)]
+    x = normal(gen, m, k).bfloat16().requires_grad_()
+    with pytest.raises(ValueError, match="gradient"):
+        ops.mxfp4_gated(x, *packed, n)
+    with torch.no_grad():
+        plain, saved = ops.mxfp4_gated(x, *packed, n, save="bf16")
+    h = Gated.apply(x, *packed, *transposed, n)
+    assert torch.equal(h, plain)
+    dh = normal(gen, m, n).bfloat16()
+    h.backward(dh)
+    assert torch.equal(x.grad, ops.mxfp4_gated_backward(dh, saved, *transposed, k)[0])
