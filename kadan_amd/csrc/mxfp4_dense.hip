@@ -12,8 +12,9 @@
 //   reduce_kernel      K slices of gemm_kernel summed in slice order, then its epilogue
 //   gate_grad_kernel   dg, du from dh and the kept pre-activations
 //
-// Times below are of one MI355X (others: up to 6 % apart where the matrix cores are the bound),
-// whose 1 GB copy runs at 5.2 TB/s and whose library 8192^3 bf16 product at 1.25 PFLOP/s.
+// mxfp4_plan.hpp chooses among them.  Times below are of single MI355X cards, up to 20 % apart
+// where the matrix cores are the bound; one's 1 GB copy runs at 5.2 TB/s and its library 8192^3
+// bf16 product at 1.25 PFLOP/s.
 #include "kdq_common.hpp"
 #include "mxfp4_plan.hpp"
 
@@ -850,13 +851,13 @@ __global__ __launch_bounds__(1024) void decode_t_kernel(Decode a) {
 // transposed weights under bf16 gradients (their scales lie along the columns, which are not
 // summed over, so the scaled MFMA cannot take them).
 //
-// bf16, 512 x 4096 -> 14336: 49-53 us, 1.13-1.22 PFLOP/s; gated projection 2048 x 4096 ->
-// 14336 387 us, 1.24, with codes kept 417, 1.15; backward of that 398 us, 1.21.  Bound by the
-// matrix cores' clock under load: products of random values alone, with nothing to load,
-// decode or wait for, run at 1.68 PFLOP/s here.  MXFP4, 2048 x 4096 -> 14336: 73-78 us, 3.1-3.3
-// PFLOP/s of 6.4 by that measure, 38 us of products: 448 tiles of 256 x 256 are 1.75 rounds of
-// the compute units, which take as long as two (43 us); the rest are waits for operands and the
-// results' way out.  (By count, at the products' own pace, operands would take a third of the
+// bf16, 512 x 4096 -> 14336: 49-59 us, 1.0-1.2 PFLOP/s; gated projection 2048 x 4096 ->
+// 14336 387 us, 1.24, with codes kept 409-426, 1.13-1.18, with bf16 values kept 430, 1.12; backward
+// of that 397-412 us, 1.17-1.21.  Bound by the matrix cores' clock under load: products of random
+// values alone, with nothing to load, decode or wait for, run at 1.68 PFLOP/s here.  MXFP4, 2048 x
+// 4096 -> 14336: 73-84 us, 2.9-3.3 PFLOP/s of 6.4 by that measure, 38 us of products: 448 tiles of
+// 256 x 256 are 1.75 rounds of the compute units, which take as long as two (43 us); the rest are
+// waits for operands and the results' way out.  (By count, at the products' own pace, operands would take a third of the
 // LDS's 128 bytes a cycle and weights and x about 30 bytes a cycle of a compute unit's loads.)
 // (Four wavefronts of 64 x 256 in place of eight took 74-96 us.)
 //
@@ -873,7 +874,8 @@ struct Gemm {
     unsigned x_second;        // kTransposed: bytes to the second matrix's values in a row
     unsigned segments;        // 16-byte segments of a row of x (of one matrix's part)
     unsigned groups, steps;   // of the packed form
-    unsigned chunks, part;    // chunks of K, and how many a part has (a multiple of 4)
+    unsigned chunks, part;    // chunks of K, and how many a part has (kFp4: any number; else a
+                              // multiple of 4, the loop's turn)
     unsigned tiles_n, tiles_m;
     Target out;
     float* partial;           // K slices: results go here
@@ -1361,8 +1363,10 @@ __global__ __launch_bounds__(256) void reduce_kernel(const float* __restrict__ p
 // g and u come as bf16 [m][2n] or as 8-bit codes with a scale per 32.  dg and du leave as bf16,
 // the operands of the product with the weights and what a framework's gradients of bf16
 // activations are: dx is off by 2.3e-3 of its root mean square for it, 1.7e-3 being its own
-// rounding.  Bound by memory: 2048 x 14336 from codes 37 us (242 MB, 6.5 TB/s), 1024 rows from
-// bf16 25 us (147 MB, 5.9 TB/s).
+// rounding.  (What the rounding leaves over, as a second bf16 operand, would double the matrix
+// products, which are nine tenths of the pass: 207 us of 1024 rows to about 400.)  Bound by
+// memory: 2048 x 14336 from codes 37 us (242 MB, 6.5 TB/s), 1024 rows from bf16 25 us (147 MB,
+// 5.9 TB/s).
 
 template <bool Q8>
 __global__ __launch_bounds__(256) void gate_grad_kernel(const uint16_t* __restrict__ dh,

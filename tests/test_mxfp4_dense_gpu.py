@@ -770,13 +770,12 @@ class Gated(torch.autograd.Function):
     def forward(ctx, x, gate, up, gate_t, up_t, n):
         h, saved = ops.mxfp4_gated(x, gate, up, n, save="bf16")
         ctx.save_for_backward(saved, gate_t, up_t)
+        ctx.k = x.shape[1]
         return h
 
     @staticmethod
     def backward(ctx, dh):
-        saved, gate_t, up_t = ctx.saved_tensors
-        k = 2 * gate_t.shape[0] * 32
-        dx, _ = ops.mxfp4_gated_backward(dh, saved, gate_t, up_t, k)
+        dx, _ = ops.mxfp4_gated_backward(dh.contiguous(), *ctx.saved_tensors, ctx.k)
         return dx, None, None, None, None, None
 
 
@@ -795,3 +794,7 @@ def test_recorded_by_a_function_and_refused_without_one(device, gen):
     dh = normal(gen, m, n).bfloat16()
     h.backward(dh)
     assert torch.equal(x.grad, ops.mxfp4_gated_backward(dh, saved, *transposed, k)[0])
+    x.grad = None
+    Gated.apply(x, *packed, *transposed, n).sum().backward()  # (a gradient of rows that overlap)
+    ones = torch.ones(m, n, dtype=BF16, device=device)
+    assert torch.equal(x.grad, ops.mxfp4_gated_backward(ones, saved, *transposed, k)[0])
