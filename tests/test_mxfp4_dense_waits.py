@@ -50,7 +50,6 @@ def run(body):
     LDS are still on their way as ("x" | "scale", number from 0), reads of LDS on their way)."""
     place = {at: i for i, (at, _) in enumerate(body)}
     flying, reads, issued, barriers, i = [], 0, {"x": 0, "scale": 0}, [], 0
-    taken = set()
     while len(barriers) < BARRIERS:
         at, text = body[i]
         op, i = text.split()[0], i + 1
