@@ -474,6 +474,52 @@ int kdq_mxfp4_gated_backward(const uint16_t* dh_bf16, size_t dh_stride, size_t m
                              uint16_t* dgu_bf16, uint16_t* dx_bf16, size_t dx_stride,
                              void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- a mixture layer in pieces, with their gradients, around kdq_moe_route and the products
+ * below (the reference runs the layer on the host and has no gradients:
+ * IW/src/models/text/qwen_layers.cpp:378-492).  Slot token * top_k + i is a token's i-th
+ * selection; `perm` is kdq_moe_route's (a permutation of the slots, those of expert 0 first).
+ * Rows are of type KDQ_F32, KDQ_F16 or KDQ_BF16, any number of values apart, aligned to their
+ * values; tokens <= 2^20, top_k <= 8, cols <= 2^20.  No output may overlap an input or another
+ * output, but for what is said at kdq_moe_combine.  No call uses a workspace, so calls on
+ * different streams may overlap, and every call may be captured. */
+
+/* rows[p] = x[perm[p] / top_k] for the tokens * top_k positions p, and place[perm[p]] = p.  An
+ * entry of perm that is no slot gives a row of zeros and no place. */
+int kdq_moe_sort(int type, const void* x, size_t x_stride, size_t tokens, size_t cols,
+                 size_t top_k, const int32_t* perm, void* rows, size_t rows_stride,
+                 int32_t* place, void* stream);
+
+/* Its gradient: dx[t] = sum over i of drows[place[t * top_k + i]], summed in fp32 in that order
+ * and rounded once.  Here and below a place that is no position contributes nothing. */
+int kdq_moe_sort_backward(int type, const void* drows, size_t drows_stride, const int32_t* place,
+                          size_t tokens, size_t cols, size_t top_k, void* dx, size_t dx_stride,
+                          void* stream);
+
+/* y[t] = residual[t] + sum over i of weights[t, i] * rows[place[t * top_k + i]], summed in fp32
+ * in that order and rounded once.  weights fp32 [tokens x top_k]; y, and residual (or null), of
+ * type y_type: the rows' or KDQ_F32.  y may be the residual itself (with its stride). */
+int kdq_moe_combine(int type, const void* rows, size_t rows_stride, const int32_t* place,
+                    const float* weights, size_t tokens, size_t cols, size_t top_k, int y_type,
+                    const void* residual, size_t residual_stride, void* y, size_t y_stride,
+                    void* stream);
+
+/* Its gradients: drows[place[t * top_k + i]] = weights[t, i] * dy[t] (of the rows' type) and
+ * dweights[t, i] = dy[t] . rows[place[t * top_k + i]] (fp32 sums); dy of type dy_type: the rows'
+ * or KDQ_F32.  The residual's gradient is dy. */
+int kdq_moe_combine_backward(int type, const void* rows, size_t rows_stride, const int32_t* place,
+                             const float* weights, size_t tokens, size_t cols, size_t top_k,
+                             int dy_type, const void* dy, size_t dy_stride, void* drows,
+                             size_t drows_stride, float* dweights, void* stream);
+
+/* The gradient of kdq_moe_route's weights with respect to its logits: for idx and weights
+ * [tokens x top_k] as it wrote them, dlogits [tokens x experts] is
+ * w_i * (dw_i - sum over j of w_j * dw_j) at idx_i and 0 elsewhere.  (The weights are a softmax
+ * over the selected logits: the floor of 2^-14 under their sum cannot act, since the largest of
+ * at most 256 probabilities is at least 2^-8.) */
+int kdq_moe_route_backward(const int32_t* idx, const float* weights, const float* dweights,
+                           size_t tokens, size_t experts, size_t top_k, float* dlogits,
+                           void* stream);
+
 /* Measurement aid, no counterpart in the reference: one streaming read of `bytes`
  * (a multiple of 16; `src` 16-byte aligned) over `workgroups` workgroups of `threads`
  * (256 or 1024) lanes.  Workgroup b folds (xor) the 32-bit words of its share, units of

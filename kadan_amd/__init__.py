@@ -96,6 +96,12 @@ _SIGNATURES = {
                         _VP],
     "kdq_mxfp4_gated_backward": [_VP, _SZ, _SZ, _VP, _VP, _VP, _VP, _VP, _SZ, _SZ, _VP, _VP, _SZ,
                                  _VP, _SZ, _VP],
+    "kdq_moe_sort": [_I, _VP, _SZ, _SZ, _SZ, _SZ, _VP, _VP, _SZ, _VP, _VP],
+    "kdq_moe_sort_backward": [_I, _VP, _SZ, _VP, _SZ, _SZ, _SZ, _VP, _SZ, _VP],
+    "kdq_moe_combine": [_I, _VP, _SZ, _VP, _VP, _SZ, _SZ, _SZ, _I, _VP, _SZ, _VP, _SZ, _VP],
+    "kdq_moe_combine_backward": [_I, _VP, _SZ, _VP, _VP, _SZ, _SZ, _SZ, _I, _VP, _SZ, _VP, _SZ,
+                                 _VP, _VP],
+    "kdq_moe_route_backward": [_VP, _VP, _VP, _SZ, _SZ, _SZ, _VP, _VP],
     "kdq_hbm_read": [_VP, _SZ, _VP, _SZ, _I, _I, C.c_uint, _VP],
     "kdq_release_scratch": [],
 }

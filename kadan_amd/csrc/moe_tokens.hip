@@ -1,0 +1,535 @@
+// Tokens sorted by expert and back, with their gradients, and the router's (include/kadan_amd.h).
+// The reference goes from expert to expert on the host (MoeLayer::forward,
+// IW/src/models/text/qwen_layers.cpp:378-492; IW = services/hikari/inference_worker) and has no
+// gradients.
+//
+//   sort_kernel            rows[p] = x[perm[p] / top_k], place[perm[p]] = p
+//   combine_kernel         y[t] = residual[t] + sum_i w[t, i] rows[place[t top_k + i]]; without
+//                          weights the gradient of sorting
+//   combine_grad_kernel    drows[place] = w dy, dw = dy . rows[place]
+//   route_grad_kernel      dlogits of the renormalised weights of the selection
+//
+// All of them move memory: a value costs a few operations at most.  A lane moves eight values
+// (16 or 32 bytes) at a time, from any element on: gfx950 loads need no alignment beyond it.
+#include "kdq_common.hpp"
+
+#include <algorithm>
+
+namespace kdq {
+namespace {
+
+constexpr unsigned kThreads = 256, kMost = 8;  // selections of a token
+
+struct Bf16 {
+    uint16_t bits;
+};
+struct F16 {
+    uint16_t bits;
+};
+
+typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ float widen(Bf16 v) {
+    return __uint_as_float(unsigned(v.bits) << 16);
+}
+__device__ __forceinline__ float widen(F16 v) {
+    return half_hw(v.bits);
+}
+__device__ __forceinline__ float widen(float v) {
+    return v;
+}
+
+template <class T> __device__ __forceinline__ T narrow(float v);
+template <> __device__ __forceinline__ float narrow<float>(float v) {
+    return v;
+}
+template <> __device__ __forceinline__ Bf16 narrow<Bf16>(float v) {
+    return {__builtin_bit_cast(uint16_t, __bf16(v))};
+}
+template <> __device__ __forceinline__ F16 narrow<F16>(float v) {
+    return {__builtin_bit_cast(uint16_t, _Float16(v))};
+}
+
+// Eight values as they lie.
+template <class T> struct Eight {
+    u32x4 w[sizeof(T) / 2];
+};
+
+template <class T> __device__ __forceinline__ Eight<T> load8(const T* p) {
+    Eight<T> v;
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(T) / 2; ++i)
+        v.w[i] = load16_a2(reinterpret_cast<const uint8_t*>(p) + 16 * i);
+    return v;
+}
+
+template <class T> __device__ __forceinline__ void store8(T* p, const Eight<T>& v) {
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(T) / 2; ++i)
+        reinterpret_cast<u32x4_a2*>(p)[i] = u32x4_a2{v.w[i].x, v.w[i].y, v.w[i].z, v.w[i].w};
+}
+
+__device__ __forceinline__ float value(const Eight<Bf16>& v, int i) {
+    const unsigned w = v.w[0][i / 2];
+    return __uint_as_float(i % 2 ? w & 0xffff0000u : w << 16);
+}
+__device__ __forceinline__ float value(const Eight<F16>& v, int i) {
+    return half_hw((v.w[0][i / 2] >> (16 * (i % 2))) & 0xffffu);
+}
+__device__ __forceinline__ float value(const Eight<float>& v, int i) {
+    return __uint_as_float(v.w[i / 4][i % 4]);
+}
+
+__device__ __forceinline__ void set(Eight<Bf16>& v, const float (&f)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        v.w[0][i] = __builtin_bit_cast(unsigned, bf16x2{__bf16(f[2 * i]), __bf16(f[2 * i + 1])});
+}
+__device__ __forceinline__ void set(Eight<F16>& v, const float (&f)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        v.w[0][i] = unsigned(narrow<F16>(f[2 * i]).bits) |
+                    unsigned(narrow<F16>(f[2 * i + 1]).bits) << 16;
+}
+__device__ __forceinline__ void set(Eight<float>& v, const float (&f)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        v.w[i / 4][i % 4] = __float_as_uint(f[i]);
+}
+
+// A row's values c .. c + 7, of which those past its end read as zeros and are not written.
+template <class T>
+__device__ __forceinline__ Eight<T> load_piece(const T* row, unsigned c, unsigned cols) {
+    if (c + 8 <= cols)
+        return load8(row + c);
+    float f[8];
+#pragma unroll
+    for (unsigned i = 0; i < 8; ++i)
+        f[i] = c + i < cols ? widen(row[c + i]) : 0.f;
+    Eight<T> v;
+    set(v, f);
+    return v;
+}
+
+template <class T>
+__device__ __forceinline__ void store_piece(T* row, unsigned c, unsigned cols, const float (&f)[8]) {
+    if (c + 8 <= cols) {
+        Eight<T> v;
+        set(v, f);
+        store8(row + c, v);
+        return;
+    }
+#pragma unroll
+    for (unsigned i = 0; i < 8; ++i)
+        if (c + i < cols)
+            row[c + i] = narrow<T>(f[i]);
+}
+
+// How a launch's workgroups share rows of `cols` values: `across` lanes (a power of two) along a
+// row, the others' along further rows.
+struct Shape {
+    unsigned across, rows, blocks;  // rows of a workgroup, workgroups of a row
+};
+
+Shape shape_of(size_t cols) {
+    const size_t pieces = (cols + 7) / 8;
+    unsigned across = 1;
+    while (across < kThreads && across < pieces)
+        across *= 2;
+    return {across, kThreads / across, unsigned((pieces + across - 1) / across)};
+}
+
+// A copy, so bits and no values.
+template <class U>
+__global__ __launch_bounds__(kThreads) void sort_kernel(const U* __restrict__ x, size_t x_stride,
+                                                        unsigned slots, unsigned cols,
+                                                        unsigned top_k, Shape s,
+                                                        const int32_t* __restrict__ perm,
+                                                        U* __restrict__ rows, size_t rows_stride,
+                                                        int32_t* __restrict__ place) {
+    const unsigned p = blockIdx.x * s.rows + threadIdx.x / s.across;
+    const unsigned c = (blockIdx.y * s.across + threadIdx.x % s.across) * 8;
+    if (p >= slots || c >= cols)
+        return;
+    const unsigned slot = unsigned(perm[p]);
+    U* to = rows + size_t(p) * rows_stride + c;
+    if (slot >= slots) {  // no slot: a row of zeros
+        for (unsigned i = 0; i < 8 && c + i < cols; ++i)
+            to[i] = U{};
+        return;
+    }
+    if (c == 0)
+        place[slot] = int32_t(p);
+    const U* from = x + size_t(slot / top_k) * x_stride + c;
+    if (c + 8 <= cols) {
+        store8(to, load8(from));
+    } else {
+        for (unsigned i = 0; c + i < cols; ++i)
+            to[i] = from[i];
+    }
+}
+
+// Sums in fp32, in the order of the selection, and one rounding.
+template <class T, class Y>
+__global__ __launch_bounds__(kThreads) void combine_kernel(
+    const T* __restrict__ rows, size_t rows_stride, const int32_t* __restrict__ place,
+    const float* __restrict__ weights, unsigned tokens, unsigned top_k, unsigned cols, Shape s,
+    const Y* residual, size_t residual_stride, Y* y, size_t y_stride) {
+    const unsigned t = blockIdx.x * s.rows + threadIdx.x / s.across;
+    const unsigned c = (blockIdx.y * s.across + threadIdx.x % s.across) * 8;
+    if (t >= tokens || c >= cols)
+        return;
+    const unsigned slots = tokens * top_k;
+    unsigned at[kMost];
+    float w[kMost];
+#pragma unroll
+    for (unsigned i = 0; i < kMost; ++i)
+        if (i < top_k) {
+            at[i] = unsigned(place[t * top_k + i]);
+            w[i] = weights ? weights[t * top_k + i] : 1.0f;
+        }
+    Eight<T> v[kMost];
+#pragma unroll
+    for (unsigned i = 0; i < kMost; ++i)
+        if (i < top_k && at[i] < slots)
+            v[i] = load_piece(rows + size_t(at[i]) * rows_stride, c, cols);
+    float sum[8] = {};
+    if (residual) {
+        const Eight<Y> r = load_piece(residual + size_t(t) * residual_stride, c, cols);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            sum[e] = value(r, e);
+    }
+#pragma unroll
+    for (unsigned i = 0; i < kMost; ++i)
+        if (i < top_k && at[i] < slots)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                sum[e] = fmaf(w[i], value(v[i], e), sum[e]);
+    store_piece(y + size_t(t) * y_stride, c, cols, sum);
+}
+
+// A workgroup takes a token: its dy is read once for all of its rows, each of which is read,
+// multiplied into its weight's gradient and written over by none (drows is another tensor).
+template <class T, class Y>
+__global__ __launch_bounds__(kThreads) void combine_grad_kernel(
+    const T* __restrict__ rows, size_t rows_stride, const Y* __restrict__ dy, size_t dy_stride,
+    const int32_t* __restrict__ place, const float* __restrict__ weights, unsigned tokens,
+    unsigned top_k, unsigned cols, T* __restrict__ drows, size_t drows_stride,
+    float* __restrict__ dweights) {
+    __shared__ float sums[kThreads / 64][kMost];
+    const unsigned t = blockIdx.x, slots = tokens * top_k;
+    const unsigned lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    unsigned at[kMost];
+    float w[kMost], dot[kMost] = {};
+#pragma unroll
+    for (unsigned i = 0; i < kMost; ++i)
+        if (i < top_k) {
+            at[i] = unsigned(place[t * top_k + i]);
+            w[i] = weights[t * top_k + i];
+        }
+    for (unsigned c = threadIdx.x * 8; c < cols; c += blockDim.x * 8) {
+        const Eight<Y> d = load_piece(dy + size_t(t) * dy_stride, c, cols);
+        Eight<T> v[kMost];
+#pragma unroll
+        for (unsigned i = 0; i < kMost; ++i)
+            if (i < top_k && at[i] < slots)
+                v[i] = load_piece(rows + size_t(at[i]) * rows_stride, c, cols);
+#pragma unroll
+        for (unsigned i = 0; i < kMost; ++i)
+            if (i < top_k && at[i] < slots) {
+                float f[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float g = value(d, e);
+                    dot[i] = fmaf(g, value(v[i], e), dot[i]);
+                    f[e] = w[i] * g;
+                }
+                store_piece(drows + size_t(at[i]) * drows_stride, c, cols, f);
+            }
+    }
+#pragma unroll
+    for (unsigned i = 0; i < kMost; ++i)
+        if (i < top_k) {
+            const float sum = wave_sum(dot[i]);
+            if (lane == 0)
+                sums[wave][i] = sum;
+        }
+    __syncthreads();
+    if (threadIdx.x < top_k) {
+        float sum = 0.f;
+        for (unsigned i = 0; i < blockDim.x / 64; ++i)
+            sum += sums[i][threadIdx.x];
+        dweights[t * top_k + threadIdx.x] = sum;
+    }
+}
+
+// w = softmax over the selected logits, so dlogit = w (dw - sum w dw) there and 0 elsewhere.  A
+// wavefront takes a token: lane i its selection i, then lanes go along the experts.
+__global__ __launch_bounds__(kThreads) void route_grad_kernel(
+    const int32_t* __restrict__ idx, const float* __restrict__ weights,
+    const float* __restrict__ dweights, unsigned tokens, unsigned experts, unsigned top_k,
+    float* __restrict__ dlogits) {
+    const unsigned t = blockIdx.x * (kThreads / 64) + threadIdx.x / 64, lane = threadIdx.x % 64;
+    if (t >= tokens)
+        return;
+    const bool chosen = lane < top_k;
+    const int e = chosen ? idx[t * top_k + lane] : -1;
+    const float w = chosen ? weights[t * top_k + lane] : 0.f;
+    const float d = chosen ? dweights[t * top_k + lane] : 0.f;
+    float sum = w * d;  // (of lanes 0 to 7, in every one of them)
+#pragma unroll
+    for (int offset = 4; offset > 0; offset >>= 1)
+        sum += __shfl_xor(sum, offset, 64);
+    const float g = w * (d - sum);
+    for (unsigned c = lane; c < experts; c += 64) {
+        float out = 0.f;
+#pragma unroll
+        for (unsigned i = 0; i < kMost; ++i)
+            if (i < top_k &&
+                unsigned(__builtin_amdgcn_readlane(e, int(i))) == c)
+                out = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(g), int(i)));
+        dlogits[size_t(t) * experts + c] = out;
+    }
+}
+
+// ------------------------------------------------------------------ arguments
+
+constexpr size_t kMaxTokens = size_t(1) << 20, kMaxCols = size_t(1) << 20;
+
+size_t size_of(int type) {
+    return type == KDQ_F32 ? 4 : type == KDQ_F16 || type == KDQ_BF16 ? 2 : 0;
+}
+
+// Rows of a call: their bytes from the first value to the last.
+struct Rows {
+    const void* p;
+    size_t stride, count;
+    int type;
+    size_t bytes(size_t cols) const {
+        return ((count - 1) * stride + cols) * size_of(type);
+    }
+};
+
+int check_sizes(size_t tokens, size_t top_k, size_t cols) {
+    if (!tokens || !top_k || !cols)
+        return KDQ_ERR_ARGUMENT;
+    return tokens > kMaxTokens || top_k > kMost || cols > kMaxCols ? KDQ_ERR_SHAPE : KDQ_OK;
+}
+
+int check_rows(const Rows& r, size_t cols) {
+    if (!size_of(r.type))
+        return KDQ_ERR_UNSUPPORTED;
+    if (r.stride < cols || r.stride > (SIZE_MAX >> 4) / r.count)
+        return KDQ_ERR_SHAPE;
+    return misaligned(r.p, size_of(r.type)) ? KDQ_ERR_ALIGNMENT : KDQ_OK;
+}
+
+int check_words(const void* p) {
+    return misaligned(p, 4) ? KDQ_ERR_ALIGNMENT : KDQ_OK;
+}
+
+#define KDQ_TRY(check)              \
+    do {                            \
+        if (const int rc_ = (check)) \
+            return rc_;             \
+    } while (0)
+
+struct Range {
+    const void* p;
+    size_t bytes;
+};
+
+template <size_t N, size_t M> bool any_overlap(const Range (&out)[N], const Range (&in)[M]) {
+    for (size_t i = 0; i < N; ++i) {
+        for (const Range& b : in)
+            if (overlaps(out[i].p, out[i].bytes, b.p, b.bytes))
+                return true;
+        for (size_t j = 0; j < i; ++j)
+            if (overlaps(out[i].p, out[i].bytes, out[j].p, out[j].bytes))
+                return true;
+    }
+    return false;
+}
+
+// f with a value of the C++ type of `type`, and (two types) one of the second: the first's or
+// fp32.
+template <class F> int by_type(int type, F&& f) {
+    switch (type) {
+    case KDQ_BF16:
+        return f(Bf16{});
+    case KDQ_F16:
+        return f(F16{});
+    default:
+        return f(0.f);
+    }
+}
+
+template <class F> int by_types(int type, int second, F&& f) {
+    return by_type(type, [&](auto t) {
+        return second == type ? f(t, t) : f(t, 0.f);
+    });
+}
+
+int combine(const Rows& rows, const int32_t* place, const float* weights, size_t tokens,
+            size_t top_k, size_t cols, const Rows& residual, const Rows& y, hipStream_t st) {
+    const Shape s = shape_of(cols);
+    return by_types(rows.type, y.type, [&](auto t, auto u) {
+        using T = decltype(t);
+        using Y = decltype(u);
+        hipLaunchKernelGGL((combine_kernel<T, Y>),
+                           dim3(unsigned((tokens + s.rows - 1) / s.rows), s.blocks),
+                           dim3(kThreads), 0, st, static_cast<const T*>(rows.p), rows.stride,
+                           place, weights, unsigned(tokens), unsigned(top_k), unsigned(cols), s,
+                           static_cast<const Y*>(residual.p), residual.stride,
+                           static_cast<Y*>(const_cast<void*>(y.p)), y.stride);
+        KDQ_HIP(hipGetLastError());
+        return int(KDQ_OK);
+    });
+}
+}  // namespace
+}  // namespace kdq
+
+using namespace kdq;
+
+extern "C" int kdq_moe_sort(int type, const void* x, size_t x_stride, size_t tokens, size_t cols,
+                            size_t top_k, const int32_t* perm, void* rows, size_t rows_stride,
+                            int32_t* place, void* stream) {
+    if (!x || !perm || !rows || !place)
+        return KDQ_ERR_ARGUMENT;
+    KDQ_TRY(check_sizes(tokens, top_k, cols));
+    const size_t slots = tokens * top_k;
+    const Rows in{x, x_stride, tokens, type}, out{rows, rows_stride, slots, type};
+    KDQ_TRY(check_rows(in, cols));
+    KDQ_TRY(check_rows(out, cols));
+    KDQ_TRY(check_words(perm));
+    KDQ_TRY(check_words(place));
+    const Range to[] = {{rows, out.bytes(cols)}, {place, slots * 4}},
+                from[] = {{x, in.bytes(cols)}, {perm, slots * 4}};
+    if (any_overlap(to, from))
+        return KDQ_ERR_ALIAS;
+    const Shape s = shape_of(cols);
+    const auto launch = [&](auto u) {
+        using U = decltype(u);
+        hipLaunchKernelGGL(sort_kernel<U>, dim3(unsigned((slots + s.rows - 1) / s.rows), s.blocks),
+                           dim3(kThreads), 0, static_cast<hipStream_t>(stream),
+                           static_cast<const U*>(x), x_stride, unsigned(slots), unsigned(cols),
+                           unsigned(top_k), s, perm, static_cast<U*>(rows), rows_stride, place);
+        KDQ_HIP(hipGetLastError());
+        return int(KDQ_OK);
+    };
+    return type == KDQ_F32 ? launch(0.f) : launch(Bf16{});
+}
+
+extern "C" int kdq_moe_sort_backward(int type, const void* drows, size_t drows_stride,
+                                     const int32_t* place, size_t tokens, size_t cols,
+                                     size_t top_k, void* dx, size_t dx_stride, void* stream) {
+    if (!drows || !place || !dx)
+        return KDQ_ERR_ARGUMENT;
+    KDQ_TRY(check_sizes(tokens, top_k, cols));
+    const size_t slots = tokens * top_k;
+    const Rows in{drows, drows_stride, slots, type}, out{dx, dx_stride, tokens, type};
+    KDQ_TRY(check_rows(in, cols));
+    KDQ_TRY(check_rows(out, cols));
+    KDQ_TRY(check_words(place));
+    const Range to[] = {{dx, out.bytes(cols)}},
+                from[] = {{drows, in.bytes(cols)}, {place, slots * 4}};
+    if (any_overlap(to, from))
+        return KDQ_ERR_ALIAS;
+    return combine(in, place, nullptr, tokens, top_k, cols, Rows{}, out,
+                   static_cast<hipStream_t>(stream));
+}
+
+extern "C" int kdq_moe_combine(int type, const void* rows, size_t rows_stride,
+                               const int32_t* place, const float* weights, size_t tokens,
+                               size_t cols, size_t top_k, int y_type, const void* residual,
+                               size_t residual_stride, void* y, size_t y_stride, void* stream) {
+    if (!rows || !place || !weights || !y)
+        return KDQ_ERR_ARGUMENT;
+    KDQ_TRY(check_sizes(tokens, top_k, cols));
+    if (y_type != type && y_type != KDQ_F32)
+        return KDQ_ERR_UNSUPPORTED;
+    const size_t slots = tokens * top_k;
+    const Rows in{rows, rows_stride, slots, type}, out{y, y_stride, tokens, y_type},
+        add{residual, residual ? residual_stride : cols, tokens, y_type};
+    KDQ_TRY(check_rows(in, cols));
+    KDQ_TRY(check_rows(out, cols));
+    KDQ_TRY(check_rows(add, cols));
+    KDQ_TRY(check_words(place));
+    KDQ_TRY(check_words(weights));
+    // (y may be the residual itself: a lane reads what it then writes)
+    const bool in_place = residual == y && residual_stride == y_stride;
+    const Range to[] = {{y, out.bytes(cols)}},
+                from[] = {{rows, in.bytes(cols)},
+                          {place, slots * 4},
+                          {weights, slots * 4},
+                          {in_place ? nullptr : residual, add.bytes(cols)}};
+    if (any_overlap(to, from))
+        return KDQ_ERR_ALIAS;
+    return combine(in, place, weights, tokens, top_k, cols, add, out,
+                   static_cast<hipStream_t>(stream));
+}
+
+extern "C" int kdq_moe_combine_backward(int type, const void* rows, size_t rows_stride,
+                                        const int32_t* place, const float* weights, size_t tokens,
+                                        size_t cols, size_t top_k, int dy_type, const void* dy,
+                                        size_t dy_stride, void* drows, size_t drows_stride,
+                                        float* dweights, void* stream) {
+    if (!rows || !place || !weights || !dy || !drows || !dweights)
+        return KDQ_ERR_ARGUMENT;
+    KDQ_TRY(check_sizes(tokens, top_k, cols));
+    if (dy_type != type && dy_type != KDQ_F32)
+        return KDQ_ERR_UNSUPPORTED;
+    const size_t slots = tokens * top_k;
+    const Rows in{rows, rows_stride, slots, type}, of{dy, dy_stride, tokens, dy_type},
+        out{drows, drows_stride, slots, type};
+    KDQ_TRY(check_rows(in, cols));
+    KDQ_TRY(check_rows(of, cols));
+    KDQ_TRY(check_rows(out, cols));
+    for (const void* p : {static_cast<const void*>(place), static_cast<const void*>(weights),
+                          static_cast<const void*>(dweights)})
+        KDQ_TRY(check_words(p));
+    const Range to[] = {{drows, out.bytes(cols)}, {dweights, slots * 4}},
+                from[] = {{rows, in.bytes(cols)},
+                          {dy, of.bytes(cols)},
+                          {place, slots * 4},
+                          {weights, slots * 4}};
+    if (any_overlap(to, from))
+        return KDQ_ERR_ALIAS;
+    const unsigned threads = unsigned(std::min<size_t>(kThreads, (cols + 511) / 512 * 64));
+    return by_types(type, dy_type, [&](auto t, auto u) {
+        using T = decltype(t);
+        using Y = decltype(u);
+        hipLaunchKernelGGL((combine_grad_kernel<T, Y>), dim3(unsigned(tokens)), dim3(threads), 0,
+                           static_cast<hipStream_t>(stream), static_cast<const T*>(rows),
+                           rows_stride, static_cast<const Y*>(dy), dy_stride, place, weights,
+                           unsigned(tokens), unsigned(top_k), unsigned(cols),
+                           static_cast<T*>(drows), drows_stride, dweights);
+        KDQ_HIP(hipGetLastError());
+        return int(KDQ_OK);
+    });
+}
+
+extern "C" int kdq_moe_route_backward(const int32_t* idx, const float* weights,
+                                      const float* dweights, size_t tokens, size_t experts,
+                                      size_t top_k, float* dlogits, void* stream) {
+    if (!idx || !weights || !dweights || !dlogits || !experts)
+        return KDQ_ERR_ARGUMENT;
+    KDQ_TRY(check_sizes(tokens, top_k, experts));
+    if (experts > 256 || top_k > experts)
+        return KDQ_ERR_SHAPE;
+    for (const void* p : {static_cast<const void*>(idx), static_cast<const void*>(weights),
+                          static_cast<const void*>(dweights), static_cast<const void*>(dlogits)})
+        KDQ_TRY(check_words(p));
+    const size_t bytes = tokens * top_k * 4;
+    const Range to[] = {{dlogits, tokens * experts * 4}},
+                from[] = {{idx, bytes}, {weights, bytes}, {dweights, bytes}};
+    if (any_overlap(to, from))
+        return KDQ_ERR_ALIAS;
+    hipLaunchKernelGGL(route_grad_kernel, dim3(unsigned((tokens + 3) / 4)), dim3(kThreads), 0,
+                       static_cast<hipStream_t>(stream), idx, weights, dweights, unsigned(tokens),
+                       unsigned(experts), unsigned(top_k), dlogits);
+    KDQ_HIP(hipGetLastError());
+    return KDQ_OK;
+}

@@ -659,6 +659,140 @@ def mxfp4_gated_backward(dh: torch.Tensor, saved, gate: torch.Tensor, up: torch.
     return out, dgu
 
 
+def _rows_of(t: torch.Tensor, name: str) -> tuple[int, int]:
+    """KDQ type of fp32, fp16 or bf16 rows, and the values from row to row."""
+    kind = _TYPES.get(t.dtype)
+    if kind is None:
+        raise ValueError(f"{name}: expected fp32, fp16 or bf16 rows")
+    return kind, _row_stride(t, t.dtype, name, 1)
+
+
+def _slots(t: torch.Tensor, slots: int, name: str, dtype=torch.int32) -> int:
+    """A contiguous tensor of a value per slot."""
+    _need(t, dtype, name)
+    if t.numel() != slots:
+        raise ValueError(f"{name}: expected {slots} values, one per selection")
+    return t.data_ptr()
+
+
+def moe_sort(x: torch.Tensor, perm: torch.Tensor, top_k: int):
+    """Tokens sorted by expert: x [tokens, cols] (fp32, fp16 or bf16) and moe_route's perm ->
+    rows [tokens * top_k, cols], rows[p] = x[perm[p] // top_k], and place int32
+    [tokens * top_k], place[perm[p]] = p (kdq_moe_sort).  Nothing is recorded for autograd: its
+    backward pass is moe_sort_backward."""
+    _no_graph(x, "x")
+    kind, stride = _rows_of(x, "x")
+    tokens, cols = x.shape
+    slots = tokens * top_k
+    order = _slots(perm, slots, "perm")
+    stream = _stream_for(x, perm)
+    rows = torch.empty(slots, cols, dtype=x.dtype, device=x.device)
+    place = torch.empty(slots, dtype=torch.int32, device=x.device)
+    call("kdq_moe_sort", kind, x.data_ptr(), stride, tokens, cols, top_k, order, rows.data_ptr(),
+         cols, place.data_ptr(), stream)
+    return rows, place
+
+
+def moe_sort_backward(drows: torch.Tensor, place: torch.Tensor, top_k: int) -> torch.Tensor:
+    """The gradient of moe_sort: drows [tokens * top_k, cols] -> dx [tokens, cols] of its type,
+    each token's rows summed (kdq_moe_sort_backward)."""
+    _no_graph(drows, "drows")
+    kind, stride = _rows_of(drows, "drows")
+    slots, cols = drows.shape
+    if top_k < 1 or slots % top_k:
+        raise ValueError("drows: expected top_k rows per token")
+    at = _slots(place, slots, "place")
+    stream = _stream_for(drows, place)
+    dx = torch.empty(slots // top_k, cols, dtype=drows.dtype, device=drows.device)
+    call("kdq_moe_sort_backward", kind, drows.data_ptr(), stride, at, slots // top_k, cols, top_k,
+         dx.data_ptr(), cols, stream)
+    return dx
+
+
+def _weights(weights: torch.Tensor, name: str) -> tuple[int, int]:
+    _need(weights, torch.float32, name)
+    if weights.dim() != 2:
+        raise ValueError(f"{name}: expected [tokens, top_k]")
+    return weights.shape
+
+
+def moe_combine(rows: torch.Tensor, weights: torch.Tensor, place: torch.Tensor,
+                residual: torch.Tensor | None = None, dtype: torch.dtype | None = None,
+                out: torch.Tensor | None = None) -> torch.Tensor:
+    """Experts' rows back to their tokens: y[t] = residual[t] + sum_i weights[t, i] *
+    rows[place[t * top_k + i]], rows [tokens * top_k, cols] (fp32, fp16 or bf16), weights fp32
+    [tokens, top_k], place from moe_sort -> y [tokens, cols] of the rows' type or fp32
+    (``dtype``; the residual's, and ``out`` may be the residual itself) (kdq_moe_combine).
+    Nothing is recorded for autograd: its backward pass is moe_combine_backward."""
+    for t, name in ((rows, "rows"), (weights, "weights"), (residual, "residual")):
+        if t is not None:
+            _no_graph(t, name)
+    kind, stride = _rows_of(rows, "rows")
+    tokens, top_k = _weights(weights, "weights")
+    slots, cols = rows.shape
+    if slots != tokens * top_k:
+        raise ValueError("rows: expected one per weight")
+    at = _slots(place, slots, "place")
+    if dtype is None:
+        dtype = rows.dtype
+    if dtype != rows.dtype and dtype != torch.float32:
+        raise ValueError("dtype: the rows' type or fp32")
+    parts, add, add_stride = [rows, weights, place], None, 0
+    if residual is not None:
+        add, add_stride = residual.data_ptr(), _output(residual, tokens, cols, dtype, "residual")
+        parts.append(residual)
+    if out is None:
+        stream, y_stride = _stream_for(*parts), cols
+        out = torch.empty(tokens, cols, dtype=dtype, device=rows.device)
+    else:
+        y_stride = _output(out, tokens, cols, dtype, "out")
+        stream = _stream_for(*parts, out)
+    call("kdq_moe_combine", kind, rows.data_ptr(), stride, at, weights.data_ptr(), tokens, cols,
+         top_k, _TYPES[dtype], add, add_stride, out.data_ptr(), y_stride, stream)
+    return out
+
+
+def moe_combine_backward(dy: torch.Tensor, rows: torch.Tensor, weights: torch.Tensor,
+                         place: torch.Tensor):
+    """The gradients of moe_combine: dy [tokens, cols] (the rows' type or fp32) and its rows,
+    weights and place -> drows [tokens * top_k, cols] of the rows' type and dweights fp32
+    [tokens, top_k] (kdq_moe_combine_backward).  The residual's gradient is dy."""
+    _no_graph(dy, "dy")
+    kind, stride = _rows_of(rows, "rows")
+    dy_kind, dy_stride = _rows_of(dy, "dy")
+    if dy_kind not in (kind, 0):
+        raise ValueError("dy: the rows' type or fp32")
+    tokens, top_k = _weights(weights, "weights")
+    slots, cols = rows.shape
+    if slots != tokens * top_k or dy.shape != (tokens, cols):
+        raise ValueError("expected rows [tokens * top_k, cols] and dy [tokens, cols]")
+    at = _slots(place, slots, "place")
+    stream = _stream_for(rows, weights, place, dy)
+    drows = torch.empty(slots, cols, dtype=rows.dtype, device=rows.device)
+    dweights = torch.empty(tokens, top_k, dtype=torch.float32, device=rows.device)
+    call("kdq_moe_combine_backward", kind, rows.data_ptr(), stride, at, weights.data_ptr(),
+         tokens, cols, top_k, dy_kind, dy.data_ptr(), dy_stride, drows.data_ptr(), cols,
+         dweights.data_ptr(), stream)
+    return drows, dweights
+
+
+def moe_route_backward(idx: torch.Tensor, weights: torch.Tensor, dweights: torch.Tensor,
+                       experts: int) -> torch.Tensor:
+    """The gradient of moe_route's weights: idx int32, weights and their gradient fp32, each
+    [tokens, top_k] -> dlogits fp32 [tokens, experts] (kdq_moe_route_backward)."""
+    _no_graph(dweights, "dweights")
+    tokens, top_k = _weights(weights, "weights")
+    _need(idx, torch.int32, "idx")
+    _need(dweights, torch.float32, "dweights")
+    if idx.shape != weights.shape or dweights.shape != weights.shape:
+        raise ValueError("idx, weights and dweights: expected one shape")
+    stream = _stream_for(idx, weights, dweights)
+    dlogits = torch.empty(tokens, experts, dtype=torch.float32, device=weights.device)
+    call("kdq_moe_route_backward", idx.data_ptr(), weights.data_ptr(), dweights.data_ptr(), tokens,
+         experts, top_k, dlogits.data_ptr(), stream)
+    return dlogits
+
+
 def hbm_read(buffer: torch.Tensor, sink: torch.Tensor, workgroups: int,
              threads: int = 256, store_all: bool = True, match: int = 0) -> None:
     """kdq_hbm_read: one streaming read of `buffer` (the HBM read ceiling's probe) over
@@ -676,5 +810,7 @@ __all__ = ["dequantize", "gemv", "gemv_batch", "quantize_q8", "gemm_q4_0", "gemm
            "moe_gguf", "moe_route",
            "mxfp4_quantize", "mxfp4_pack", "mxfp4_product", "mxfp4_product_quantized",
            "mxfp4_gated", "mxfp4_gated_backward",
+           "moe_sort", "moe_sort_backward", "moe_combine", "moe_combine_backward",
+           "moe_route_backward",
            "mxfp4_dequantize", "moe_mxfp4", "moe_mxfp4_pack", "moe_mxfp4_packed", "lib",
            "BLOCK_BYTES", "BLOCK_VALUES"]
