@@ -330,6 +330,26 @@ inline bool overlaps(const void* a, size_t an, const void* b, size_t bn) {
     return x <= y ? y - x < an : x - y < bn;
 }
 
+struct Range {
+    const void* p;
+    size_t bytes;
+};
+
+// Whether one of the ranges that a call writes (its workspace among them, as far as the caller
+// says it may) overlaps one that it reads, or another that it writes.
+template <size_t N, size_t M>
+bool any_overlap(const Range (&out)[N], const Range (&in)[M]) {
+    for (size_t i = 0; i < N; ++i) {
+        for (const Range& b : in)
+            if (overlaps(out[i].p, out[i].bytes, b.p, b.bytes))
+                return true;
+        for (size_t j = 0; j < i; ++j)
+            if (overlaps(out[i].p, out[i].bytes, out[j].p, out[j].bytes))
+                return true;
+    }
+    return false;
+}
+
 inline bool misaligned(const void* p, size_t alignment) {
     return reinterpret_cast<uintptr_t>(p) % alignment != 0;
 }

@@ -336,23 +336,6 @@ int check_words(const void* p) {
             return rc_;             \
     } while (0)
 
-struct Range {
-    const void* p;
-    size_t bytes;
-};
-
-template <size_t N, size_t M> bool any_overlap(const Range (&out)[N], const Range (&in)[M]) {
-    for (size_t i = 0; i < N; ++i) {
-        for (const Range& b : in)
-            if (overlaps(out[i].p, out[i].bytes, b.p, b.bytes))
-                return true;
-        for (size_t j = 0; j < i; ++j)
-            if (overlaps(out[i].p, out[i].bytes, out[j].p, out[j].bytes))
-                return true;
-    }
-    return false;
-}
-
 // f with a value of the C++ type of `type`, and (two types) one of the second: the first's or
 // fp32.
 template <class F> int by_type(int type, F&& f) {

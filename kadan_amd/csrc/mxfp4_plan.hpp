@@ -1,4 +1,4 @@
-// Which kernel of mxfp4_dense.hip a call runs, in which tile and how many K slices.  Plain host
+// Which kernel of mxfp4_kernels.hpp a call runs, in which tile and how many K slices.  Plain host
 // arithmetic over sizes and a number of compute units, so that tests can ask which variant a
 // size reaches.
 #pragma once
@@ -13,8 +13,8 @@ constexpr size_t ceil_div(size_t a, size_t b) {
 }
 
 // What gemm_kernel multiplies: bf16 or MXFP4 rows of x by the packed form, or bf16 gradients by
-// the transposed one.
-enum Operands { kBf16, kFp4, kTransposed };
+// the transposed one (kOneTransposed, for plans only: a single matrix, where kTransposed has two).
+enum Operands { kBf16, kFp4, kTransposed, kOneTransposed };
 
 constexpr unsigned kTileFloats = 2 * 16 * 64;  // a wavefront's two result tiles
 constexpr unsigned kStagedBytes = 32 * 1024;   // of x that decode_kernel passes through LDS
@@ -48,7 +48,7 @@ inline Cost cost_of(int ops, int tt) {
     if (ops == kFp4)
         return {2.0 + 0.75 * tt, 0.05 + 0.55 * tt, 0.1 + 1.35 * tt};
     const double fixed = 2.5 + 0.9 * tt;
-    return ops == kTransposed ? Cost{fixed, tt == 1 ? 0.5 : 0.4 + 0.3 * tt, 0.7 + 0.6 * tt}
+    return ops >= kTransposed ? Cost{fixed, tt == 1 ? 0.5 : 0.4 + 0.3 * tt, 0.7 + 0.6 * tt}
                               : Cost{fixed, 0.03 + 0.33 * tt, 0.05 + 0.66 * tt};
 }
 
@@ -82,7 +82,7 @@ inline Plan plan_gemm(size_t m, size_t wave_groups, size_t chunks, int ops, size
                                 (each > 1 ? 1.5 : 0.0)
                           : double(each) * (split ? alone : 0.93 * alone);
         if (p.slices > 1)  // (the backward pass's third launch, which is its caller's time too)
-            t += (ops == kTransposed ? 4.5 : 3.5) + double(partial_bytes(p, m)) / 2.5e6;
+            t += (ops >= kTransposed ? 4.5 : 3.5) + double(partial_bytes(p, m)) / 2.5e6;
         if (!best.slices || t < best.cost) {
             best = p;
             best.cost = t;
@@ -185,6 +185,58 @@ inline Plan plan_backward(size_t m, size_t n, size_t k, size_t cus) {
     Plan p = plan_gemm(m, ceil_div(k, 64), ceil_div(n, 64), kTransposed, cus);
     const double units = double(ceil_div(n, 128)) * double(ceil_div(k / 32, cus));
     p.decode = m <= 32 && 2.5 + 0.2 * units * (1.0 + double(m) / 14) < p.cost;
+    return p;
+}
+
+inline Plan plan_one_backward(size_t m, size_t n, size_t k, size_t cus) {
+    return plan_gemm(m, ceil_div(k, 64), ceil_div(n, 64), kOneTransposed, cus);
+}
+
+// The most tiles of `rows` rows that m rows of x, sorted by expert, may make: an expert's last one
+// may hold a single row.
+constexpr size_t most_tiles(size_t m, size_t experts, size_t rows) {
+    return (m + (rows - 1) * std::min(experts, m)) / rows;
+}
+
+// How the experts' products run: decode_kernel over tiles of 16 rows, or gemm_kernel over tiles of
+// tt * 32, `most` tiles at most (the device alone knows how many).
+struct ExpertsPlan {
+    bool decode;
+    DecodeShape shape;
+    int tt;
+    size_t tiles_n, most;
+};
+
+inline ExpertsPlan plan_experts(size_t m, size_t experts, size_t n, size_t k, bool gated,
+                                bool kept, size_t cus) {
+    ExpertsPlan p{};
+    const size_t reached = std::min(experts, m), mean = m / reached;
+    p.decode = !kept && mean <= 8;
+    if (p.decode) {
+        const size_t units = ceil_div(k, 128);
+        DecodeShape& s = p.shape;
+        s.wide = ceil_div(n, 32) * reached >= cus;
+        s.tb = 1;
+        s.waves = units <= 8 ? 2 : units <= 16 ? 4 : 8;
+        s.units = unsigned(ceil_div(ceil_div(units, s.waves), 2) * 2);
+        s.staged = m <= 16 && m * staged_pitch(unsigned(k * 2)) <= kStagedBytes &&
+                   m * k * 2 <= s.waves * 64 * 16 * 8;
+        p.most = most_tiles(m, experts, 16);
+        return p;
+    }
+    p.tt = mean <= 32 ? 1 : mean <= 64 ? 2 : mean <= 96 ? 3 : 4;
+    p.tiles_n = ceil_div(n, gated ? 128 : 256);
+    p.most = most_tiles(m, experts, size_t(p.tt) * 32);
+    return p;
+}
+
+inline ExpertsPlan plan_experts_backward(size_t m, size_t experts, size_t k, size_t cus) {
+    ExpertsPlan p{};
+    const size_t mean = m / std::min(experts, m);
+    (void)cus;
+    p.tt = mean <= 32 ? 1 : mean <= 64 ? 2 : mean <= 96 ? 3 : 4;
+    p.tiles_n = ceil_div(k, 256);
+    p.most = most_tiles(m, experts, size_t(p.tt) * 32);
     return p;
 }
 

@@ -453,6 +453,8 @@ def _mxfp4_sizes(*sizes):
 
 
 _PACKED, _TRANSPOSED = "kdq_mxfp4_packed_bytes", "kdq_mxfp4_packed_transposed_bytes"
+_EXPERTS = "kdq_mxfp4_experts_packed_bytes"
+_EXPERTS_TRANSPOSED = "kdq_mxfp4_experts_packed_transposed_bytes"
 
 
 # The two packed forms of a matrix may take the same number of bytes (14336 x 4096 does), so
@@ -464,7 +466,8 @@ def _matrix(packed: torch.Tensor, size: int, name: str, dims: int = 1) -> int:
         raise ValueError(f"{name}: not the packed size of this call's matrix")
     if packed.dim() != dims:
         raise ValueError(f"{name}: expected mxfp4_pack's flat form" if dims == 1 else
-                         f"{name}: expected the form of mxfp4_pack(..., transposed=True)")
+                         f"{name}: expected the form of mxfp4_pack(..., transposed=True)" +
+                         (" of a stack" if dims == 3 else ""))
     return packed.data_ptr()
 
 
@@ -518,9 +521,14 @@ def mxfp4_quantize(x: torch.Tensor, status: torch.Tensor | None = None):
 def mxfp4_pack(blocks: torch.Tensor, scales: torch.Tensor,
                transposed: bool = False) -> torch.Tensor:
     """An MXFP4 matrix in the form the products read, uint8 [bytes] (kdq_mxfp4_pack), or,
-    ``transposed``, in the one that mxfp4_gated_backward reads, uint8 [ceil(cols / 64), bytes of
+    ``transposed``, in the one that the backward passes read, uint8 [ceil(cols / 64), bytes of
     64 columns] (kdq_mxfp4_pack_transposed).  The shape is what tells the two forms apart; of
-    matrices of other sizes the calls see the number of bytes alone."""
+    matrices of other sizes the calls see the number of bytes alone.  A stack of experts' matrices
+    (blocks and scales with a first dimension of experts) gives the experts' forms: uint8 [bytes],
+    which for rows of whole 32s and cols of whole 64s is moe_mxfp4_pack's, and uint8 [experts,
+    ceil(cols / 64), bytes] (kdq_mxfp4_experts_pack, kdq_mxfp4_experts_pack_transposed)."""
+    if blocks.dim() == 3:
+        return _pack_experts(blocks, scales, transposed)
     rows, cols = _blocks(blocks, scales)
     stream = _stream_for(blocks, scales)
     size = _mxfp4_size(_TRANSPOSED if transposed else _PACKED, rows, cols)
@@ -531,6 +539,25 @@ def mxfp4_pack(blocks: torch.Tensor, scales: torch.Tensor,
                          device=blocks.device)
     call("kdq_mxfp4_pack_transposed" if transposed else "kdq_mxfp4_pack", blocks.data_ptr(),
          scales.data_ptr(), rows, cols, packed.data_ptr(), stream)
+    return packed
+
+
+def _pack_experts(blocks: torch.Tensor, scales: torch.Tensor, transposed: bool) -> torch.Tensor:
+    _need(blocks, torch.uint8, "blocks")
+    _need(scales, torch.uint8, "scales")
+    experts, rows, width = blocks.shape
+    if scales.shape != (experts, rows, width // 16) or width % 16:
+        raise ValueError("expected blocks [experts, rows, cols/2], scales [experts, rows, cols/32]")
+    cols = 2 * width
+    stream = _stream_for(blocks, scales)
+    size = _mxfp4_size(_EXPERTS_TRANSPOSED if transposed else _EXPERTS, experts, rows, cols)
+    if not size:
+        raise ValueError(f"{experts} matrices of {rows} x {cols} have no packed form")
+    groups = (cols + 63) // 64
+    packed = torch.empty((experts, groups, size // (experts * groups)) if transposed else size,
+                         dtype=torch.uint8, device=blocks.device)
+    call("kdq_mxfp4_experts_pack_transposed" if transposed else "kdq_mxfp4_experts_pack",
+         blocks.data_ptr(), scales.data_ptr(), experts, rows, cols, packed.data_ptr(), stream)
     return packed
 
 
@@ -631,20 +658,7 @@ def mxfp4_gated_backward(dh: torch.Tensor, saved, gate: torch.Tensor, up: torch.
                                  n, n_in)
     wg = _transposed_matrix(gate, weights, n_in, "gate")
     wu = _transposed_matrix(up, weights, n_in, "up")
-    kept = codes = scales = None
-    if isinstance(saved, torch.Tensor):
-        _need(saved, _BF16, "saved")
-        parts = (saved,)
-        kept = saved.data_ptr()
-    else:
-        parts = q, d = saved
-        _need(q, torch.int8, "saved codes")
-        _need(d, torch.float32, "saved scales")
-        if d.shape != (m, n // 16):
-            raise ValueError("saved: scales of another shape")
-        codes, scales = q.data_ptr(), d.data_ptr()
-    if parts[0].shape != (m, 2 * n):
-        raise ValueError("saved: of another shape than dh")
+    parts, (kept, codes, scales) = _saved_gates(saved, m, n)
     device = dh.device
     if out is None:
         stream, dx_stride = _stream_for(dh, gate, up, *parts), n_in
@@ -656,6 +670,241 @@ def mxfp4_gated_backward(dh: torch.Tensor, saved, gate: torch.Tensor, up: torch.
     scratch = _scratch(size, device)
     call("kdq_mxfp4_gated_backward", dh.data_ptr(), stride, m, kept, codes, scales, wg, wu, n,
          n_in, dgu.data_ptr(), out.data_ptr(), dx_stride, _ptr(scratch), size, stream)
+    return out, dgu
+
+
+_ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2}  # KDQ_ACT_NONE, _SILU, _GELU
+_GATES = {"silu": 1, "clamped": 3}              # KDQ_ACT_SILU, _CLAMPED
+
+
+def _activation(kinds: dict, activation) -> int:
+    if activation not in kinds:
+        raise ValueError(f"activation: one of {', '.join(map(repr, kinds))}")
+    return kinds[activation]
+
+
+def _offsets(offsets: torch.Tensor) -> int:
+    """The number of experts."""
+    _need(offsets, torch.int32, "offsets")
+    experts = offsets.numel() - 1
+    if offsets.dim() != 1 or not 1 <= experts <= 256:
+        raise ValueError("offsets: expected 1 to 256 experts' offsets and the end of the last")
+    return experts
+
+
+def _bias(bias: torch.Tensor | None, name: str, *shape: int) -> int | None:
+    if bias is None:
+        return None
+    _no_graph(bias, name)
+    _need(bias, torch.float32, name)
+    if bias.shape != shape:
+        raise ValueError(f"{name}: expected {list(shape)}")
+    return bias.data_ptr()
+
+
+def _stack(packed: torch.Tensor, function: str, experts: int, rows: int, cols: int,
+           name: str) -> int:
+    """A stack's packed form."""
+    size = _mxfp4_size(function, experts, rows, cols)
+    if function == _EXPERTS:
+        return _matrix(packed, size, name)
+    at = _matrix(packed, size, name, 3)
+    if packed.shape[:2] != (experts, (cols + 63) // 64):
+        raise ValueError(f"{name}: another stack's packed form")
+    return at
+
+
+def mxfp4_linear(x: torch.Tensor, packed: torch.Tensor, n_out: int,
+                 bias: torch.Tensor | None = None, activation: str | None = None,
+                 residual: torch.Tensor | None = None, dtype: torch.dtype = torch.float32,
+                 offsets: torch.Tensor | None = None, save: bool = False,
+                 out: torch.Tensor | None = None):
+    """y = residual + act(x W^T + bias): bf16 [m, k] and a packed MXFP4 matrix (mxfp4_pack) of
+    n_out rows -> fp32 or bf16 [m, n_out], with a bias fp32 [n_out], an activation (None, "silu"
+    or "gelu", the tanh form) and a residual of y's type, each or none of them (``out`` may be the
+    residual itself).  With ``offsets`` int32 [experts + 1] (moe_route's) the rows are sorted by
+    expert (moe_sort) and each is multiplied by its own expert's matrix of a packed stack, with
+    its bias of [experts, n_out]; rows that no expert has are left as they are in ``out``.  With
+    ``save`` the pre-activations are kept for mxfp4_linear_backward, bf16 [m, n_out], and
+    (y, saved) returned.  Nothing is recorded for autograd (kdq_mxfp4_linear)."""
+    _no_graph(x, "x")
+    stride = _row_stride(x, _BF16, "x")
+    kind, act = _type(dtype), _activation(_ACTIVATIONS, activation)
+    if save and not act:
+        raise ValueError("save: without an activation there is nothing to keep")
+    m, k = x.shape
+    parts, size = [x, packed], 0
+    if offsets is None:
+        experts, table = 1, None
+        weights, size = _mxfp4_sizes(_PACKED, n_out, k, "kdq_mxfp4_linear_workspace", m, n_out, k)
+        w = _matrix(packed, weights, "packed")
+        b = _bias(bias, "bias", n_out)
+    else:
+        experts, table = _offsets(offsets), offsets.data_ptr()
+        w = _stack(packed, _EXPERTS, experts, n_out, k, "packed")
+        b = _bias(bias, "bias", experts, n_out)
+        parts.append(offsets)
+    if bias is not None:
+        parts.append(bias)
+    add, add_stride = None, 0
+    if residual is not None:
+        _no_graph(residual, "residual")
+        add, add_stride = residual.data_ptr(), _output(residual, m, n_out, dtype, "residual")
+        parts.append(residual)
+    device = x.device
+    if out is None:
+        stream, y_stride = _stream_for(*parts), n_out
+        out = torch.empty(m, n_out, dtype=dtype, device=device)
+    else:
+        y_stride = _output(out, m, n_out, dtype, "out")
+        stream = _stream_for(*parts, out)
+    saved = torch.empty(m, n_out, dtype=_BF16, device=device) if save else None
+    scratch = _scratch(size, device)
+    call("kdq_mxfp4_linear", x.data_ptr(), stride, m, table, experts, w, n_out, k, b, act, add,
+         add_stride, kind, out.data_ptr(), y_stride, _ptr(saved), _ptr(scratch), size, stream)
+    return (out, saved) if save else out
+
+
+def mxfp4_linear_backward(dy: torch.Tensor, packed: torch.Tensor, n_in: int,
+                          saved: torch.Tensor | None = None, activation: str | None = None,
+                          offsets: torch.Tensor | None = None, out: torch.Tensor | None = None):
+    """The backward pass of mxfp4_linear over frozen weights: dy bf16 [m, n_out]
+    (n_out % 8 == 0), with an activation what its forward pass saved, and the matrix or stack from
+    mxfp4_pack(..., transposed=True) -> dx bf16 [m, n_in] and dpre bf16 [m, n_out], the gradient
+    before the activation (dy itself without one; the bias's gradient is the sum of its rows)
+    (kdq_mxfp4_linear_backward)."""
+    _no_graph(dy, "dy")
+    stride = _row_stride(dy, _BF16, "dy")
+    act = _activation(_ACTIVATIONS, activation)
+    m, n = dy.shape
+    if n % 8 or n_in % 32 or not n_in:
+        raise ValueError("n_out must be a multiple of 8, n_in of 32")
+    if (saved is None) == bool(act):
+        raise ValueError("saved: expected with an activation, and only with one")
+    parts, size = [dy, packed], 0
+    if offsets is None:
+        experts, table = 1, None
+        weights, size = _mxfp4_sizes(_TRANSPOSED, n, n_in, "kdq_mxfp4_linear_backward_workspace",
+                                     m, n, n_in)
+        w = _transposed_matrix(packed, weights, n_in, "packed")
+    else:
+        experts, table = _offsets(offsets), offsets.data_ptr()
+        w = _stack(packed, _EXPERTS_TRANSPOSED, experts, n, n_in, "packed")
+        parts.append(offsets)
+    device = dy.device
+    dpre = dy
+    if act:
+        _need(saved, _BF16, "saved")
+        if saved.shape != (m, n):
+            raise ValueError("saved: of another shape than dy")
+        parts.append(saved)
+        dpre = torch.empty(m, n, dtype=_BF16, device=device)
+    if out is None:
+        stream, dx_stride = _stream_for(*parts), n_in
+        out = torch.empty(m, n_in, dtype=_BF16, device=device)
+    else:
+        dx_stride = _output(out, m, n_in, _BF16, "out")
+        stream = _stream_for(*parts, out)
+    scratch = _scratch(size, device)
+    call("kdq_mxfp4_linear_backward", dy.data_ptr(), stride, m, table, experts, _ptr(saved), act,
+         w, n, n_in, dpre.data_ptr() if act else None, out.data_ptr(), dx_stride, _ptr(scratch),
+         size, stream)
+    return out, dpre
+
+
+def mxfp4_experts_gated(x: torch.Tensor, offsets: torch.Tensor, gate: torch.Tensor,
+                        up: torch.Tensor, n_out: int, gate_bias: torch.Tensor | None = None,
+                        up_bias: torch.Tensor | None = None, activation: str = "silu",
+                        save: str | None = None, out: torch.Tensor | None = None):
+    """mxfp4_gated of a mixture's experts: bf16 [m, k] rows sorted by expert (moe_sort), offsets
+    int32 [experts + 1] (moe_route's) and two packed stacks (mxfp4_pack) of n_out rows
+    (n_out % 32 == 0), with biases fp32 [experts, n_out] or none -> h bf16 [m, n_out]:
+    silu(g) * u, or, "clamped", with g' = min(g, 7) and u' = u between -7 and 7,
+    g' sigmoid(1.702 g') (u' + 1).  Rows that no expert has are left as they are in ``out``.
+    ``save`` as for mxfp4_gated.  Nothing is recorded for autograd (kdq_mxfp4_experts_gated)."""
+    _no_graph(x, "x")
+    stride = _row_stride(x, _BF16, "x")
+    act = _activation(_GATES, activation)
+    if save not in (None, "bf16", "q8"):
+        raise ValueError('save: None, "bf16" or "q8"')
+    if n_out % 32:
+        raise ValueError("n_out must be a multiple of 32")
+    if (gate_bias is None) != (up_bias is None):
+        raise ValueError("expected both biases or none")
+    m, k = x.shape
+    experts = _offsets(offsets)
+    wg = _stack(gate, _EXPERTS, experts, n_out, k, "gate")
+    wu = _stack(up, _EXPERTS, experts, n_out, k, "up")
+    bg = _bias(gate_bias, "gate_bias", experts, n_out)
+    bu = _bias(up_bias, "up_bias", experts, n_out)
+    parts = [x, offsets, gate, up]
+    if bg is not None:
+        parts += [gate_bias, up_bias]
+    device = x.device
+    if out is None:
+        stream, h_stride = _stream_for(*parts), n_out
+        out = torch.empty(m, n_out, dtype=_BF16, device=device)
+    else:
+        h_stride = _output(out, m, n_out, _BF16, "out")
+        stream = _stream_for(*parts, out)
+    saved = kept = codes = scales = None
+    if save == "bf16":
+        saved = torch.empty(m, 2 * n_out, dtype=_BF16, device=device)
+        kept = saved.data_ptr()
+    elif save == "q8":
+        saved = (torch.empty(m, 2 * n_out, dtype=torch.int8, device=device),
+                 torch.empty(m, n_out // 16, dtype=torch.float32, device=device))
+        codes, scales = saved[0].data_ptr(), saved[1].data_ptr()
+    call("kdq_mxfp4_experts_gated", x.data_ptr(), stride, m, offsets.data_ptr(), experts, wg, wu,
+         n_out, k, bg, bu, act, out.data_ptr(), h_stride, kept, codes, scales, stream)
+    return out if save is None else (out, saved)
+
+
+def _saved_gates(saved, m: int, n: int):
+    """Kept pre-activations: the tensors, and the pointers to bf16 values, codes and scales."""
+    if isinstance(saved, torch.Tensor):
+        _need(saved, _BF16, "saved")
+        parts, at = (saved,), (saved.data_ptr(), None, None)
+    else:
+        parts = q, d = saved
+        _need(q, torch.int8, "saved codes")
+        _need(d, torch.float32, "saved scales")
+        if d.shape != (m, n // 16):
+            raise ValueError("saved: scales of another shape")
+        at = (None, q.data_ptr(), d.data_ptr())
+    if parts[0].shape != (m, 2 * n):
+        raise ValueError("saved: of another shape than dh")
+    return parts, at
+
+
+def mxfp4_experts_gated_backward(dh: torch.Tensor, offsets: torch.Tensor, saved,
+                                 gate: torch.Tensor, up: torch.Tensor, n_in: int,
+                                 activation: str = "silu", out: torch.Tensor | None = None):
+    """The backward pass of mxfp4_experts_gated over frozen weights: dh bf16 [m, n_out], its
+    offsets, ``saved`` from its forward pass, the stacks from mxfp4_pack(..., transposed=True)
+    -> dx bf16 [m, n_in] and the pre-activations' gradients bf16 [m, 2 n_out], gates then ups
+    (kdq_mxfp4_experts_gated_backward)."""
+    _no_graph(dh, "dh")
+    stride = _row_stride(dh, _BF16, "dh")
+    act = _activation(_GATES, activation)
+    m, n = dh.shape
+    if n % 32 or n_in % 32 or not n_in:
+        raise ValueError("n_out and n_in must be multiples of 32")
+    experts = _offsets(offsets)
+    wg = _stack(gate, _EXPERTS_TRANSPOSED, experts, n, n_in, "gate")
+    wu = _stack(up, _EXPERTS_TRANSPOSED, experts, n, n_in, "up")
+    parts, (kept, codes, scales) = _saved_gates(saved, m, n)
+    device = dh.device
+    if out is None:
+        stream, dx_stride = _stream_for(dh, offsets, gate, up, *parts), n_in
+        out = torch.empty(m, n_in, dtype=_BF16, device=device)
+    else:
+        dx_stride = _output(out, m, n_in, _BF16, "out")
+        stream = _stream_for(dh, offsets, gate, up, out, *parts)
+    dgu = torch.empty(m, 2 * n, dtype=_BF16, device=device)
+    call("kdq_mxfp4_experts_gated_backward", dh.data_ptr(), stride, m, offsets.data_ptr(),
+         experts, kept, codes, scales, act, wg, wu, n, n_in, dgu.data_ptr(), out.data_ptr(),
+         dx_stride, stream)
     return out, dgu
 
 
@@ -811,6 +1060,7 @@ __all__ = ["dequantize", "gemv", "gemv_batch", "quantize_q8", "gemm_q4_0", "gemm
            "mxfp4_quantize", "mxfp4_pack", "mxfp4_product", "mxfp4_product_quantized",
            "mxfp4_gated", "mxfp4_gated_backward",
            "moe_sort", "moe_sort_backward", "moe_combine", "moe_combine_backward",
-           "moe_route_backward",
+           "moe_route_backward", "mxfp4_linear", "mxfp4_linear_backward", "mxfp4_experts_gated",
+           "mxfp4_experts_gated_backward",
            "mxfp4_dequantize", "moe_mxfp4", "moe_mxfp4_pack", "moe_mxfp4_packed", "lib",
            "BLOCK_BYTES", "BLOCK_VALUES"]
