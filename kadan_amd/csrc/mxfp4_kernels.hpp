@@ -430,38 +430,11 @@ __device__ __forceinline__ void store_f32(float* p, unsigned c, unsigned n, cons
     }
 }
 
-// N sums of a row from column c on, to y; kept: the pre-activations as bf16 [m][n].
-template <int N>
-__device__ __forceinline__ void finish(const Target& t, unsigned row, unsigned c, float (&v)[N],
-                                       const float (&bias)[N]) {
-    if (row >= t.m || c >= t.n)
-        return;
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-        v[i] += bias[i];
-    if (t.kept)
-        store_bf16(t.kept + size_t(row) * t.n, c, t.n, v);
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-        v[i] = act_value(v[i], t.e.act);
-    if (t.e.residual) {
-        float r[N];
-        if (t.e.f32)
-            load_f32(static_cast<const float*>(t.e.residual) + size_t(row) * t.e.residual_stride,
-                     c, t.n, r);
-        else
-            load_bf16(static_cast<const uint16_t*>(t.e.residual) +
-                          size_t(row) * t.e.residual_stride,
-                      c, t.n, r);
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            v[i] += r[i];
-    }
-    if (t.e.f32)
-        store_f32(static_cast<float*>(t.y) + size_t(row) * t.stride, c, t.n, v);
-    else
-        store_bf16(static_cast<uint16_t*>(t.y) + size_t(row) * t.stride, c, t.n, v);
-}
+// What an epilogue adds to N values of a row from column c on.  It is asked for ahead of the sums
+// it is added to, so that its way from memory is not waited for behind theirs.
+template <int N> struct Added {
+    float bias[N], residual[N];
+};
 
 template <int N>
 __device__ __forceinline__ void bias_of(const float* bias, unsigned c, unsigned n,
@@ -474,10 +447,52 @@ __device__ __forceinline__ void bias_of(const float* bias, unsigned c, unsigned 
             b[i] = 0.f;
 }
 
-__device__ __forceinline__ void finish4(const Target& t, unsigned row, unsigned c, f32x4 v) {
-    float f[4] = {v.x, v.y, v.z, v.w}, b[4];
-    bias_of(t.e.bias, c, t.n, b);
-    finish(t, row, c, f, b);
+template <int N>
+__device__ __forceinline__ void residual_of(const Target& t, unsigned row, unsigned c,
+                                            float (&r)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        r[i] = 0.f;
+    if (!t.e.residual || row >= t.m)
+        return;
+    const size_t at = size_t(row) * t.e.residual_stride;
+    if (t.e.f32)
+        load_f32(static_cast<const float*>(t.e.residual) + at, c, t.n, r);
+    else
+        load_bf16(static_cast<const uint16_t*>(t.e.residual) + at, c, t.n, r);
+}
+
+// N sums of a row from column c on, to y; kept: the pre-activations as bf16 [m][n].
+template <int N>
+__device__ __forceinline__ void finish(const Target& t, unsigned row, unsigned c, float (&v)[N],
+                                       const float (&bias)[N], const float (&residual)[N]) {
+    if (row >= t.m || c >= t.n)
+        return;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        v[i] += bias[i];
+    if (t.kept)
+        store_bf16(t.kept + size_t(row) * t.n, c, t.n, v);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        v[i] = act_value(v[i], t.e.act) + residual[i];
+    if (t.e.f32)
+        store_f32(static_cast<float*>(t.y) + size_t(row) * t.stride, c, t.n, v);
+    else
+        store_bf16(static_cast<uint16_t*>(t.y) + size_t(row) * t.stride, c, t.n, v);
+}
+
+__device__ __forceinline__ Added<4> added4(const Target& t, unsigned row, unsigned c) {
+    Added<4> a;
+    bias_of(t.e.bias, c, t.n, a.bias);
+    residual_of(t, row, c, a.residual);
+    return a;
+}
+
+__device__ __forceinline__ void finish4(const Target& t, unsigned row, unsigned c, f32x4 v,
+                                        const Added<4>& a) {
+    float f[4] = {v.x, v.y, v.z, v.w};
+    finish(t, row, c, f, a.bias, a.residual);
 }
 
 // Quad j of a wavefront's two 32 x 32 result tiles (group G, row `token` of x, lane half
@@ -495,9 +510,6 @@ __device__ __forceinline__ void store_quad(const Target& t, unsigned G, unsigned
     } else if constexpr (OUT == kOutBf16) {
         store4_bf16(static_cast<uint16_t*>(t.y), t.stride, t.n, token, 64 * G + r, v0);
         store4_bf16(static_cast<uint16_t*>(t.y), t.stride, t.n, token, 64 * G + 32 + r, v1);
-    } else if constexpr (of_linear(OUT)) {
-        finish4(t, token, 64 * G + r, v0);
-        finish4(t, token, 64 * G + 32 + r, v1);
     } else if constexpr (OUT == kOutGated) {
         const unsigned c = 32 * G + r;
         const f32x4 hv{gate_value(v0.x, v1.x), gate_value(v0.y, v1.y), gate_value(v0.z, v1.z),
@@ -634,6 +646,12 @@ __device__ __forceinline__ unsigned wide_at(unsigned row, unsigned piece) {
 __device__ __forceinline__ void store_linear(const Target& t, unsigned G, unsigned T,
                                              uint8_t* patch, const f32x16& a0, const f32x16& a1) {
     const unsigned lane = threadIdx.x % 64, h = lane / 32;
+    const unsigned eighth = lane % 8, c = 64 * G + 8 * eighth;
+    float bias[8], residual[4][8];
+    bias_of(t.e.bias, c, t.n, bias);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        residual_of(t, T * 32 + 8 * i + lane / 8, c, residual[i]);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -642,16 +660,13 @@ __device__ __forceinline__ void store_linear(const Target& t, unsigned G, unsign
                 quad_of(i ? a1 : a0, j);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-    const unsigned eighth = lane % 8, c = 64 * G + 8 * eighth;
-    float bias[8];
-    bias_of(t.e.bias, c, t.n, bias);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const unsigned row = 8 * i + lane / 8;
         const f32x4 lo = *reinterpret_cast<const f32x4*>(patch + wide_at(row, 2 * eighth));
         const f32x4 hi = *reinterpret_cast<const f32x4*>(patch + wide_at(row, 2 * eighth + 1));
         float v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-        finish(t, T * 32 + row, c, v, bias);
+        finish(t, T * 32 + row, c, v, bias, residual[i]);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -1118,7 +1133,7 @@ __global__ __launch_bounds__(1024) void decode_kernel(Decode a) {
                       gate_value(v.w, u.w)};
         }
         if constexpr (of_linear(OUT))
-            finish4(a.out, token, at, v);
+            finish4(a.out, token, at, v, added4(a.out, token, at));
         else if constexpr (OUT == kOutF32)
             store4_f32(static_cast<float*>(a.out.y), a.out.stride, a.out.n, token, at, v);
         else
@@ -1351,6 +1366,10 @@ __global__ __launch_bounds__(512, (shares_unit<TT, OPS> ? 4 : 2)) void gemm_kern
     const unsigned G = tile_n * 4 + rg;  // the wavefront's pair of tiles
 
     // this wavefront group's part of K, in chunks
+    // (the experts' products with an epilogue take parts of whole half turns, two chunks: K of 768
+    // is 6 + 6 chunks in place of 8 + 4, 4096 rows over 128 experts of 768 -> 2048 160 -> 145 us;
+    // the others' longer turns gain less than the branch costs them, 3 to 15 %)
+    constexpr bool kHalfTurns = OUT == kOutExpertsLinear;
     constexpr bool kTwoParts = SPLIT && (OPS != kTransposed || of_one_backward(OUT));
     const auto part_of = [&](unsigned set) {
         return kTwoParts ? blockIdx.y * 2 + set : blockIdx.y;
@@ -1520,6 +1539,9 @@ __global__ __launch_bounds__(512, (shares_unit<TT, OPS> ? 4 : 2)) void gemm_kern
     constexpr int kBuffers = shares_unit<TT, OPS> ? 1 : 2;
     Codes codes[kAhead];
     Scales scales, next;
+    // (parts that are no whole turns may begin within a dword's four steps: two dwords give one)
+    const unsigned shift = kHalfTurns ? begin_step % 4 : 0, scale_step = begin_step - shift;
+    Scales after, shifted;
     // the x operands of a chunk's step S, and (bf16) the chunk's weights of it
     auto read_x = [&]<int S>(const uint8_t* buf, u4 (&v)[TT]) {
 #pragma unroll
@@ -1536,7 +1558,8 @@ __global__ __launch_bounds__(512, (shares_unit<TT, OPS> ? 4 : 2)) void gemm_kern
         } else {
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-                v[i] = decode8(codes[C % kAhead].w[i][S], scale_of(scales.w[i], C));
+                v[i] = decode8(codes[C % kAhead].w[i][S],
+                               scale_of(kHalfTurns ? shifted.w[i] : scales.w[i], C));
         }
     };
     issue_order();
@@ -1545,7 +1568,9 @@ __global__ __launch_bounds__(512, (shares_unit<TT, OPS> ? 4 : 2)) void gemm_kern
     stage(0, 0);
     stage(1, 1);
     stage(2, 2);
-    load_scales(begin_step, scales);
+    load_scales(scale_step, scales);
+    if constexpr (kHalfTurns)
+        load_scales(scale_step + 4, after);
 #pragma unroll
     for (int i = 0; i < kAhead; ++i)
         load_codes(begin_step + i, codes[i]);
@@ -1621,11 +1646,18 @@ __global__ __launch_bounds__(512, (shares_unit<TT, OPS> ? 4 : 2)) void gemm_kern
             asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kBehindFirst) : "memory");
         for (unsigned c0 = 0; c0 < a.part; c0 += 4) {
             static_for<4>([&]<int C>() {
+                if constexpr (kHalfTurns && C >= 2)
+                    if (c0 + 2 >= a.part) [[unlikely]]
+                        return;
                 arrive.template operator()<kBehind + (C == 0 ? 0 : kScaleLoads)>();
                 const uint8_t* buf = x_lane + C * kStageBytes;
                 stage(c0 + C + 3, (C + 3) % kStages);
                 if constexpr (C == 0)
-                    load_scales(begin_step + c0 + 4, next);
+                    load_scales(scale_step + c0 + (kHalfTurns ? 8 : 4), next);
+                if constexpr (C == 0 && kHalfTurns)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        shifted.w[i] = __builtin_amdgcn_alignbyte(after.w[i], scales.w[i], shift);
                 u4 xv[kBuffers][TT];
                 bf16x8 wv[kBuffers][2];
                 if constexpr (kBuffers == 2) {
@@ -1653,7 +1685,8 @@ __global__ __launch_bounds__(512, (shares_unit<TT, OPS> ? 4 : 2)) void gemm_kern
                 issue_order();
                 load_codes(begin_step + c0 + C + kAhead, codes[C % kAhead]);
             });
-            scales = next;
+            scales = kHalfTurns ? after : next;
+            after = next;
         }
     }
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // no copy outlives the loop
@@ -1781,6 +1814,12 @@ __global__ __launch_bounds__(256) void reduce_kernel(const float* __restrict__ p
     const size_t step = pairs * (kTileFloats / 4);
     constexpr int kQuads = WHOLE ? 4 : 1;
     const unsigned j0 = WHOLE ? 0 : unsigned(w % 4);
+    const unsigned token = T * 32 + lane % 32, h = lane / 32;
+    Added<4> added[2];
+    if constexpr (of_linear(OUT))
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            added[i] = added4(out, token, 64 * G + 32 * i + 8 * j0 + 4 * h);
     f32x4 v[2][kQuads];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
@@ -1794,10 +1833,15 @@ __global__ __launch_bounds__(256) void reduce_kernel(const float* __restrict__ p
 #pragma unroll
             for (int j = 0; j < kQuads; ++j)
                 v[i][j] += from[s * step + (i * 4 + j0 + j) * 64];
-    const unsigned token = T * 32 + lane % 32, h = lane / 32;
+    if constexpr (of_linear(OUT)) {
 #pragma unroll
-    for (int j = 0; j < kQuads; ++j)
-        store_quad<OUT>(out, G, token, h, j0 + j, v[0][j], v[1][j]);
+        for (int i = 0; i < 2; ++i)
+            finish4(out, token, 64 * G + 32 * i + 8 * j0 + 4 * h, v[i][0], added[i]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < kQuads; ++j)
+            store_quad<OUT>(out, G, token, h, j0 + j, v[0][j], v[1][j]);
+    }
     if constexpr (WHOLE) {
         if (32 * G < out.n) {
             keep_q8(out, 32 * G, token, h, v[0]);
@@ -1924,6 +1968,14 @@ int launch_gemm(const Gemm& a, const Plan& p, hipStream_t st) {
     return KDQ_OK;
 }
 
+template <int OPS, int OUT> int launch_tall(const Gemm& a, const Plan& p, hipStream_t st) {
+    if constexpr (of_experts(OUT))  // (no plan of theirs has such tiles)
+        return KDQ_ERR_UNSUPPORTED;
+    else
+        return p.tt == 3 ? launch_gemm<3, true, OPS, OUT>(a, p, st)
+                         : launch_gemm<4, true, OPS, OUT>(a, p, st);
+}
+
 template <int OUT> int run_reduce(const Gemm& a, const Plan& p, hipStream_t st) {
     const unsigned row_tiles = unsigned(ceil_div(a.out.m, 32));
     const size_t pairs = size_t(p.tiles_n) * 4 * row_tiles;
@@ -1957,8 +2009,7 @@ template <int OPS, int OUT> int run_gemm(Gemm a, const Plan& p, void* workspace,
     } else {
         rc = p.tt == 1   ? launch_gemm<1, true, OPS, OUT>(a, p, st)
              : p.tt == 2 ? launch_gemm<2, true, OPS, OUT>(a, p, st)
-             : p.tt == 3 ? launch_gemm<3, true, OPS, OUT>(a, p, st)
-                         : launch_gemm<4, true, OPS, OUT>(a, p, st);
+                         : launch_tall<OPS, OUT>(a, p, st);
     }
     if constexpr (!of_experts(OUT)) {  // (theirs have no slices)
         if (!rc && p.slices > 1)
@@ -1984,14 +2035,14 @@ int launch_decode(Decode a, unsigned waves, hipStream_t st) {
     return KDQ_OK;
 }
 
+// (x is read by every wavefront: through LDS a token's projections took as long)
 template <bool GATED, int OUT>
 int run_experts_decode(Decode a, const DecodeShape& s, hipStream_t st) {
     a.units = s.units;
-    if (s.staged)
-        return s.wide ? launch_decode<2, 1, GATED, false, true, OUT>(a, s.waves, st)
-                      : launch_decode<1, 1, GATED, false, true, OUT>(a, s.waves, st);
-    return s.wide ? launch_decode<2, 1, GATED, false, false, OUT>(a, s.waves, st)
-                  : launch_decode<1, 1, GATED, false, false, OUT>(a, s.waves, st);
+    if constexpr (!GATED)
+        if (s.wide)
+            return launch_decode<2, 1, GATED, false, false, OUT>(a, s.waves, st);
+    return launch_decode<1, 1, GATED, false, false, OUT>(a, s.waves, st);
 }
 
 template <int OPS, int OUT>
@@ -2004,7 +2055,8 @@ int run_experts_gemm(Gemm a, const ExpertsPlan& e, size_t chunks, hipStream_t st
     p.slices = 1;
     p.chunks = unsigned(chunks);
     const size_t sets = OPS != kTransposed || of_one_backward(OUT) ? 2 : 1;
-    p.part = unsigned(ceil_div(ceil_div(chunks, sets), 4) * 4);
+    const size_t unit = OUT == kOutExpertsLinear ? 2 : 4;  // (gemm_kernel's turns)
+    p.part = unsigned(ceil_div(ceil_div(chunks, sets), unit) * unit);
     return run_gemm<OPS, OUT>(a, p, nullptr, st);
 }
 

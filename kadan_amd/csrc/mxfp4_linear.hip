@@ -209,7 +209,7 @@ extern "C" int kdq_mxfp4_linear_backward(const uint16_t* dy_bf16, size_t dy_stri
     Plan p{};
     ExpertsPlan e{};
     if (offsets) {
-        e = plan_experts_backward(m, experts, k, compute_units());
+        e = plan_experts_backward(m, experts, k);
         if (!launches(e))
             return KDQ_ERR_SHAPE;
     } else {
@@ -316,7 +316,7 @@ extern "C" int kdq_mxfp4_experts_gated_backward(
                         {up_transposed, bytes_of(f, experts)}};
     if (any_overlap(out, in))
         return KDQ_ERR_ALIAS;
-    const ExpertsPlan p = plan_experts_backward(m, experts, k, compute_units());
+    const ExpertsPlan p = plan_experts_backward(m, experts, k);
     if (!launches(p))
         return KDQ_ERR_SHAPE;
     const auto st = static_cast<hipStream_t>(stream);

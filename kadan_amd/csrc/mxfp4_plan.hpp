@@ -199,7 +199,22 @@ constexpr size_t most_tiles(size_t m, size_t experts, size_t rows) {
 }
 
 // How the experts' products run: decode_kernel over tiles of 16 rows, or gemm_kernel over tiles of
-// tt * 32, `most` tiles at most (the device alone knows how many).
+// tt * 32; `most` tiles at most (the device alone knows how many), each in tiles_n workgroups.
+//
+// gemm_kernel takes weights at the memory's rate as soon as there are workgroups of it for most
+// compute units, also where an expert has one row (256 sorted rows over 25 of 32 experts of
+// 2880 x 2880, gated: 41 us, 235 MB at 5.7 TB/s; decode_kernel 50).  Fewer, as for a token or two,
+// leave units without any, and decode_kernel's narrower shares are the quicker: 1 token to 4 of 32
+// experts gated 11.6 us against 15.5, then down 7.7 against 12.8; 2 tokens gated (184 workgroups)
+// 15.9 against 14.4, down (96) 9.8 against 12.8.  It reads a row of x once for each of its
+// workgroups: 16 tokens to 2 of 8 experts 5632 -> 4096 20.5 us against 20.4, 32 tokens 28 against
+// 21.
+//
+// Tiles of 32 rows waste least where experts have few, tiles of 64 reuse weights and operands
+// twice as much (two workgroups of either share a compute unit): 2048 rows of 32 experts gated 95
+// us against 102, back 133 against 143; 2800 rows 118 against 117, back 179 against 158; 4096
+// rows 163 against 154, back 241 against 207.  Tiles of 96 and 128 rows have a unit to themselves
+// and lose by 5 to 50 % up to 512 rows an expert, at 2048 they are within 2 % of those of 64.
 struct ExpertsPlan {
     bool decode;
     DecodeShape shape;
@@ -210,31 +225,30 @@ struct ExpertsPlan {
 inline ExpertsPlan plan_experts(size_t m, size_t experts, size_t n, size_t k, bool gated,
                                 bool kept, size_t cus) {
     ExpertsPlan p{};
-    const size_t reached = std::min(experts, m), mean = m / reached;
-    p.decode = !kept && mean <= 8;
+    const size_t reached = std::min(experts, m), mean = m / reached;  // (at most, at least)
+    p.tiles_n = ceil_div(n, gated ? 128 : 256);
+    p.decode = !(gated && kept) && p.tiles_n * reached * 9 <= cus * 5 && mean <= 4;
     if (p.decode) {
+        // (wavefronts of four units, whose loads are all in flight at once; two matrices' are
+        // twice as many, and their wavefronts take longer runs: gated 2880 -> 2880 of a token
+        // 11.6 us over 4, 12.3 over 6, 4096 -> 5632 12.8 over 4, 14.1 over 8; down 5632 -> 4096
+        // 8.2 over 12, 9.3 over 6)
         const size_t units = ceil_div(k, 128);
-        DecodeShape& s = p.shape;
-        s.wide = ceil_div(n, 32) * reached >= cus;
-        s.tb = 1;
-        s.waves = units <= 8 ? 2 : units <= 16 ? 4 : 8;
-        s.units = unsigned(ceil_div(ceil_div(units, s.waves), 2) * 2);
-        s.staged = m <= 16 && m * staged_pitch(unsigned(k * 2)) <= kStagedBytes &&
-                   m * k * 2 <= s.waves * 64 * 16 * 8;
+        p.shape.wide = !gated && ceil_div(n, 32) * reached >= cus;
+        p.shape.tb = 1;
+        p.shape.waves = unsigned(std::min<size_t>(ceil_div(units, 4), gated ? 4 : 16));
+        p.shape.units = unsigned(ceil_div(ceil_div(units, p.shape.waves), 2) * 2);
         p.most = most_tiles(m, experts, 16);
         return p;
     }
-    p.tt = mean <= 32 ? 1 : mean <= 64 ? 2 : mean <= 96 ? 3 : 4;
-    p.tiles_n = ceil_div(n, gated ? 128 : 256);
+    p.tt = mean < 96 ? 1 : 2;
     p.most = most_tiles(m, experts, size_t(p.tt) * 32);
     return p;
 }
 
-inline ExpertsPlan plan_experts_backward(size_t m, size_t experts, size_t k, size_t cus) {
+inline ExpertsPlan plan_experts_backward(size_t m, size_t experts, size_t k) {
     ExpertsPlan p{};
-    const size_t mean = m / std::min(experts, m);
-    (void)cus;
-    p.tt = mean <= 32 ? 1 : mean <= 64 ? 2 : mean <= 96 ? 3 : 4;
+    p.tt = m / std::min(experts, m) < 80 ? 1 : 2;
     p.tiles_n = ceil_div(k, 256);
     p.most = most_tiles(m, experts, size_t(p.tt) * 32);
     return p;
