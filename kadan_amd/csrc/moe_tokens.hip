@@ -3,14 +3,20 @@
 // IW/src/models/text/qwen_layers.cpp:378-492; IW = services/hikari/inference_worker) and has no
 // gradients.
 //
-//   sort_kernel            rows[p] = x[perm[p] / top_k], place[perm[p]] = p
+//   sort_kernel            rows[p] = x[perm[p] / top_k], place[perm[p]] = p, by positions
+//   place_kernel, spread_kernel   the same by tokens
 //   combine_kernel         y[t] = residual[t] + sum_i w[t, i] rows[place[t top_k + i]]; without
 //                          weights the gradient of sorting
 //   combine_grad_kernel    drows[place] = w dy, dw = dy . rows[place]
 //   route_grad_kernel      dlogits of the renormalised weights of the selection
 //
-// All of them move memory: a value costs a few operations at most.  A lane moves eight values
-// (16 or 32 bytes) at a time, from any element on: gfx950 loads need no alignment beyond it.
+// All of them move memory: a value costs a few operations at most, and up to a few hundred tokens
+// a call is its launch.  A lane moves 16 bytes at a time (32 where types differ), from any element
+// on: gfx950 loads need no alignment beyond it.  Times below are of single MI355X cards, whose
+// 1 GB copy runs at 5.2 TB/s and whose reads alone at 7.  Stores keep the caches' default policy:
+// streaming ones shorten what follows where that reads something else (combining 32768 rows of
+// 2048 bf16 values and back 90 -> 77 us) and lengthen it where it reads the rows, as the experts'
+// products do (back and the down product's gradient 173 -> 183).
 #include "kdq_common.hpp"
 
 #include <algorithm>
@@ -51,80 +57,91 @@ template <> __device__ __forceinline__ F16 narrow<F16>(float v) {
     return {__builtin_bit_cast(uint16_t, _Float16(v))};
 }
 
-// Eight values as they lie.
-template <class T> struct Eight {
-    u32x4 w[sizeof(T) / 2];
+// N values as they lie, 16 bytes or twice as many.
+template <class T, int N> struct Piece {
+    u32x4 w[N * sizeof(T) / 16];
 };
 
-template <class T> __device__ __forceinline__ Eight<T> load8(const T* p) {
-    Eight<T> v;
+// Values a lane moves at a time: 16 bytes of the narrower type, so that a wavefront's access is
+// whole lines of it.
+template <class T, class Y> constexpr int kValues = sizeof(T) == 4 && sizeof(Y) == 4 ? 4 : 8;
+
+template <int N, class T> __device__ __forceinline__ Piece<T, N> load_whole(const T* p) {
+    Piece<T, N> v;
 #pragma unroll
-    for (unsigned i = 0; i < sizeof(T) / 2; ++i)
+    for (unsigned i = 0; i < N * sizeof(T) / 16; ++i)
         v.w[i] = load16_a2(reinterpret_cast<const uint8_t*>(p) + 16 * i);
     return v;
 }
 
-template <class T> __device__ __forceinline__ void store8(T* p, const Eight<T>& v) {
+template <int N, class T> __device__ __forceinline__ void store_whole(T* p, const Piece<T, N>& v) {
 #pragma unroll
-    for (unsigned i = 0; i < sizeof(T) / 2; ++i)
+    for (unsigned i = 0; i < N * sizeof(T) / 16; ++i)
         reinterpret_cast<u32x4_a2*>(p)[i] = u32x4_a2{v.w[i].x, v.w[i].y, v.w[i].z, v.w[i].w};
 }
 
-__device__ __forceinline__ float value(const Eight<Bf16>& v, int i) {
-    const unsigned w = v.w[0][i / 2];
+template <int N> __device__ __forceinline__ float value(const Piece<Bf16, N>& v, int i) {
+    const unsigned w = v.w[i / 8][i / 2 % 4];
     return __uint_as_float(i % 2 ? w & 0xffff0000u : w << 16);
 }
-__device__ __forceinline__ float value(const Eight<F16>& v, int i) {
-    return half_hw((v.w[0][i / 2] >> (16 * (i % 2))) & 0xffffu);
+template <int N> __device__ __forceinline__ float value(const Piece<F16, N>& v, int i) {
+    return half_hw((v.w[i / 8][i / 2 % 4] >> (16 * (i % 2))) & 0xffffu);
 }
-__device__ __forceinline__ float value(const Eight<float>& v, int i) {
+template <int N> __device__ __forceinline__ float value(const Piece<float, N>& v, int i) {
     return __uint_as_float(v.w[i / 4][i % 4]);
 }
 
-__device__ __forceinline__ void set(Eight<Bf16>& v, const float (&f)[8]) {
+template <int N> __device__ __forceinline__ void set(Piece<Bf16, N>& v, const float (&f)[N]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        v.w[0][i] = __builtin_bit_cast(unsigned, bf16x2{__bf16(f[2 * i]), __bf16(f[2 * i + 1])});
+    for (int i = 0; i < N; i += 2)
+        v.w[i / 8][i / 2 % 4] =
+            __builtin_bit_cast(unsigned, bf16x2{__bf16(f[i]), __bf16(f[i + 1])});
 }
-__device__ __forceinline__ void set(Eight<F16>& v, const float (&f)[8]) {
+template <int N> __device__ __forceinline__ void set(Piece<F16, N>& v, const float (&f)[N]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        v.w[0][i] = unsigned(narrow<F16>(f[2 * i]).bits) |
-                    unsigned(narrow<F16>(f[2 * i + 1]).bits) << 16;
+    for (int i = 0; i < N; i += 2)
+        v.w[i / 8][i / 2 % 4] =
+            unsigned(narrow<F16>(f[i]).bits) | unsigned(narrow<F16>(f[i + 1]).bits) << 16;
 }
-__device__ __forceinline__ void set(Eight<float>& v, const float (&f)[8]) {
+template <int N> __device__ __forceinline__ void set(Piece<float, N>& v, const float (&f)[N]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < N; ++i)
         v.w[i / 4][i % 4] = __float_as_uint(f[i]);
 }
 
-// A row's values c .. c + 7, of which those past its end read as zeros and are not written.
-template <class T>
-__device__ __forceinline__ Eight<T> load_piece(const T* row, unsigned c, unsigned cols) {
-    if (c + 8 <= cols)
-        return load8(row + c);
-    float f[8];
+// A row's values from c on, of which those past its end read as zeros and are not written.
+template <int N, class T>
+__device__ __forceinline__ Piece<T, N> load_piece(const T* row, unsigned c, unsigned cols) {
+    if (c + N <= cols)
+        return load_whole<N>(row + c);
+    float f[N];
 #pragma unroll
-    for (unsigned i = 0; i < 8; ++i)
+    for (unsigned i = 0; i < N; ++i)
         f[i] = c + i < cols ? widen(row[c + i]) : 0.f;
-    Eight<T> v;
+    Piece<T, N> v;
     set(v, f);
     return v;
 }
 
-template <class T>
-__device__ __forceinline__ void store_piece(T* row, unsigned c, unsigned cols, const float (&f)[8]) {
-    if (c + 8 <= cols) {
-        Eight<T> v;
+template <int N, class T>
+__device__ __forceinline__ void store_piece(T* row, unsigned c, unsigned cols,
+                                            const float (&f)[N]) {
+    if (c + N <= cols) {
+        Piece<T, N> v;
         set(v, f);
-        store8(row + c, v);
+        store_whole<N>(row + c, v);
         return;
     }
 #pragma unroll
-    for (unsigned i = 0; i < 8; ++i)
+    for (unsigned i = 0; i < N; ++i)
         if (c + i < cols)
             row[c + i] = narrow<T>(f[i]);
 }
+
+// From this many bytes of rows on they are written by tokens, in two launches: 32768 rows of 2048
+// bf16 values 26.6 us against 37.5 by positions (5.7 TB/s of what has to move), 8192 of 2880 13.3
+// against 14.8, 4096 of 2048 (17 MB) 7.4 against 6.3.
+constexpr size_t kSpreadBytes = size_t(32) << 20;
 
 // How a launch's workgroups share rows of `cols` values: `across` lanes (a power of two) along a
 // row, the others' along further rows.
@@ -132,15 +149,16 @@ struct Shape {
     unsigned across, rows, blocks;  // rows of a workgroup, workgroups of a row
 };
 
-Shape shape_of(size_t cols) {
-    const size_t pieces = (cols + 7) / 8;
+Shape shape_of(size_t cols, int values) {
+    const size_t pieces = (cols + values - 1) / values;
     unsigned across = 1;
     while (across < kThreads && across < pieces)
         across *= 2;
     return {across, kThreads / across, unsigned((pieces + across - 1) / across)};
 }
 
-// A copy, so bits and no values.
+// A copy, so bits and no values.  By positions: a row of x is read for each of its places, from
+// the caches but for the first time.
 template <class U>
 __global__ __launch_bounds__(kThreads) void sort_kernel(const U* __restrict__ x, size_t x_stride,
                                                         unsigned slots, unsigned cols,
@@ -148,36 +166,90 @@ __global__ __launch_bounds__(kThreads) void sort_kernel(const U* __restrict__ x,
                                                         const int32_t* __restrict__ perm,
                                                         U* __restrict__ rows, size_t rows_stride,
                                                         int32_t* __restrict__ place) {
+    constexpr unsigned N = kValues<U, U>;
     const unsigned p = blockIdx.x * s.rows + threadIdx.x / s.across;
-    const unsigned c = (blockIdx.y * s.across + threadIdx.x % s.across) * 8;
+    const unsigned c = (blockIdx.y * s.across + threadIdx.x % s.across) * N;
     if (p >= slots || c >= cols)
         return;
     const unsigned slot = unsigned(perm[p]);
     U* to = rows + size_t(p) * rows_stride + c;
     if (slot >= slots) {  // no slot: a row of zeros
-        for (unsigned i = 0; i < 8 && c + i < cols; ++i)
+        for (unsigned i = 0; i < N && c + i < cols; ++i)
             to[i] = U{};
         return;
     }
     if (c == 0)
         place[slot] = int32_t(p);
     const U* from = x + size_t(slot / top_k) * x_stride + c;
-    if (c + 8 <= cols) {
-        store8(to, load8(from));
+    if (c + N <= cols) {
+        store_whole<N>(to, load_whole<N>(from));
     } else {
         for (unsigned i = 0; c + i < cols; ++i)
             to[i] = from[i];
     }
 }
 
-// Sums in fp32, in the order of the selection, and one rounding.
+// The same by tokens, once the places are known: a row of x is read once.
+template <class U>
+__global__ __launch_bounds__(kThreads) void place_kernel(const int32_t* __restrict__ perm,
+                                                         unsigned slots, unsigned cols,
+                                                         U* __restrict__ rows, size_t rows_stride,
+                                                         int32_t* __restrict__ place) {
+    const unsigned p = blockIdx.x * kThreads + threadIdx.x;
+    if (p >= slots)
+        return;
+    if (unsigned(perm[p]) < slots) {
+        place[perm[p]] = int32_t(p);
+    } else {
+        for (unsigned c = 0; c < cols; ++c)
+            rows[size_t(p) * rows_stride + c] = U{};
+    }
+}
+
+template <class U>
+__global__ __launch_bounds__(kThreads) void spread_kernel(const U* __restrict__ x, size_t x_stride,
+                                                          unsigned tokens, unsigned cols,
+                                                          unsigned top_k, Shape s,
+                                                          const int32_t* __restrict__ perm,
+                                                          const int32_t* __restrict__ place,
+                                                          U* __restrict__ rows,
+                                                          size_t rows_stride) {
+    constexpr unsigned N = kValues<U, U>;
+    const unsigned t = blockIdx.x * s.rows + threadIdx.x / s.across;
+    const unsigned c = (blockIdx.y * s.across + threadIdx.x % s.across) * N;
+    if (t >= tokens || c >= cols)
+        return;
+    const unsigned slots = tokens * top_k;
+    const bool whole = c + N <= cols;
+    const U* from = x + size_t(t) * x_stride + c;
+    Piece<U, N> v;
+    if (whole)
+        v = load_whole<N>(from);
+    for (unsigned i = 0; i < top_k; ++i) {
+        const unsigned slot = t * top_k + i, p = unsigned(place[slot]);
+        if (p >= slots || unsigned(perm[p]) != slot)  // (a slot that perm does not name)
+            continue;
+        U* to = rows + size_t(p) * rows_stride + c;
+        if (whole) {
+            store_whole<N>(to, v);
+        } else {
+            for (unsigned j = 0; c + j < cols; ++j)
+                to[j] = from[j];
+        }
+    }
+}
+
+// Sums in fp32, in the order of the selection, and one rounding.  Every row of a token is asked for
+// at once.  32768 rows of 2048 bf16 values to 4096 tokens 24.7 us (6.1 TB/s), with weights and a
+// residual 28 (6.0); a few tokens 3 us, the launch and two loads, one behind the other.
 template <class T, class Y>
 __global__ __launch_bounds__(kThreads) void combine_kernel(
     const T* __restrict__ rows, size_t rows_stride, const int32_t* __restrict__ place,
     const float* __restrict__ weights, unsigned tokens, unsigned top_k, unsigned cols, Shape s,
     const Y* residual, size_t residual_stride, Y* y, size_t y_stride) {
+    constexpr int N = kValues<T, Y>;
     const unsigned t = blockIdx.x * s.rows + threadIdx.x / s.across;
-    const unsigned c = (blockIdx.y * s.across + threadIdx.x % s.across) * 8;
+    const unsigned c = (blockIdx.y * s.across + threadIdx.x % s.across) * N;
     if (t >= tokens || c >= cols)
         return;
     const unsigned slots = tokens * top_k;
@@ -189,35 +261,37 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(
             at[i] = unsigned(place[t * top_k + i]);
             w[i] = weights ? weights[t * top_k + i] : 1.0f;
         }
-    Eight<T> v[kMost];
+    Piece<T, N> v[kMost];
 #pragma unroll
     for (unsigned i = 0; i < kMost; ++i)
         if (i < top_k && at[i] < slots)
-            v[i] = load_piece(rows + size_t(at[i]) * rows_stride, c, cols);
-    float sum[8] = {};
+            v[i] = load_piece<N>(rows + size_t(at[i]) * rows_stride, c, cols);
+    float sum[N] = {};
     if (residual) {
-        const Eight<Y> r = load_piece(residual + size_t(t) * residual_stride, c, cols);
+        const Piece<Y, N> r = load_piece<N>(residual + size_t(t) * residual_stride, c, cols);
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
+        for (int e = 0; e < N; ++e)
             sum[e] = value(r, e);
     }
 #pragma unroll
     for (unsigned i = 0; i < kMost; ++i)
         if (i < top_k && at[i] < slots)
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
+            for (int e = 0; e < N; ++e)
                 sum[e] = fmaf(w[i], value(v[i], e), sum[e]);
-    store_piece(y + size_t(t) * y_stride, c, cols, sum);
+    store_piece<N>(y + size_t(t) * y_stride, c, cols, sum);
 }
 
-// A workgroup takes a token: its dy is read once for all of its rows, each of which is read,
-// multiplied into its weight's gradient and written over by none (drows is another tensor).
+// A workgroup takes a token: its dy is read once for all of its rows, and one pass over those gives
+// both gradients; dot products are summed lane by lane, then over lanes and wavefronts in their
+// order, so results do not depend on the run.  32768 rows of 2048 bf16 values 49 us (5.8 TB/s).
 template <class T, class Y>
 __global__ __launch_bounds__(kThreads) void combine_grad_kernel(
     const T* __restrict__ rows, size_t rows_stride, const Y* __restrict__ dy, size_t dy_stride,
     const int32_t* __restrict__ place, const float* __restrict__ weights, unsigned tokens,
     unsigned top_k, unsigned cols, T* __restrict__ drows, size_t drows_stride,
     float* __restrict__ dweights) {
+    constexpr int N = kValues<T, Y>;
     __shared__ float sums[kThreads / 64][kMost];
     const unsigned t = blockIdx.x, slots = tokens * top_k;
     const unsigned lane = threadIdx.x % 64, wave = threadIdx.x / 64;
@@ -229,24 +303,24 @@ __global__ __launch_bounds__(kThreads) void combine_grad_kernel(
             at[i] = unsigned(place[t * top_k + i]);
             w[i] = weights[t * top_k + i];
         }
-    for (unsigned c = threadIdx.x * 8; c < cols; c += blockDim.x * 8) {
-        const Eight<Y> d = load_piece(dy + size_t(t) * dy_stride, c, cols);
-        Eight<T> v[kMost];
+    for (unsigned c = threadIdx.x * N; c < cols; c += blockDim.x * N) {
+        const Piece<Y, N> d = load_piece<N>(dy + size_t(t) * dy_stride, c, cols);
+        Piece<T, N> v[kMost];
 #pragma unroll
         for (unsigned i = 0; i < kMost; ++i)
             if (i < top_k && at[i] < slots)
-                v[i] = load_piece(rows + size_t(at[i]) * rows_stride, c, cols);
+                v[i] = load_piece<N>(rows + size_t(at[i]) * rows_stride, c, cols);
 #pragma unroll
         for (unsigned i = 0; i < kMost; ++i)
             if (i < top_k && at[i] < slots) {
-                float f[8];
+                float f[N];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
+                for (int e = 0; e < N; ++e) {
                     const float g = value(d, e);
                     dot[i] = fmaf(g, value(v[i], e), dot[i]);
                     f[e] = w[i] * g;
                 }
-                store_piece(drows + size_t(at[i]) * drows_stride, c, cols, f);
+                store_piece<N>(drows + size_t(at[i]) * drows_stride, c, cols, f);
             }
     }
 #pragma unroll
@@ -266,7 +340,8 @@ __global__ __launch_bounds__(kThreads) void combine_grad_kernel(
 }
 
 // w = softmax over the selected logits, so dlogit = w (dw - sum w dw) there and 0 elsewhere.  A
-// wavefront takes a token: lane i its selection i, then lanes go along the experts.
+// wavefront takes a token: lane i its selection i, then lanes go along the experts.  4096 tokens of
+// 128 experts 3.7 us, of which 2.5 are the launch.
 __global__ __launch_bounds__(kThreads) void route_grad_kernel(
     const int32_t* __restrict__ idx, const float* __restrict__ weights,
     const float* __restrict__ dweights, unsigned tokens, unsigned experts, unsigned top_k,
@@ -357,10 +432,10 @@ template <class F> int by_types(int type, int second, F&& f) {
 
 int combine(const Rows& rows, const int32_t* place, const float* weights, size_t tokens,
             size_t top_k, size_t cols, const Rows& residual, const Rows& y, hipStream_t st) {
-    const Shape s = shape_of(cols);
     return by_types(rows.type, y.type, [&](auto t, auto u) {
         using T = decltype(t);
         using Y = decltype(u);
+        const Shape s = shape_of(cols, kValues<T, Y>);
         hipLaunchKernelGGL((combine_kernel<T, Y>),
                            dim3(unsigned((tokens + s.rows - 1) / s.rows), s.blocks),
                            dim3(kThreads), 0, st, static_cast<const T*>(rows.p), rows.stride,
@@ -392,13 +467,27 @@ extern "C" int kdq_moe_sort(int type, const void* x, size_t x_stride, size_t tok
                 from[] = {{x, in.bytes(cols)}, {perm, slots * 4}};
     if (any_overlap(to, from))
         return KDQ_ERR_ALIAS;
-    const Shape s = shape_of(cols);
+    const auto st = static_cast<hipStream_t>(stream);
     const auto launch = [&](auto u) {
         using U = decltype(u);
-        hipLaunchKernelGGL(sort_kernel<U>, dim3(unsigned((slots + s.rows - 1) / s.rows), s.blocks),
-                           dim3(kThreads), 0, static_cast<hipStream_t>(stream),
-                           static_cast<const U*>(x), x_stride, unsigned(slots), unsigned(cols),
-                           unsigned(top_k), s, perm, static_cast<U*>(rows), rows_stride, place);
+        const Shape s = shape_of(cols, kValues<U, U>);
+        const auto blocks = [&](size_t count) {
+            return dim3(unsigned((count + s.rows - 1) / s.rows), s.blocks);
+        };
+        if (top_k > 1 && slots * cols * size_of(type) >= kSpreadBytes) {
+            hipLaunchKernelGGL(place_kernel<U>, dim3(unsigned((slots + kThreads - 1) / kThreads)),
+                               dim3(kThreads), 0, st, perm, unsigned(slots), unsigned(cols),
+                               static_cast<U*>(rows), rows_stride, place);
+            hipLaunchKernelGGL(spread_kernel<U>, blocks(tokens), dim3(kThreads), 0, st,
+                               static_cast<const U*>(x), x_stride, unsigned(tokens),
+                               unsigned(cols), unsigned(top_k), s, perm, place,
+                               static_cast<U*>(rows), rows_stride);
+        } else {
+            hipLaunchKernelGGL(sort_kernel<U>, blocks(slots), dim3(kThreads), 0, st,
+                               static_cast<const U*>(x), x_stride, unsigned(slots),
+                               unsigned(cols), unsigned(top_k), s, perm, static_cast<U*>(rows),
+                               rows_stride, place);
+        }
         KDQ_HIP(hipGetLastError());
         return int(KDQ_OK);
     };

@@ -1381,6 +1381,8 @@ __global__ __launch_bounds__(512, (shares_unit<TT, OPS> ? 4 : 2)) void gemm_kern
     // segments past the part's end, or the row's, read as zeros
     const unsigned first_row = tile_m * kRows;
     const unsigned rows = min(kRows, a.out.m - first_row);
+    // (a tile of the experts' that holds one of its two halves multiplies one)
+    const bool both = rows > 32;
     const auto xs = buffer(a.x + size_t(first_row) * a.x_stride,
                            (rows - 1) * a.x_stride + a.x_second * (OPS == kTransposed) +
                                a.segments * 16);
@@ -1674,13 +1676,16 @@ __global__ __launch_bounds__(512, (shares_unit<TT, OPS> ? 4 : 2)) void gemm_kern
                         decode_w.template operator()<C, S + kBuffers - 1>(
                             wv[(S + kBuffers - 1) % kBuffers]);
 #pragma unroll
-                    for (int t = 0; t < TT; ++t)
+                    for (int t = 0; t < TT; ++t) {
+                        if (of_experts(OUT) && t > 0 && !both)
+                            continue;
 #pragma unroll
                         for (int i = 0; i < 2; ++i)
                             acc[i][t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
                                 wv[S % kBuffers][i],
                                 __builtin_bit_cast(bf16x8, xv[S % kBuffers][t]),
                                 acc[i][t], 0, 0, 0);
+                    }
                 });
                 issue_order();
                 load_codes(begin_step + c0 + C + kAhead, codes[C % kAhead]);

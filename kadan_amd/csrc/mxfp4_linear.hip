@@ -209,7 +209,7 @@ extern "C" int kdq_mxfp4_linear_backward(const uint16_t* dy_bf16, size_t dy_stri
     Plan p{};
     ExpertsPlan e{};
     if (offsets) {
-        e = plan_experts_backward(m, experts, k);
+        e = plan_experts_backward(m, experts, k, false);
         if (!launches(e))
             return KDQ_ERR_SHAPE;
     } else {
@@ -316,7 +316,7 @@ extern "C" int kdq_mxfp4_experts_gated_backward(
                         {up_transposed, bytes_of(f, experts)}};
     if (any_overlap(out, in))
         return KDQ_ERR_ALIAS;
-    const ExpertsPlan p = plan_experts_backward(m, experts, k);
+    const ExpertsPlan p = plan_experts_backward(m, experts, k, true);
     if (!launches(p))
         return KDQ_ERR_SHAPE;
     const auto st = static_cast<hipStream_t>(stream);

@@ -210,11 +210,13 @@ constexpr size_t most_tiles(size_t m, size_t experts, size_t rows) {
 // workgroups: 16 tokens to 2 of 8 experts 5632 -> 4096 20.5 us against 20.4, 32 tokens 28 against
 // 21.
 //
-// Tiles of 32 rows waste least where experts have few, tiles of 64 reuse weights and operands
-// twice as much (two workgroups of either share a compute unit): 2048 rows of 32 experts gated 95
-// us against 102, back 133 against 143; 2800 rows 118 against 117, back 179 against 158; 4096
-// rows 163 against 154, back 241 against 207.  Tiles of 96 and 128 rows have a unit to themselves
-// and lose by 5 to 50 % up to 512 rows an expert, at 2048 they are within 2 % of those of 64.
+// Tiles of 64 rows (two workgroups of either share a compute unit; a half that is empty is not
+// multiplied) decode a weight once for twice the rows, tiles of 32 are more, and fill the last
+// round of workgroups better: 2048 rows of 32 experts of 2880 x 2880 gated 97 us against 101, down
+// 60 against 54, back 135 against 137 and 66 against 64; 8192 rows of 128 of 2048 x 768 70 against
+// 73, 52 against 54, 97 against 110 and 46 against 46; 256 rows of the 32 gated 73 against 64.
+// Tiles of 96 and 128 rows have a unit to themselves and lose by 5 to 50 % up to 512 rows an
+// expert; at 2048 they are within 2 % of those of 64.
 struct ExpertsPlan {
     bool decode;
     DecodeShape shape;
@@ -241,14 +243,15 @@ inline ExpertsPlan plan_experts(size_t m, size_t experts, size_t n, size_t k, bo
         p.most = most_tiles(m, experts, 16);
         return p;
     }
-    p.tt = mean < 96 ? 1 : 2;
+    p.tt = mean < (gated ? 48 : 96) ? 1 : 2;
     p.most = most_tiles(m, experts, size_t(p.tt) * 32);
     return p;
 }
 
-inline ExpertsPlan plan_experts_backward(size_t m, size_t experts, size_t k) {
+// (`gated`: two matrices)
+inline ExpertsPlan plan_experts_backward(size_t m, size_t experts, size_t k, bool gated) {
     ExpertsPlan p{};
-    p.tt = m / std::min(experts, m) < 80 ? 1 : 2;
+    p.tt = m / std::min(experts, m) < (gated ? 48 : 80) ? 1 : 2;
     p.tiles_n = ceil_div(k, 256);
     p.most = most_tiles(m, experts, size_t(p.tt) * 32);
     return p;

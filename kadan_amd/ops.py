@@ -692,9 +692,7 @@ def _offsets(offsets: torch.Tensor) -> int:
     return experts
 
 
-def _bias(bias: torch.Tensor | None, name: str, *shape: int) -> int | None:
-    if bias is None:
-        return None
+def _bias(bias: torch.Tensor, name: str, shape: tuple) -> int:
     _no_graph(bias, name)
     _need(bias, torch.float32, name)
     if bias.shape != shape:
@@ -733,33 +731,31 @@ def mxfp4_linear(x: torch.Tensor, packed: torch.Tensor, n_out: int,
     if save and not act:
         raise ValueError("save: without an activation there is nothing to keep")
     m, k = x.shape
-    parts, size = [x, packed], 0
     if offsets is None:
         experts, table = 1, None
         weights, size = _mxfp4_sizes(_PACKED, n_out, k, "kdq_mxfp4_linear_workspace", m, n_out, k)
         w = _matrix(packed, weights, "packed")
-        b = _bias(bias, "bias", n_out)
+        stream = _stream_for(x, packed)
     else:
-        experts, table = _offsets(offsets), offsets.data_ptr()
+        experts, table, size = _offsets(offsets), offsets.data_ptr(), 0
         w = _stack(packed, _EXPERTS, experts, n_out, k, "packed")
-        b = _bias(bias, "bias", experts, n_out)
-        parts.append(offsets)
+        stream = _stream_for(x, packed, offsets)
+    b = add = None
     if bias is not None:
-        parts.append(bias)
-    add, add_stride = None, 0
+        b = _bias(bias, "bias", (n_out,) if table is None else (experts, n_out))
+        _stream_for(bias)
+    add_stride = 0
     if residual is not None:
         _no_graph(residual, "residual")
         add, add_stride = residual.data_ptr(), _output(residual, m, n_out, dtype, "residual")
-        parts.append(residual)
-    device = x.device
+        _stream_for(residual)
     if out is None:
-        stream, y_stride = _stream_for(*parts), n_out
-        out = torch.empty(m, n_out, dtype=dtype, device=device)
+        y_stride, out = n_out, x.new_empty(m, n_out, dtype=dtype)
     else:
         y_stride = _output(out, m, n_out, dtype, "out")
-        stream = _stream_for(*parts, out)
-    saved = torch.empty(m, n_out, dtype=_BF16, device=device) if save else None
-    scratch = _scratch(size, device)
+        _stream_for(out)
+    saved = x.new_empty(m, n_out) if save else None
+    scratch = _scratch(size, x.device) if size else None
     call("kdq_mxfp4_linear", x.data_ptr(), stride, m, table, experts, w, n_out, k, b, act, add,
          add_stride, kind, out.data_ptr(), y_stride, _ptr(saved), _ptr(scratch), size, stream)
     return (out, saved) if save else out
@@ -835,25 +831,24 @@ def mxfp4_experts_gated(x: torch.Tensor, offsets: torch.Tensor, gate: torch.Tens
     experts = _offsets(offsets)
     wg = _stack(gate, _EXPERTS, experts, n_out, k, "gate")
     wu = _stack(up, _EXPERTS, experts, n_out, k, "up")
-    bg = _bias(gate_bias, "gate_bias", experts, n_out)
-    bu = _bias(up_bias, "up_bias", experts, n_out)
-    parts = [x, offsets, gate, up]
-    if bg is not None:
-        parts += [gate_bias, up_bias]
-    device = x.device
+    stream = _stream_for(x, offsets, gate, up)
+    bg = bu = None
+    if gate_bias is not None:
+        bg = _bias(gate_bias, "gate_bias", (experts, n_out))
+        bu = _bias(up_bias, "up_bias", (experts, n_out))
+        _stream_for(gate_bias, up_bias)
     if out is None:
-        stream, h_stride = _stream_for(*parts), n_out
-        out = torch.empty(m, n_out, dtype=_BF16, device=device)
+        h_stride, out = n_out, x.new_empty(m, n_out)
     else:
         h_stride = _output(out, m, n_out, _BF16, "out")
-        stream = _stream_for(*parts, out)
+        _stream_for(out)
     saved = kept = codes = scales = None
     if save == "bf16":
-        saved = torch.empty(m, 2 * n_out, dtype=_BF16, device=device)
+        saved = x.new_empty(m, 2 * n_out)
         kept = saved.data_ptr()
     elif save == "q8":
-        saved = (torch.empty(m, 2 * n_out, dtype=torch.int8, device=device),
-                 torch.empty(m, n_out // 16, dtype=torch.float32, device=device))
+        saved = (x.new_empty(m, 2 * n_out, dtype=torch.int8),
+                 x.new_empty(m, n_out // 16, dtype=torch.float32))
         codes, scales = saved[0].data_ptr(), saved[1].data_ptr()
     call("kdq_mxfp4_experts_gated", x.data_ptr(), stride, m, offsets.data_ptr(), experts, wg, wu,
          n_out, k, bg, bu, act, out.data_ptr(), h_stride, kept, codes, scales, stream)
@@ -935,8 +930,7 @@ def moe_sort(x: torch.Tensor, perm: torch.Tensor, top_k: int):
     slots = tokens * top_k
     order = _slots(perm, slots, "perm")
     stream = _stream_for(x, perm)
-    rows = torch.empty(slots, cols, dtype=x.dtype, device=x.device)
-    place = torch.empty(slots, dtype=torch.int32, device=x.device)
+    rows, place = x.new_empty(slots, cols), perm.new_empty(slots)
     call("kdq_moe_sort", kind, x.data_ptr(), stride, tokens, cols, top_k, order, rows.data_ptr(),
          cols, place.data_ptr(), stream)
     return rows, place
@@ -952,7 +946,7 @@ def moe_sort_backward(drows: torch.Tensor, place: torch.Tensor, top_k: int) -> t
         raise ValueError("drows: expected top_k rows per token")
     at = _slots(place, slots, "place")
     stream = _stream_for(drows, place)
-    dx = torch.empty(slots // top_k, cols, dtype=drows.dtype, device=drows.device)
+    dx = drows.new_empty(slots // top_k, cols)
     call("kdq_moe_sort_backward", kind, drows.data_ptr(), stride, at, slots // top_k, cols, top_k,
          dx.data_ptr(), cols, stream)
     return dx
@@ -973,9 +967,8 @@ def moe_combine(rows: torch.Tensor, weights: torch.Tensor, place: torch.Tensor,
     [tokens, top_k], place from moe_sort -> y [tokens, cols] of the rows' type or fp32
     (``dtype``; the residual's, and ``out`` may be the residual itself) (kdq_moe_combine).
     Nothing is recorded for autograd: its backward pass is moe_combine_backward."""
-    for t, name in ((rows, "rows"), (weights, "weights"), (residual, "residual")):
-        if t is not None:
-            _no_graph(t, name)
+    _no_graph(rows, "rows")
+    _no_graph(weights, "weights")
     kind, stride = _rows_of(rows, "rows")
     tokens, top_k = _weights(weights, "weights")
     slots, cols = rows.shape
@@ -986,16 +979,17 @@ def moe_combine(rows: torch.Tensor, weights: torch.Tensor, place: torch.Tensor,
         dtype = rows.dtype
     if dtype != rows.dtype and dtype != torch.float32:
         raise ValueError("dtype: the rows' type or fp32")
-    parts, add, add_stride = [rows, weights, place], None, 0
+    stream = _stream_for(rows, weights, place)
+    add, add_stride = None, 0
     if residual is not None:
+        _no_graph(residual, "residual")
         add, add_stride = residual.data_ptr(), _output(residual, tokens, cols, dtype, "residual")
-        parts.append(residual)
+        _stream_for(residual)
     if out is None:
-        stream, y_stride = _stream_for(*parts), cols
-        out = torch.empty(tokens, cols, dtype=dtype, device=rows.device)
+        y_stride, out = cols, rows.new_empty(tokens, cols, dtype=dtype)
     else:
         y_stride = _output(out, tokens, cols, dtype, "out")
-        stream = _stream_for(*parts, out)
+        _stream_for(out)
     call("kdq_moe_combine", kind, rows.data_ptr(), stride, at, weights.data_ptr(), tokens, cols,
          top_k, _TYPES[dtype], add, add_stride, out.data_ptr(), y_stride, stream)
     return out
@@ -1017,8 +1011,7 @@ def moe_combine_backward(dy: torch.Tensor, rows: torch.Tensor, weights: torch.Te
         raise ValueError("expected rows [tokens * top_k, cols] and dy [tokens, cols]")
     at = _slots(place, slots, "place")
     stream = _stream_for(rows, weights, place, dy)
-    drows = torch.empty(slots, cols, dtype=rows.dtype, device=rows.device)
-    dweights = torch.empty(tokens, top_k, dtype=torch.float32, device=rows.device)
+    drows, dweights = rows.new_empty(slots, cols), weights.new_empty(tokens, top_k)
     call("kdq_moe_combine_backward", kind, rows.data_ptr(), stride, at, weights.data_ptr(),
          tokens, cols, top_k, dy_kind, dy.data_ptr(), dy_stride, drows.data_ptr(), cols,
          dweights.data_ptr(), stream)
@@ -1036,7 +1029,7 @@ def moe_route_backward(idx: torch.Tensor, weights: torch.Tensor, dweights: torch
     if idx.shape != weights.shape or dweights.shape != weights.shape:
         raise ValueError("idx, weights and dweights: expected one shape")
     stream = _stream_for(idx, weights, dweights)
-    dlogits = torch.empty(tokens, experts, dtype=torch.float32, device=weights.device)
+    dlogits = weights.new_empty(tokens, experts)
     call("kdq_moe_route_backward", idx.data_ptr(), weights.data_ptr(), dweights.data_ptr(), tokens,
          experts, top_k, dlogits.data_ptr(), stream)
     return dlogits
