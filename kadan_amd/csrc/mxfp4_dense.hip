@@ -226,12 +226,9 @@ extern "C" int kdq_mxfp4_gated_backward(const uint16_t* dh_bf16, size_t dh_strid
         return rc;
     const auto st = static_cast<hipStream_t>(stream);
     const dim3 grid(unsigned(ceil_div(m * (n / 8), 256)));
-    if (kept_q8)
-        hipLaunchKernelGGL((gate_grad_kernel<true, false>), grid, dim3(256), 0, st, dh_bf16, dh_stride,
-                           unsigned(m), unsigned(n), kept_bf16, kept_q8, kept_scales, dgu_bf16);
-    else
-        hipLaunchKernelGGL((gate_grad_kernel<false, false>), grid, dim3(256), 0, st, dh_bf16, dh_stride,
-                           unsigned(m), unsigned(n), kept_bf16, kept_q8, kept_scales, dgu_bf16);
+    const auto kernel = kept_q8 ? gate_grad_kernel<true, false> : gate_grad_kernel<false, false>;
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, dh_bf16, dh_stride, unsigned(m), unsigned(n),
+                       kept_bf16, kept_q8, kept_scales, dgu_bf16);
     KDQ_HIP(hipGetLastError());
     const Form f = transposed_form(n, k);
     const Target t{dx_bf16, dx_stride, unsigned(m), unsigned(k), nullptr, nullptr, nullptr};

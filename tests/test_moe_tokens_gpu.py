@@ -16,8 +16,8 @@ BITS = {F32: torch.int32, F16: torch.int16, BF16: torch.int16}
 
 # tokens, experts, top_k, cols: one of each, odd rows, every way rows share a workgroup, rows of
 # several workgroups
-SIZES = [(1, 1, 1, 1), (1, 4, 4, 2880), (3, 5, 2, 7), (5, 32, 4, 2880), (17, 8, 3, 8), (33, 16, 8, 9),
-         (64, 128, 8, 65), (7, 256, 5, 1023), (100, 12, 6, 511), (257, 9, 7, 128),
+SIZES = [(1, 1, 1, 1), (1, 4, 4, 2880), (3, 5, 2, 7), (5, 32, 4, 2880), (17, 8, 3, 8),
+         (33, 16, 8, 9), (64, 128, 8, 65), (7, 256, 5, 1023), (100, 12, 6, 511), (257, 9, 7, 128),
          (1000, 64, 4, 333), (6, 4, 4, 2049), (2, 3, 3, 8192), (513, 128, 8, 2048)]
 
 
@@ -118,6 +118,25 @@ def test_strided_rows_and_given_outputs(gen, dtype):
     for a, b in zip(got, ops.moe_combine_backward(x.contiguous(), part.contiguous(), weights,
                                                   place)):
         assert same(a, b)
+
+
+@pytest.mark.parametrize("dtype,tokens,top_k,cols", [
+    (BF16, 1100, 8, 2050), (F16, 4100, 2, 2047), (F32, 900, 3, 4101), (F32, 140, 8, 8200)])
+def test_sort_of_many_rows_by_tokens(gen, dtype, tokens, top_k, cols):
+    """32 MB of rows and more: odd rows apart, and entries that are no slot or a slot again."""
+    wide = normal(gen, tokens, cols + 5).to(dtype)
+    x = wide[:, 3:3 + cols]
+    _, _, _, perm = routed(gen, tokens, 32, top_k)
+    rows, place = ops.moe_sort(x, perm, top_k)
+    assert rows.numel() * rows.element_size() >= 32 << 20
+    assert same(rows, x[perm.long() // top_k])
+    assert torch.equal(place[perm.long()].long(), torch.arange(tokens * top_k, device=x.device))
+    bad = perm.clone()
+    bad[5], bad[77], bad[-1] = -1, tokens * top_k, 2 ** 31 - 1
+    got, _ = ops.moe_sort(x, bad, top_k)
+    want = x[perm.long() // top_k]
+    want[[5, 77, tokens * top_k - 1]] = 0
+    assert same(got, want)
 
 
 def test_combine_onto_the_residual_itself(gen):

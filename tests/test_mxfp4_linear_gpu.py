@@ -58,7 +58,8 @@ LINEAR = [  # m, n, k: decode and larger tiles, K slices, ragged in each directi
     (1, 1, 32), (1, 16, 64), (2, 33, 96), (3, 8, 14336), (9, 2880, 2880), (16, 70, 128),
     (17, 65, 256), (31, 100, 288), (32, 8192, 672), (1, 8161, 32), (33, 70, 96), (65, 257, 544),
     (77, 4096, 1440), (127, 130, 1056), (129, 63, 4128), (257, 1030, 288), (2933, 525, 544),
-    (833, 4756, 544), (2083, 2856, 1632), (65, 11414, 12448), (520, 2048, 608)]
+    (833, 4756, 544), (2083, 2856, 1632), (65, 11414, 12448), (520, 2048, 608),
+    (16, 8412, 544), (2872, 3, 12608), (3017, 525, 10528)]
 EPILOGUES = [(None, True, False), ("silu", False, True), ("gelu", True, True),
              ("gelu", False, False), (None, False, True)]
 
@@ -93,7 +94,8 @@ def test_linear_of_nothing_is_the_product(gen):
 # m, n, k of dy [m, n] and dx [m, k]
 BACKWARD = [(1, 8, 32), (2, 40, 64), (7, 2880, 2880), (33, 72, 96), (65, 264, 544),
             (77, 4096, 1440), (129, 64, 4128), (300, 1032, 288), (1025, 520, 2048),
-            (2083, 1632, 2848), (64, 14336, 1024), (520, 608, 5024)]
+            (2083, 1632, 2848), (64, 14336, 1024), (520, 608, 5024),
+            (3272, 8, 1056), (2846, 16584, 64), (2832, 14744, 32), (2739, 15568, 32)]
 
 
 @pytest.mark.parametrize("act", [None, "silu", "gelu"])
@@ -193,12 +195,15 @@ def test_experts_gated(gen, m, experts, n, k, kind, act, with_bias, save):
     epi.by_expert(check, offsets.tolist(), x, h, saved if save else h)
 
 
-@pytest.mark.parametrize("act", [None, "gelu"])
-@pytest.mark.parametrize("m,experts,n,k,kind", [
+EXPERTS_BACKWARD = [
     (1, 1, 8, 32, "even"), (4, 32, 96, 64, "even"), (16, 3, 104, 288, "odd"),
     (64, 32, 2880, 1440, "odd"), (100, 256, 136, 160, "odd"), (129, 2, 64, 4128, "even"),
     (256, 8, 776, 544, "odd"), (400, 12, 320, 1440, "even"), (513, 5, 504, 224, "odd"),
-    (700, 3, 2104, 608, "even"), (1000, 9, 96, 2912, "one"), (5000, 255, 288, 128, "odd")])
+    (700, 3, 2104, 608, "even"), (1000, 9, 96, 2912, "one"), (5000, 255, 288, 128, "odd")]
+
+
+@pytest.mark.parametrize("act", [None, "gelu"])
+@pytest.mark.parametrize("m,experts,n,k,kind", EXPERTS_BACKWARD)
 def test_experts_linear_backward(gen, m, experts, n, k, kind, act):
     w = stack(gen, experts, n, k)
     offsets = offsets_of(counts_of(gen, m, experts, kind))
@@ -219,13 +224,16 @@ def test_experts_linear_backward(gen, m, experts, n, k, kind, act):
                                            BF16), "dpre")
 
 
-@pytest.mark.parametrize("save", ["bf16", "q8"])
-@pytest.mark.parametrize("act", ["silu", "clamped"])
-@pytest.mark.parametrize("m,experts,n,k,kind", [
+GATED_BACKWARD = [
     (1, 1, 32, 32, "even"), (4, 32, 96, 64, "even"), (16, 3, 96, 288, "odd"),
     (64, 32, 2880, 1440, "odd"), (100, 256, 160, 160, "odd"), (129, 2, 64, 4128, "even"),
     (256, 8, 768, 544, "odd"), (400, 12, 320, 1440, "even"), (513, 5, 512, 224, "odd"),
-    (700, 3, 2112, 608, "even"), (5000, 255, 288, 128, "odd")])
+    (700, 3, 2112, 608, "even"), (5000, 255, 288, 128, "odd")]
+
+
+@pytest.mark.parametrize("save", ["bf16", "q8"])
+@pytest.mark.parametrize("act", ["silu", "clamped"])
+@pytest.mark.parametrize("m,experts,n,k,kind", GATED_BACKWARD)
 def test_experts_gated_backward(gen, m, experts, n, k, kind, act, save):
     gate, up = stack(gen, experts, n, k), stack(gen, experts, n, k)
     offsets = offsets_of(counts_of(gen, m, experts, kind))
@@ -348,7 +356,8 @@ def test_values_that_are_not_finite_stay_in_their_rows(gen, m, bad):
     w, v = ops.mxfp4_pack(*stack(gen, experts, n, k)), ops.mxfp4_pack(*stack(gen, experts, n, k))
     offsets = torch.tensor([0, m // 2, m // 2, m], dtype=torch.int32, device=gen.device)
     x = normal(gen, m, k).bfloat16()
-    clean = (ops.mxfp4_linear(x, w, n, offsets=offsets), ops.mxfp4_experts_gated(x, offsets, w, v, n))
+    clean = (ops.mxfp4_linear(x, w, n, offsets=offsets),
+             ops.mxfp4_experts_gated(x, offsets, w, v, n))
     row = m // 2 - 1
     x[row] = bad
     spoilt = (ops.mxfp4_linear(x, w, n, offsets=offsets),
@@ -504,7 +513,8 @@ def test_wrapper_refusals(gen):
         lambda: ops.mxfp4_linear(x, ws, n, bias=bias, offsets=offsets),
         lambda: ops.mxfp4_linear(x, w, n, activation="clamped"),
         lambda: ops.mxfp4_linear(x, w, n, activation="relu"),
-        lambda: ops.mxfp4_linear(x, w, n, residual=dy), lambda: ops.mxfp4_linear(x, w, n, save=True),
+        lambda: ops.mxfp4_linear(x, w, n, residual=dy),
+        lambda: ops.mxfp4_linear(x, w, n, save=True),
         lambda: ops.mxfp4_linear(x, w, n, dtype=torch.float16),
         lambda: ops.mxfp4_linear(x, w, n, bias=bias.requires_grad_(True)),
         lambda: ops.mxfp4_linear(x.float().requires_grad_(True).bfloat16(), w, n),
