@@ -205,7 +205,7 @@ constexpr size_t most_tiles(size_t m, size_t experts, size_t rows) {
 // compute units, also where an expert has one row (256 sorted rows over 25 of 32 experts of
 // 2880 x 2880, gated: 41 us, 235 MB at 5.7 TB/s; decode_kernel 50).  Fewer, as for a token or two,
 // leave units without any, and decode_kernel's narrower shares are the quicker: 1 token to 4 of 32
-// experts gated 11.6 us against 15.5, then down 7.7 against 12.8; 2 tokens gated (184 workgroups)
+// experts gated 10.7 us against 15.5, then down 7.7 against 12.8; 2 tokens gated (184 workgroups)
 // 15.9 against 14.4, down (96) 9.8 against 12.8.  It reads a row of x once for each of its
 // workgroups: 16 tokens to 2 of 8 experts 5632 -> 4096 20.5 us against 20.4, 32 tokens 28 against
 // 21.
@@ -231,15 +231,18 @@ inline ExpertsPlan plan_experts(size_t m, size_t experts, size_t n, size_t k, bo
     p.tiles_n = ceil_div(n, gated ? 128 : 256);
     p.decode = !(gated && kept) && p.tiles_n * reached * 9 <= cus * 5 && mean <= 4;
     if (p.decode) {
-        // (wavefronts of four units, whose loads are all in flight at once; two matrices' are
-        // twice as many, and their wavefronts take longer runs: gated 2880 -> 2880 of a token
-        // 11.6 us over 4, 12.3 over 6, 4096 -> 5632 12.8 over 4, 14.1 over 8; down 5632 -> 4096
-        // 8.2 over 12, 9.3 over 6)
-        const size_t units = ceil_div(k, 128);
-        p.shape.wide = !gated && ceil_div(n, 32) * reached >= cus;
-        p.shape.tb = 1;
-        p.shape.waves = unsigned(std::min<size_t>(ceil_div(units, 4), gated ? 4 : 16));
+        // (runs of four units, a batch whose loads are all in flight at once, and where two matrices
+        // are twice as many, of eight: gated 2880 -> 2880 of a token 10.7 us over 3 wavefronts, 11.4
+        // over 4, 12.1 over 6, 2048 -> 768 6.2 over 4, 7.3 over 2; down 5632 -> 4096 8.2 over 11,
+        // 9.3 over 6)
+        const size_t units = ceil_div(k, 128), run = gated && units > 16 ? 8 : 4;
+        p.shape.waves = unsigned(std::min<size_t>(ceil_div(units, run), 16));
         p.shape.units = unsigned(ceil_div(ceil_div(units, p.shape.waves), 2) * 2);
+        // (whole blocks of 32 rows where there is work enough for half as many workgroups, each
+        // counted as a wavefront more than it has: down 2880 -> 2880 of a token 7.9 us against 7.7,
+        // of two 9.8 against 10.9; 5632 -> 4096 of a token 8.1 against 8.7)
+        p.shape.wide = !gated && ceil_div(n, 16) * reached * (p.shape.waves + 1) >= 21 * cus;
+        p.shape.tb = 1;
         p.most = most_tiles(m, experts, 16);
         return p;
     }

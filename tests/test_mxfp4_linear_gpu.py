@@ -121,6 +121,7 @@ def test_linear_backward(gen, m, n, k, act):
 EXPERTS = [  # m, experts, n, k, rows: every kernel, one and no row, odd and long ones
     (1, 1, 1, 32, "even"), (1, 32, 96, 64, "even"), (4, 32, 2880, 2880, "even"),
     (4, 128, 2048, 768, "odd"), (5, 5, 33, 96, "even"), (16, 3, 100, 288, "odd"),
+    (16, 128, 2048, 768, "even"), (14, 64, 2030, 800, "odd"),
     (16, 16, 8192, 96, "odd"), (24, 4, 300, 1056, "odd"), (32, 256, 640, 512, "even"),
     (40, 7, 257, 2080, "one"), (64, 32, 2880, 2880, "odd"), (100, 256, 130, 160, "odd"),
     (129, 2, 64, 4128, "even"), (256, 8, 777, 544, "odd"), (333, 32, 1030, 288, "odd"),
