@@ -694,10 +694,16 @@ def _offsets(offsets: torch.Tensor) -> int:
 
 def _bias(bias: torch.Tensor, name: str, shape: tuple) -> int:
     _no_graph(bias, name)
-    _need(bias, torch.float32, name)
-    if bias.shape != shape:
-        raise ValueError(f"{name}: expected {list(shape)}")
+    if (bias.dtype != torch.float32 or bias.shape != shape or not bias.is_contiguous()
+            or bias.get_device() != _current_device()):
+        raise ValueError(f"{name}: expected a contiguous fp32 tensor of {list(shape)} on the "
+                         "current device")
     return bias.data_ptr()
+
+
+def _here(t: torch.Tensor, name: str) -> None:
+    if t.get_device() != _current_device():
+        raise ValueError(f"{name}: expected on the current device")
 
 
 def _stack(packed: torch.Tensor, function: str, experts: int, rows: int, cols: int,
@@ -743,17 +749,16 @@ def mxfp4_linear(x: torch.Tensor, packed: torch.Tensor, n_out: int,
     b = add = None
     if bias is not None:
         b = _bias(bias, "bias", (n_out,) if table is None else (experts, n_out))
-        _stream_for(bias)
     add_stride = 0
     if residual is not None:
         _no_graph(residual, "residual")
         add, add_stride = residual.data_ptr(), _output(residual, m, n_out, dtype, "residual")
-        _stream_for(residual)
+        _here(residual, "residual")
     if out is None:
         y_stride, out = n_out, x.new_empty(m, n_out, dtype=dtype)
     else:
         y_stride = _output(out, m, n_out, dtype, "out")
-        _stream_for(out)
+        _here(out, "out")
     saved = x.new_empty(m, n_out) if save else None
     scratch = _scratch(size, x.device) if size else None
     call("kdq_mxfp4_linear", x.data_ptr(), stride, m, table, experts, w, n_out, k, b, act, add,
@@ -836,12 +841,11 @@ def mxfp4_experts_gated(x: torch.Tensor, offsets: torch.Tensor, gate: torch.Tens
     if gate_bias is not None:
         bg = _bias(gate_bias, "gate_bias", (experts, n_out))
         bu = _bias(up_bias, "up_bias", (experts, n_out))
-        _stream_for(gate_bias, up_bias)
     if out is None:
         h_stride, out = n_out, x.new_empty(m, n_out)
     else:
         h_stride = _output(out, m, n_out, _BF16, "out")
-        _stream_for(out)
+        _here(out, "out")
     saved = kept = codes = scales = None
     if save == "bf16":
         saved = x.new_empty(m, 2 * n_out)
@@ -984,12 +988,12 @@ def moe_combine(rows: torch.Tensor, weights: torch.Tensor, place: torch.Tensor,
     if residual is not None:
         _no_graph(residual, "residual")
         add, add_stride = residual.data_ptr(), _output(residual, tokens, cols, dtype, "residual")
-        _stream_for(residual)
+        _here(residual, "residual")
     if out is None:
         y_stride, out = cols, rows.new_empty(tokens, cols, dtype=dtype)
     else:
         y_stride = _output(out, tokens, cols, dtype, "out")
-        _stream_for(out)
+        _here(out, "out")
     call("kdq_moe_combine", kind, rows.data_ptr(), stride, at, weights.data_ptr(), tokens, cols,
          top_k, _TYPES[dtype], add, add_stride, out.data_ptr(), y_stride, stream)
     return out
