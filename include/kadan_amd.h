@@ -552,7 +552,7 @@ int kdq_mxfp4_experts_gated_backward(const uint16_t* dh_bf16, size_t dh_stride, 
                                      size_t dx_stride, void* stream);
 
 /* ---- a mixture layer in pieces, with their gradients, around kdq_moe_route and the products
- * below (the reference runs the layer on the host and has no gradients:
+ * above (the reference runs the layer on the host and has no gradients:
  * IW/src/models/text/qwen_layers.cpp:378-492).  Slot token * top_k + i is a token's i-th
  * selection; `perm` is kdq_moe_route's (a permutation of the slots, those of expert 0 first).
  * Rows are of type KDQ_F32, KDQ_F16 or KDQ_BF16, any number of values apart, aligned to their
@@ -561,7 +561,8 @@ int kdq_mxfp4_experts_gated_backward(const uint16_t* dh_bf16, size_t dh_stride, 
  * different streams may overlap, and every call may be captured. */
 
 /* rows[p] = x[perm[p] / top_k] for the tokens * top_k positions p, and place[perm[p]] = p.  An
- * entry of perm that is no slot gives a row of zeros and no place. */
+ * entry of perm that is no slot gives a row of zeros and no place; perm may not name a slot
+ * twice. */
 int kdq_moe_sort(int type, const void* x, size_t x_stride, size_t tokens, size_t cols,
                  size_t top_k, const int32_t* perm, void* rows, size_t rows_stride,
                  int32_t* place, void* stream);

@@ -369,6 +369,59 @@ def test_values_that_are_not_finite_stay_in_their_rows(gen, m, bad):
         assert not bool(torch.isfinite(b[row].float()).all())
 
 
+@pytest.mark.parametrize("m", [4, 40, 500])
+@pytest.mark.parametrize("k", [352, 768, 2080])
+def test_a_block_without_a_scale_reaches_its_own_results_only(gen, m, k):
+    """Scale byte 255 (NaN) in one row of one expert's matrix."""
+    experts, n = 3, 96
+    (blocks, scales), other = stack(gen, experts, n, k), ops.mxfp4_pack(*stack(gen, experts, n, k))
+    offsets = torch.tensor([0, m // 4, m // 2, m], dtype=torch.int32, device=gen.device)
+    x = normal(gen, m, k).bfloat16()
+    for block in (0, k // 64, k // 32 - 1):
+        w = ops.mxfp4_pack(blocks, scales)
+        bad = scales.clone()
+        bad[1, 37, block] = 255
+        v = ops.mxfp4_pack(blocks, bad)
+        hit = torch.zeros(m, n, dtype=torch.bool, device=gen.device)
+        hit[m // 4:m // 2, 37] = True
+        for f in (lambda p: ops.mxfp4_linear(x, p, n, offsets=offsets),
+                  lambda p: ops.mxfp4_experts_gated(x, offsets, p, other, n),
+                  lambda p: ops.mxfp4_experts_gated(x, offsets, other, p, n)):
+            want, got = f(w), f(v)
+            assert torch.equal(got[~hit], want[~hit]) and bool(torch.isnan(got[hit]).all())
+
+
+def test_two_calls_at_once(gen):
+    """Calls on two streams share nothing."""
+    experts, n, k, top_k = 8, 160, 288, 2
+    w = ops.mxfp4_pack(*stack(gen, experts, n, k))
+    turned = ops.mxfp4_pack(*stack(gen, experts, n, k), transposed=True)
+    batches = []
+    for tokens in (7, 300):
+        x = normal(gen, tokens, k).bfloat16()
+        _, weights, offsets, perm = ops.moe_route(normal(gen, tokens, experts), top_k)
+        batches.append((x, weights, offsets, perm))
+
+    def chain(x, weights, offsets, perm):
+        rows, place = ops.moe_sort(x, perm, top_k)
+        y = ops.mxfp4_linear(rows, w, n, activation="gelu", dtype=BF16, offsets=offsets)
+        d, dw = ops.moe_combine_backward(ops.moe_combine(y, weights, place), y, weights, place)
+        return y, d, dw, ops.mxfp4_linear_backward(d, turned, k, offsets=offsets)[0]
+
+    want = [chain(*b) for b in batches]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(8):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(chain(*batches[i]))
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        for run in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(run, want[i]))
+
+
 @pytest.mark.parametrize("m", [4, 64, 700])
 def test_on_another_stream_and_captured(gen, m):
     """A graph of the experts' projections and their gradients, replayed with other inputs, and
