@@ -907,19 +907,24 @@ def mxfp4_experts_gated_backward(dh: torch.Tensor, offsets: torch.Tensor, saved,
     return out, dgu
 
 
+# (A few tokens' rows take 2-4 us on the device, their wrappers more than that: so few steps.)
+_F32, _I32 = torch.float32, torch.int32
+
+
 def _rows_of(t: torch.Tensor, name: str) -> tuple[int, int]:
     """KDQ type of fp32, fp16 or bf16 rows, and the values from row to row."""
-    kind = _TYPES.get(t.dtype)
+    dtype = t.dtype
+    kind = _TYPES.get(dtype)
     if kind is None:
         raise ValueError(f"{name}: expected fp32, fp16 or bf16 rows")
-    return kind, _row_stride(t, t.dtype, name, 1)
+    return kind, _row_stride(t, dtype, name, 1)
 
 
-def _slots(t: torch.Tensor, slots: int, name: str, dtype=torch.int32) -> int:
-    """A contiguous tensor of a value per slot."""
-    _need(t, dtype, name)
-    if t.numel() != slots:
-        raise ValueError(f"{name}: expected {slots} values, one per selection")
+def _slots(t: torch.Tensor, slots: int, name: str) -> int:
+    """A contiguous int32 tensor of a value per slot."""
+    if t.dtype != _I32 or not t.is_cuda or not t.is_contiguous() or t.numel() != slots:
+        raise ValueError(f"{name}: expected a contiguous int32 device tensor of {slots} values, "
+                         "one per selection")
     return t.data_ptr()
 
 
@@ -956,10 +961,10 @@ def moe_sort_backward(drows: torch.Tensor, place: torch.Tensor, top_k: int) -> t
     return dx
 
 
-def _weights(weights: torch.Tensor, name: str) -> tuple[int, int]:
-    _need(weights, torch.float32, name)
-    if weights.dim() != 2:
-        raise ValueError(f"{name}: expected [tokens, top_k]")
+def _weights(weights: torch.Tensor) -> tuple[int, int]:
+    if (weights.dtype != _F32 or not weights.is_cuda or weights.dim() != 2
+            or not weights.is_contiguous()):
+        raise ValueError("weights: expected a contiguous fp32 device tensor [tokens, top_k]")
     return weights.shape
 
 
@@ -974,7 +979,7 @@ def moe_combine(rows: torch.Tensor, weights: torch.Tensor, place: torch.Tensor,
     _no_graph(rows, "rows")
     _no_graph(weights, "weights")
     kind, stride = _rows_of(rows, "rows")
-    tokens, top_k = _weights(weights, "weights")
+    tokens, top_k = _weights(weights)
     slots, cols = rows.shape
     if slots != tokens * top_k:
         raise ValueError("rows: expected one per weight")
@@ -1009,7 +1014,7 @@ def moe_combine_backward(dy: torch.Tensor, rows: torch.Tensor, weights: torch.Te
     dy_kind, dy_stride = _rows_of(dy, "dy")
     if dy_kind not in (kind, 0):
         raise ValueError("dy: the rows' type or fp32")
-    tokens, top_k = _weights(weights, "weights")
+    tokens, top_k = _weights(weights)
     slots, cols = rows.shape
     if slots != tokens * top_k or dy.shape != (tokens, cols):
         raise ValueError("expected rows [tokens * top_k, cols] and dy [tokens, cols]")
@@ -1027,11 +1032,11 @@ def moe_route_backward(idx: torch.Tensor, weights: torch.Tensor, dweights: torch
     """The gradient of moe_route's weights: idx int32, weights and their gradient fp32, each
     [tokens, top_k] -> dlogits fp32 [tokens, experts] (kdq_moe_route_backward)."""
     _no_graph(dweights, "dweights")
-    tokens, top_k = _weights(weights, "weights")
-    _need(idx, torch.int32, "idx")
-    _need(dweights, torch.float32, "dweights")
-    if idx.shape != weights.shape or dweights.shape != weights.shape:
-        raise ValueError("idx, weights and dweights: expected one shape")
+    tokens, top_k = _weights(weights)
+    if (idx.dtype != _I32 or dweights.dtype != _F32 or idx.shape != weights.shape
+            or dweights.shape != weights.shape or not idx.is_contiguous()
+            or not dweights.is_contiguous()):
+        raise ValueError("expected contiguous idx int32 and dweights fp32 of the weights' shape")
     stream = _stream_for(idx, weights, dweights)
     dlogits = weights.new_empty(tokens, experts)
     call("kdq_moe_route_backward", idx.data_ptr(), weights.data_ptr(), dweights.data_ptr(), tokens,
