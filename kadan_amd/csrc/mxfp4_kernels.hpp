@@ -870,12 +870,14 @@ __device__ __forceinline__ unsigned lanes_up_to(unsigned v) {
 
 constexpr unsigned kMaxExperts = 256;
 
-// A quad of experts of each lane: their first rows and the tiles of each.
-struct Tiles {
+// A quad of experts of each lane: their rows, and how many tiles of `rows` they make: in the low
+// half of a word, and in the high half those whose last tile has at most half the rows (where
+// HALVES tells them apart: it is then in no low half).
+template <unsigned ROWS, bool HALVES> struct Tiles {
     unsigned first[4], end[4], tiles[4], before, total;
 
     // Offsets are taken as they are, but for those outside of the rows (m of them).
-    __device__ __forceinline__ Tiles(const Stack& s, unsigned m, unsigned rows_of_tile) {
+    __device__ __forceinline__ Tiles(const Stack& s, unsigned m) {
         const unsigned lane = threadIdx.x % 64;
         unsigned at[5], sum = 0;
 #pragma unroll
@@ -885,7 +887,10 @@ struct Tiles {
         for (unsigned j = 0; j < 4; ++j) {  // (past the last expert: no rows)
             first[j] = at[j];
             end[j] = max(at[j], at[j + 1]);
-            tiles[j] = (end[j] - first[j] + rows_of_tile - 1) / rows_of_tile;
+            const unsigned rows = end[j] - first[j];
+            tiles[j] = (rows + (HALVES ? ROWS / 2 - 1 : ROWS - 1)) / ROWS;
+            if (HALVES && rows > tiles[j] * ROWS)
+                tiles[j] |= 1u << 16;
             sum += tiles[j];
         }
         const unsigned through = lanes_up_to(sum);
@@ -893,24 +898,37 @@ struct Tiles {
         total = unsigned(__builtin_amdgcn_readlane(int(through), 63));
     }
 
+    __device__ __forceinline__ unsigned whole() const {
+        return total & 0xffffu;
+    }
+    __device__ __forceinline__ unsigned halves() const {
+        return total >> 16;
+    }
+
     struct Place {
-        unsigned expert, first, end, before, tiles;  // rows; tiles before the expert's, and its
+        // rows of the expert from its first such tile on; such tiles before the expert's, and its
+        unsigned expert, first, end, before, tiles;
     };
 
-    // The expert whose tiles the tile `t` (below total) is among.
-    __device__ __forceinline__ Place of(unsigned t) const {
-        unsigned from = before, e = 0, lo = 0, hi = 0, b = 0, n = 0;
+    // The expert whose whole tiles (or halves) number `t` is among; no tiles where there is none,
+    // as offsets that decrease might have it.
+    __device__ __forceinline__ Place of(unsigned t, bool half) const {
+        const unsigned shift = half ? 16 : 0;
+        unsigned from = before >> shift & 0xffffu, e = 0, lo = 0, hi = 0, b = 0, n = 0;
         bool mine = false;
 #pragma unroll
         for (unsigned j = 0; j < 4; ++j) {
-            if (t >= from && t < from + tiles[j]) {
+            const unsigned count = tiles[j] >> shift & 0xffffu;
+            if (t >= from && t < from + count) {
                 mine = true;
                 e = 4 * (threadIdx.x % 64) + j;
-                lo = first[j], hi = end[j], b = from, n = tiles[j];
+                lo = first[j] + (half ? (tiles[j] & 0xffffu) * ROWS : 0);
+                hi = end[j], b = from, n = count;
             }
-            from += tiles[j];
+            from += count;
         }
-        const int lane = int(__builtin_ctzll(__builtin_amdgcn_ballot_w64(mine)));
+        const uint64_t who = __builtin_amdgcn_ballot_w64(mine);
+        const int lane = who ? int(__builtin_ctzll(who)) : 0;
         const auto read = [&](unsigned v) {
             return unsigned(__builtin_amdgcn_readlane(int(v), lane));
         };
@@ -967,10 +985,10 @@ __global__ __launch_bounds__(1024) void decode_kernel(Decode a) {
     unsigned first_row = blockIdx.y * (16 * TB);
     size_t expert = 0;
     if constexpr (of_experts(OUT)) {
-        const Tiles list(a.stack, a.out.m, 16 * TB);
-        if (blockIdx.y >= list.total)
+        const Tiles<16 * TB, false> list(a.stack, a.out.m);
+        const auto p = list.of(blockIdx.y, false);
+        if (!p.tiles)
             return;
-        const auto p = list.of(blockIdx.y);
         first_row = p.first + (blockIdx.y - p.before) * (16 * TB);
         move_to<OUT>(a.out, p.expert, first_row, min(p.end - first_row, 16u * TB));
         a.x += size_t(first_row) * a.x_stride;
@@ -1377,12 +1395,24 @@ __global__ __launch_bounds__(512, (shares_unit<TT, OPS> ? 4 : 2)) void gemm_kern
     size_t expert = 0;
     unsigned tile_m, tile_n;
     if constexpr (of_experts(OUT)) {
-        const Tiles list(a.stack, a.out.m, kRows);
-        tiles = list.total * a.tiles_n;
-        if (blockIdx.x / 8 >= tiles / 8 + (xcd < tiles % 8)) [[unlikely]]
+        // (whole tiles first, then the halves, so that what is left at a launch's end is small: an
+        // XCD has its share of either: 2048 rows of 32 experts of 2880 x 2880 gated 91 us against 97,
+        // 4096 rows 146 against 156)
+        const Tiles<kRows, (TT > 1)> list(a.stack, a.out.m);
+        const auto share = [&](unsigned n) {
+            return n / 8 + (xcd < n % 8);
+        };
+        unsigned turn = blockIdx.x / 8;
+        tiles = list.whole() * a.tiles_n;
+        const bool half = turn >= share(tiles);
+        if (half) {
+            turn -= share(tiles);
+            tiles = list.halves() * a.tiles_n;
+        }
+        const unsigned tile = xcd * (tiles / 8) + min(xcd, tiles % 8) + turn;
+        const auto p = list.of(tile / a.tiles_n, half);
+        if (turn >= share(tiles) || !p.tiles) [[unlikely]]
             return;
-        const unsigned tile = xcd * (tiles / 8) + min(xcd, tiles % 8) + blockIdx.x / 8;
-        const auto p = list.of(tile / a.tiles_n);
         const unsigned within = tile - p.before * a.tiles_n;
         const unsigned first = p.first + within % p.tiles * kRows;
         tile_m = 0;
@@ -1431,7 +1461,8 @@ __global__ __launch_bounds__(512, (shares_unit<TT, OPS> ? 4 : 2)) void gemm_kern
         const unsigned from = b * 8 + seg;
         x_at[j] = int(row * a.x_stride + from * 16 +
                       (OPS == kTransposed && set ? a.x_second : 0));
-        x_limit[j] = e > from ? e - from : 0;
+        // (the experts' tiles are seldom full: rows past the last are zeros)
+        x_limit[j] = e > from && (!of_experts(OUT) || place < rows) ? e - from : 0;
     }
     // kFp4: the scales of four chunks are 32 bytes of a row, copied as the nine dwords that
     // hold them (a row's bytes start anywhere; the buffer ends with the dword of the last one)
@@ -2017,8 +2048,10 @@ int launch_gemm(const Gemm& a, const Plan& p, hipStream_t st) {
             configured.fetch_or(bit, std::memory_order_relaxed);
         }
     }
-    // (the experts': p.tiles_m is the most that they may have)
-    hipLaunchKernelGGL(f, dim3(p.tiles_n * p.tiles_m, p.slices), dim3(512), kLds, st, a);
+    // (the experts': p.tiles_m is the most that they may have, and eight XCDs' shares of two kinds
+    // are rounded up)
+    const unsigned tiles = p.tiles_n * p.tiles_m + (of_experts(OUT) ? 16 : 0);
+    hipLaunchKernelGGL(f, dim3(tiles, p.slices), dim3(512), kLds, st, a);
     KDQ_HIP(hipGetLastError());
     return KDQ_OK;
 }

@@ -46,7 +46,7 @@ size_t offset_bytes(const int32_t* offsets, size_t experts) {
 
 // (a launch's threads are counted in 32 bits)
 bool launches(const ExpertsPlan& p) {
-    return p.decode ? p.most <= 65535 : p.most * p.tiles_n <= UINT32_MAX / 512;
+    return p.decode ? p.most <= 65535 : p.most * p.tiles_n + 16 <= UINT32_MAX / 512;
 }
 
 Gemm gemm_of(const uint8_t* w0, const uint8_t* w1, const uint16_t* x, size_t x_stride,
@@ -209,7 +209,7 @@ extern "C" int kdq_mxfp4_linear_backward(const uint16_t* dy_bf16, size_t dy_stri
     Plan p{};
     ExpertsPlan e{};
     if (offsets) {
-        e = plan_experts_backward(m, experts, k, false);
+        e = plan_experts_backward(m, experts, k);
         if (!launches(e))
             return KDQ_ERR_SHAPE;
     } else {
@@ -316,7 +316,7 @@ extern "C" int kdq_mxfp4_experts_gated_backward(
                         {up_transposed, bytes_of(f, experts)}};
     if (any_overlap(out, in))
         return KDQ_ERR_ALIAS;
-    const ExpertsPlan p = plan_experts_backward(m, experts, k, true);
+    const ExpertsPlan p = plan_experts_backward(m, experts, k);
     if (!launches(p))
         return KDQ_ERR_SHAPE;
     const auto st = static_cast<hipStream_t>(stream);

@@ -212,9 +212,11 @@ constexpr size_t most_tiles(size_t m, size_t experts, size_t rows) {
 //
 // Tiles of 64 rows (two workgroups of either share a compute unit; a half that is empty is not
 // multiplied) decode a weight once for twice the rows, tiles of 32 are more, and fill the last
-// round of workgroups better: 2048 rows of 32 experts of 2880 x 2880 gated 97 us against 101, down
-// 60 against 54, back 135 against 137 and 66 against 64; 8192 rows of 128 of 2048 x 768 70 against
-// 73, 52 against 54, 97 against 110 and 46 against 46; 256 rows of the 32 gated 73 against 64.
+// round of workgroups better.  Rows an expert, in us over tiles of 32 and of 64: 32 experts of 2880
+// x 2880 gated 16 59, 57; 32 70, 73; 64 100, 91; down 16 33, 37; 32 40, 39; 64 52, 56; 128 83, 80;
+// their gradients gated 16 76, 83; 32 100, 89; down 16 32, 38; 32 49, 42; 64 65, 62; 128 experts of
+// 2048 x 768 gated 32 53, 52; 64 73, 67; down (K of 768, where a workgroup's fixed part is the
+// larger) 32 38, 38; 64 54, 50; gradients gated 16 55, 54; 32 71, 67; down 16 24, 27; 32 34, 29.
 // Tiles of 96 and 128 rows have a unit to themselves and lose by 5 to 50 % up to 512 rows an
 // expert; at 2048 they are within 2 % of those of 64.
 struct ExpertsPlan {
@@ -246,15 +248,14 @@ inline ExpertsPlan plan_experts(size_t m, size_t experts, size_t n, size_t k, bo
         p.most = most_tiles(m, experts, 16);
         return p;
     }
-    p.tt = mean < (gated ? 48 : 96) ? 1 : 2;
+    p.tt = mean < (gated || k <= 1536 ? 48 : 96) ? 1 : 2;
     p.most = most_tiles(m, experts, size_t(p.tt) * 32);
     return p;
 }
 
-// (`gated`: two matrices)
-inline ExpertsPlan plan_experts_backward(size_t m, size_t experts, size_t k, bool gated) {
+inline ExpertsPlan plan_experts_backward(size_t m, size_t experts, size_t k) {
     ExpertsPlan p{};
-    p.tt = m / std::min(experts, m) < (gated ? 48 : 80) ? 1 : 2;
+    p.tt = m / std::min(experts, m) < 24 ? 1 : 2;
     p.tiles_n = ceil_div(k, 256);
     p.most = most_tiles(m, experts, size_t(p.tt) * 32);
     return p;

@@ -1,6 +1,6 @@
 // Prints what kadan_amd/csrc/mxfp4_plan.hpp picks for the calls on standard input, one a line:
 //   linear m n k | back m n k | experts m experts n k gated kept |
-//   experts_back m experts n k gated | tiles m experts rows
+//   experts_back m experts n k 0 | tiles m experts rows
 // as "decode wide staged tb", "gemm tt split sliced", "experts decode wide", "experts gemm tt" or
 // a number of tiles, on `argv[1]` compute units.
 #include "mxfp4_plan.hpp"
@@ -36,7 +36,7 @@ int main(int, char** argv) {
         if (path == "experts")
             std::cin >> kept;
         const ExpertsPlan p = path == "experts" ? plan_experts(m, a, b, c, gated, kept, cus)
-                                                : plan_experts_backward(m, a, c, gated);
+                                                : plan_experts_backward(m, a, c);
         if (p.decode)
             std::cout << "experts decode " << p.shape.wide << '\n';
         else

@@ -46,8 +46,8 @@ TESTED = {
     ("experts", False, False): experts("experts", sizes.EXPERTS, False, False),
     ("experts", True, False): experts("experts", sizes.GATED, True, False),
     ("experts", True, True): experts("experts", sizes.GATED, True, True),
-    ("experts_back", False): experts("experts_back", sizes.EXPERTS_BACKWARD, False),
-    ("experts_back", True): experts("experts_back", sizes.GATED_BACKWARD, True),
+    ("experts_back", 0): experts("experts_back", sizes.EXPERTS_BACKWARD, 0),
+    ("experts_back", 1): experts("experts_back", sizes.GATED_BACKWARD, 0),
 }
 
 
