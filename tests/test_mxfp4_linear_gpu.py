@@ -348,6 +348,47 @@ def test_strided_rows_and_given_outputs(gen, m):
         assert torch.equal(dx, want) and torch.equal(dpre, dwant)
 
 
+@pytest.mark.parametrize("m", [6, 100, 700])
+def test_strided_rows_of_experts(gen, m):
+    experts, n, k = 4, 96, 160
+    gate, up, down = stack(gen, experts, n, k), stack(gen, experts, n, k), stack(gen, experts, k, n)
+    fwd = [ops.mxfp4_pack(*s) for s in (gate, up, down)]
+    back = [ops.mxfp4_pack(*s, transposed=True) for s in (gate, up, down)]
+    padded = torch.zeros(experts + 2, dtype=torch.int32, device=gen.device)
+    padded[1:] = offsets_of(counts_of(gen, m, experts, "odd"))
+    offsets = padded[1:]  # from any element on
+    x = normal(gen, m, 2 * k).bfloat16()[:, 24:24 + k]
+    around = normal(gen, m, n + 9).bfloat16()
+    before, h = around.clone(), around[:, 5:5 + n]
+    ops.mxfp4_experts_gated(x, offsets, fwd[0], fwd[1], n, out=h)
+    want = ops.mxfp4_experts_gated(x.contiguous(), offsets.clone(), fwd[0], fwd[1], n)
+    assert torch.equal(h, want)
+    assert torch.equal(around[:, :5], before[:, :5])
+    assert torch.equal(around[:, 5 + n:], before[:, 5 + n:])
+    for dtype in (F32, BF16):
+        residual = normal(gen, m, k + 3).to(dtype)[:, 2:2 + k]
+        y = normal(gen, m, k + 5).to(dtype)[:, 1:1 + k]
+        ops.mxfp4_linear(want, fwd[2], k, residual=residual, dtype=dtype, offsets=offsets, out=y)
+        plain = ops.mxfp4_linear(want, fwd[2], k, residual=residual.contiguous(), dtype=dtype,
+                                 offsets=offsets)
+        assert torch.equal(y, plain)
+        same = residual.contiguous()
+        ops.mxfp4_linear(want, fwd[2], k, residual=same, dtype=dtype, offsets=offsets, out=same)
+        assert torch.equal(same, plain)
+    dy = normal(gen, m, 2 * k).bfloat16()[:, 8:8 + k]
+    dh = normal(gen, m, n + 11).bfloat16()[:, 3:3 + n]
+    ops.mxfp4_linear_backward(dy, back[2], n, offsets=offsets, out=dh)
+    plain, _ = ops.mxfp4_linear_backward(dy.contiguous(), back[2], n, offsets=offsets)
+    assert torch.equal(dh, plain)
+    saved = normal(gen, m, 2 * n).bfloat16()
+    wide = normal(gen, m, n + 8).bfloat16()
+    wide[:, 8:] = plain
+    dx = normal(gen, m, k + 1).bfloat16()[:, 1:]
+    ops.mxfp4_experts_gated_backward(wide[:, 8:], offsets, saved, back[0], back[1], k, out=dx)
+    plain, _ = ops.mxfp4_experts_gated_backward(plain, offsets, saved, back[0], back[1], k)
+    assert torch.equal(dx, plain)
+
+
 @pytest.mark.parametrize("m", [4, 500])
 @pytest.mark.parametrize("bad", [float("inf"), float("nan")])
 def test_values_that_are_not_finite_stay_in_their_rows(gen, m, bad):
