@@ -913,11 +913,12 @@ _F32, _I32 = torch.float32, torch.int32
 
 def _rows_of(t: torch.Tensor, name: str) -> tuple[int, int]:
     """KDQ type of fp32, fp16 or bf16 rows, and the values from row to row."""
-    dtype = t.dtype
-    kind = _TYPES.get(dtype)
+    kind = _TYPES.get(t.dtype)
     if kind is None:
         raise ValueError(f"{name}: expected fp32, fp16 or bf16 rows")
-    return kind, _row_stride(t, dtype, name, 1)
+    if t.is_contiguous() and t.dim() == 2:
+        return kind, t.shape[1]
+    return kind, _row_stride(t, t.dtype, name, 1)
 
 
 def _slots(t: torch.Tensor, slots: int, name: str) -> int:
@@ -933,13 +934,14 @@ def moe_sort(x: torch.Tensor, perm: torch.Tensor, top_k: int):
     rows [tokens * top_k, cols], rows[p] = x[perm[p] // top_k], and place int32
     [tokens * top_k], place[perm[p]] = p (kdq_moe_sort).  Nothing is recorded for autograd: its
     backward pass is moe_sort_backward."""
-    _no_graph(x, "x")
+    if x.requires_grad:
+        _no_graph(x, "x")
     kind, stride = _rows_of(x, "x")
     tokens, cols = x.shape
     slots = tokens * top_k
     order = _slots(perm, slots, "perm")
     stream = _stream_for(x, perm)
-    rows, place = x.new_empty(slots, cols), perm.new_empty(slots)
+    rows, place = x.new_empty(slots, cols), torch.empty_like(perm)
     call("kdq_moe_sort", kind, x.data_ptr(), stride, tokens, cols, top_k, order, rows.data_ptr(),
          cols, place.data_ptr(), stream)
     return rows, place
@@ -948,7 +950,8 @@ def moe_sort(x: torch.Tensor, perm: torch.Tensor, top_k: int):
 def moe_sort_backward(drows: torch.Tensor, place: torch.Tensor, top_k: int) -> torch.Tensor:
     """The gradient of moe_sort: drows [tokens * top_k, cols] -> dx [tokens, cols] of its type,
     each token's rows summed (kdq_moe_sort_backward)."""
-    _no_graph(drows, "drows")
+    if drows.requires_grad:
+        _no_graph(drows, "drows")
     kind, stride = _rows_of(drows, "drows")
     slots, cols = drows.shape
     if top_k < 1 or slots % top_k:
@@ -976,8 +979,10 @@ def moe_combine(rows: torch.Tensor, weights: torch.Tensor, place: torch.Tensor,
     [tokens, top_k], place from moe_sort -> y [tokens, cols] of the rows' type or fp32
     (``dtype``; the residual's, and ``out`` may be the residual itself) (kdq_moe_combine).
     Nothing is recorded for autograd: its backward pass is moe_combine_backward."""
-    _no_graph(rows, "rows")
-    _no_graph(weights, "weights")
+    if rows.requires_grad:
+        _no_graph(rows, "rows")
+    if weights.requires_grad:
+        _no_graph(weights, "weights")
     kind, stride = _rows_of(rows, "rows")
     tokens, top_k = _weights(weights)
     slots, cols = rows.shape
@@ -991,7 +996,8 @@ def moe_combine(rows: torch.Tensor, weights: torch.Tensor, place: torch.Tensor,
     stream = _stream_for(rows, weights, place)
     add, add_stride = None, 0
     if residual is not None:
-        _no_graph(residual, "residual")
+        if residual.requires_grad:
+            _no_graph(residual, "residual")
         add, add_stride = residual.data_ptr(), _output(residual, tokens, cols, dtype, "residual")
         _here(residual, "residual")
     if out is None:
@@ -1009,7 +1015,8 @@ def moe_combine_backward(dy: torch.Tensor, rows: torch.Tensor, weights: torch.Te
     """The gradients of moe_combine: dy [tokens, cols] (the rows' type or fp32) and its rows,
     weights and place -> drows [tokens * top_k, cols] of the rows' type and dweights fp32
     [tokens, top_k] (kdq_moe_combine_backward).  The residual's gradient is dy."""
-    _no_graph(dy, "dy")
+    if dy.requires_grad:
+        _no_graph(dy, "dy")
     kind, stride = _rows_of(rows, "rows")
     dy_kind, dy_stride = _rows_of(dy, "dy")
     if dy_kind not in (kind, 0):
@@ -1031,7 +1038,8 @@ def moe_route_backward(idx: torch.Tensor, weights: torch.Tensor, dweights: torch
                        experts: int) -> torch.Tensor:
     """The gradient of moe_route's weights: idx int32, weights and their gradient fp32, each
     [tokens, top_k] -> dlogits fp32 [tokens, experts] (kdq_moe_route_backward)."""
-    _no_graph(dweights, "dweights")
+    if dweights.requires_grad:
+        _no_graph(dweights, "dweights")
     tokens, top_k = _weights(weights)
     if (idx.dtype != _I32 or dweights.dtype != _F32 or idx.shape != weights.shape
             or dweights.shape != weights.shape or not idx.is_contiguous()
