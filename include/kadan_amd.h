@@ -508,8 +508,8 @@ int kdq_mxfp4_experts_pack_transposed(const uint8_t* blocks, const uint8_t* scal
  * activation (KDQ_ACT_NONE, _SILU or _GELU) and residual in fp32, one rounding.  bias fp32 [n] or
  * null; residual of y's type, rows residual_stride apart, or null: y may be the residual itself
  * (with its stride).  kept_bf16 (or null): pre as bf16 [m x n], 2-byte aligned, for the backward pass.
- * Dense where offsets is null (experts = 1); of experts: bias [experts x n], and no workspace. */
-size_t kdq_mxfp4_linear_workspace(size_t m, size_t n, size_t k);
+ * Dense where offsets is null (experts = 1; the workspace's: 0); of experts: bias [experts x n]. */
+size_t kdq_mxfp4_linear_workspace(size_t m, size_t experts, size_t n, size_t k);
 int kdq_mxfp4_linear(const uint16_t* x_bf16, size_t x_stride, size_t m, const int32_t* offsets,
                      size_t experts, const uint8_t* packed, size_t n, size_t k, const float* bias,
                      int activation, const void* residual, size_t residual_stride, int type,
@@ -520,9 +520,9 @@ int kdq_mxfp4_linear(const uint16_t* x_bf16, size_t x_stride, size_t m, const in
  * kept_bf16, and dx [m x k] bf16 = dpre W, the products of the rounded dpre exact and their sums
  * fp32.  (KDQ_ACT_NONE: dpre is dy; kept_bf16 and dpre are null.)  The bias's gradient is the sum
  * of dpre's rows, the residual's is dy.  Weights from kdq_mxfp4_pack_transposed, or
- * kdq_mxfp4_experts_pack_transposed with offsets; n % 8 == 0; of experts: no workspace, dx of rows
- * that no expert has is left as it was (dpre is not). */
-size_t kdq_mxfp4_linear_backward_workspace(size_t m, size_t n, size_t k);
+ * kdq_mxfp4_experts_pack_transposed with offsets; n % 8 == 0; of experts: dx of rows that no expert
+ * has is left as it was (dpre is not); the workspace's `experts` is 0 for dense calls. */
+size_t kdq_mxfp4_linear_backward_workspace(size_t m, size_t experts, size_t n, size_t k);
 int kdq_mxfp4_linear_backward(const uint16_t* dy_bf16, size_t dy_stride, size_t m,
                               const int32_t* offsets, size_t experts, const uint16_t* kept_bf16,
                               int activation, const uint8_t* transposed, size_t n, size_t k,
@@ -532,24 +532,29 @@ int kdq_mxfp4_linear_backward(const uint16_t* dy_bf16, size_t dy_stride, size_t 
 /* kdq_mxfp4_gated of experts, with biases: g = x Wg^T + gate_bias, u = x Wu^T + up_bias (both
  * fp32 [experts x n], or both null) and h [m x n] bf16 = silu(g) u (KDQ_ACT_SILU) or, with
  * g' = min(g, 7) and u' = u between -7 and 7, g' sigmoid(1.702 g') (u' + 1) (KDQ_ACT_CLAMPED).
- * n % 32 == 0.  The pre-activations g and u may be kept as kdq_mxfp4_gated keeps them. */
+ * n % 32 == 0.  The pre-activations g and u may be kept as kdq_mxfp4_gated keeps them (workspace
+ * with kept = 1). */
+size_t kdq_mxfp4_experts_gated_workspace(size_t m, size_t experts, size_t n, size_t k, int kept);
 int kdq_mxfp4_experts_gated(const uint16_t* x_bf16, size_t x_stride, size_t m,
                             const int32_t* offsets, size_t experts, const uint8_t* gate_packed,
                             const uint8_t* up_packed, size_t n, size_t k, const float* gate_bias,
                             const float* up_bias, int activation, uint16_t* h_bf16,
                             size_t h_stride, uint16_t* kept_bf16, int8_t* kept_q8,
-                            float* kept_scales, void* stream);
+                            float* kept_scales, void* workspace, size_t workspace_bytes,
+                            void* stream);
 
 /* Its backward pass over frozen weights, as kdq_mxfp4_gated_backward (the clamped form's dg is 0
  * where g is above 7, its du where |u| is).  dx of rows that no expert has is left as it was (dgu
  * is not). */
+size_t kdq_mxfp4_experts_gated_backward_workspace(size_t m, size_t experts, size_t n, size_t k);
 int kdq_mxfp4_experts_gated_backward(const uint16_t* dh_bf16, size_t dh_stride, size_t m,
                                      const int32_t* offsets, size_t experts,
                                      const uint16_t* kept_bf16, const int8_t* kept_q8,
                                      const float* kept_scales, int activation,
                                      const uint8_t* gate_transposed, const uint8_t* up_transposed,
                                      size_t n, size_t k, uint16_t* dgu_bf16, uint16_t* dx_bf16,
-                                     size_t dx_stride, void* stream);
+                                     size_t dx_stride, void* workspace, size_t workspace_bytes,
+                                     void* stream);
 
 /* ---- a mixture layer in pieces, with their gradients, around kdq_moe_route and the products
  * above (the reference runs the layer on the host and has no gradients:

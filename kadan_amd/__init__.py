@@ -103,9 +103,9 @@ _SIGNATURES = {
     "kdq_mxfp4_linear_backward": [_VP, _SZ, _SZ, _VP, _SZ, _VP, _I, _VP, _SZ, _SZ, _VP, _VP, _SZ,
                                   _VP, _SZ, _VP],
     "kdq_mxfp4_experts_gated": [_VP, _SZ, _SZ, _VP, _SZ, _VP, _VP, _SZ, _SZ, _VP, _VP, _I, _VP,
-                                _SZ, _VP, _VP, _VP, _VP],
+                                _SZ, _VP, _VP, _VP, _VP, _SZ, _VP],
     "kdq_mxfp4_experts_gated_backward": [_VP, _SZ, _SZ, _VP, _SZ, _VP, _VP, _VP, _I, _VP, _VP,
-                                         _SZ, _SZ, _VP, _VP, _SZ, _VP],
+                                         _SZ, _SZ, _VP, _VP, _SZ, _VP, _SZ, _VP],
     "kdq_moe_sort": [_I, _VP, _SZ, _SZ, _SZ, _SZ, _VP, _VP, _SZ, _VP, _VP],
     "kdq_moe_sort_backward": [_I, _VP, _SZ, _VP, _SZ, _SZ, _SZ, _VP, _SZ, _VP],
     "kdq_moe_combine": [_I, _VP, _SZ, _VP, _VP, _SZ, _SZ, _SZ, _I, _VP, _SZ, _VP, _SZ, _VP],
@@ -132,8 +132,10 @@ _OTHER = {
     "kdq_mxfp4_gated_backward_workspace": (_SZ, [_SZ, _SZ, _SZ]),
     "kdq_mxfp4_experts_packed_bytes": (_SZ, [_SZ, _SZ, _SZ]),
     "kdq_mxfp4_experts_packed_transposed_bytes": (_SZ, [_SZ, _SZ, _SZ]),
-    "kdq_mxfp4_linear_workspace": (_SZ, [_SZ, _SZ, _SZ]),
-    "kdq_mxfp4_linear_backward_workspace": (_SZ, [_SZ, _SZ, _SZ]),
+    "kdq_mxfp4_linear_workspace": (_SZ, [_SZ, _SZ, _SZ, _SZ]),
+    "kdq_mxfp4_linear_backward_workspace": (_SZ, [_SZ, _SZ, _SZ, _SZ]),
+    "kdq_mxfp4_experts_gated_workspace": (_SZ, [_SZ, _SZ, _SZ, _SZ, _I]),
+    "kdq_mxfp4_experts_gated_backward_workspace": (_SZ, [_SZ, _SZ, _SZ, _SZ]),
 }
 
 _lib = None

@@ -510,10 +510,15 @@ __device__ __forceinline__ void store_quad(const Target& t, unsigned G, unsigned
     } else if constexpr (OUT == kOutBf16) {
         store4_bf16(static_cast<uint16_t*>(t.y), t.stride, t.n, token, 64 * G + r, v0);
         store4_bf16(static_cast<uint16_t*>(t.y), t.stride, t.n, token, 64 * G + 32 + r, v1);
-    } else if constexpr (OUT == kOutGated) {
+    } else if constexpr (of_gated(OUT)) {
         const unsigned c = 32 * G + r;
-        const f32x4 hv{gate_value(v0.x, v1.x), gate_value(v0.y, v1.y), gate_value(v0.z, v1.z),
-                       gate_value(v0.w, v1.w)};
+        const auto gate = [&](float g, float u) {
+            if constexpr (OUT == kOutExpertsGated)
+                return gate_value(g, u, t.e.act);
+            else
+                return gate_value(g, u);
+        };
+        const f32x4 hv{gate(v0.x, v1.x), gate(v0.y, v1.y), gate(v0.z, v1.z), gate(v0.w, v1.w)};
         store4_bf16(static_cast<uint16_t*>(t.y), t.stride, t.n, token, c, hv);
         if (t.kept && c < t.n) {  // (n % 32 == 0)
             store4_bf16(t.kept, 2 * size_t(t.n), 2 * t.n, token, c, v0);
@@ -1393,7 +1398,7 @@ __global__ __launch_bounds__(512, (shares_unit<TT, OPS> ? 4 : 2)) void gemm_kern
     unsigned tiles = a.tiles_n * a.tiles_m;
     const unsigned xcd = blockIdx.x % 8;
     size_t expert = 0;
-    unsigned tile_m, tile_n;
+    unsigned tile_m, tile_n, spot = 0;  // spot: the experts' tile among all of them
     if constexpr (of_experts(OUT)) {
         // (whole tiles first, then the halves, so that what is left at a launch's end is small: an
         // XCD has its share of either: 2048 rows of 32 experts of 2880 x 2880 gated 91 us against 97,
@@ -1415,6 +1420,7 @@ __global__ __launch_bounds__(512, (shares_unit<TT, OPS> ? 4 : 2)) void gemm_kern
             return;
         const unsigned within = tile - p.before * a.tiles_n;
         const unsigned first = p.first + within % p.tiles * kRows;
+        spot = (half ? list.whole() : 0) + p.before + within % p.tiles;
         tile_m = 0;
         tile_n = within / p.tiles;
         move_to<OUT>(a.out, p.expert, first, min(p.end - first, kRows));
@@ -1818,7 +1824,7 @@ __global__ __launch_bounds__(512, (shares_unit<TT, OPS> ? 4 : 2)) void gemm_kern
     const unsigned own = SPLIT && kg ? kOther : kOwn;
     if constexpr (OUT == kOutExpertsGated) {  // (n % 32 == 0)
         const unsigned c = 32 * G + 4 * h;
-        if (a.out.e.bias && 32 * G < a.out.n) {
+        if (a.out.e.bias && !a.partial && 32 * G < a.out.n) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 float bg[4], bu[4];
@@ -1860,11 +1866,11 @@ __global__ __launch_bounds__(512, (shares_unit<TT, OPS> ? 4 : 2)) void gemm_kern
             break;
         const unsigned T = first_tile + t;
         if (a.partial) {
-            const unsigned row_tiles = (a.out.m + 31) / 32;
-            if (T < row_tiles) {
+            if (T < (a.out.m + 31) / 32) {
+                const unsigned row_tiles = of_experts(OUT) ? a.tiles_m * TT : (a.out.m + 31) / 32;
                 auto* to = reinterpret_cast<f32x4*>(
                                a.partial + ((size_t(blockIdx.y) * (a.tiles_n * 4) + G) * row_tiles +
-                                            T) * kTileFloats) +
+                                            spot * TT + T) * kTileFloats) +
                            lane;
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
@@ -1885,19 +1891,13 @@ __global__ __launch_bounds__(512, (shares_unit<TT, OPS> ? 4 : 2)) void gemm_kern
 // (42 MB in all, 5.8 TB/s).  (A last workgroup that sums in place of this launch has to make
 // the others' partial results visible first: backward of 1024 rows 225 -> 299 us.)
 template <int OUT, bool WHOLE>
-__global__ __launch_bounds__(256) void reduce_kernel(const float* __restrict__ partial,
-                                                     unsigned slices, size_t pairs,
-                                                     unsigned row_tiles, Target out) {
+__device__ __forceinline__ void finish_slices(const float* partial, unsigned slices, size_t pairs,
+                                              size_t pair, unsigned G, unsigned T, unsigned j0,
+                                              const Target& out) {
     const unsigned lane = threadIdx.x % 64;
-    const size_t w = size_t(blockIdx.x) * 4 + threadIdx.x / 64;
-    const size_t pair = WHOLE ? w : w / 4;
-    if (pair >= pairs)
-        return;
-    const unsigned G = unsigned(pair / row_tiles), T = unsigned(pair % row_tiles);
     const auto* from = reinterpret_cast<const f32x4*>(partial + pair * kTileFloats) + lane;
     const size_t step = pairs * (kTileFloats / 4);
     constexpr int kQuads = WHOLE ? 4 : 1;
-    const unsigned j0 = WHOLE ? 0 : unsigned(w % 4);
     const unsigned token = T * 32 + lane % 32, h = lane / 32;
     Added<4> added[2];
     if constexpr (of_linear(OUT))
@@ -1917,6 +1917,19 @@ __global__ __launch_bounds__(256) void reduce_kernel(const float* __restrict__ p
 #pragma unroll
             for (int j = 0; j < kQuads; ++j)
                 v[i][j] += from[s * step + (i * 4 + j0 + j) * 64];
+    if constexpr (OUT == kOutExpertsGated) {
+        if (out.e.bias && 32 * G < out.n) {  // (n % 32 == 0)
+#pragma unroll
+            for (int j = 0; j < kQuads; ++j) {
+                const unsigned c = 32 * G + 8 * (j0 + j) + 4 * h;
+                float bg[4], bu[4];
+                load_f32(out.e.bias, c, out.n, bg);
+                load_f32(out.e.bias_up, c, out.n, bu);
+                v[0][j] += f32x4{bg[0], bg[1], bg[2], bg[3]};
+                v[1][j] += f32x4{bu[0], bu[1], bu[2], bu[3]};
+            }
+        }
+    }
     if constexpr (of_linear(OUT)) {
 #pragma unroll
         for (int i = 0; i < 2; ++i)
@@ -1932,6 +1945,42 @@ __global__ __launch_bounds__(256) void reduce_kernel(const float* __restrict__ p
             keep_q8(out, out.n + 32 * G, token, h, v[1]);
         }
     }
+}
+
+template <int OUT, bool WHOLE>
+__global__ __launch_bounds__(256) void reduce_kernel(const float* __restrict__ partial,
+                                                     unsigned slices, size_t pairs,
+                                                     unsigned row_tiles, Target out) {
+    const size_t w = size_t(blockIdx.x) * 4 + threadIdx.x / 64;
+    const size_t pair = WHOLE ? w : w / 4;
+    if (pair >= pairs)
+        return;
+    finish_slices<OUT, WHOLE>(partial, slices, pairs, pair, unsigned(pair / row_tiles),
+                              unsigned(pair % row_tiles), WHOLE ? 0 : unsigned(w % 4), out);
+}
+
+// The same for the experts' tiles of TT * 32 rows, of which there may be fewer than `spots`.
+template <int TT, int OUT, bool WHOLE>
+__global__ __launch_bounds__(256) void experts_reduce_kernel(const float* __restrict__ partial,
+                                                             unsigned slices, size_t pairs,
+                                                             unsigned spots, Stack stack,
+                                                             Target out) {
+    const size_t w = size_t(blockIdx.x) * 4 + threadIdx.x / 64;
+    const size_t pair = WHOLE ? w : w / 4;
+    if (pair >= pairs)
+        return;
+    const unsigned row_tile = uniform(unsigned(pair % (spots * TT)));
+    const unsigned spot = row_tile / TT, T = row_tile % TT;
+    const Tiles<TT * 32, (TT > 1)> list(stack, out.m);
+    const bool half = spot >= list.whole();
+    const unsigned number = half ? spot - list.whole() : spot;
+    const auto p = list.of(number, half);
+    const unsigned first = p.first + (number - p.before) * (half ? 0 : TT * 32);
+    if (!p.tiles || first + T * 32 >= p.end)
+        return;
+    move_to<OUT>(out, p.expert, first, min(p.end - first, TT * 32u));
+    finish_slices<OUT, WHOLE>(partial, slices, pairs, pair, unsigned(pair / (spots * TT)), T,
+                              WHOLE ? 0 : unsigned(w % 4), out);
 }
 
 // ------------------------------------------------------------------ dg and du
@@ -2056,6 +2105,21 @@ int launch_gemm(const Gemm& a, const Plan& p, hipStream_t st) {
     return KDQ_OK;
 }
 
+template <int TT, int OUT>
+int run_experts_reduce(const Gemm& a, const Plan& p, hipStream_t st) {
+    const size_t pairs = size_t(p.tiles_n) * 4 * p.tiles_m * TT;
+    const auto launch = [&](auto kernel, size_t blocks) {
+        hipLaunchKernelGGL(kernel, dim3(unsigned(blocks)), dim3(256), 0, st, a.partial, p.slices,
+                           pairs, p.tiles_m, a.stack, a.out);
+        KDQ_HIP(hipGetLastError());
+        return int(KDQ_OK);
+    };
+    if constexpr (OUT == kOutExpertsGated)
+        if (a.out.kept_q)
+            return launch(experts_reduce_kernel<TT, OUT, true>, ceil_div(pairs, 4));
+    return launch(experts_reduce_kernel<TT, OUT, false>, pairs);
+}
+
 template <int OPS, int OUT> int launch_tall(const Gemm& a, const Plan& p, hipStream_t st) {
     if constexpr (of_experts(OUT))  // (no plan of theirs has such tiles)
         return KDQ_ERR_UNSUPPORTED;
@@ -2099,8 +2163,11 @@ template <int OPS, int OUT> int run_gemm(Gemm a, const Plan& p, void* workspace,
              : p.tt == 2 ? launch_gemm<2, true, OPS, OUT>(a, p, st)
                          : launch_tall<OPS, OUT>(a, p, st);
     }
-    if constexpr (!of_experts(OUT)) {  // (theirs have no slices)
-        if (!rc && p.slices > 1)
+    if (!rc && p.slices > 1) {
+        if constexpr (of_experts(OUT))
+            rc = p.tt == 1 ? run_experts_reduce<1, OUT>(a, p, st)
+                           : run_experts_reduce<2, OUT>(a, p, st);
+        else
             rc = run_reduce<OUT>(a, p, st);
     }
     return rc;
@@ -2134,18 +2201,16 @@ int run_experts_decode(Decode a, const DecodeShape& s, hipStream_t st) {
 }
 
 template <int OPS, int OUT>
-int run_experts_gemm(Gemm a, const ExpertsPlan& e, size_t chunks, hipStream_t st) {
+int run_experts_gemm(Gemm a, const ExpertsPlan& e, void* workspace, hipStream_t st) {
     Plan p{};
     p.split = true;
     p.tt = e.tt;
     p.tiles_n = unsigned(e.tiles_n);
     p.tiles_m = unsigned(e.most);
-    p.slices = 1;
-    p.chunks = unsigned(chunks);
-    const size_t sets = OPS != kTransposed || of_one_backward(OUT) ? 2 : 1;
-    const size_t unit = OUT == kOutExpertsLinear ? 2 : 4;  // (gemm_kernel's turns)
-    p.part = unsigned(ceil_div(ceil_div(chunks, sets), unit) * unit);
-    return run_gemm<OPS, OUT>(a, p, nullptr, st);
+    p.slices = e.slices;
+    p.chunks = e.chunks;
+    p.part = e.part;
+    return run_gemm<OPS, OUT>(a, p, workspace, st);
 }
 
 template <bool GATED, bool FP4, int OUT> int run_decode(Decode a, hipStream_t st) {

@@ -46,7 +46,9 @@ size_t offset_bytes(const int32_t* offsets, size_t experts) {
 
 // (a launch's threads are counted in 32 bits)
 bool launches(const ExpertsPlan& p) {
-    return p.decode ? p.most <= 65535 : p.most * p.tiles_n + 16 <= UINT32_MAX / 512;
+    return p.decode ? p.most <= 65535
+                    : p.most * p.tiles_n + 16 <= UINT32_MAX / 512 &&
+                          (p.slices == 1 || p.tiles_n * 4 * p.most * p.tt <= UINT32_MAX / 256);
 }
 
 Gemm gemm_of(const uint8_t* w0, const uint8_t* w1, const uint16_t* x, size_t x_stride,
@@ -107,8 +109,12 @@ extern "C" int kdq_mxfp4_experts_pack_transposed(const uint8_t* blocks, const ui
     return launch_pack(pack_t_kernel, f, blocks, scales, rows, cols, packed, stream, experts);
 }
 
-extern "C" size_t kdq_mxfp4_linear_workspace(size_t m, size_t n, size_t k) {
-    return kdq_mxfp4_product_workspace(m, n, k, 0);
+extern "C" size_t kdq_mxfp4_linear_workspace(size_t m, size_t experts, size_t n, size_t k) {
+    if (!experts)
+        return kdq_mxfp4_product_workspace(m, n, k, 0);
+    if (!m || !n || !k || experts > kMaxExperts || !sizes_ok(m, n, k))
+        return 0;
+    return partial_bytes(plan_experts(m, experts, n, k, false, false, compute_units()));
 }
 
 extern "C" int kdq_mxfp4_linear(const uint16_t* x_bf16, size_t x_stride, size_t m,
@@ -156,10 +162,12 @@ extern "C" int kdq_mxfp4_linear(const uint16_t* x_bf16, size_t x_stride, size_t 
         const ExpertsPlan p = plan_experts(m, experts, n, k, false, false, compute_units());
         if (!launches(p))
             return KDQ_ERR_SHAPE;
+        if (const int rc = check_workspace(partial_bytes(p), workspace, workspace_bytes))
+            return rc;
         g.stack = stack_of(offsets, experts, f);
         return p.decode
                    ? run_experts_decode<false, kOutExpertsLinear>(decode_of(g, k), p.shape, st)
-                   : run_experts_gemm<kBf16, kOutExpertsLinear>(g, p, ceil_div(k, 64), st);
+                   : run_experts_gemm<kBf16, kOutExpertsLinear>(g, p, workspace, st);
     }
     const Plan p = plan_product(m, n, k, false, compute_units());
     if (const int rc = check_workspace(partial_bytes(p, m), workspace, workspace_bytes))
@@ -168,10 +176,13 @@ extern "C" int kdq_mxfp4_linear(const uint16_t* x_bf16, size_t x_stride, size_t 
                     : run_gemm<kBf16, kOutLinear>(g, p, workspace, st);
 }
 
-extern "C" size_t kdq_mxfp4_linear_backward_workspace(size_t m, size_t n, size_t k) {
-    if (!m || !n || !k || m > kMaxRows || !packs_transposed(n, k))
+extern "C" size_t kdq_mxfp4_linear_backward_workspace(size_t m, size_t experts, size_t n,
+                                                      size_t k) {
+    if (!m || !n || !k || m > kMaxRows || experts > kMaxExperts || !packs_transposed(n, k))
         return 0;
-    return partial_bytes(plan_one_backward(m, n, k, compute_units()), m);
+    const size_t cus = compute_units();
+    return experts ? partial_bytes(plan_experts_backward(m, experts, n, k, false, cus))
+                   : partial_bytes(plan_one_backward(m, n, k, cus), m);
 }
 
 extern "C" int kdq_mxfp4_linear_backward(const uint16_t* dy_bf16, size_t dy_stride, size_t m,
@@ -209,9 +220,11 @@ extern "C" int kdq_mxfp4_linear_backward(const uint16_t* dy_bf16, size_t dy_stri
     Plan p{};
     ExpertsPlan e{};
     if (offsets) {
-        e = plan_experts_backward(m, experts, k);
+        e = plan_experts_backward(m, experts, n, k, false, compute_units());
         if (!launches(e))
             return KDQ_ERR_SHAPE;
+        if (const int rc = check_workspace(partial_bytes(e), workspace, workspace_bytes))
+            return rc;
     } else {
         p = plan_one_backward(m, n, k, compute_units());
         if (const int rc = check_workspace(partial_bytes(p, m), workspace, workspace_bytes))
@@ -230,7 +243,21 @@ extern "C" int kdq_mxfp4_linear_backward(const uint16_t* dy_bf16, size_t dy_stri
     if (!offsets)
         return run_gemm<kTransposed, kOutOneBackward>(g, p, workspace, st);
     g.stack = stack_of(offsets, experts, f);
-    return run_experts_gemm<kTransposed, kOutExpertsOneBackward>(g, e, ceil_div(n, 64), st);
+    return run_experts_gemm<kTransposed, kOutExpertsOneBackward>(g, e, workspace, st);
+}
+
+extern "C" size_t kdq_mxfp4_experts_gated_workspace(size_t m, size_t experts, size_t n, size_t k,
+                                                    int kept) {
+    if (!m || !n || !k || !experts || experts > kMaxExperts || !sizes_ok(m, n, k) || n % 32)
+        return 0;
+    return partial_bytes(plan_experts(m, experts, n, k, true, kept != 0, compute_units()));
+}
+
+extern "C" size_t kdq_mxfp4_experts_gated_backward_workspace(size_t m, size_t experts, size_t n,
+                                                             size_t k) {
+    if (!m || !n || !k || !experts || experts > kMaxExperts || !backward_sizes_ok(m, n, k))
+        return 0;
+    return partial_bytes(plan_experts_backward(m, experts, n, k, true, compute_units()));
 }
 
 extern "C" int kdq_mxfp4_experts_gated(const uint16_t* x_bf16, size_t x_stride, size_t m,
@@ -239,7 +266,8 @@ extern "C" int kdq_mxfp4_experts_gated(const uint16_t* x_bf16, size_t x_stride, 
                                        size_t n, size_t k, const float* gate_bias,
                                        const float* up_bias, int activation, uint16_t* h_bf16,
                                        size_t h_stride, uint16_t* kept_bf16, int8_t* kept_q8,
-                                       float* kept_scales, void* stream) {
+                                       float* kept_scales, void* workspace,
+                                       size_t workspace_bytes, void* stream) {
     if (!x_bf16 || !offsets || !gate_packed || !up_packed || !h_bf16 || !m || !n || !k ||
         (kept_bf16 && kept_q8) || !kept_q8 != !kept_scales || !gate_bias != !up_bias)
         return KDQ_ERR_ARGUMENT;
@@ -261,7 +289,8 @@ extern "C" int kdq_mxfp4_experts_gated(const uint16_t* x_bf16, size_t x_stride, 
     const Range out[] = {{h_bf16, extent(m, h_stride, n, 2)},
                          {kept_bf16, 4 * m * n},
                          {kept_q8, 2 * m * n},
-                         {kept_scales, m * n / 4}},
+                         {kept_scales, m * n / 4},
+                         {workspace, workspace_bytes}},
                 in[] = {{x_bf16, extent(m, x_stride, k, 2)},
                         {offsets, offset_bytes(offsets, experts)},
                         {gate_bias, experts * n * 4},
@@ -274,20 +303,23 @@ extern "C" int kdq_mxfp4_experts_gated(const uint16_t* x_bf16, size_t x_stride, 
         plan_experts(m, experts, n, k, true, kept_bf16 || kept_q8, compute_units());
     if (!launches(p))
         return KDQ_ERR_SHAPE;
+    if (const int rc = check_workspace(partial_bytes(p), workspace, workspace_bytes))
+        return rc;
     const auto st = static_cast<hipStream_t>(stream);
     Target t{h_bf16, h_stride, unsigned(m), unsigned(n), kept_bf16, kept_q8, kept_scales};
     t.e = {gate_bias, up_bias, nullptr, 0, activation, false};
     Gemm g = gemm_of(gate_packed, up_packed, x_bf16, x_stride, k, f, t);
     g.stack = stack_of(offsets, experts, f);
     return p.decode ? run_experts_decode<true, kOutExpertsGated>(decode_of(g, k), p.shape, st)
-                    : run_experts_gemm<kBf16, kOutExpertsGated>(g, p, ceil_div(k, 64), st);
+                    : run_experts_gemm<kBf16, kOutExpertsGated>(g, p, workspace, st);
 }
 
 extern "C" int kdq_mxfp4_experts_gated_backward(
     const uint16_t* dh_bf16, size_t dh_stride, size_t m, const int32_t* offsets, size_t experts,
     const uint16_t* kept_bf16, const int8_t* kept_q8, const float* kept_scales, int activation,
     const uint8_t* gate_transposed, const uint8_t* up_transposed, size_t n, size_t k,
-    uint16_t* dgu_bf16, uint16_t* dx_bf16, size_t dx_stride, void* stream) {
+    uint16_t* dgu_bf16, uint16_t* dx_bf16, size_t dx_stride, void* workspace,
+    size_t workspace_bytes, void* stream) {
     if (!dh_bf16 || !offsets || !gate_transposed || !up_transposed || !dgu_bf16 || !dx_bf16 ||
         !m || !n || !k || !kept_bf16 == !kept_q8 || !kept_q8 != !kept_scales)
         return KDQ_ERR_ARGUMENT;
@@ -306,7 +338,9 @@ extern "C" int kdq_mxfp4_experts_gated_backward(
         misaligned(dgu_bf16, 16))
         return KDQ_ERR_ALIGNMENT;
     const Form f = transposed_form(n, k);
-    const Range out[] = {{dgu_bf16, 4 * m * n}, {dx_bf16, extent(m, dx_stride, k, 2)}},
+    const Range out[] = {{dgu_bf16, 4 * m * n},
+                         {dx_bf16, extent(m, dx_stride, k, 2)},
+                         {workspace, workspace_bytes}},
                 in[] = {{dh_bf16, extent(m, dh_stride, n, 2)},
                         {offsets, offset_bytes(offsets, experts)},
                         {kept_bf16, 4 * m * n},
@@ -316,9 +350,11 @@ extern "C" int kdq_mxfp4_experts_gated_backward(
                         {up_transposed, bytes_of(f, experts)}};
     if (any_overlap(out, in))
         return KDQ_ERR_ALIAS;
-    const ExpertsPlan p = plan_experts_backward(m, experts, k);
+    const ExpertsPlan p = plan_experts_backward(m, experts, n, k, true, compute_units());
     if (!launches(p))
         return KDQ_ERR_SHAPE;
+    if (const int rc = check_workspace(partial_bytes(p), workspace, workspace_bytes))
+        return rc;
     const auto st = static_cast<hipStream_t>(stream);
     const auto gradients = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3(unsigned(ceil_div(m * (n / 8), 256))), dim3(256), 0, st,
@@ -336,5 +372,5 @@ extern "C" int kdq_mxfp4_experts_gated_backward(
     Gemm g = gemm_of(gate_transposed, up_transposed, dgu_bf16, 2 * n, n, f, t);
     g.x_second = unsigned(n * 2);
     g.stack = stack_of(offsets, experts, f);
-    return run_experts_gemm<kTransposed, kOutExpertsBackward>(g, p, ceil_div(n, 64), st);
+    return run_experts_gemm<kTransposed, kOutExpertsBackward>(g, p, workspace, st);
 }

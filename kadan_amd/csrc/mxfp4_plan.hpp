@@ -3,6 +3,7 @@
 // size reaches.
 #pragma once
 #include <algorithm>
+#include <cmath>
 #include <cstddef>
 
 namespace kdq {
@@ -224,7 +225,47 @@ struct ExpertsPlan {
     DecodeShape shape;
     int tt;
     size_t tiles_n, most;
+    unsigned slices, chunks, part;  // of K, in chunks
 };
+
+inline size_t partial_bytes(const ExpertsPlan& p) {
+    return p.decode || p.slices == 1
+               ? 0
+               : size_t(p.slices) * p.tiles_n * 4 * p.most * p.tt * kTileFloats * 4;
+}
+
+// K slices where the tiles are too few to fill the compute units: by plan_gemm's estimate, and no
+// shorter than `reached` experts' `bytes` take; over the tiles that as many experts with half a tile
+// more than whole ones would make. `sets`: parts of K that a workgroup takes, of `unit` chunks.
+// (slices of measured calls, with rows an expert as a batch leaves them, us:
+//  gated backward of 4 rows, 3392 -> 1024: 37 as one, 16.9 in 6, 15.7 in 8, 18.1 in 16
+//  594 rows of 6 experts, 5920 -> 416: product 37 as one, 18.8 in 6, 22 in 12; gated backward 89, 32, 33
+//  64 rows of 8 experts, 5632 -> 4096, which reads 92 MB: 24 as one, 29 in 2, 27 in 4)
+inline void slice_experts(ExpertsPlan& p, size_t m, size_t reached, double bytes, size_t chunks,
+                          size_t sets, size_t unit, int ops, size_t cus) {
+    const double tiles =
+        std::min(double(p.most), std::max(double(m) / double(p.tt * 32) + 0.5 * double(reached),
+                                          0.85 * double(reached)));
+    const Cost c = cost_of(ops, p.tt);
+    double best = 0;
+    p.chunks = unsigned(chunks);
+    for (size_t slices = 1; slices <= 16; ++slices) {
+        const size_t part = ceil_div(ceil_div(chunks, slices * sets), unit) * unit;
+        const size_t real = ceil_div(chunks, part * sets);
+        const double groups = tiles * double(p.tiles_n) * double(real);
+        const double each = std::ceil(groups / double(cus));
+        const double alone = c.fixed + double(part) * c.turn;
+        const double both = c.fixed + double(part) * c.turn_of_two;
+        double t = std::max(each <= 1 ? alone : each / 2 * both, bytes / 4.5e6);
+        if (real > 1)
+            t += 2 + 0.25 * double(real) + groups * p.tt * 4 * kTileFloats * 4 / 2e6;
+        if (slices == 1 || t < best) {
+            best = slices == 1 ? 0.9 * t : t;  // (a tenth less, or not at all)
+            p.slices = unsigned(real);
+            p.part = unsigned(part);
+        }
+    }
+}
 
 inline ExpertsPlan plan_experts(size_t m, size_t experts, size_t n, size_t k, bool gated,
                                 bool kept, size_t cus) {
@@ -250,14 +291,21 @@ inline ExpertsPlan plan_experts(size_t m, size_t experts, size_t n, size_t k, bo
     }
     p.tt = mean < (gated || k <= 1536 ? 48 : 96) ? 1 : 2;
     p.most = most_tiles(m, experts, size_t(p.tt) * 32);
+    slice_experts(p, m, reached, double(reached) * double(n * k) * (gated ? 17 : 8.5) / 16,
+                  ceil_div(k, 64), 2, gated ? 4 : 2, kBf16, cus);
     return p;
 }
 
-inline ExpertsPlan plan_experts_backward(size_t m, size_t experts, size_t k) {
+// (`gated`: two matrices, each of a wavefront group's own)
+inline ExpertsPlan plan_experts_backward(size_t m, size_t experts, size_t n, size_t k, bool gated,
+                                         size_t cus) {
     ExpertsPlan p{};
-    p.tt = m / std::min(experts, m) < 24 ? 1 : 2;
+    const size_t reached = std::min(experts, m);
+    p.tt = m / reached < 24 ? 1 : 2;
     p.tiles_n = ceil_div(k, 256);
     p.most = most_tiles(m, experts, size_t(p.tt) * 32);
+    slice_experts(p, m, reached, double(reached) * double(n * k) * (gated ? 17 : 8.5) / 16,
+                  ceil_div(n, 64), gated ? 1 : 2, 4, kTransposed, cus);
     return p;
 }
 

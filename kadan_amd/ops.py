@@ -452,6 +452,17 @@ def _mxfp4_sizes(*sizes):
     return _mxfp4_sizes_on(_current_device(), *sizes)
 
 
+@functools.lru_cache(maxsize=4096, typed=True)
+def _experts_sizes_on(device: int, stack: str, experts: int, rows: int, cols: int, workspace: str,
+                      *sizes: int):
+    return _mxfp4_size(stack, experts, rows, cols), int(getattr(lib(), workspace)(*sizes))
+
+
+def _experts_sizes(*sizes):
+    """The same for a stack of experts' matrices."""
+    return _experts_sizes_on(_current_device(), *sizes)
+
+
 _PACKED, _TRANSPOSED = "kdq_mxfp4_packed_bytes", "kdq_mxfp4_packed_transposed_bytes"
 _EXPERTS = "kdq_mxfp4_experts_packed_bytes"
 _EXPERTS_TRANSPOSED = "kdq_mxfp4_experts_packed_transposed_bytes"
@@ -706,12 +717,7 @@ def _here(t: torch.Tensor, name: str) -> None:
         raise ValueError(f"{name}: expected on the current device")
 
 
-def _stack(packed: torch.Tensor, function: str, experts: int, rows: int, cols: int,
-           name: str) -> int:
-    """A stack's packed form."""
-    size = _mxfp4_size(function, experts, rows, cols)
-    if function == _EXPERTS:
-        return _matrix(packed, size, name)
+def _transposed_stack(packed: torch.Tensor, size: int, experts: int, cols: int, name: str) -> int:
     at = _matrix(packed, size, name, 3)
     if packed.shape[:2] != (experts, (cols + 63) // 64):
         raise ValueError(f"{name}: another stack's packed form")
@@ -739,12 +745,15 @@ def mxfp4_linear(x: torch.Tensor, packed: torch.Tensor, n_out: int,
     m, k = x.shape
     if offsets is None:
         experts, table = 1, None
-        weights, size = _mxfp4_sizes(_PACKED, n_out, k, "kdq_mxfp4_linear_workspace", m, n_out, k)
+        weights, size = _mxfp4_sizes(_PACKED, n_out, k, "kdq_mxfp4_linear_workspace", m, 0, n_out,
+                                     k)
         w = _matrix(packed, weights, "packed")
         stream = _stream_for(x, packed)
     else:
-        experts, table, size = _offsets(offsets), offsets.data_ptr(), 0
-        w = _stack(packed, _EXPERTS, experts, n_out, k, "packed")
+        experts, table = _offsets(offsets), offsets.data_ptr()
+        weights, size = _experts_sizes(_EXPERTS, experts, n_out, k, "kdq_mxfp4_linear_workspace", m,
+                                       experts, n_out, k)
+        w = _matrix(packed, weights, "packed")
         stream = _stream_for(x, packed, offsets)
     b = add = None
     if bias is not None:
@@ -782,15 +791,17 @@ def mxfp4_linear_backward(dy: torch.Tensor, packed: torch.Tensor, n_in: int,
         raise ValueError("n_out must be a multiple of 8, n_in of 32")
     if (saved is None) == bool(act):
         raise ValueError("saved: expected with an activation, and only with one")
-    parts, size = [dy, packed], 0
+    parts = [dy, packed]
     if offsets is None:
         experts, table = 1, None
         weights, size = _mxfp4_sizes(_TRANSPOSED, n, n_in, "kdq_mxfp4_linear_backward_workspace",
-                                     m, n, n_in)
+                                     m, 0, n, n_in)
         w = _transposed_matrix(packed, weights, n_in, "packed")
     else:
         experts, table = _offsets(offsets), offsets.data_ptr()
-        w = _stack(packed, _EXPERTS_TRANSPOSED, experts, n, n_in, "packed")
+        weights, size = _experts_sizes(_EXPERTS_TRANSPOSED, experts, n, n_in,
+                                       "kdq_mxfp4_linear_backward_workspace", m, experts, n, n_in)
+        w = _transposed_stack(packed, weights, experts, n_in, "packed")
         parts.append(offsets)
     device = dy.device
     dpre = dy
@@ -834,8 +845,9 @@ def mxfp4_experts_gated(x: torch.Tensor, offsets: torch.Tensor, gate: torch.Tens
         raise ValueError("expected both biases or none")
     m, k = x.shape
     experts = _offsets(offsets)
-    wg = _stack(gate, _EXPERTS, experts, n_out, k, "gate")
-    wu = _stack(up, _EXPERTS, experts, n_out, k, "up")
+    weights, size = _experts_sizes(_EXPERTS, experts, n_out, k, "kdq_mxfp4_experts_gated_workspace",
+                                   m, experts, n_out, k, 0 if save is None else 1)
+    wg, wu = _matrix(gate, weights, "gate"), _matrix(up, weights, "up")
     stream = _stream_for(x, offsets, gate, up)
     bg = bu = None
     if gate_bias is not None:
@@ -854,8 +866,10 @@ def mxfp4_experts_gated(x: torch.Tensor, offsets: torch.Tensor, gate: torch.Tens
         saved = (x.new_empty(m, 2 * n_out, dtype=torch.int8),
                  x.new_empty(m, n_out // 16, dtype=torch.float32))
         codes, scales = saved[0].data_ptr(), saved[1].data_ptr()
+    scratch = _scratch(size, x.device) if size else None
     call("kdq_mxfp4_experts_gated", x.data_ptr(), stride, m, offsets.data_ptr(), experts, wg, wu,
-         n_out, k, bg, bu, act, out.data_ptr(), h_stride, kept, codes, scales, stream)
+         n_out, k, bg, bu, act, out.data_ptr(), h_stride, kept, codes, scales, _ptr(scratch), size,
+         stream)
     return out if save is None else (out, saved)
 
 
@@ -890,8 +904,11 @@ def mxfp4_experts_gated_backward(dh: torch.Tensor, offsets: torch.Tensor, saved,
     if n % 32 or n_in % 32 or not n_in:
         raise ValueError("n_out and n_in must be multiples of 32")
     experts = _offsets(offsets)
-    wg = _stack(gate, _EXPERTS_TRANSPOSED, experts, n, n_in, "gate")
-    wu = _stack(up, _EXPERTS_TRANSPOSED, experts, n, n_in, "up")
+    weights, size = _experts_sizes(_EXPERTS_TRANSPOSED, experts, n, n_in,
+                                   "kdq_mxfp4_experts_gated_backward_workspace", m, experts, n,
+                                   n_in)
+    wg = _transposed_stack(gate, weights, experts, n_in, "gate")
+    wu = _transposed_stack(up, weights, experts, n_in, "up")
     parts, (kept, codes, scales) = _saved_gates(saved, m, n)
     device = dh.device
     if out is None:
@@ -901,9 +918,10 @@ def mxfp4_experts_gated_backward(dh: torch.Tensor, offsets: torch.Tensor, saved,
         dx_stride = _output(out, m, n_in, _BF16, "out")
         stream = _stream_for(dh, offsets, gate, up, out, *parts)
     dgu = torch.empty(m, 2 * n, dtype=_BF16, device=device)
+    scratch = _scratch(size, device)
     call("kdq_mxfp4_experts_gated_backward", dh.data_ptr(), stride, m, offsets.data_ptr(),
          experts, kept, codes, scales, act, wg, wu, n, n_in, dgu.data_ptr(), out.data_ptr(),
-         dx_stride, stream)
+         dx_stride, _ptr(scratch), size, stream)
     return out, dgu
 
 

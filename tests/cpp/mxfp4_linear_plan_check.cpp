@@ -1,7 +1,7 @@
 // Prints what kadan_amd/csrc/mxfp4_plan.hpp picks for the calls on standard input, one a line:
 //   linear m n k | back m n k | experts m experts n k gated kept |
-//   experts_back m experts n k 0 | tiles m experts rows
-// as "decode wide staged tb", "gemm tt split sliced", "experts decode wide", "experts gemm tt" or
+//   experts_back m experts n k gated | tiles m experts rows
+// as "decode wide staged tb", "gemm tt split sliced", "experts decode wide", "experts gemm tt sliced" or
 // a number of tiles, on `argv[1]` compute units.
 #include "mxfp4_plan.hpp"
 
@@ -36,10 +36,10 @@ int main(int, char** argv) {
         if (path == "experts")
             std::cin >> kept;
         const ExpertsPlan p = path == "experts" ? plan_experts(m, a, b, c, gated, kept, cus)
-                                                : plan_experts_backward(m, a, c);
+                                                : plan_experts_backward(m, a, b, c, gated, cus);
         if (p.decode)
             std::cout << "experts decode " << p.shape.wide << '\n';
         else
-            std::cout << "experts gemm " << p.tt << '\n';
+            std::cout << "experts gemm " << p.tt << ' ' << (p.slices > 1) << '\n';
     }
 }

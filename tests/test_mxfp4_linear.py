@@ -31,10 +31,20 @@ def test_packed_sizes():
     assert size(256, 1, 32) and turned(256, 1, 32)
     for f in (size, turned):
         assert f(0, 64, 64) == f(257, 64, 64) == f(4, 0, 64) == f(4, 64, 48) == 0
-    assert lib.kdq_mxfp4_linear_workspace(64, 4096, 14336) == \
+    assert lib.kdq_mxfp4_linear_workspace(64, 0, 4096, 14336) == \
         lib.kdq_mxfp4_product_workspace(64, 4096, 14336, 0)
     work = lib.kdq_mxfp4_linear_backward_workspace
-    assert work(64, 14336, 4096) and work(0, 64, 64) == work(64, 64, 48) == 0
+    assert work(64, 0, 14336, 4096) and work(0, 0, 64, 64) == work(64, 0, 64, 48) == 0
+    # of experts: partial sums where the tiles are few, and none where they are many
+    fits = [(lib.kdq_mxfp4_linear_workspace, ()), (work, ()),
+            (lib.kdq_mxfp4_experts_gated_workspace, (1,)),
+            (lib.kdq_mxfp4_experts_gated_backward_workspace, ())]
+    for f, last in fits:
+        assert f(64, 1, 4096, 14336, *last) and f(32768, 32, 2880, 2880, *last) == 0
+        assert f(0, 2, 64, 64, *last) == f(64, 257, 2880, 2880, *last) == 0
+        assert f(64, 2, 2880, 2872, *last) == 0
+    assert lib.kdq_mxfp4_experts_gated_workspace(4, 32, 2880, 2880, 0) == 0  # (one kernel)
+    assert lib.kdq_mxfp4_experts_gated_workspace(64, 2, 0, 64, 0) == 0
 
 
 def test_pack_refusals():
@@ -77,11 +87,15 @@ def test_linear_refusals(experts):
     if experts:
         assert call(y=O) == 4 and call(o=O + 2) == 7 and call(e=257) == 2
         assert call(y=B + 3 * 40 * 4) == 4  # (the last expert's bias)
+        many = dict(m=64, e=1, n=4096, k=14336, xs=14336, ys=4096, rs=4096)
+        need = kadan_amd.lib().kdq_mxfp4_linear_workspace(64, 1, 4096, 14336)
+        assert call(**many) == 6 and call(**many, ws=Z, wb=need - 16) == 6
+        assert call(**many, ws=Z + 8, wb=need) == 7 and call(**many, ws=O, wb=need) == 4
     else:
         assert call(e=2) == 1
         # K slices need their workspace, aligned and apart from everything else
         many = dict(m=64, n=4096, k=14336, xs=14336, ys=4096, rs=4096)
-        need = kadan_amd.lib().kdq_mxfp4_linear_workspace(64, 4096, 14336)
+        need = kadan_amd.lib().kdq_mxfp4_linear_workspace(64, 0, 4096, 14336)
         assert call(**many) == 6 and call(**many, ws=Z, wb=need - 16) == 6
         assert call(**many, ws=Z + 8, wb=need) == 7 and call(**many, ws=X, wb=need) == 4
         assert call(**many, ws=K, wb=need) == 4 and call(**many, ws=R, wb=need) == 4
@@ -109,17 +123,21 @@ def test_linear_backward_refusals(experts):
     assert call(dx=W + 16) == 4
     if experts:
         assert call(dx=O) == 4 and call(o=O + 1) == 7 and call(e=257) == 2
+        many = dict(m=64, e=1, n=14336, k=4096, ds=14336, dxs=4096)
+        need = kadan_amd.lib().kdq_mxfp4_linear_backward_workspace(64, 1, 14336, 4096)
+        assert call(**many) == 6 and call(**many, ws=Z + 8, wb=need) == 7
+        assert call(**many, ws=O, wb=need) == 4 and call(**many, ws=Q, wb=need) == 4
     else:
         many = dict(m=64, n=14336, k=4096, ds=14336, dxs=4096)
-        need = kadan_amd.lib().kdq_mxfp4_linear_backward_workspace(64, 14336, 4096)
+        need = kadan_amd.lib().kdq_mxfp4_linear_backward_workspace(64, 0, 14336, 4096)
         assert call(**many) == 6 and call(**many, ws=Z + 8, wb=need) == 7
         assert call(**many, ws=Q, wb=need) == 4
 
 
 def test_experts_gated_refusals():
-    call = caller("kdq_mxfp4_experts_gated", "x xs m o e g u n k bg bu act h hs kb kq ks",
+    call = caller("kdq_mxfp4_experts_gated", "x xs m o e g u n k bg bu act h hs kb kq ks ws wb",
                   dict(x=X, xs=64, m=2, o=O, e=4, g=W, u=V, n=32, k=64, bg=B, bu=R, act=1, h=Y,
-                       hs=32, kb=None, kq=Q, ks=S))
+                       hs=32, kb=None, kq=Q, ks=S, ws=None, wb=0))
     for name in ("x", "o", "g", "u", "h", "bg", "bu", "kq", "ks"):
         assert call(**{name: None}) == 1
     for name in ("m", "n", "k", "e"):
@@ -132,12 +150,17 @@ def test_experts_gated_refusals():
     assert call(o=O + 2) == 7 and call(bg=B + 2) == 7 and call(ks=S + 2) == 7
     assert call(h=X) == 4 and call(h=B) == 4 and call(kq=R) == 4 and call(ks=Y) == 4
     assert call(h=O) == 4 and call(kb=V, kq=None, ks=None) == 4
+    many = dict(m=64, e=1, n=4096, k=14336, xs=14336, hs=4096)
+    need = kadan_amd.lib().kdq_mxfp4_experts_gated_workspace(64, 1, 4096, 14336, 1)
+    assert call(**many) == 6 and call(**many, ws=Z + 8, wb=need) == 7
+    assert call(**many, ws=O, wb=need) == 4 and call(**many, ws=S, wb=need) == 4
 
 
 def test_experts_gated_backward_refusals():
-    call = caller("kdq_mxfp4_experts_gated_backward", "d ds m o e kb kq ks act g u n k dgu dx dxs",
+    call = caller("kdq_mxfp4_experts_gated_backward", "d ds m o e kb kq ks act g u n k dgu dx dxs ws "
+                  "wb",
                   dict(d=Y, ds=32, m=2, o=O, e=4, kb=K, kq=None, ks=None, act=3, g=W, u=V, n=32,
-                       k=64, dgu=Q, dx=X, dxs=64))
+                       k=64, dgu=Q, dx=X, dxs=64, ws=None, wb=0))
     for name in ("d", "o", "kb", "g", "u", "dgu", "dx"):
         assert call(**{name: None}) == 1
     for name in ("m", "n", "k", "e"):
@@ -148,6 +171,10 @@ def test_experts_gated_backward_refusals():
     assert call(d=Y + 8) == 7 and call(g=W + 8) == 7 and call(dgu=Q + 8) == 7 and call(o=O + 2) == 7
     assert call(dx=Y) == 4 and call(dgu=K) == 4 and call(dx=Q) == 4 and call(dgu=V) == 4
     assert call(dx=O) == 4
+    many = dict(m=64, e=1, n=14336, k=4096, ds=14336, dxs=4096)
+    need = kadan_amd.lib().kdq_mxfp4_experts_gated_backward_workspace(64, 1, 14336, 4096)
+    assert call(**many) == 6 and call(**many, ws=Z + 8, wb=need) == 7
+    assert call(**many, ws=O, wb=need) == 4 and call(**many, ws=V, wb=need) == 4
 
 
 @pytest.mark.parametrize("act", ["silu", "gelu"])

@@ -127,7 +127,8 @@ EXPERTS = [  # m, experts, n, k, rows: every kernel, one and no row, odd and lon
     (129, 2, 64, 4128, "even"), (256, 8, 777, 544, "odd"), (333, 32, 1030, 288, "odd"),
     (400, 12, 320, 1440, "even"), (513, 5, 500, 224, "odd"), (700, 3, 2100, 608, "even"),
     (1000, 9, 96, 2912, "one"), (2048, 32, 520, 352, "odd"), (2000, 16, 4096, 96, "even"),
-    (5000, 255, 288, 128, "odd")]
+    (5000, 255, 288, 128, "odd"), (27, 7, 385, 2912, "odd"), (90, 2, 72, 8192, "odd"),
+    (330, 3, 257, 3968, "odd")]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
@@ -159,7 +160,8 @@ GATED = [(1, 1, 32, 32, "even"), (4, 32, 2880, 2880, "even"), (4, 128, 768, 2048
          (40, 7, 256, 2080, "one"), (64, 32, 2880, 1440, "odd"), (100, 256, 160, 160, "odd"),
          (129, 2, 64, 4128, "even"), (256, 8, 768, 544, "odd"), (400, 12, 320, 1440, "even"),
          (513, 5, 512, 224, "odd"), (700, 3, 2112, 608, "even"), (2048, 32, 544, 352, "odd"),
-         (5000, 255, 288, 128, "odd")]
+         (5000, 255, 288, 128, "odd"), (1, 3, 96, 4160, "odd"), (27, 7, 384, 2912, "odd"),
+         (90, 2, 64, 8192, "odd"), (330, 3, 288, 3968, "odd")]
 
 
 @pytest.mark.parametrize("save", [None, "bf16", "q8"])
@@ -200,7 +202,8 @@ EXPERTS_BACKWARD = [
     (1, 1, 8, 32, "even"), (4, 32, 96, 64, "even"), (16, 3, 104, 288, "odd"),
     (64, 32, 2880, 1440, "odd"), (100, 256, 136, 160, "odd"), (129, 2, 64, 4128, "even"),
     (256, 8, 776, 544, "odd"), (400, 12, 320, 1440, "even"), (513, 5, 504, 224, "odd"),
-    (700, 3, 2104, 608, "even"), (1000, 9, 96, 2912, "one"), (5000, 255, 288, 128, "odd")]
+    (700, 3, 2104, 608, "even"), (1000, 9, 96, 2912, "one"), (5000, 255, 288, 128, "odd"),
+    (1, 3, 2600, 32, "odd"), (27, 7, 2904, 416, "odd"), (330, 3, 3960, 288, "odd")]
 
 
 @pytest.mark.parametrize("act", [None, "gelu"])
@@ -229,7 +232,8 @@ GATED_BACKWARD = [
     (1, 1, 32, 32, "even"), (4, 32, 96, 64, "even"), (16, 3, 96, 288, "odd"),
     (64, 32, 2880, 1440, "odd"), (100, 256, 160, 160, "odd"), (129, 2, 64, 4128, "even"),
     (256, 8, 768, 544, "odd"), (400, 12, 320, 1440, "even"), (513, 5, 512, 224, "odd"),
-    (700, 3, 2112, 608, "even"), (5000, 255, 288, 128, "odd")]
+    (700, 3, 2112, 608, "even"), (5000, 255, 288, 128, "odd"), (4, 28, 3392, 96, "odd"),
+    (27, 7, 2912, 416, "odd"), (330, 3, 3968, 288, "odd")]
 
 
 @pytest.mark.parametrize("save", ["bf16", "q8"])

@@ -46,8 +46,8 @@ TESTED = {
     ("experts", False, False): experts("experts", sizes.EXPERTS, False, False),
     ("experts", True, False): experts("experts", sizes.GATED, True, False),
     ("experts", True, True): experts("experts", sizes.GATED, True, True),
-    ("experts_back", 0): experts("experts_back", sizes.EXPERTS_BACKWARD, 0),
-    ("experts_back", 1): experts("experts_back", sizes.GATED_BACKWARD, 0),
+    ("experts_back", False): experts("experts_back", sizes.EXPERTS_BACKWARD, False),
+    ("experts_back", True): experts("experts_back", sizes.GATED_BACKWARD, True),
 }
 
 
@@ -77,12 +77,15 @@ def test_every_variant_is_reached_by_a_tested_size(plan, path):
 
 @pytest.mark.parametrize("call,kernel", [
     (("experts", 4, 32, 2880, 2880, 1, 0), "experts decode 0"),      # a token gated
-    (("experts", 8, 32, 2880, 2880, 1, 0), "experts gemm 1"),        # two
+    (("experts", 8, 32, 2880, 2880, 1, 0), "experts gemm 1 0"),      # two
     (("experts", 8, 32, 2880, 2880, 0, 0), "experts decode 1"),      # their down projection
-    (("experts", 16, 32, 2880, 2880, 0, 0), "experts gemm 1"),
-    (("experts", 64, 8, 4096, 5632, 0, 0), "experts gemm 1"),        # eight rows an expert
-    (("experts", 4, 32, 2880, 2880, 1, 1), "experts gemm 1"),        # kept: for a backward pass
-    (("experts", 32768, 128, 768, 2048, 1, 1), "experts gemm 2")])
+    (("experts", 16, 32, 2880, 2880, 0, 0), "experts gemm 1 0"),
+    (("experts", 64, 8, 4096, 5632, 0, 0), "experts gemm 1 0"),      # eight rows an expert
+    (("experts", 4, 32, 2880, 2880, 1, 1), "experts gemm 1 0"),      # kept: for a backward pass
+    (("experts", 32768, 128, 768, 2048, 1, 1), "experts gemm 2 0"),
+    (("experts", 594, 6, 416, 5920, 0, 0), "experts gemm 2 1"),      # few tiles, a long K
+    (("experts_back", 4, 28, 3392, 1024, 1), "experts gemm 1 1"),
+    (("experts_back", 594, 6, 5920, 416, 1), "experts gemm 2 1")])
 def test_kernels_of_measured_sizes(plan, call, kernel):
     assert plan([call]) == [kernel]
 
