@@ -278,7 +278,8 @@ def test_packed_stack_is_the_mixture_layers(gen):
     assert torch.equal(turned[0], ops.mxfp4_pack(blocks[0], scales[0], transposed=True))
 
 
-@pytest.mark.parametrize("m,experts,n,k", [(9, 4, 70, 96), (600, 4, 160, 96)])
+@pytest.mark.parametrize("m,experts,n,k", [(9, 4, 70, 96), (600, 4, 160, 96),
+                                           (60, 4, 96, 4160), (60, 4, 4160, 96)])
 def test_rows_that_no_expert_has_stay(gen, m, experts, n, k):
     """Rows before the first offset and behind the last."""
     n = n // 32 * 32
@@ -353,8 +354,9 @@ def test_strided_rows_and_given_outputs(gen, m):
 
 
 @pytest.mark.parametrize("m", [6, 100, 700])
-def test_strided_rows_of_experts(gen, m):
-    experts, n, k = 4, 96, 160
+@pytest.mark.parametrize("n,k", [(96, 160), (96, 4160), (4160, 160)])  # (K slices of the long ones)
+def test_strided_rows_of_experts(gen, m, n, k):
+    experts = 4
     gate, up, down = stack(gen, experts, n, k), stack(gen, experts, n, k), stack(gen, experts, k, n)
     fwd = [ops.mxfp4_pack(*s) for s in (gate, up, down)]
     back = [ops.mxfp4_pack(*s, transposed=True) for s in (gate, up, down)]
@@ -436,9 +438,10 @@ def test_a_block_without_a_scale_reaches_its_own_results_only(gen, m, k):
             assert torch.equal(got[~hit], want[~hit]) and bool(torch.isnan(got[hit]).all())
 
 
-def test_two_calls_at_once(gen):
+@pytest.mark.parametrize("n,k", [(160, 288), (160, 4160), (4160, 288)])
+def test_two_calls_at_once(gen, n, k):
     """Calls on two streams share nothing."""
-    experts, n, k, top_k = 8, 160, 288, 2
+    experts, top_k = 8, 2
     w = ops.mxfp4_pack(*stack(gen, experts, n, k))
     turned = ops.mxfp4_pack(*stack(gen, experts, n, k), transposed=True)
     batches = []
@@ -468,10 +471,11 @@ def test_two_calls_at_once(gen):
 
 
 @pytest.mark.parametrize("m", [4, 64, 700])
-def test_on_another_stream_and_captured(gen, m):
+@pytest.mark.parametrize("n,k", [(96, 160), (96, 4160), (4160, 160)])
+def test_on_another_stream_and_captured(gen, m, n, k):
     """A graph of the experts' projections and their gradients, replayed with other inputs, and
     other rows for each expert, between eager work."""
-    experts, n, k = 6, 96, 160
+    experts = 6
     gate, up, down = stack(gen, experts, n, k), stack(gen, experts, n, k), stack(gen, experts, k, n)
     fwd = [ops.mxfp4_pack(*s) for s in (gate, up, down)]
     back = [ops.mxfp4_pack(*s, transposed=True) for s in (gate, up, down)]
