@@ -1355,6 +1355,7 @@ struct Gemm {
     unsigned tiles_n, tiles_m;
     Target out;
     float* partial;           // K slices: results go here
+    unsigned slices;
     Stack stack;
 };
 
@@ -1398,23 +1399,32 @@ __global__ __launch_bounds__(512, (shares_unit<TT, OPS> ? 4 : 2)) void gemm_kern
     unsigned tiles = a.tiles_n * a.tiles_m;
     const unsigned xcd = blockIdx.x % 8;
     size_t expert = 0;
-    unsigned tile_m, tile_n, spot = 0;  // spot: the experts' tile among all of them
+    unsigned tile_m, tile_n, slice = blockIdx.y;
+    unsigned spot = 0;  // the experts' tile among all of them
     if constexpr (of_experts(OUT)) {
         // (whole tiles first, then the halves, so that what is left at a launch's end is small: an
-        // XCD has its share of either: 2048 rows of 32 experts of 2880 x 2880 gated 91 us against 97,
-        // 4096 rows 146 against 156)
+        // XCD has its share of either: 2048 rows of 32 experts of 2880 x 2880 gated 91 us against
+        // 97, 4096 rows 146 against 156; all K slices before the workgroups that have no tile, or two
+        // share a compute unit while others are idle: gated backward of 40 rows of 8 experts, 5888
+        // -> 1120 in six slices 22 us against 28)
         const Tiles<kRows, (TT > 1)> list(a.stack, a.out.m);
         const auto share = [&](unsigned n) {
             return n / 8 + (xcd < n % 8);
         };
         unsigned turn = blockIdx.x / 8;
-        tiles = list.whole() * a.tiles_n;
+        tiles = list.whole() * a.tiles_n * a.slices;
         const bool half = turn >= share(tiles);
         if (half) {
             turn -= share(tiles);
-            tiles = list.halves() * a.tiles_n;
+            tiles = list.halves() * a.tiles_n * a.slices;
         }
-        const unsigned tile = xcd * (tiles / 8) + min(xcd, tiles % 8) + turn;
+        const unsigned item = xcd * (tiles / 8) + min(xcd, tiles % 8) + turn;
+        unsigned tile = item;
+        slice = 0;
+        if (a.slices > 1) [[unlikely]] {
+            slice = item / max(tiles / a.slices, 1u);
+            tile -= slice * (tiles / a.slices);
+        }
         const auto p = list.of(tile / a.tiles_n, half);
         if (turn >= share(tiles) || !p.tiles) [[unlikely]]
             return;
@@ -1439,7 +1449,7 @@ __global__ __launch_bounds__(512, (shares_unit<TT, OPS> ? 4 : 2)) void gemm_kern
     constexpr bool kHalfTurns = OUT == kOutExpertsLinear;
     constexpr bool kTwoParts = SPLIT && (OPS != kTransposed || of_one_backward(OUT));
     const auto part_of = [&](unsigned set) {
-        return kTwoParts ? blockIdx.y * 2 + set : blockIdx.y;
+        return kTwoParts ? slice * 2 + set : slice;
     };
     const unsigned begin = min(a.chunks, part_of(kg) * a.part);
     const unsigned end = min(a.chunks, begin + a.part);
@@ -1869,7 +1879,7 @@ __global__ __launch_bounds__(512, (shares_unit<TT, OPS> ? 4 : 2)) void gemm_kern
             if (T < (a.out.m + 31) / 32) {
                 const unsigned row_tiles = of_experts(OUT) ? a.tiles_m * TT : (a.out.m + 31) / 32;
                 auto* to = reinterpret_cast<f32x4*>(
-                               a.partial + ((size_t(blockIdx.y) * (a.tiles_n * 4) + G) * row_tiles +
+                               a.partial + ((size_t(slice) * (a.tiles_n * 4) + G) * row_tiles +
                                             spot * TT + T) * kTileFloats) +
                            lane;
 #pragma unroll
@@ -2099,8 +2109,9 @@ int launch_gemm(const Gemm& a, const Plan& p, hipStream_t st) {
     }
     // (the experts': p.tiles_m is the most that they may have, and eight XCDs' shares of two kinds
     // are rounded up)
-    const unsigned tiles = p.tiles_n * p.tiles_m + (of_experts(OUT) ? 16 : 0);
-    hipLaunchKernelGGL(f, dim3(tiles, p.slices), dim3(512), kLds, st, a);
+    const dim3 grid = of_experts(OUT) ? dim3(p.tiles_n * p.tiles_m * p.slices + 16)
+                                      : dim3(p.tiles_n * p.tiles_m, p.slices);
+    hipLaunchKernelGGL(f, grid, dim3(512), kLds, st, a);
     KDQ_HIP(hipGetLastError());
     return KDQ_OK;
 }
@@ -2151,6 +2162,7 @@ template <int OPS, int OUT> int run_gemm(Gemm a, const Plan& p, void* workspace,
     a.part = p.part;
     a.tiles_n = p.tiles_n;
     a.tiles_m = p.tiles_m;
+    a.slices = p.slices;
     a.partial = p.slices > 1 ? static_cast<float*>(workspace) : nullptr;
     int rc;
     if (!p.split) {

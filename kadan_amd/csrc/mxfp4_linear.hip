@@ -47,7 +47,7 @@ size_t offset_bytes(const int32_t* offsets, size_t experts) {
 // (a launch's threads are counted in 32 bits)
 bool launches(const ExpertsPlan& p) {
     return p.decode ? p.most <= 65535
-                    : p.most * p.tiles_n + 16 <= UINT32_MAX / 512 &&
+                    : p.most * p.tiles_n * p.slices + 16 <= UINT32_MAX / 512 &&
                           (p.slices == 1 || p.tiles_n * 4 * p.most * p.tt <= UINT32_MAX / 256);
 }
 

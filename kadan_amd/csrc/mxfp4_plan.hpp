@@ -235,12 +235,15 @@ inline size_t partial_bytes(const ExpertsPlan& p) {
 }
 
 // K slices where the tiles are too few to fill the compute units: by plan_gemm's estimate, and no
-// shorter than `reached` experts' `bytes` take; over the tiles that as many experts with half a tile
-// more than whole ones would make. `sets`: parts of K that a workgroup takes, of `unit` chunks.
-// (slices of measured calls, with rows an expert as a batch leaves them, us:
-//  gated backward of 4 rows, 3392 -> 1024: 37 as one, 16.9 in 6, 15.7 in 8, 18.1 in 16
-//  594 rows of 6 experts, 5920 -> 416: product 37 as one, 18.8 in 6, 22 in 12; gated backward 89, 32, 33
-//  64 rows of 8 experts, 5632 -> 4096, which reads 92 MB: 24 as one, 29 in 2, 27 in 4)
+// shorter than `reached` experts' `bytes` take, longer where few workgroups ask for them; over the
+// tiles that as many experts with half a tile more than whole ones would make. `sets`: parts of K
+// that a workgroup takes, of `unit` chunks.
+// (measured calls, us by slices, the gated backward's with its gate gradients:
+//  gated backward of 4 rows, 3392 -> 1024: 36.6 as one, 16.8 in 6, 15.7 in 8, 16.2 in 16
+//  594 rows of 6 experts, 5920 -> 416: 88 as one, 31.7 in 6, 29.7 in 8, 33.0 in 12; product 37.6,
+//  19.5 in 6, 23.5 in 12
+//  64 rows of 8 experts, 5632 -> 4096: backward 60 as one, 44 in 2, 48 in 4; product, which reads
+//  92 MB, 24.7, 22.8, 26.2)
 inline void slice_experts(ExpertsPlan& p, size_t m, size_t reached, double bytes, size_t chunks,
                           size_t sets, size_t unit, int ops, size_t cus) {
     const double tiles =
@@ -256,7 +259,8 @@ inline void slice_experts(ExpertsPlan& p, size_t m, size_t reached, double bytes
         const double each = std::ceil(groups / double(cus));
         const double alone = c.fixed + double(part) * c.turn;
         const double both = c.fixed + double(part) * c.turn_of_two;
-        double t = std::max(each <= 1 ? alone : each / 2 * both, bytes / 4.5e6);
+        const double rate = 4.5e6 * std::sqrt(std::min(1.0, groups / (0.75 * double(cus))));
+        double t = std::max(each <= 1 ? alone : each / 2 * both, bytes / rate);
         if (real > 1)
             t += 2 + 0.25 * double(real) + groups * p.tt * 4 * kTileFloats * 4 / 2e6;
         if (slices == 1 || t < best) {
