@@ -482,9 +482,10 @@ int kdq_mxfp4_gated_backward(const uint16_t* dh_bf16, size_t dh_stride, size_t m
  * Of experts: `offsets` (device memory, experts + 1 of them, as kdq_moe_route writes them) says
  * that rows offsets[e] .. offsets[e + 1] - 1 of x, sorted by expert (kdq_moe_sort), are expert e's;
  * it is a stack of `experts` matrices (1 to 256) that the rows are multiplied by, each by its own.
- * Offsets may not decrease; those outside of 0 .. m count as the nearer end.  Results of rows that
- * no expert has are left as they were.  The number of rows of each expert is read on the device
- * only: no call waits for it, and a captured call takes new ones at every replay. */
+ * Offsets may not decrease (the results of a call whose offsets do are undefined, but it reads and
+ * writes no memory that is not its own); those outside of 0 .. m count as the nearer end.  Results
+ * of rows that no expert has are left as they were.  The number of rows of each expert is read on
+ * the device only: no call waits for it, and a captured call takes new ones at every replay. */
 enum kdq_activation {
     KDQ_ACT_NONE = 0,
     KDQ_ACT_SILU = 1,    /* v sigmoid(v) */

@@ -892,10 +892,7 @@ template <unsigned ROWS, bool HALVES> struct Tiles {
         for (unsigned j = 0; j < 4; ++j) {  // (past the last expert: no rows)
             first[j] = at[j];
             end[j] = max(at[j], at[j + 1]);
-            const unsigned rows = end[j] - first[j];
-            tiles[j] = (rows + (HALVES ? ROWS / 2 - 1 : ROWS - 1)) / ROWS;
-            if (HALVES && rows > tiles[j] * ROWS)
-                tiles[j] |= 1u << 16;
+            tiles[j] = tiles_of(end[j] - first[j], ROWS, HALVES);
             sum += tiles[j];
         }
         const unsigned through = lanes_up_to(sum);
@@ -1408,29 +1405,17 @@ __global__ __launch_bounds__(512, (shares_unit<TT, OPS> ? 4 : 2)) void gemm_kern
         // share a compute unit while others are idle: gated backward of 40 rows of 8 experts, 5888
         // -> 1120 in six slices 22 us against 28)
         const Tiles<kRows, (TT > 1)> list(a.stack, a.out.m);
-        const auto share = [&](unsigned n) {
-            return n / 8 + (xcd < n % 8);
-        };
-        unsigned turn = blockIdx.x / 8;
-        tiles = list.whole() * a.tiles_n * a.slices;
-        const bool half = turn >= share(tiles);
-        if (half) {
-            turn -= share(tiles);
-            tiles = list.halves() * a.tiles_n * a.slices;
-        }
-        const unsigned item = xcd * (tiles / 8) + min(xcd, tiles % 8) + turn;
-        unsigned tile = item;
-        slice = 0;
-        if (a.slices > 1) [[unlikely]] {
-            slice = item / max(tiles / a.slices, 1u);
-            tile -= slice * (tiles / a.slices);
-        }
-        const auto p = list.of(tile / a.tiles_n, half);
-        if (turn >= share(tiles) || !p.tiles) [[unlikely]]
+        const ExpertsItem item =
+            experts_item(blockIdx.x, list.whole(), list.halves(), a.tiles_n, a.slices);
+        const auto p = list.of(item.tile / a.tiles_n, item.half);
+        if (!item.there || !p.tiles) [[unlikely]]
             return;
-        const unsigned within = tile - p.before * a.tiles_n;
+        slice = item.slice;
+        const unsigned within = item.tile - p.before * a.tiles_n;
         const unsigned first = p.first + within % p.tiles * kRows;
-        spot = (half ? list.whole() : 0) + p.before + within % p.tiles;
+        spot = (item.half ? list.whole() : 0) + p.before + within % p.tiles;
+        if (a.slices > 1 && !has_partials(spot, a.tiles_m)) [[unlikely]]
+            return;  // (offsets that decrease, which no call may have)
         tile_m = 0;
         tile_n = within / p.tiles;
         move_to<OUT>(a.out, p.expert, first, min(p.end - first, kRows));
@@ -1877,10 +1862,13 @@ __global__ __launch_bounds__(512, (shares_unit<TT, OPS> ? 4 : 2)) void gemm_kern
         const unsigned T = first_tile + t;
         if (a.partial) {
             if (T < (a.out.m + 31) / 32) {
-                const unsigned row_tiles = of_experts(OUT) ? a.tiles_m * TT : (a.out.m + 31) / 32;
                 auto* to = reinterpret_cast<f32x4*>(
-                               a.partial + ((size_t(slice) * (a.tiles_n * 4) + G) * row_tiles +
-                                            spot * TT + T) * kTileFloats) +
+                               a.partial + (of_experts(OUT)
+                                                ? partial_tile(slice, G, spot, T, a.tiles_n, TT,
+                                                               a.tiles_m)
+                                                : (size_t(slice) * (a.tiles_n * 4) + G) *
+                                                          ((a.out.m + 31) / 32) + T) *
+                                               kTileFloats) +
                            lane;
 #pragma unroll
                 for (int i = 0; i < 2; ++i)

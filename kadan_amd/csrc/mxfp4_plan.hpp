@@ -199,6 +199,56 @@ constexpr size_t most_tiles(size_t m, size_t experts, size_t rows) {
     return (m + (rows - 1) * std::min(experts, m)) / rows;
 }
 
+// Tiles of `rows` rows that an expert's `count` rows make: in the low half of a word, and in the high
+// half whether the last has at most half the rows (where `halves` tells such apart: it is then not in
+// the low half).
+constexpr unsigned tiles_of(unsigned count, unsigned rows, bool halves) {
+    const unsigned tiles = (count + (halves ? rows / 2 - 1 : rows - 1)) / rows;
+    return halves && count > tiles * rows ? tiles | 1u << 16 : tiles;
+}
+
+// What workgroup `block` of the experts' launch of gemm_kernel takes: a workgroup's share of whole
+// tile `tile / tiles_n` (or half), or nothing. Workgroups go round the eight XCDs, and an XCD has
+// its share of whole tiles, then of halves, all K slices of either before its workgroups of neither.
+struct ExpertsItem {
+    unsigned tile, slice;
+    bool half, there;
+};
+
+constexpr ExpertsItem experts_item(unsigned block, unsigned whole, unsigned halves,
+                                   unsigned tiles_n, unsigned slices) {
+    const unsigned xcd = block % 8;
+    unsigned turn = block / 8, tiles = whole * tiles_n * slices;
+    unsigned share = tiles / 8 + (xcd < tiles % 8);
+    const bool half = turn >= share;
+    if (half) {
+        turn -= share;
+        tiles = halves * tiles_n * slices;
+        share = tiles / 8 + (xcd < tiles % 8);
+    }
+    ExpertsItem item{xcd * (tiles / 8) + (xcd < tiles % 8 ? xcd : tiles % 8) + turn, 0, half,
+                     turn < share};
+    if (slices > 1) [[unlikely]] {
+        const unsigned each = tiles / slices;
+        item.slice = item.tile / (each ? each : 1);
+        item.tile -= item.slice * each;
+    }
+    return item;
+}
+
+// Where a K slice's partial sums of row tile T (of 32 rows) of the launch's tile `spot` lie, for the
+// wavefronts of row group G: in tiles of kTileFloats, of which there are partial_bytes' for `most`
+// tiles of `tt` row tiles.
+constexpr size_t partial_tile(unsigned slice, unsigned G, unsigned spot, unsigned T,
+                              unsigned tiles_n, unsigned tt, unsigned most) {
+    return (size_t(slice) * (tiles_n * 4) + G) * (most * tt) + spot * tt + T;
+}
+
+// Offsets that decrease may make more tiles than `most`: those have no partial sums.
+constexpr bool has_partials(unsigned spot, unsigned most) {
+    return spot < most;
+}
+
 // How the experts' products run: decode_kernel over tiles of 16 rows, or gemm_kernel over tiles of
 // tt * 32; `most` tiles at most (the device alone knows how many), each in tiles_n workgroups.
 //
