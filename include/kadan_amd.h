@@ -567,8 +567,8 @@ int kdq_mxfp4_experts_gated_backward(const uint16_t* dh_bf16, size_t dh_stride, 
  * different streams may overlap, and every call may be captured. */
 
 /* rows[p] = x[perm[p] / top_k] for the tokens * top_k positions p, and place[perm[p]] = p.  An
- * entry of perm that is no slot gives a row of zeros and no place; perm may not name a slot
- * twice. */
+ * entry of perm that is no slot gives a row of zeros, and a slot that perm does not name (its
+ * selection is dropped) the place -1; perm may not name a slot twice. */
 int kdq_moe_sort(int type, const void* x, size_t x_stride, size_t tokens, size_t cols,
                  size_t top_k, const int32_t* perm, void* rows, size_t rows_stride,
                  int32_t* place, void* stream);

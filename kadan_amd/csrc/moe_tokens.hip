@@ -4,7 +4,7 @@
 // gradients.
 //
 //   sort_kernel            rows[p] = x[perm[p] / top_k], place[perm[p]] = p, by positions
-//   place_kernel, spread_kernel   the same by tokens
+//   place_kernel, spread_kernel   the same by tokens; in both, -1 for a slot that perm does not name
 //   combine_kernel         y[t] = residual[t] + sum_i w[t, i] rows[place[t top_k + i]]; without
 //                          weights the gradient of sorting
 //   combine_grad_kernel    drows[place] = w dy, dw = dy . rows[place]
@@ -157,8 +157,58 @@ Shape shape_of(size_t cols, int values) {
     return {across, kThreads / across, unsigned((pieces + across - 1) / across)};
 }
 
+// The inverse of the permutation, -1 for a slot that it does not name.  A workgroup takes kPlaces
+// slots through LDS and goes over the whole permutation for them, beside the rows' workgroups: 4 and
+// 2048 slots of 2880 bf16 values 2.5 and 4.9 us, as without.  Of narrow rows the scan is what is
+// seen: 64 values, 4096 slots 4.0 us against 2.5, 16384 6.2, 32768 8.7.  By tokens, which needs no
+// scan, those take 7.0 and 7.5, but in two launches, and the second is 3 us of the host.
+constexpr unsigned kPlaces = 4096, kOwnPlaces = 32768;
+
+constexpr unsigned places_groups(unsigned slots) {
+    return (slots + kPlaces - 1) / kPlaces;
+}
+
+__device__ __forceinline__ void write_places(const int32_t* __restrict__ perm, unsigned slots,
+                                             unsigned first, int32_t* __restrict__ place) {
+    __shared__ int32_t at[kPlaces];
+    constexpr unsigned kAhead = 4, kTurn = kAhead * kThreads * 4;
+    const unsigned mine = min(slots - first, kPlaces);
+    for (unsigned s = threadIdx.x; s < mine; s += kThreads)
+        at[s] = -1;
+    __syncthreads();
+    const auto put = [&](int32_t slot, unsigned p) {
+        if (unsigned(slot) < slots && unsigned(slot) - first < mine)
+            at[unsigned(slot) - first] = int32_t(p);
+    };
+    unsigned p0 = 0;
+    for (; p0 + kTurn <= slots; p0 += kTurn) {
+        Piece<float, 4> v[kAhead];
+#pragma unroll
+        for (unsigned i = 0; i < kAhead; ++i)
+            v[i] = load_whole<4>(reinterpret_cast<const float*>(perm) + p0 +
+                                 (i * kThreads + threadIdx.x) * 4);
+#pragma unroll
+        for (unsigned i = 0; i < kAhead; ++i)
+#pragma unroll
+            for (unsigned j = 0; j < 4; ++j)
+                put(int32_t(v[i].w[0][j]), p0 + (i * kThreads + threadIdx.x) * 4 + j);
+    }
+    int32_t rest[kTurn / kThreads];
+#pragma unroll
+    for (unsigned i = 0; i < kTurn / kThreads; ++i) {
+        const unsigned p = p0 + i * kThreads + threadIdx.x;
+        rest[i] = p < slots ? perm[p] : -1;
+    }
+#pragma unroll
+    for (unsigned i = 0; i < kTurn / kThreads; ++i)
+        put(rest[i], p0 + i * kThreads + threadIdx.x);
+    __syncthreads();
+    for (unsigned s = threadIdx.x; s < mine; s += kThreads)
+        place[first + s] = at[s];
+}
+
 // A copy, so bits and no values.  By positions: a row of x is read for each of its places, from
-// the caches but for the first time.
+// the caches but for the first time.  The first of the workgroups take the places.
 template <class U>
 __global__ __launch_bounds__(kThreads) void sort_kernel(const U* __restrict__ x, size_t x_stride,
                                                         unsigned slots, unsigned cols,
@@ -167,7 +217,13 @@ __global__ __launch_bounds__(kThreads) void sort_kernel(const U* __restrict__ x,
                                                         U* __restrict__ rows, size_t rows_stride,
                                                         int32_t* __restrict__ place) {
     constexpr unsigned N = kValues<U, U>;
-    const unsigned p = blockIdx.x * s.rows + threadIdx.x / s.across;
+    const unsigned own = places_groups(slots);
+    if (blockIdx.x < own) {
+        if (blockIdx.y == 0)
+            write_places(perm, slots, blockIdx.x * kPlaces, place);
+        return;
+    }
+    const unsigned p = (blockIdx.x - own) * s.rows + threadIdx.x / s.across;
     const unsigned c = (blockIdx.y * s.across + threadIdx.x % s.across) * N;
     if (p >= slots || c >= cols)
         return;
@@ -178,8 +234,6 @@ __global__ __launch_bounds__(kThreads) void sort_kernel(const U* __restrict__ x,
             to[i] = U{};
         return;
     }
-    if (c == 0)
-        place[slot] = int32_t(p);
     const U* from = x + size_t(slot / top_k) * x_stride + c;
     if (c + N <= cols) {
         store_whole<N>(to, load_whole<N>(from));
@@ -211,8 +265,7 @@ __global__ __launch_bounds__(kThreads) void spread_kernel(const U* __restrict__ 
                                                           unsigned tokens, unsigned cols,
                                                           unsigned top_k, Shape s,
                                                           const int32_t* __restrict__ perm,
-                                                          const int32_t* __restrict__ place,
-                                                          U* __restrict__ rows,
+                                                          int32_t* place, U* __restrict__ rows,
                                                           size_t rows_stride) {
     constexpr unsigned N = kValues<U, U>;
     const unsigned t = blockIdx.x * s.rows + threadIdx.x / s.across;
@@ -227,8 +280,11 @@ __global__ __launch_bounds__(kThreads) void spread_kernel(const U* __restrict__ 
         v = load_whole<N>(from);
     for (unsigned i = 0; i < top_k; ++i) {
         const unsigned slot = t * top_k + i, p = unsigned(place[slot]);
-        if (p >= slots || unsigned(perm[p]) != slot)  // (a slot that perm does not name)
+        if (p >= slots || unsigned(perm[p]) != slot) {  // a slot that perm does not name
+            if (c == 0)
+                place[slot] = -1;  // (another lane finds either value to be none)
             continue;
+        }
         U* to = rows + size_t(p) * rows_stride + c;
         if (whole) {
             store_whole<N>(to, v);
@@ -474,7 +530,7 @@ extern "C" int kdq_moe_sort(int type, const void* x, size_t x_stride, size_t tok
         const auto blocks = [&](size_t count) {
             return dim3(unsigned((count + s.rows - 1) / s.rows), s.blocks);
         };
-        if (top_k > 1 && slots * cols * size_of(type) >= kSpreadBytes) {
+        if (slots > kOwnPlaces || (top_k > 1 && slots * cols * size_of(type) >= kSpreadBytes)) {
             hipLaunchKernelGGL(place_kernel<U>, dim3(unsigned((slots + kThreads - 1) / kThreads)),
                                dim3(kThreads), 0, st, perm, unsigned(slots), unsigned(cols),
                                static_cast<U*>(rows), rows_stride, place);
@@ -483,7 +539,9 @@ extern "C" int kdq_moe_sort(int type, const void* x, size_t x_stride, size_t tok
                                unsigned(cols), unsigned(top_k), s, perm, place,
                                static_cast<U*>(rows), rows_stride);
         } else {
-            hipLaunchKernelGGL(sort_kernel<U>, blocks(slots), dim3(kThreads), 0, st,
+            dim3 grid = blocks(slots);
+            grid.x += places_groups(unsigned(slots));
+            hipLaunchKernelGGL(sort_kernel<U>, grid, dim3(kThreads), 0, st,
                                static_cast<const U*>(x), x_stride, unsigned(slots),
                                unsigned(cols), unsigned(top_k), s, perm, static_cast<U*>(rows),
                                rows_stride, place);

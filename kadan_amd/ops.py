@@ -950,8 +950,10 @@ def _slots(t: torch.Tensor, slots: int, name: str) -> int:
 def moe_sort(x: torch.Tensor, perm: torch.Tensor, top_k: int):
     """Tokens sorted by expert: x [tokens, cols] (fp32, fp16 or bf16) and moe_route's perm ->
     rows [tokens * top_k, cols], rows[p] = x[perm[p] // top_k], and place int32
-    [tokens * top_k], place[perm[p]] = p (kdq_moe_sort).  Nothing is recorded for autograd: its
-    backward pass is moe_sort_backward."""
+    [tokens * top_k], place[perm[p]] = p.  An entry of perm that is no slot (-1, say) gives a row of
+    zeros, and a slot that perm does not name the place -1: a dropped selection, which the calls
+    that take place leave out (kdq_moe_sort).  Nothing is recorded for autograd: its backward pass
+    is moe_sort_backward."""
     if x.requires_grad:
         _no_graph(x, "x")
     kind, stride = _rows_of(x, "x")
