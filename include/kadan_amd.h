@@ -589,7 +589,8 @@ int kdq_moe_combine(int type, const void* rows, size_t rows_stride, const int32_
 
 /* Its gradients: drows[place[t * top_k + i]] = weights[t, i] * dy[t] (of the rows' type) and
  * dweights[t, i] = dy[t] . rows[place[t * top_k + i]] (fp32 sums); dy of type dy_type: the rows'
- * or KDQ_F32.  The residual's gradient is dy. */
+ * or KDQ_F32.  Rows of drows that no place names get zeros, dweights of a place that is no position
+ * 0; no two places may name one position.  The residual's gradient is dy. */
 int kdq_moe_combine_backward(int type, const void* rows, size_t rows_stride, const int32_t* place,
                              const float* weights, size_t tokens, size_t cols, size_t top_k,
                              int dy_type, const void* dy, size_t dy_stride, void* drows,

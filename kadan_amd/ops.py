@@ -1034,7 +1034,8 @@ def moe_combine_backward(dy: torch.Tensor, rows: torch.Tensor, weights: torch.Te
                          place: torch.Tensor):
     """The gradients of moe_combine: dy [tokens, cols] (the rows' type or fp32) and its rows,
     weights and place -> drows [tokens * top_k, cols] of the rows' type and dweights fp32
-    [tokens, top_k] (kdq_moe_combine_backward).  The residual's gradient is dy."""
+    [tokens, top_k] (kdq_moe_combine_backward); zeros for dropped selections (places of -1) and for
+    the rows that no place names.  The residual's gradient is dy."""
     if dy.requires_grad:
         _no_graph(dy, "dy")
     kind, stride = _rows_of(rows, "rows")

@@ -107,3 +107,32 @@ def test_dropped_selections_on_their_way_back(gen, tokens, top_k, cols, dtype):
     slot = perm[~gone].long()
     want = dy.double()[slot // top_k] * weights.double().reshape(-1, 1)[slot]
     within(drows[~gone], want, HALF[F32] * want.abs())
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("tokens,top_k,cols", SIZES + [(1024, 8, 500), (1025, 8, 500),
+                                                       (4096, 8, 1600), (10923, 3, 1537)])
+def test_rows_that_no_place_names_have_a_gradient_of_zero(gen, tokens, top_k, cols, dtype):
+    """Into rows of NaN, some values apart; the values between them stay."""
+    slots = tokens * top_k
+    perm, gone = dropped(gen, slots, 0.25)
+    place = places(perm)
+    place[place < 0] = torch.tensor([-1, slots, 2 ** 31 - 1, -(2 ** 31)], dtype=torch.int32,
+                                    device=gen.device).repeat(slots)[:int((place < 0).sum())]
+    rows, dy = normal(gen, slots, cols).to(dtype), normal(gen, tokens, cols).to(dtype)
+    weights = torch.rand(tokens, top_k, generator=gen, device=gen.device)
+    drows = torch.full((slots, cols + 3), float("nan"), dtype=dtype, device=gen.device)
+    dweights = torch.full((tokens, top_k), float("nan"), device=gen.device)
+    kadan_amd.call("kdq_moe_combine_backward", KIND[dtype], rows.data_ptr(), cols, place.data_ptr(),
+                   weights.data_ptr(), tokens, cols, top_k, KIND[dtype], dy.data_ptr(), cols,
+                   drows.data_ptr(), cols + 3, dweights.data_ptr(),
+                   torch.cuda.current_stream().cuda_stream)
+    assert bool(drows[:, cols:].isnan().all())
+    assert not bool(drows[gone, :cols].any())
+    slot = perm[~gone].long()
+    want = dy.double()[slot // top_k] * weights.double().reshape(-1, 1)[slot]
+    off = (drows[~gone, :cols].double() - want).abs()
+    bound = HALF[F32] * want.abs()
+    assert bool((off <= bound + (want.abs() + bound) * HALF[dtype] + LEAST[dtype]).all())
+    again, dw = ops.moe_combine_backward(dy, rows, weights, place)
+    assert torch.equal(again, drows[:, :cols]) and torch.equal(dw, dweights)
