@@ -237,35 +237,23 @@ __global__ __launch_bounds__(kThreads) void sort_kernel(const U* __restrict__ x,
         return;
     const unsigned slot = unsigned(perm[p]);
     U* to = rows + size_t(p) * rows_stride + c;
-    if (slot >= slots) {  // no slot: a row of zeros
-        for (unsigned i = 0; i < N && c + i < cols; ++i)
-            to[i] = U{};
-        return;
-    }
-    const U* from = x + size_t(slot / top_k) * x_stride + c;
+    const bool some = slot < slots;  // (no slot: a row of zeros)
+    const U* from = x + size_t(some ? slot / top_k : 0) * x_stride + c;
     if (c + N <= cols) {
-        store_whole<N>(to, load_whole<N>(from));
+        store_whole<N>(to, some ? load_whole<N>(from) : Piece<U, N>{});
     } else {
         for (unsigned i = 0; c + i < cols; ++i)
-            to[i] = from[i];
+            to[i] = some ? from[i] : U{};
     }
 }
 
 // The same by tokens, once the places are known: a row of x is read once.
-template <class U>
 __global__ __launch_bounds__(kThreads) void place_kernel(const int32_t* __restrict__ perm,
-                                                         unsigned slots, unsigned cols,
-                                                         U* __restrict__ rows, size_t rows_stride,
+                                                         unsigned slots,
                                                          int32_t* __restrict__ place) {
     const unsigned p = blockIdx.x * kThreads + threadIdx.x;
-    if (p >= slots)
-        return;
-    if (unsigned(perm[p]) < slots) {
+    if (p < slots && unsigned(perm[p]) < slots)
         place[perm[p]] = int32_t(p);
-    } else {
-        for (unsigned c = 0; c < cols; ++c)
-            rows[size_t(p) * rows_stride + c] = U{};
-    }
 }
 
 template <class U>
@@ -286,8 +274,10 @@ __global__ __launch_bounds__(kThreads) void spread_kernel(const U* __restrict__ 
     Piece<U, N> v;
     if (whole)
         v = load_whole<N>(from);
+    bool holes = false;
     for (unsigned i = 0; i < top_k; ++i) {
         const unsigned slot = t * top_k + i, p = unsigned(place[slot]);
+        holes |= unsigned(perm[slot]) >= slots;
         if (p >= slots || unsigned(perm[p]) != slot) {  // a slot that perm does not name
             if (c == 0)
                 place[slot] = -1;  // (another lane finds either value to be none)
@@ -301,6 +291,17 @@ __global__ __launch_bounds__(kThreads) void spread_kernel(const U* __restrict__ 
                 to[j] = from[j];
         }
     }
+    if (holes) [[unlikely]]  // entries that are no slot: rows of zeros
+        for (unsigned p = t * top_k; p < (t + 1) * top_k; ++p)
+            if (unsigned(perm[p]) >= slots) {
+                U* to = rows + size_t(p) * rows_stride + c;
+                if (whole) {
+                    store_whole<N>(to, Piece<U, N>{});
+                } else {
+                    for (unsigned j = 0; c + j < cols; ++j)
+                        to[j] = U{};
+                }
+            }
 }
 
 // Sums in fp32, in the order of the selection, and one rounding.  Every row of a token is asked for
@@ -348,49 +349,48 @@ __global__ __launch_bounds__(kThreads) void combine_kernel(
 
 // Zeros in every row from `first` on whose lane asks for them, by the whole wavefront.
 template <class T>
-__device__ __forceinline__ void zero_rows(bool mine, unsigned first, unsigned cols, T* drows,
-                                          size_t drows_stride) {
+__device__ __forceinline__ void zero_rows(bool mine, unsigned first, unsigned cols, T* rows,
+                                          size_t stride) {
     constexpr int N = kValues<T, T>;
     const float zeros[N] = {};
     for (uint64_t left = __builtin_amdgcn_ballot_w64(mine); left; left &= left - 1) {
-        T* row = drows + size_t(first + unsigned(__builtin_ctzll(left))) * drows_stride;
+        T* row = rows + size_t(first + unsigned(__builtin_ctzll(left))) * stride;
         for (unsigned c = threadIdx.x % 64 * N; c < cols; c += 64 * N)
             store_piece<N>(row, c, cols, zeros);
     }
 }
 
-// Rows of drows that no place names (as many as selections are dropped) get zeros.  A workgroup
-// takes kPlaces positions and marks those that one of all the places names, beside the tokens'
-// workgroups: one launch for as many slots as its threads scan about as fast as another two launches
-// begin.  4096 slots of 2048 bf16 values 9.9 us against 9.1 without, 4096 of 128 (64 threads) 12.2
-// against 6.4, in three launches 10.0 and 6 us more of the host; 32768 of 2048 in three 51 against 47
-// (in one 59, by the registers that the scan takes from the rows').
-constexpr size_t most_marked(unsigned threads) {
-    return threads * 64;
-}
+// Rows of drows that no place names (as many as selections are dropped) get zeros.  Up to
+// kMostMarked slots this is the tokens' launch: a workgroup goes over all the places and marks which
+// of its kMarked positions they name.  5 slots' tokens 6.0 us against 5.3 without, 4096 slots of 2048
+// bf16 values 10.0 against 9.1, 16384 of 512 14.2 against 9.1, in three launches 12.9 and 6 us more
+// of the host; 32768 of 2048 in three launches 51 against 47, in one 57.
+constexpr unsigned kMarked = 64, kMostMarked = 16384;
 
 template <class T>
 __device__ __forceinline__ void zero_unnamed(const int32_t* __restrict__ place, unsigned slots,
                                              unsigned first, unsigned cols, T* drows,
                                              size_t drows_stride) {
-    __shared__ uint8_t named[kPlaces];
-    const unsigned mine = min(slots - first, kPlaces);
-    for (unsigned p = threadIdx.x; p < mine; p += blockDim.x)
-        named[p] = 0;
+    __shared__ uint8_t named[kMarked];
+    if (threadIdx.x < kMarked)
+        named[threadIdx.x] = 0;
     __syncthreads();
     for_each(place, slots, blockDim.x, [&](int32_t p, unsigned) {
-        if (unsigned(p) < slots && unsigned(p) - first < mine)
+        if (unsigned(p) < slots && unsigned(p) - first < kMarked)
             named[unsigned(p) - first] = 1;
     });
     __syncthreads();
-    for (unsigned p = threadIdx.x / 64 * 64; p < mine; p += blockDim.x) {
-        const unsigned at = p + threadIdx.x % 64;
-        zero_rows(at < mine && !named[at], first + p, cols, drows, drows_stride);
-    }
+    const unsigned waves = blockDim.x / 64, share = (kMarked + waves - 1) / waves;
+    const unsigned lane = threadIdx.x % 64, at = threadIdx.x / 64 * share;
+    zero_rows(lane < share && at + lane < kMarked && first + at + lane < slots && !named[at + lane],
+              first + at, cols, drows, drows_stride);
 }
 
 // The same ahead of the tokens' launch, by the places' inverse, which goes where the weights'
 // gradients will be.  It needs no clearing: what is left there of another use does not lead back.
+// A wavefront takes kZeroed positions.
+constexpr unsigned kZeroed = 8;
+
 __global__ __launch_bounds__(kThreads) void inverse_kernel(const int32_t* __restrict__ place,
                                                            unsigned slots,
                                                            int32_t* __restrict__ slot) {
@@ -405,10 +405,11 @@ __global__ __launch_bounds__(kThreads) void zero_kernel(const int32_t* __restric
                                                         unsigned slots, unsigned cols,
                                                         T* __restrict__ drows,
                                                         size_t drows_stride) {
-    const unsigned p = blockIdx.x * kThreads + threadIdx.x;
-    const unsigned of = p < slots ? unsigned(slot[p]) : 0;
-    zero_rows(p < slots && (of >= slots || unsigned(place[of]) != p), p / 64 * 64, cols, drows,
-              drows_stride);
+    const unsigned lane = threadIdx.x % 64;
+    const unsigned first = (blockIdx.x * kThreads + threadIdx.x) / 64 * kZeroed, p = first + lane;
+    const bool mine = lane < kZeroed && p < slots;
+    const unsigned of = mine ? unsigned(slot[p]) : 0;
+    zero_rows(mine && (of >= slots || unsigned(place[of]) != p), first, cols, drows, drows_stride);
 }
 
 // A workgroup takes a token: its dy is read once for all of its rows, and one pass over those gives
@@ -423,9 +424,9 @@ __global__ __launch_bounds__(kThreads) void combine_grad_kernel(
     constexpr int N = kValues<T, Y>;
     __shared__ float sums[kThreads / 64][kMost];
     const unsigned slots = tokens * top_k;
-    const unsigned zeroing = ZEROES ? places_groups(slots) : 0;
+    const unsigned zeroing = ZEROES ? (slots + kMarked - 1) / kMarked : 0;
     if (blockIdx.x < zeroing) {  // (the first, so that none is waited for in the end)
-        zero_unnamed(place, slots, blockIdx.x * kPlaces, cols, drows, drows_stride);
+        zero_unnamed(place, slots, blockIdx.x * kMarked, cols, drows, drows_stride);
         return;
     }
     const unsigned t = blockIdx.x - zeroing;
@@ -610,9 +611,8 @@ extern "C" int kdq_moe_sort(int type, const void* x, size_t x_stride, size_t tok
             return dim3(unsigned((count + s.rows - 1) / s.rows), s.blocks);
         };
         if (slots > kOwnPlaces || (top_k > 1 && slots * cols * size_of(type) >= kSpreadBytes)) {
-            hipLaunchKernelGGL(place_kernel<U>, dim3(unsigned((slots + kThreads - 1) / kThreads)),
-                               dim3(kThreads), 0, st, perm, unsigned(slots), unsigned(cols),
-                               static_cast<U*>(rows), rows_stride, place);
+            hipLaunchKernelGGL(place_kernel, dim3(unsigned((slots + kThreads - 1) / kThreads)),
+                               dim3(kThreads), 0, st, perm, unsigned(slots), place);
             hipLaunchKernelGGL(spread_kernel<U>, blocks(tokens), dim3(kThreads), 0, st,
                                static_cast<const U*>(x), x_stride, unsigned(tokens),
                                unsigned(cols), unsigned(top_k), s, perm, place,
@@ -711,16 +711,18 @@ extern "C" int kdq_moe_combine_backward(int type, const void* rows, size_t rows_
         using T = decltype(t);
         using Y = decltype(u);
         const auto st = static_cast<hipStream_t>(stream);
-        const bool marked = slots <= most_marked(threads);
-        const unsigned zeroing = marked ? places_groups(unsigned(slots)) : 0;
+        const bool marked = slots <= kMostMarked;
+        const unsigned zeroing = marked ? unsigned((slots + kMarked - 1) / kMarked) : 0;
         if (!marked) {
             auto* slot = reinterpret_cast<int32_t*>(dweights);
-            const dim3 grid(unsigned((slots + kThreads - 1) / kThreads));
-            hipLaunchKernelGGL(inverse_kernel, grid, dim3(kThreads), 0, st, place,
+            const auto grid = [&](unsigned each) {  // positions of a workgroup
+                return dim3(unsigned((slots + each - 1) / each));
+            };
+            hipLaunchKernelGGL(inverse_kernel, grid(kThreads), dim3(kThreads), 0, st, place,
                                unsigned(slots), slot);
-            hipLaunchKernelGGL(zero_kernel<T>, grid, dim3(kThreads), 0, st, place, slot,
-                               unsigned(slots), unsigned(cols), static_cast<T*>(drows),
-                               drows_stride);
+            hipLaunchKernelGGL(zero_kernel<T>, grid(kThreads / 64 * kZeroed), dim3(kThreads), 0,
+                               st, place, slot, unsigned(slots), unsigned(cols),
+                               static_cast<T*>(drows), drows_stride);
         }
         const auto kernel =
             marked ? combine_grad_kernel<T, Y, true> : combine_grad_kernel<T, Y, false>;

@@ -110,8 +110,9 @@ def test_dropped_selections_on_their_way_back(gen, tokens, top_k, cols, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
-@pytest.mark.parametrize("tokens,top_k,cols", SIZES + [(1024, 8, 500), (1025, 8, 500),
-                                                       (4096, 8, 1600), (10923, 3, 1537)])
+@pytest.mark.parametrize("tokens,top_k,cols", SIZES + [(512, 8, 500), (513, 8, 500),
+                                                       (700, 6, 1400), (2048, 8, 1600),
+                                                       (10923, 3, 1537)])
 def test_rows_that_no_place_names_have_a_gradient_of_zero(gen, tokens, top_k, cols, dtype):
     """Into rows of NaN, some values apart; the values between them stay."""
     slots = tokens * top_k
@@ -136,3 +137,32 @@ def test_rows_that_no_place_names_have_a_gradient_of_zero(gen, tokens, top_k, co
     assert bool((off <= bound + (want.abs() + bound) * HALF[dtype] + LEAST[dtype]).all())
     again, dw = ops.moe_combine_backward(dy, rows, weights, place)
     assert torch.equal(again, drows[:, :cols]) and torch.equal(dw, dweights)
+
+
+@pytest.mark.parametrize("way", ["sort", "back"])
+@pytest.mark.parametrize("tokens,top_k,cols", [(4096, 8, 2048), (600, 8, 16384), (500, 8, 16384)])
+def test_dropped_selections_cost_no_more_than_the_others(gen, tokens, top_k, cols, way):
+    """Rows of zeros are written by as many lanes as rows of tokens: a permutation of which half is
+    dropped takes no twice as long as one of which nothing is."""
+    slots = tokens * top_k
+    x = normal(gen, tokens, cols).bfloat16()
+    rows, weights = normal(gen, slots, cols).bfloat16(), normal(gen, tokens, top_k)
+    took = []
+    for share in (None, 0.5):
+        perm = (dropped(gen, slots, share)[0] if share else
+                torch.randperm(slots, generator=gen, device=gen.device).int())
+        place = places(perm)
+        times = []
+        for _ in range(7):
+            begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            begin.record()
+            for _ in range(5):
+                if way == "sort":
+                    ops.moe_sort(x, perm, top_k)
+                else:
+                    ops.moe_combine_backward(x, rows, weights, place)
+            end.record()
+            end.synchronize()
+            times.append(begin.elapsed_time(end))
+        took.append(sorted(times)[len(times) // 2])
+    assert took[1] <= 2 * took[0]
