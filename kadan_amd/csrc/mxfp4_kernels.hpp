@@ -1516,6 +1516,9 @@ __global__ __launch_bounds__(512, (shares_unit<TT, OPS> ? 4 : 2)) void gemm_kern
     // (in scalar registers, or every load would loop over its buffer's possible values)
     const unsigned end_step = uniform(min(a.steps, end * kStepsPerChunk));
     const unsigned begin_step = uniform(begin * kStepsPerChunk);
+    // (a part of nothing begins where K ends, within four steps' scales: zero codes times another
+    // row's scale there would be NaN where that is)
+    const bool some = begin_step < end_step;
     const unsigned scale_groups = (a.steps + 3) / 4;
     __amdgpu_buffer_rsrc_t codes_buf[2], scales_buf[2];
 #pragma unroll
@@ -1535,7 +1538,8 @@ __global__ __launch_bounds__(512, (shares_unit<TT, OPS> ? 4 : 2)) void gemm_kern
         if constexpr (OPS == kTransposed)
             scales_buf[t] = buffer(s + g * a.steps * 128, there ? end_step * 128 : 0);
         else
-            scales_buf[t] = buffer(s + g * scale_groups * 256, there ? scale_groups * 256 : 0);
+            scales_buf[t] =
+                buffer(s + g * scale_groups * 256, there && some ? scale_groups * 256 : 0);
     }
     // steps (registers for two are left, or several workgroups share a compute unit)
     constexpr int kAhead =
