@@ -520,9 +520,10 @@ int kdq_mxfp4_linear(const uint16_t* x_bf16, size_t x_stride, size_t m, const in
 /* Its backward pass over frozen weights: dpre [m x n] bf16 = dy * act'(pre) from dy bf16 and
  * kept_bf16, and dx [m x k] bf16 = dpre W, the products of the rounded dpre exact and their sums
  * fp32.  (KDQ_ACT_NONE: dpre is dy; kept_bf16 and dpre are null.)  The bias's gradient is the sum
- * of dpre's rows, the residual's is dy.  Weights from kdq_mxfp4_pack_transposed, or
- * kdq_mxfp4_experts_pack_transposed with offsets; n % 8 == 0; of experts: dx of rows that no expert
- * has is left as it was (dpre is not); the workspace's `experts` is 0 for dense calls. */
+ * of dpre's rows (an expert's of its own rows), the residual's is dy.  Weights from
+ * kdq_mxfp4_pack_transposed, or kdq_mxfp4_experts_pack_transposed with offsets; n % 8 == 0; of
+ * experts: dx of rows that no expert has is left as it was (dpre is not); the workspace's `experts`
+ * is 0 for dense calls. */
 size_t kdq_mxfp4_linear_backward_workspace(size_t m, size_t experts, size_t n, size_t k);
 int kdq_mxfp4_linear_backward(const uint16_t* dy_bf16, size_t dy_stride, size_t m,
                               const int32_t* offsets, size_t experts, const uint16_t* kept_bf16,

@@ -4,7 +4,7 @@
 // gradients.
 //
 //   sort_kernel            rows[p] = x[perm[p] / top_k], place[perm[p]] = p, by positions
-//   place_kernel, spread_kernel   the same by tokens; in both, -1 for a slot that perm does not name
+//   place_kernel, spread_kernel   the same by tokens (-1 for a slot that perm does not name)
 //   combine_kernel         y[t] = residual[t] + sum_i w[t, i] rows[place[t top_k + i]]; without
 //                          weights the gradient of sorting
 //   combine_grad_kernel    drows[place] = w dy, dw = dy . rows[place]
@@ -140,8 +140,9 @@ __device__ __forceinline__ void store_piece(T* row, unsigned c, unsigned cols,
 }
 
 // From this many bytes of rows on they are written by tokens, in two launches: 32768 rows of 2048
-// bf16 values 26.6 us against 37.5 by positions (5.7 TB/s of what has to move), 8192 of 2880 13.3
-// against 14.8, 4096 of 2048 (17 MB) 7.4 against 6.3.
+// bf16 values 33.3 us against 38.5 by positions (4.5 TB/s of what has to move, of tensors that are
+// not in the caches), 8192 of 2880 (45 MB) 14.2 against 15.5, 8192 of 2048 (32 MB) 11.4 against
+// 11.1, 4096 of 2048 (16 MB) 8.5 against 6.7.
 constexpr size_t kSpreadBytes = size_t(32) << 20;
 
 // How a launch's workgroups share rows of `cols` values: `across` lanes (a power of two) along a
@@ -159,10 +160,10 @@ Shape shape_of(size_t cols, int values) {
 }
 
 // The inverse of the permutation, -1 for a slot that it does not name.  A workgroup takes kPlaces
-// slots through LDS and goes over the whole permutation for them, beside the rows' workgroups: 4 and
-// 2048 slots of 2880 bf16 values 2.5 and 4.9 us, as without.  Of narrow rows the scan is what is
-// seen: 64 values, 4096 slots 4.0 us against 2.5, 16384 6.2, 32768 8.7.  By tokens, which needs no
-// scan, those take 7.0 and 7.5, but in two launches, and the second is 3 us of the host.
+// slots through LDS and goes over the whole permutation for them, beside the rows' workgroups: 4
+// and 2048 slots of 2880 bf16 values 2.5 and 4.9 us, as without.  Of narrow rows the scan is what
+// is seen: 64 values, 4096 slots 4.0 us against 2.5, 16384 6.2, 32768 8.7.  By tokens, which needs
+// no scan, those take 7.0 and 7.5, but in two launches, and the second is 3 us of the host.
 constexpr unsigned kPlaces = 4096, kOwnPlaces = 32768;
 
 constexpr unsigned places_groups(unsigned slots) {
@@ -305,8 +306,9 @@ __global__ __launch_bounds__(kThreads) void spread_kernel(const U* __restrict__ 
 }
 
 // Sums in fp32, in the order of the selection, and one rounding.  Every row of a token is asked for
-// at once.  32768 rows of 2048 bf16 values to 4096 tokens 24.7 us (6.1 TB/s), with weights and a
-// residual 28 (6.0); a few tokens 3 us, the launch and two loads, one behind the other.
+// at once.  32768 rows of 2048 bf16 values to 4096 tokens 33 us (4.6 TB/s), with weights and a
+// residual 43 (3.9), of tensors that are not in the caches; a few tokens 3.4 us, the launch and two
+// loads, one behind the other.
 template <class T, class Y>
 __global__ __launch_bounds__(kThreads) void combine_kernel(
     const T* __restrict__ rows, size_t rows_stride, const int32_t* __restrict__ place,
@@ -361,10 +363,10 @@ __device__ __forceinline__ void zero_rows(bool mine, unsigned first, unsigned co
 }
 
 // Rows of drows that no place names (as many as selections are dropped) get zeros.  Up to
-// kMostMarked slots this is the tokens' launch: a workgroup goes over all the places and marks which
-// of its kMarked positions they name.  5 slots' tokens 6.0 us against 5.3 without, 4096 slots of 2048
-// bf16 values 10.0 against 9.1, 16384 of 512 14.2 against 9.1, in three launches 12.9 and 6 us more
-// of the host; 32768 of 2048 in three launches 51 against 47, in one 57.
+// kMostMarked slots this is the tokens' launch: a workgroup goes over all the places and marks
+// which of its kMarked positions they name.  20 slots of 2880 bf16 values 6.0 us against 5.3
+// without, 4096 of 2048 10.0 against 9.1, 16384 of 512 14.2 against 9.1, in three launches 12.9 and
+// 6 us more of the host; 32768 of 2048 in three launches 51 against 47, in one 57.
 constexpr unsigned kMarked = 64, kMostMarked = 16384;
 
 template <class T>
@@ -414,7 +416,7 @@ __global__ __launch_bounds__(kThreads) void zero_kernel(const int32_t* __restric
 
 // A workgroup takes a token: its dy is read once for all of its rows, and one pass over those gives
 // both gradients; dot products are summed lane by lane, then over lanes and wavefronts in their
-// order, so results do not depend on the run.  32768 rows of 2048 bf16 values 49 us (5.8 TB/s).
+// order, so results do not depend on the run.  32768 rows of 2048 bf16 values 48 us (6.0 TB/s).
 template <class T, class Y, bool ZEROES>
 __global__ __launch_bounds__(kThreads) void combine_grad_kernel(
     const T* __restrict__ rows, size_t rows_stride, const Y* __restrict__ dy, size_t dy_stride,

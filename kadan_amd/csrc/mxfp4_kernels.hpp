@@ -1,7 +1,8 @@
 // The kernels of MXFP4 dense layers for gfx950 and their launches: products with a packed matrix,
-// the gated feed-forward projection and its backward pass (include/kadan_amd.h; entry points in
-// mxfp4_dense.hip).  The reference multiplies MXFP4 rows on the host only
-// (IW/src/weights/quantization.cpp:207-247; IW = services/hikari/inference_worker).
+// the gated feed-forward projection and its backward pass, dense and of a mixture's experts
+// (include/kadan_amd.h; entry points in mxfp4_dense.hip and mxfp4_linear.hip).  The reference
+// multiplies MXFP4 rows on the host only (IW/src/weights/quantization.cpp:207-247; IW =
+// services/hikari/inference_worker).
 //
 //   pack_kernel        rows -> the packed form every product reads
 //   pack_t_kernel      rows -> the form the backward pass reads (summed over the rows)
@@ -272,7 +273,7 @@ __device__ __forceinline__ unsigned bf16_pair(float a, float b) {
     return bits(v);
 }
 
-// silu(g) * u with the hardware exp2 and reciprocal (about 2^-22 relative; h leaves as bf16)
+// silu(g) * u with the hardware exp2 and reciprocal (2^-21 (1 + |g|) relative; h leaves as bf16)
 __device__ __forceinline__ float gate_value(float g, float u) {
     const float e = __builtin_amdgcn_exp2f(-1.44269504f * g);
     return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
@@ -314,7 +315,8 @@ __device__ __forceinline__ void store4_f32(float* y, size_t stride, unsigned n, 
     }
 }
 
-// sigmoid, by the hardware exp2 and reciprocal (about 2^-22 relative)
+// sigmoid, by the hardware exp2 and reciprocal: each is within 2^-22, and the argument, rounded to
+// fp32 twice, adds 2^-21 |z| (all relative); below about -88 the result is 0.
 __device__ __forceinline__ float sigmoid_value(float z) {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504f * z));
 }
@@ -851,8 +853,9 @@ struct Decode {
 // The rows of x are sorted by expert, and only the device knows where each expert's begin, so a
 // launch has as many workgroups as any sizes could need and each finds its own: every wavefront
 // reads all the offsets (a quad of experts a lane), counts the tiles of `rows_of_tile` rows and
-// adds up the counts along the lanes.  About a microsecond ahead of the first load of weights;
-// a launch that wrote a list of tiles first would take several.
+// adds up the counts along the lanes.  That takes 0.6 to 0.8 us ahead of the first load of
+// weights, 0.9 to 1.1 where the offsets come out of memory (32 to 256 experts); a launch that wrote
+// a list of tiles first would take several.
 
 __device__ __forceinline__ unsigned uniform(unsigned v) {
     return unsigned(__builtin_amdgcn_readfirstlane(int(v)));
@@ -1401,9 +1404,9 @@ __global__ __launch_bounds__(512, (shares_unit<TT, OPS> ? 4 : 2)) void gemm_kern
     if constexpr (of_experts(OUT)) {
         // (whole tiles first, then the halves, so that what is left at a launch's end is small: an
         // XCD has its share of either: 2048 rows of 32 experts of 2880 x 2880 gated 91 us against
-        // 97, 4096 rows 146 against 156; all K slices before the workgroups that have no tile, or two
-        // share a compute unit while others are idle: gated backward of 40 rows of 8 experts, 5888
-        // -> 1120 in six slices 22 us against 28)
+        // 97, 4096 rows 146 against 156; all K slices before the workgroups that have no tile, or
+        // two share a compute unit while others are idle: gated backward of 40 rows of 8 experts,
+        // 5888 -> 1120 in six slices 22 us against 28)
         const Tiles<kRows, (TT > 1)> list(a.stack, a.out.m);
         const ExpertsItem item =
             experts_item(blockIdx.x, list.whole(), list.halves(), a.tiles_n, a.slices);
@@ -2059,7 +2062,9 @@ __global__ __launch_bounds__(256) void gate_grad_kernel(const uint16_t* __restri
               bf16_pair(ru[6], ru[7])};
 }
 
-// dpre = dy act'(pre) of a product's activation, eight columns a lane (n % 8 == 0).
+// dpre = dy act'(pre) of a product's activation, eight columns a lane (n % 8 == 0).  It leaves as
+// bf16 for dg's and du's reasons (above): dx is off by 2.3e-3 of its root mean square, 1.7e-3 being
+// its own rounding.  Bound by memory: 1024 x 14336 17 us (88 MB, 5.2 TB/s).
 __global__ __launch_bounds__(256) void act_grad_kernel(const uint16_t* __restrict__ dy,
                                                        size_t dy_stride, unsigned m, unsigned n,
                                                        const uint16_t* __restrict__ kept, int act,

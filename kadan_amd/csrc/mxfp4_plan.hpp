@@ -199,9 +199,9 @@ constexpr size_t most_tiles(size_t m, size_t experts, size_t rows) {
     return (m + (rows - 1) * std::min(experts, m)) / rows;
 }
 
-// Tiles of `rows` rows that an expert's `count` rows make: in the low half of a word, and in the high
-// half whether the last has at most half the rows (where `halves` tells such apart: it is then not in
-// the low half).
+// Tiles of `rows` rows that an expert's `count` rows make: in the low half of a word, and in the
+// high half whether the last has at most half the rows (where `halves` tells such apart: it is then
+// not in the low half).
 constexpr unsigned tiles_of(unsigned count, unsigned rows, bool halves) {
     const unsigned tiles = (count + (halves ? rows / 2 - 1 : rows - 1)) / rows;
     return halves && count > tiles * rows ? tiles | 1u << 16 : tiles;
@@ -209,7 +209,8 @@ constexpr unsigned tiles_of(unsigned count, unsigned rows, bool halves) {
 
 // What workgroup `block` of the experts' launch of gemm_kernel takes: a workgroup's share of whole
 // tile `tile / tiles_n` (or half), or nothing. Workgroups go round the eight XCDs, and an XCD has
-// its share of whole tiles, then of halves, all K slices of either before its workgroups of neither.
+// its share of whole tiles, then of halves, all K slices of either before its workgroups of
+// neither.
 struct ExpertsItem {
     unsigned tile, slice;
     bool half, there;
@@ -236,9 +237,9 @@ constexpr ExpertsItem experts_item(unsigned block, unsigned whole, unsigned halv
     return item;
 }
 
-// Where a K slice's partial sums of row tile T (of 32 rows) of the launch's tile `spot` lie, for the
-// wavefronts of row group G: in tiles of kTileFloats, of which there are partial_bytes' for `most`
-// tiles of `tt` row tiles.
+// Where a K slice's partial sums of row tile T (of 32 rows) of the launch's tile `spot` lie, for
+// the wavefronts of row group G: in tiles of kTileFloats, of which there are partial_bytes' for
+// `most` tiles of `tt` row tiles.
 constexpr size_t partial_tile(unsigned slice, unsigned G, unsigned spot, unsigned T,
                               unsigned tiles_n, unsigned tt, unsigned most) {
     return (size_t(slice) * (tiles_n * 4) + G) * (most * tt) + spot * tt + T;
@@ -268,6 +269,7 @@ constexpr bool has_partials(unsigned spot, unsigned most) {
 // their gradients gated 16 76, 83; 32 100, 89; down 16 32, 38; 32 49, 42; 64 65, 62; 128 experts of
 // 2048 x 768 gated 32 53, 52; 64 73, 67; down (K of 768, where a workgroup's fixed part is the
 // larger) 32 38, 38; 64 54, 50; gradients gated 16 55, 54; 32 71, 67; down 16 24, 27; 32 34, 29.
+// (That border of K, 1536, lies between the two widths measured, 768 and 2880.)
 // Tiles of 96 and 128 rows have a unit to themselves and lose by 5 to 50 % up to 512 rows an
 // expert; at 2048 they are within 2 % of those of 64.
 struct ExpertsPlan {
@@ -331,7 +333,7 @@ inline ExpertsPlan plan_experts(size_t m, size_t experts, size_t n, size_t k, bo
         // (runs of four units, a batch whose loads are all in flight at once, and where two matrices
         // are twice as many, of eight: gated 2880 -> 2880 of a token 10.7 us over 3 wavefronts, 11.4
         // over 4, 12.1 over 6, 2048 -> 768 6.2 over 4, 7.3 over 2; down 5632 -> 4096 8.2 over 11,
-        // 9.3 over 6)
+        // 9.3 over 6; the border, 2048, is the last width measured the one way, 2880 the next)
         const size_t units = ceil_div(k, 128), run = gated && units > 16 ? 8 : 4;
         p.shape.waves = unsigned(std::min<size_t>(ceil_div(units, run), 16));
         p.shape.units = unsigned(ceil_div(ceil_div(units, p.shape.waves), 2) * 2);

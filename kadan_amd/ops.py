@@ -734,9 +734,10 @@ def mxfp4_linear(x: torch.Tensor, packed: torch.Tensor, n_out: int,
     or "gelu", the tanh form) and a residual of y's type, each or none of them (``out`` may be the
     residual itself).  With ``offsets`` int32 [experts + 1] (moe_route's) the rows are sorted by
     expert (moe_sort) and each is multiplied by its own expert's matrix of a packed stack, with
-    its bias of [experts, n_out]; rows that no expert has are left as they are in ``out``.  With
-    ``save`` the pre-activations are kept for mxfp4_linear_backward, bf16 [m, n_out], and
-    (y, saved) returned.  Nothing is recorded for autograd (kdq_mxfp4_linear)."""
+    its bias of [experts, n_out]; rows that no expert has are left as they are in ``out`` (and are
+    undefined in a new tensor, and in what is saved).  With ``save`` the pre-activations are kept
+    for mxfp4_linear_backward, bf16 [m, n_out], and (y, saved) returned.  Nothing is recorded for
+    autograd (kdq_mxfp4_linear)."""
     _no_graph(x, "x")
     stride = _row_stride(x, _BF16, "x")
     kind, act = _type(dtype), _activation(_ACTIVATIONS, activation)
@@ -781,8 +782,9 @@ def mxfp4_linear_backward(dy: torch.Tensor, packed: torch.Tensor, n_in: int,
     """The backward pass of mxfp4_linear over frozen weights: dy bf16 [m, n_out]
     (n_out % 8 == 0), with an activation what its forward pass saved, and the matrix or stack from
     mxfp4_pack(..., transposed=True) -> dx bf16 [m, n_in] and dpre bf16 [m, n_out], the gradient
-    before the activation (dy itself without one; the bias's gradient is the sum of its rows)
-    (kdq_mxfp4_linear_backward)."""
+    before the activation (dy itself without one; the bias's gradient is the sum of its rows, an
+    expert's of its own rows).  Of rows that no expert has dx is left as it is in ``out`` (undefined
+    in a new tensor) and dpre undefined (kdq_mxfp4_linear_backward)."""
     _no_graph(dy, "dy")
     stride = _row_stride(dy, _BF16, "dy")
     act = _activation(_ACTIVATIONS, activation)
@@ -832,8 +834,9 @@ def mxfp4_experts_gated(x: torch.Tensor, offsets: torch.Tensor, gate: torch.Tens
     int32 [experts + 1] (moe_route's) and two packed stacks (mxfp4_pack) of n_out rows
     (n_out % 32 == 0), with biases fp32 [experts, n_out] or none -> h bf16 [m, n_out]:
     silu(g) * u, or, "clamped", with g' = min(g, 7) and u' = u between -7 and 7,
-    g' sigmoid(1.702 g') (u' + 1).  Rows that no expert has are left as they are in ``out``.
-    ``save`` as for mxfp4_gated.  Nothing is recorded for autograd (kdq_mxfp4_experts_gated)."""
+    g' sigmoid(1.702 g') (u' + 1).  Rows that no expert has are left as they are in ``out`` (and are
+    undefined in a new tensor, and in what is saved).  ``save`` as for mxfp4_gated.  Nothing is
+    recorded for autograd (kdq_mxfp4_experts_gated)."""
     _no_graph(x, "x")
     stride = _row_stride(x, _BF16, "x")
     act = _activation(_GATES, activation)
@@ -895,8 +898,9 @@ def mxfp4_experts_gated_backward(dh: torch.Tensor, offsets: torch.Tensor, saved,
                                  activation: str = "silu", out: torch.Tensor | None = None):
     """The backward pass of mxfp4_experts_gated over frozen weights: dh bf16 [m, n_out], its
     offsets, ``saved`` from its forward pass, the stacks from mxfp4_pack(..., transposed=True)
-    -> dx bf16 [m, n_in] and the pre-activations' gradients bf16 [m, 2 n_out], gates then ups
-    (kdq_mxfp4_experts_gated_backward)."""
+    -> dx bf16 [m, n_in] and the pre-activations' gradients bf16 [m, 2 n_out], gates then ups.  Of
+    rows that no expert has dx is left as it is in ``out`` (undefined in a new tensor) and the
+    gradients undefined (kdq_mxfp4_experts_gated_backward)."""
     _no_graph(dh, "dh")
     stride = _row_stride(dh, _BF16, "dh")
     act = _activation(_GATES, activation)

@@ -30,8 +30,8 @@ def normal(g, *shape):
 
 
 def dropped(g, slots, share):
-    """A permutation of the slots with a share of its entries, one at least, replaced by numbers that
-    are none, and which positions those are."""
+    """A permutation of the slots with a share of its entries, one at least, replaced by numbers
+    that are none, and which positions those are."""
     perm = torch.randperm(slots, generator=g, device=g.device).int()
     gone = torch.rand(slots, generator=g, device=g.device) < share
     gone[torch.randint(slots, (1,), generator=g, device=g.device)] = True
