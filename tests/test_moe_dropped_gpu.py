@@ -166,3 +166,34 @@ def test_dropped_selections_cost_no_more_than_the_others(gen, tokens, top_k, col
             times.append(begin.elapsed_time(end))
         took.append(sorted(times)[len(times) // 2])
     assert took[1] <= 2 * took[0]
+
+
+@pytest.mark.parametrize("tokens,top_k,cols", [(64, 4, 72), (4097, 4, 40), (9000, 4, 40),
+                                               (2100, 8, 1100)])
+def test_captured_with_other_drops_at_every_replay(gen, tokens, top_k, cols):
+    slots = tokens * top_k
+    x, dy = normal(gen, tokens, cols).bfloat16(), normal(gen, tokens, cols).bfloat16()
+    weights = torch.rand(tokens, top_k, generator=gen, device=gen.device)
+    perm, _ = dropped(gen, slots, 0.2)
+
+    def chain():
+        rows, place = ops.moe_sort(x, perm, top_k)
+        y = ops.moe_combine(rows, weights, place, residual=x)
+        drows, dweights = ops.moe_combine_backward(dy, rows, weights, place)
+        return rows, place, y, drows, dweights, ops.moe_sort_backward(drows, place, top_k)
+
+    chain()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = chain()
+    for share in (0.5, 0.0, 1.0, 0.1):
+        other, gone = dropped(gen, slots, share)
+        perm.copy_(other)
+        x.copy_(normal(gen, tokens, cols))
+        eager = chain()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(eager, captured))
+        assert not bool(captured[0][gone].any()) and not bool(captured[3][gone].any())
+        assert torch.equal(captured[1], places(perm))
